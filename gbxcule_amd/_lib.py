@@ -39,8 +39,36 @@ BUF_MEM, BUF_PIX, BUF_PIX_PACKED, BUF_OBS, BUF_REWARD, BUF_ACTIONS, BUF_CART_RAM
     INFO_STEP_WAVES,
 ) = range(12)
 
+F32, BF16, F16 = range(3)
+
+_vp, _i32, _i64, _f32, _f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
+
+
+class ScanIn(ctypes.Structure):
+    """``gbx_scan_in``."""
+
+    _fields_ = [
+        *((k, _i32) for k in ("steps", "envs", "dim", "groups", "states", "elem", "softplus")),
+        *((k, _vp) for k in ("x", "dt", "z", "b", "c")),
+        *((k, _i64) for k in ("x_step", "x_env", "dt_step", "dt_env", "z_step", "z_env")),
+        *((k, _i64) for k in ("b_step", "b_env", "b_group", "c_step", "c_env", "c_group")),
+        *((k, _vp) for k in ("a", "skip", "bias", "resets")),
+    ]
+
+
+class AdamwIn(ctypes.Structure):
+    """``gbx_adamw_in``."""
+
+    _fields_ = [
+        *((k, _i32) for k in ("count", "elem", "grad_elem", "state_bits")),
+        *((k, _vp) for k in ("params", "grads", "sizes", "starts", "exp_avg", "exp_avg_sq")),
+        *((k, _vp) for k in ("exp_avg_scale", "exp_avg_sq_scale", "grad_scale")),
+        *((k, _f64) for k in ("beta1", "beta2", "step_size", "inv_root2", "eps", "keep")),
+        ("key", ctypes.c_uint32),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
-_vp, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 _P64 = ctypes.POINTER(ctypes.c_int64)
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_last_error": (ctypes.c_char_p, []),
@@ -75,6 +103,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_buffer": (ctypes.c_int, [_vp, _i32, ctypes.POINTER(_vp), _P64]),
     "gbx_info": (ctypes.c_int, [_vp, _i32, _P64]),
     "gbx_set_debug": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32]),
+    "gbx_rms_norm": (ctypes.c_int, [_i64, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp]),
+    "gbx_rms_norm_grad_work": (_i64, [_i64, _i32]),
+    "gbx_rms_norm_grad": (
+        ctypes.c_int, [_i64, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "gbx_causal_conv": (ctypes.c_int, [*[_i32] * 6, _vp, _i64, _i64, *[_vp] * 7]),
+    "gbx_causal_conv_grad_work": (_i64, [_i32] * 4),
+    "gbx_causal_conv_grad": (ctypes.c_int, [*[_i32] * 6, _vp, _i64, _i64, *[_vp] * 5, _i64, _i64, *[_vp] * 5]),
+    "gbx_causal_conv_step": (ctypes.c_int, [*[_i32] * 5, _vp, _i64, *[_vp] * 6]),
+    "gbx_selective_scan_work": (_i64, [ctypes.POINTER(ScanIn)]),
+    "gbx_selective_scan": (ctypes.c_int, [ctypes.POINTER(ScanIn), *[_vp] * 6]),
+    "gbx_selective_scan_grad_work": (_i64, [ctypes.POINTER(ScanIn)]),
+    "gbx_selective_scan_grad": (ctypes.c_int, [ctypes.POINTER(ScanIn), _vp, _vp, _i64, _i64, *[_vp] * 10]),
+    "gbx_selective_scan_step": (ctypes.c_int, [ctypes.POINTER(ScanIn), *[_vp] * 3]),
+    "gbx_adamw": (ctypes.c_int, [ctypes.POINTER(AdamwIn), _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

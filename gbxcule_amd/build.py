@@ -10,13 +10,16 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libgbx_hip.so"
-SOURCES = ("gbx_step.hip", "gbx_aux.hip", "gbx_api.hip")
+SOURCES = (
+    "gbx_step.hip", "gbx_aux.hip", "gbx_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_adamw.hip", "gbx_api.hip",
+)  # fmt: skip
 ARCH = os.environ.get("GBX_OFFLOAD_ARCH", "gfx950")
 # -O2 with the iterative ILP machine scheduler: on the step kernel's hot
 # loop this schedules the dependent loads earlier than -O3 with the default
@@ -43,26 +46,29 @@ def hipcc() -> str:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP source and link the shared library (always rebuilds)."""
+    """Compile every HIP source and link the shared library (always rebuilds).
+    The sources compile side by side."""
     LIB_DIR.mkdir(exist_ok=True)
     tmp = LIB_DIR / "libgbx_hip.so.tmp"
-    cmd = [
-        hipcc(),
-        *DEVICE_FLAGS,
-        "-fPIC",
-        "-shared",
-        "-I",
-        str(PKG.parent / "include"),
-        "-o",
-        str(tmp),
-        *[str(CSRC / s) for s in SOURCES],
+    include = ["-I", str(PKG.parent / "include")]
+    objects = [LIB_DIR / f"{Path(s).stem}.o" for s in SOURCES]
+    commands = [
+        [hipcc(), *DEVICE_FLAGS, "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)] for s, o in zip(SOURCES, objects)
     ]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("hipcc failed building libgbx_hip.so")
+    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+        done = list(pool.map(lambda cmd: subprocess.run(cmd, capture_output=True, text=True), commands))
+    link = [hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", str(tmp), *map(str, objects)]
+    if all(res.returncode == 0 for res in done):
+        commands.append(link)
+        done.append(subprocess.run(link, capture_output=True, text=True))
+    for cmd, res in zip(commands, done):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError(f"hipcc failed: {cmd[-3]}" if cmd is not link else "hipcc failed linking libgbx_hip.so")
+    for o in objects:
+        o.unlink()
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

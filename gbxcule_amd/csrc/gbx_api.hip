@@ -10,6 +10,7 @@
 #include "../../include/gbx_hip.h"
 #include "gbx_aux.h"
 #include "gbx_decode.h"
+#include "gbx_policy.h"
 
 using namespace gbx;
 
@@ -236,6 +237,44 @@ int check_rect(const gbx_ctx* ctx, int32_t env_lo, int32_t env_hi, int32_t lo, i
   if (env_lo < 0 || env_hi > ctx->s.n || env_lo > env_hi)
     return fail(GBX_E_INVALID, "env range out of bounds");
   if (lo < 0 || hi > kMemSize || lo > hi) return fail(GBX_E_INVALID, "address range out of bounds");
+  return GBX_OK;
+}
+
+// Argument checks of the policy operators.  The limits keep every count that
+// a kernel holds in 32 bits there; offsets are 64-bit.
+constexpr int64_t kMaxDim = 1 << 20, kMaxRows = (int64_t)1 << 40;
+int check_norm(int64_t rows, int32_t dim, int32_t elem) {
+  if (rows < 0 || rows > kMaxRows) return fail(GBX_E_INVALID, "row count out of range");
+  if (dim < 1 || dim > kMaxDim) return fail(GBX_E_INVALID, "channel count out of range");
+  if (elem < GBX_F32 || elem > GBX_F16) return fail(GBX_E_INVALID, "bad element type");
+  return GBX_OK;
+}
+int check_rows(int32_t steps, int32_t envs) {
+  if (steps < 1 || steps > 1 << 30) return fail(GBX_E_INVALID, "step count out of range");
+  if (envs < 1 || envs > 1 << 26) return fail(GBX_E_INVALID, "env count out of range");
+  return GBX_OK;
+}
+int check_conv(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem) {
+  if (int e = check_rows(steps, envs)) return e;
+  if (int e = check_norm(0, dim, elem)) return e;
+  if (width < 2 || width > 4) return fail(GBX_E_INVALID, "width must be 2, 3 or 4");
+  return GBX_OK;
+}
+int scan_args(const gbx_scan_in* in, ScanArgs& a) {
+  if (!in) return fail(GBX_E_INVALID, "in is NULL");
+  if (int e = check_rows(in->steps, in->envs)) return e;
+  if (int e = check_norm(0, in->dim, in->elem)) return e;
+  if (in->states < 1 || in->states > kMaxStates) return fail(GBX_E_INVALID, "1 to 32 states are supported");
+  if (in->groups < 1 || in->dim % in->groups) return fail(GBX_E_INVALID, "dim must be a multiple of groups");
+  if (!in->x || !in->dt || !in->b || !in->c || !in->a) return fail(GBX_E_INVALID, "x, dt, a, b or c is NULL");
+  a = ScanArgs{};
+  a.steps = in->steps, a.envs = in->envs, a.dim = in->dim, a.groups = in->groups, a.states = in->states;
+  a.elem = in->elem, a.softplus = in->softplus;
+  a.x = in->x, a.dt = in->dt, a.z = in->z, a.b = in->b, a.c = in->c;
+  a.x_step = in->x_step, a.x_env = in->x_env, a.dt_step = in->dt_step, a.dt_env = in->dt_env;
+  a.z_step = in->z_step, a.z_env = in->z_env, a.b_step = in->b_step, a.b_env = in->b_env, a.b_group = in->b_group;
+  a.c_step = in->c_step, a.c_env = in->c_env, a.c_group = in->c_group;
+  a.a = in->a, a.skip = in->skip, a.bias = in->bias, a.resets = in->resets;
   return GBX_OK;
 }
 
@@ -799,6 +838,146 @@ int gbx_set_debug(gbx_ctx* ctx, int32_t rst38, int32_t trap_pc, int32_t max_inst
   ctx->dbg[1] = trap_pc & 0xFFFF;
   ctx->dbg[2] = max_instr > 0 ? max_instr : 0;
   ctx->dbg[3] = watch_addr & 0xFFFF;
+  return GBX_OK;
+}
+
+// ---- operators of a policy with memory ----
+
+int gbx_rms_norm(int64_t rows, int32_t dim, int32_t elem, float eps, const void* x, int64_t x_stride,
+                 const void* residual, int64_t residual_stride, const float* weight, void* out, void* summed,
+                 float* scale, int32_t group, void* stream) {
+  if (int e = check_norm(rows, dim, elem)) return e;
+  if (group != 0 && group != 128) return fail(GBX_E_INVALID, "group must be 0 or 128");
+  if (rows == 0) return GBX_OK;
+  if (!x || !weight || !out) return fail(GBX_E_INVALID, "x, weight or out is NULL");
+  if (!residual != !summed) return fail(GBX_E_INVALID, "residual and summed go together");
+  NormArgs a{rows, dim, elem, eps, x, residual, x_stride, residual_stride, weight, out, summed, scale, group};
+  HIP_TRY(launch_rms_norm(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int64_t gbx_rms_norm_grad_work(int64_t rows, int32_t dim) {
+  if (int e = check_norm(rows, dim, GBX_F32)) return e;
+  return norm_grad_work(rows, dim);
+}
+int gbx_rms_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const void* summed, int64_t summed_stride,
+                      const void* dy, int64_t dy_stride, const void* dsummed, int64_t dsummed_stride,
+                      const float* weight, void* dx, float* dweight, float* work, void* stream) {
+  if (int e = check_norm(rows, dim, elem)) return e;
+  if (rows == 0) return fail(GBX_E_INVALID, "no rows");
+  if (!summed || !dy || !weight || !dx || !dweight || !work) return fail(GBX_E_INVALID, "an argument is NULL");
+  NormGradArgs a{rows, dim, elem, eps, summed, dy, dsummed, summed_stride, dy_stride, dsummed_stride, weight, dx, dweight, work};
+  HIP_TRY(launch_rms_norm_grad(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
+int gbx_causal_conv(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu, const void* x,
+                    int64_t x_step, int64_t x_env, const float* weight, const float* bias, const void* state,
+                    const uint8_t* resets, void* y, void* last, void* stream) {
+  if (int e = check_conv(steps, envs, dim, width, elem)) return e;
+  if (!x || !weight || !y || !last) return fail(GBX_E_INVALID, "x, weight, y or last is NULL");
+  ConvArgs a{};
+  a.steps = steps, a.envs = envs, a.dim = dim, a.width = width, a.elem = elem, a.silu = silu;
+  a.x = x, a.x_step = x_step, a.x_env = x_env, a.weight = weight, a.bias = bias;
+  a.state = state, a.resets = resets, a.y = y, a.last = last;
+  HIP_TRY(launch_conv(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int64_t gbx_causal_conv_grad_work(int32_t steps, int32_t envs, int32_t dim, int32_t width) {
+  if (int e = check_conv(steps, envs, dim, width, GBX_F32)) return e;
+  return conv_grad_work(steps, envs, dim, width);
+}
+int gbx_causal_conv_grad(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu,
+                         const void* x, int64_t x_step, int64_t x_env, const float* weight, const float* bias,
+                         const void* state, const uint8_t* resets, const void* dy, int64_t dy_step, int64_t dy_env,
+                         void* dx, float* dweight, float* dbias, float* work, void* stream) {
+  if (int e = check_conv(steps, envs, dim, width, elem)) return e;
+  if (!x || !weight || !dy || !dx || !dweight || !work) return fail(GBX_E_INVALID, "an argument is NULL");
+  ConvArgs a{};
+  a.steps = steps, a.envs = envs, a.dim = dim, a.width = width, a.elem = elem, a.silu = silu;
+  a.x = x, a.x_step = x_step, a.x_env = x_env, a.weight = weight, a.bias = bias;
+  a.state = state, a.resets = resets, a.dy = dy, a.dy_step = dy_step, a.dy_env = dy_env;
+  a.dx = dx, a.dweight = dweight, a.dbias = dbias, a.work = work;
+  HIP_TRY(launch_conv_grad(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int gbx_causal_conv_step(int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu, const void* x,
+                         int64_t x_env, const float* weight, const float* bias, void* state, const uint8_t* resets,
+                         void* y, void* stream) {
+  if (int e = check_conv(1, envs, dim, width, elem)) return e;
+  if (!x || !weight || !state || !y) return fail(GBX_E_INVALID, "x, weight, state or y is NULL");
+  ConvArgs a{};
+  a.steps = 1, a.envs = envs, a.dim = dim, a.width = width, a.elem = elem, a.silu = silu;
+  a.x = x, a.x_env = x_env, a.weight = weight, a.bias = bias, a.resets = resets, a.y = y, a.last = state;
+  HIP_TRY(launch_conv_step(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
+int64_t gbx_selective_scan_work(const gbx_scan_in* in) {
+  ScanArgs a;
+  if (int e = scan_args(in, a)) return e;
+  return scan_work(a.steps, a.envs, a.dim, a.groups, a.states);
+}
+int gbx_selective_scan(const gbx_scan_in* in, const float* state, void* y, float* last, float* saved, float* work,
+                       void* stream) {
+  ScanArgs a;
+  if (int e = scan_args(in, a)) return e;
+  if (!y || !last) return fail(GBX_E_INVALID, "y or last is NULL");
+  if (!work && scan_work(a.steps, a.envs, a.dim, a.groups, a.states) > 0) return fail(GBX_E_INVALID, "work is NULL");
+  a.state = state, a.y = y, a.last = last, a.saved = saved, a.work = work;
+  HIP_TRY(launch_scan(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int64_t gbx_selective_scan_grad_work(const gbx_scan_in* in) {
+  ScanArgs a;
+  if (int e = scan_args(in, a)) return e;
+  return scan_grad_work(a.steps, a.envs, a.dim, a.groups, a.states);
+}
+int gbx_selective_scan_grad(const gbx_scan_in* in, const float* saved, const void* dy, int64_t dy_step, int64_t dy_env,
+                            void* dx, void* ddt, void* dz, void* db, void* dc, float* da, float* dskip, float* dbias,
+                            float* work, void* stream) {
+  ScanArgs a;
+  if (int e = scan_args(in, a)) return e;
+  if (!saved || !dy || !dx || !ddt || !db || !dc || !da || !work) return fail(GBX_E_INVALID, "an argument is NULL");
+  if (!dz != !a.z) return fail(GBX_E_INVALID, "z and dz go together");
+  a.saved = const_cast<float*>(saved), a.dy = dy, a.dy_step = dy_step, a.dy_env = dy_env;
+  a.dx = dx, a.ddt = ddt, a.dz = dz, a.db = db, a.dc = dc, a.da = da, a.dskip = dskip, a.dbias = dbias, a.work = work;
+  HIP_TRY(launch_scan_grad(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* stream) {
+  ScanArgs a;
+  if (int e = scan_args(in, a)) return e;
+  if (a.steps != 1) return fail(GBX_E_INVALID, "steps must be 1");
+  if (!state || !y) return fail(GBX_E_INVALID, "state or y is NULL");
+  a.last = state, a.y = y;
+  HIP_TRY(launch_scan_step(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
+int gbx_adamw(const gbx_adamw_in* in, void* stream) {
+  if (!in || in->count < 0) return fail(GBX_E_INVALID, "in is NULL or its count negative");
+  if (in->count == 0) return GBX_OK;
+  if (in->elem < GBX_F32 || in->elem > GBX_F16 || (in->grad_elem != in->elem && in->grad_elem != GBX_F32))
+    return fail(GBX_E_INVALID, "parameters and gradients of these types are not supported");
+  if (in->state_bits != 8 && in->state_bits != 32) return fail(GBX_E_INVALID, "state_bits must be 8 or 32");
+  if (!in->params || !in->grads || !in->sizes || !in->starts || !in->exp_avg || !in->exp_avg_sq ||
+      (in->state_bits == 8 && (!in->exp_avg_scale || !in->exp_avg_sq_scale)))
+    return fail(GBX_E_INVALID, "an argument is NULL");
+  for (int i = 0; i < in->count; ++i) {
+    if (in->sizes[i] < 0 || in->sizes[i] > (int64_t)1 << 34) return fail(GBX_E_INVALID, "tensor size out of range");
+    if (in->starts[i] < 0 || in->starts[i] % kStateBlock || in->starts[i] / kStateBlock > UINT32_MAX)
+      return fail(GBX_E_INVALID, "states start at multiples of 256");
+    if (in->sizes[i] > 0 && (!in->params[i] || !in->grads[i])) return fail(GBX_E_INVALID, "a tensor is NULL");
+  }
+  AdamArgs a{};
+  a.count = in->count, a.elem = in->elem, a.grad_elem = in->grad_elem, a.small = in->state_bits == 8;
+  a.params = in->params, a.grads = in->grads, a.sizes = in->sizes, a.starts = in->starts;
+  a.exp_avg = in->exp_avg, a.exp_avg_sq = in->exp_avg_sq;
+  a.exp_avg_scale = in->exp_avg_scale, a.exp_avg_sq_scale = in->exp_avg_sq_scale, a.grad_scale = in->grad_scale;
+  a.beta1 = (float)in->beta1, a.rest1 = (float)(1.0 - in->beta1), a.beta2 = (float)in->beta2, a.rest2 = (float)(1.0 - in->beta2);
+  a.step_size = (float)in->step_size, a.inv_root2 = (float)in->inv_root2, a.eps = (float)in->eps, a.keep = (float)in->keep;
+  a.key = in->key;
+  HIP_TRY(launch_adamw(a, (hipStream_t)stream));
   return GBX_OK;
 }
 

@@ -1,0 +1,332 @@
+// gbx_norm.hip -- root-mean-square norm with the residual's addition, its
+// gradient and its output in 8 bits, and the column sums that the gradients
+// of shared inputs end with.
+#include "gbx_policy.h"
+
+#include <algorithm>
+
+namespace gbx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;  // channels a lane takes at a time: 16 bytes of a 16-bit type
+
+// Sum (or, of bit patterns of absolute values, maximum) over LANES
+// neighbouring lanes; 256 lanes are the whole workgroup.
+template <int LANES>
+__device__ __forceinline__ float sum_over(float v, float* lds) {
+#pragma unroll
+  for (int m = 1; m < (LANES < 64 ? LANES : 64); m <<= 1) v += __shfl_xor(v, m, 64);
+  if constexpr (LANES == 256) {
+    __syncthreads();  // the last use of lds has been read
+    if ((threadIdx.x & 63u) == 0u) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  }
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t max_over(uint32_t v, float* lds) {
+#pragma unroll
+  for (int m = 1; m < (LANES < 64 ? LANES : 64); m <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
+    v = o > v ? o : v;
+  }
+  if constexpr (LANES == 256) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(lds);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0u) w[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const uint32_t a = w[0] > w[1] ? w[0] : w[1], b = w[2] > w[3] ? w[2] : w[3];
+    v = a > b ? a : b;
+  }
+  return v;
+}
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kScaleFloor = 1e-30f;  // keeps the scale of an all-zero group positive
+
+// y = s * rsqrt(mean(s^2) + eps) * weight with s = x + residual rounded to the
+// stream's type, so that the gradient sees the s that was normalised.
+//
+// LANES lanes hold one row, kVec * NV channels each, in registers: x and the
+// residual are read once, y and s written once.  NV = 0 takes rows of any
+// length in steps of the workgroup and reads the row a second time.
+template <typename T, int LANES, int NV, bool FP8>
+__global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
+  constexpr int kRows = kThreads / LANES, kHeld = NV ? NV : 1;
+  __shared__ float lds[4];
+  const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, dim = a.dim;
+  const int rounds = NV ? NV : (dim + kVec * LANES - 1) / (kVec * LANES);
+  const float inv_dim = 1.0f / (float)dim;
+  float w[kHeld][kVec];
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LANES + lane) * kVec;
+      load_row<kVec>(a.weight + c, dim - c, w[k]);
+    }
+  }
+  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.rows; row += (int64_t)gridDim.x * kRows) {
+    const T* x = (const T*)a.x + row * a.x_stride;
+    const T* r = (const T*)a.residual + row * a.residual_stride;
+    T* out = (T*)a.out + row * dim;
+    T* summed = (T*)a.summed + row * dim;
+    float s[kHeld][kVec], ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < rounds; ++k) {
+      const int c = (k * LANES + lane) * kVec;
+      float(&v)[kVec] = s[NV ? k : 0];
+      load_row<kVec>(x + c, dim - c, v);
+      if (a.residual) {
+        float o[kVec];
+        load_row<kVec>(r + c, dim - c, o);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = (float)(T)(v[i] + o[i]);
+        store_row<kVec>(summed + c, dim - c, v);
+      }
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) ss = fmaf(v[i], v[i], ss);
+    }
+    const float rstd = rsqrtf(fmaf(sum_over<LANES>(ss, lds), inv_dim, a.eps));
+    auto normed = [&](int k, float (&y)[kVec]) {
+      const int c = (k * LANES + lane) * kVec;
+      if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) y[i] = s[k][i] * rstd * w[k][i];
+      } else {
+        float wk[kVec];
+        load_row<kVec>(a.residual ? summed + c : x + c, dim - c, y);
+        load_row<kVec>(a.weight + c, dim - c, wk);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) y[i] *= rstd * wk[i];
+      }
+    };
+    auto most = [](const float (&y)[kVec], uint32_t m) {
+      // bit patterns of absolute values order as the values do, NaN above all
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t b = __float_as_uint(y[i]) & 0x7FFFFFFFu;
+        m = b > m ? b : m;
+      }
+      return m;
+    };
+    if constexpr (FP8) {
+      uint32_t row_most = 0;
+      if (a.group == 0) {
+#pragma unroll
+        for (int k = 0; k < rounds; ++k) {
+          float y[kVec];
+          normed(k, y);
+          row_most = most(y, row_most);
+        }
+        row_most = max_over<LANES>(row_most, lds);
+      }
+      uint8_t* q = (uint8_t*)a.out + row * dim;
+      const int groups = a.group ? (dim + 127) / 128 : 1;
+#pragma unroll
+      for (int k = 0; k < rounds; ++k) {
+        const int c = (k * LANES + lane) * kVec;
+        float y[kVec];
+        normed(k, y);
+        // 128 channels are 16 neighbouring lanes
+        const uint32_t m = a.group ? max_over<16>(most(y, 0u), lds) : row_most;
+        const float top = m > 0x7F800000u ? __uint_as_float(m) : fmaxf(__uint_as_float(m), kScaleFloor);
+        const float inv = kE4m3Max / top;
+        if (a.group ? (lane % 16 == 0 && c < dim) : (lane == 0 && k == 0)) a.scale[row * groups + (a.group ? c / 128 : 0)] = top / kE4m3Max;
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * inv, y[1] * inv, 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * inv, y[3] * inv, lo, true);
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
+        const uint64_t both = (uint32_t)lo | (uint64_t)(uint32_t)hi << 32;
+        if (dim - c >= kVec) {
+          __builtin_memcpy(q + c, &both, 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i)
+            if (i < dim - c) q[c + i] = (uint8_t)(both >> (8 * i));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < rounds; ++k) {
+        const int c = (k * LANES + lane) * kVec;
+        float y[kVec];
+        normed(k, y);
+        store_row<kVec>(out + c, dim - c, y);
+      }
+    }
+  }
+}
+
+// With g = weight * dy and r = rsqrt(mean(s^2) + eps):
+//   ds = r * g - s * r^3 * mean(g * s) + dsummed,   dweight = sum over rows of dy * s * r.
+// The row stays in registers as in the forward kernel; both means come from
+// one pass, so nothing but s itself has to be kept from the forward.  A
+// workgroup sums dweight over its rows in registers, then over its row slots
+// in LDS, and writes one row of partial sums: no atomics, one order.
+template <typename T, int LANES, int NV>
+__global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kRows = kThreads / LANES, kHeld = NV ? NV : 1;
+  __shared__ float lds[4];
+  const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, dim = a.dim;
+  const int rounds = NV ? NV : (dim + kVec * LANES - 1) / (kVec * LANES);
+  const float inv_dim = 1.0f / (float)dim;
+  float* part = a.work + (int64_t)blockIdx.x * dim;
+  float w[kHeld][kVec], dw[kHeld][kVec];
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LANES + lane) * kVec;
+      load_row<kVec>(a.weight + c, dim - c, w[k]);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) dw[k][i] = 0.0f;
+    }
+  }
+  const int64_t first = (int64_t)blockIdx.x * kRows + sub;
+  for (int64_t row = first; row < a.rows; row += (int64_t)gridDim.x * kRows) {
+    const T* sp = (const T*)a.summed + row * a.summed_stride;
+    const T* dyp = (const T*)a.dy + row * a.dy_stride;
+    const T* dsp = (const T*)a.dsummed + row * a.dsummed_stride;
+    T* dxp = (T*)a.dx + row * dim;
+    float s[kHeld][kVec], dy[kHeld][kVec], ss = 0.0f, gs = 0.0f;
+#pragma unroll
+    for (int k = 0; k < rounds; ++k) {
+      const int c = (k * LANES + lane) * kVec, h = NV ? k : 0;
+      load_row<kVec>(sp + c, dim - c, s[h]);
+      load_row<kVec>(dyp + c, dim - c, dy[h]);
+      if constexpr (NV == 0) load_row<kVec>(a.weight + c, dim - c, w[0]);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        ss = fmaf(s[h][i], s[h][i], ss);
+        gs = fmaf(s[h][i], dy[h][i] * w[h][i], gs);
+      }
+    }
+    const float rstd = rsqrtf(fmaf(sum_over<LANES>(ss, lds), inv_dim, a.eps));
+    const float pull = sum_over<LANES>(gs, lds) * inv_dim * rstd * rstd;
+#pragma unroll
+    for (int k = 0; k < rounds; ++k) {
+      const int c = (k * LANES + lane) * kVec, h = NV ? k : 0;
+      if constexpr (NV == 0) {
+        load_row<kVec>(sp + c, dim - c, s[0]);
+        load_row<kVec>(dyp + c, dim - c, dy[0]);
+        load_row<kVec>(a.weight + c, dim - c, w[0]);
+      }
+      float dx[kVec];
+      if (a.dsummed) {
+        load_row<kVec>(dsp + c, dim - c, dx);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) dx[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        dx[i] = fmaf(rstd, fmaf(-s[h][i], pull, dy[h][i] * w[h][i]), dx[i]);
+        const float grow = dy[h][i] * (s[h][i] * rstd);
+        if constexpr (NV > 0) dw[k][i] += grow;
+        else if (c + i < dim) part[c + i] = row == first ? grow : part[c + i] + grow;
+      }
+      store_row<kVec>(dxp + c, dim - c, dx);
+    }
+  }
+  if constexpr (NV > 0) {
+    if constexpr (kRows > 1) {
+      __shared__ float tile[kThreads * NV * kVec];
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) tile[sub * (LANES * NV * kVec) + (k * LANES + lane) * kVec + i] = dw[k][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < dim; c += kThreads) {
+        float v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) v += tile[r * (LANES * NV * kVec) + c];
+        part[c] = v;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * LANES + lane) * kVec;
+        store_row<kVec>(part + c, dim - c, dw[k]);
+      }
+    }
+  }
+}
+
+// out[c] = sum of in[r][c] over r: 16 columns by 64 rows of a workgroup at a
+// time, so that a few columns still fill the chip's memory pipes; one order.
+constexpr int kSumCols = 16, kSumRows = 64;
+__global__ __launch_bounds__(kSumCols* kSumRows) void column_sum_kernel(const float* in, int64_t stride, int rows, int cols, float* out) {
+  __shared__ float tile[kSumRows][kSumCols + 1];
+  const int c = blockIdx.x * kSumCols + threadIdx.x % kSumCols, r0 = threadIdx.x / kSumCols;
+  float v = 0.0f;
+  if (c < cols)
+    for (int r = r0; r < rows; r += kSumRows) v += in[(int64_t)r * stride + c];
+  tile[r0][threadIdx.x % kSumCols] = v;
+  __syncthreads();
+#pragma unroll
+  for (int m = kSumRows / 2; m > 0; m >>= 1) {
+    if (r0 < m) tile[r0][threadIdx.x % kSumCols] += tile[r0 + m][threadIdx.x % kSumCols];
+    __syncthreads();
+  }
+  if (r0 == 0 && c < cols) out[c] = tile[0][threadIdx.x];
+}
+
+template <typename F>
+void by_row_length(int dim, F&& f) {
+  // lanes of a row and 8-channel pieces of a lane: the fewest that hold it
+  if (dim <= 128) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  else if (dim <= 256) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+  else if (dim <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+  else if (dim <= 1024) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  else if (dim <= 2048) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  else if (dim <= 4096) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+  else if (dim <= 8192) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
+}
+int lanes_of(int dim) {
+  int lanes = 0;
+  by_row_length(dim, [&](auto l, auto) { lanes = l; });
+  return lanes;
+}
+constexpr int kGradBlocks = 1024;  // workgroups of the gradient, each a row of partial sums
+int grad_blocks(int64_t rows, int dim) {
+  const int per = kThreads / lanes_of(dim);
+  return (int)std::min<int64_t>((rows + per - 1) / per, kGradBlocks);
+}
+
+}  // namespace
+
+hipError_t launch_column_sum(const float* in, int64_t stride, int rows, int cols, float* out, hipStream_t st) {
+  hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((cols + kSumCols - 1) / kSumCols)), dim3(kSumCols * kSumRows), 0, st, in, stride, rows, cols, out);
+  return hipGetLastError();
+}
+
+hipError_t launch_rms_norm(const NormArgs& a, hipStream_t st) {
+  by_element(a.elem, [&](auto t) {
+    using T = decltype(t);
+    by_row_length(a.dim, [&](auto lanes, auto nv) {
+      const int64_t per = kThreads / lanes;
+      const dim3 grid((unsigned)std::min<int64_t>((a.rows + per - 1) / per, 1 << 16));
+      if (a.scale) hipLaunchKernelGGL((norm_kernel<T, lanes, nv, true>), grid, dim3(kThreads), 0, st, a);
+      else hipLaunchKernelGGL((norm_kernel<T, lanes, nv, false>), grid, dim3(kThreads), 0, st, a);
+    });
+  });
+  return hipGetLastError();
+}
+
+int64_t norm_grad_work(int64_t rows, int dim) { return (int64_t)grad_blocks(rows, dim) * dim; }
+
+hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t st) {
+  const int blocks = grad_blocks(a.rows, a.dim);
+  by_element(a.elem, [&](auto t) {
+    using T = decltype(t);
+    by_row_length(a.dim, [&](auto lanes, auto nv) {
+      hipLaunchKernelGGL((norm_grad_kernel<T, lanes, nv>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
+    });
+  });
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  return launch_column_sum(a.work, a.dim, blocks, a.dim, a.dweight, st);
+}
+
+}  // namespace gbx

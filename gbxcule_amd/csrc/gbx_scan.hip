@@ -1,0 +1,705 @@
+// gbx_scan.hip -- selective state space scan along the steps of each env, its
+// gradient and its single step.  For every channel d with `states` states s:
+//
+//   delta = softplus(dt + bias)                        (or dt + bias as it is)
+//   h[s]  = exp(delta * A[d][s]) * h[s] + delta * x * B[s]     (h = 0 first where an episode begins)
+//   y     = (sum over s of C[s] * h[s] + skip * x) * silu(z)
+//
+// A state costs one exponential and six other operations a step for 8/16
+// bytes of 16-bit input and output, so the kernels are bound by the vector
+// units, not by memory.  States, step sizes and sums are 32-bit throughout.
+#include <algorithm>
+
+#include "gbx_policy.h"
+
+namespace gbx {
+namespace {
+
+constexpr int kWave = 64;
+constexpr int kWaves = 4;  // wavefronts of a forward workgroup
+
+// log(1 + e^v).  log1p(e) for small e as log(u) * e / (u - 1) with u = 1 + e
+// rounded: the rounding error of u cancels (Goldberg, "What every computer
+// scientist should know about floating-point arithmetic", theorem 4).
+__device__ __forceinline__ float softplus(float v) {
+  const float e = exp2_fast(-kLog2e * fabsf(v));
+  const float u = 1.0f + e;
+  const float log1p = u == 1.0f ? e : __builtin_amdgcn_logf(u) * kLn2 * (e * rcp_fast(u - 1.0f));
+  return fmaxf(v, 0.0f) + log1p;
+}
+
+template <int SP, typename T>
+struct RowBits {  // SP elements of a row as the dwords that a scalar load takes
+  static constexpr int kWords = SP * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+};
+template <typename T>
+__device__ __forceinline__ float unpack(const uint32_t* w, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+  else if constexpr (__is_same(T, __bf16)) return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+}
+typedef const uint32_t __attribute__((address_space(4))) * ScalarPtr;
+template <int SP, typename T>
+__device__ __forceinline__ void load_scalar(const T* p, RowBits<SP, T>& r) {
+  ScalarPtr q = (ScalarPtr)(uintptr_t)p;
+#pragma unroll
+  for (int i = 0; i < RowBits<SP, T>::kWords; ++i) r.w[i] = q[i];
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
+// How the steps are divided.  A wavefront takes 64 channels (of one group) of
+// one env and one piece of the steps.
+struct Pieces {
+  int blocks, blocks_per_group;  // channel blocks of a wavefront
+  int chunk, chunks;             // steps of a piece, pieces
+};
+
+enum { FULL, ENDS, BACK };  // what scan_kernel computes
+
+// A lane is a channel and holds its states; B and C are the same for all lanes
+// of a wavefront and come through scalar registers: SCALAR loads them as
+// dwords (rows that start on 4 bytes and hold exactly SP states), else each
+// lane loads one element and the wavefront reads lanes.
+//
+// FULL: y and the last state.  Where there are too few rows to fill the chip
+// the steps are cut: ENDS computes, for each piece, the state that it ends
+// with when it starts from zero and the sum of its step sizes, whose decay
+// carries any start state across the piece (h_end = exp(A * sum) * h_start +
+// ends); join_kernel runs over the pieces; FULL then starts each piece from
+// its own state.  BACK is ENDS for the gradient, against the steps: the
+// gradient of the state before a piece when nothing flows into its end.
+template <typename T, int SP, int WHAT, bool SCALAR>
+__global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces p, float* ends, float* sums) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = block_id() * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = wave / p.blocks;
+  const int block = (int)(wave % p.blocks);
+  const int env = (int)(item % a.envs), piece = (int)(item / a.envs);
+  if (piece >= p.chunks) return;
+  const int group = block / p.blocks_per_group, per_group = a.dim / a.groups;
+  const int in_group = (block % p.blocks_per_group) * kWave + lane;
+  const bool live = in_group < per_group;
+  const int d = group * per_group + min(in_group, per_group - 1);
+  const int t0 = piece * p.chunk, t1 = min(t0 + p.chunk, a.steps), count = t1 - t0;
+  const bool gated = a.z != nullptr;
+
+  float decay[SP], h[SP];  // A in powers of two; the states, or their gradient
+#pragma unroll
+  for (int s = 0; s < SP; ++s) {
+    decay[s] = s < a.states ? a.a[(int64_t)d * a.states + s] * kLog2e : 0.0f;
+    h[s] = 0.0f;
+  }
+  const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
+  if constexpr (WHAT == FULL) {
+    if (p.chunks > 1) {
+#pragma unroll
+      for (int s = 0; s < SP; ++s)
+        if (s < a.states) h[s] = ends[((int64_t)item * a.states + s) * a.dim + d];
+    } else if (a.state) {
+#pragma unroll
+      for (int s = 0; s < SP; ++s)
+        if (s < a.states) h[s] = a.state[((int64_t)env * a.dim + d) * a.states + s];
+    }
+  }
+
+  const T* x = (const T*)(WHAT == BACK ? a.dy : a.x) + (int64_t)env * (WHAT == BACK ? a.dy_env : a.x_env) + d;
+  const int64_t x_step = WHAT == BACK ? a.dy_step : a.x_step;
+  const T* dt = (const T*)a.dt + (int64_t)env * a.dt_env + d;
+  const T* z = (const T*)a.z + (int64_t)env * a.z_env + d;
+  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
+  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
+  const uint8_t* resets = a.resets + env;
+  T* y = (T*)a.y + (int64_t)env * a.dim + d;
+
+  constexpr int kAhead = 4;  // steps whose loads are in flight together
+  T xs[kAhead], dts[kAhead], zs[kAhead], bcs[kAhead];
+  uint8_t rs[kAhead];
+  const bool lane_is_c = lane >= 32;
+  const bool lane_holds = (lane & 31) < a.states;
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = min(k0 + i, count - 1);
+      const int t = WHAT == BACK ? t1 - 1 - k : t0 + k;
+      xs[i] = x[(int64_t)t * x_step];
+      dts[i] = dt[(int64_t)t * a.dt_step];
+      if (gated && WHAT != ENDS) zs[i] = z[(int64_t)t * a.z_step];
+      if (a.resets) rs[i] = resets[(int64_t)t * a.envs];
+      if constexpr (!SCALAR) {
+        const T* row = lane_is_c ? c + (int64_t)t * a.c_step : b + (int64_t)t * a.b_step;
+        bcs[i] = lane_holds ? row[lane & 31] : (T)0.0f;
+      }
+    }
+  };
+  float sum = 0.0f;
+  bool began = false;
+  fetch(0);
+  for (int k0 = 0; k0 < count; k0 += kAhead) {
+    float xv[kAhead], dtv[kAhead], zv[kAhead], bcv[kAhead];
+    bool begins[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      xv[i] = (float)xs[i];
+      dtv[i] = (float)dts[i];
+      zv[i] = gated && WHAT != ENDS ? (float)zs[i] : 0.0f;
+      if constexpr (!SCALAR) bcv[i] = (float)bcs[i];
+      begins[i] = a.resets && __builtin_amdgcn_readfirstlane((int)rs[i]) != 0;
+    }
+    if (k0 + kAhead < count) fetch(k0 + kAhead);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (k0 + i >= count) break;
+      const int t = WHAT == BACK ? t1 - 1 - k0 - i : t0 + k0 + i;
+      float delta = dtv[i] + bias;
+      if (a.softplus) delta = softplus(delta);
+      float bv[SP], cv[SP];
+      if constexpr (SCALAR) {
+        RowBits<SP, T> rb, rc;
+        if constexpr (WHAT != BACK) {
+          load_scalar(b + (int64_t)t * a.b_step, rb);
+#pragma unroll
+          for (int s = 0; s < SP; ++s) bv[s] = unpack<T>(rb.w, s);
+        }
+        if constexpr (WHAT != ENDS) {
+          load_scalar(c + (int64_t)t * a.c_step, rc);
+#pragma unroll
+          for (int s = 0; s < SP; ++s) cv[s] = unpack<T>(rc.w, s);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+          if constexpr (WHAT != BACK) bv[s] = lane_value(bcv[i], s);
+          if constexpr (WHAT != ENDS) cv[s] = lane_value(bcv[i], 32 + s);
+        }
+      }
+      if constexpr (WHAT == BACK) {
+        const float dv = gated ? xv[i] * zv[i] * sigmoid(zv[i]) : xv[i];
+#pragma unroll
+        for (int s = 0; s < SP; ++s) h[s] = fmaf(cv[s], dv, h[s]) * exp2_fast(delta * decay[s]);
+        if (begins[i]) {
+#pragma unroll
+          for (int s = 0; s < SP; ++s) h[s] = 0.0f;
+        }
+        sum += delta;
+        began = began || begins[i];
+      } else {
+        if (begins[i]) {
+#pragma unroll
+          for (int s = 0; s < SP; ++s) h[s] = 0.0f;
+        }
+        if constexpr (WHAT == FULL) {
+          if (a.saved && t % kSegment == 0 && live) {
+            float* to = a.saved + ((int64_t)(t / kSegment) * a.envs + env) * a.states * a.dim + d;
+#pragma unroll
+            for (int s = 0; s < SP; ++s)
+              if (s < a.states) to[(int64_t)s * a.dim] = h[s];
+          }
+        }
+        const float u = delta * xv[i];
+        float part[2] = {skip * xv[i], 0.0f};
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+          h[s] = fmaf(h[s], exp2_fast(delta * decay[s]), u * bv[s]);
+          if constexpr (WHAT == FULL) part[s & 1] = fmaf(h[s], cv[s], part[s & 1]);
+        }
+        if constexpr (WHAT == FULL) {
+          float out = part[0] + part[1];
+          if (gated) out *= zv[i] * sigmoid(zv[i]);
+          if (live) y[(int64_t)t * a.envs * a.dim] = (T)out;
+        } else {
+          sum = begins[i] ? delta : sum + delta;
+          began = began || begins[i];
+        }
+      }
+    }
+  }
+  if (!live) return;
+  if constexpr (WHAT == FULL) {
+    if (t1 == a.steps) {
+#pragma unroll
+      for (int s = 0; s < SP; ++s)
+        if (s < a.states) a.last[((int64_t)env * a.dim + d) * a.states + s] = h[s];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < SP; ++s)
+      if (s < a.states) ends[((int64_t)item * a.states + s) * a.dim + d] = h[s];
+    // an episode that begins inside lets nothing through: infinity says so
+    sums[(int64_t)item * a.dim + d] = began ? __builtin_inff() : sum;
+  }
+}
+
+// Runs over the pieces, first to last (BACKWARD: last to first), and leaves in
+// `ends` what each piece starts from.  A lane is one env, state and channel.
+template <bool BACKWARD>
+__global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float* ends, const float* sums) {
+  const int64_t i = block_id() * 256 + threadIdx.x, each = (int64_t)a.envs * a.states * a.dim;
+  if (i >= each) return;
+  const int d = (int)(i % a.dim), s = (int)(i / a.dim % a.states), env = (int)(i / a.dim / a.states);
+  const float decay = a.a[(int64_t)d * a.states + s] * kLog2e;
+  float h = !BACKWARD && a.state ? a.state[((int64_t)env * a.dim + d) * a.states + s] : 0.0f;
+  constexpr int kAhead = 8;
+  for (int k0 = 0; k0 < chunks; k0 += kAhead) {
+    float e[kAhead], sum[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = min(k0 + k, chunks - 1), piece = BACKWARD ? chunks - 1 - j : j;
+      e[k] = ends[piece * each + i];
+      sum[k] = sums[((int64_t)piece * a.envs + env) * a.dim + d];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k0 + k >= chunks) break;
+      const int piece = BACKWARD ? chunks - 1 - k0 - k : k0 + k;
+      ends[piece * each + i] = h;
+      h = sum[k] == __builtin_inff() ? e[k] : fmaf(h, exp2_fast(sum[k] * decay), e[k]);
+    }
+  }
+}
+
+// Gradient.  With d = dy * silu(z) and g the gradient of the state,
+//   g = C d + a' g' (a', g': the next step's),  dC = sum over channels of d h,  dB = sum over channels of g delta x,
+//   through = sum over s of g B,  by = g a h_before,
+//   dA = sum over steps and envs of by delta,  ddelta = through x + sum over s of by A,  dx = through delta + skip d.
+//
+// A wavefront takes CH channels (16 lanes along channels, C of them in each
+// lane) and all states (4 lanes, Q states in each): 8 states of channels a
+// lane, so that both sums, over states within 4 lanes and over channels, are
+// cheap.  It walks the steps backwards in segments of 16: from the saved state
+// before the segment it computes the 16 states again into registers, then goes
+// back through them.  What a channel needs at a step (delta, x, d) and the
+// rows of B and C are converted once into LDS.
+template <typename T, int SP>
+struct GradShape {
+  static constexpr int Q = SP / 4, C = 8 / Q, CH = 16 * C, kWavesHere = 2;
+  struct Lds {
+    float delta[kSegment][CH], x[kSegment][CH], d[kSegment][CH];
+    float through[kSegment][CH], by[kSegment][CH], plain[kSegment][CH];  // sums over states
+    float b[kSegment][SP], c[kSegment][SP];
+    float cross[16][2 * SP];  // dB and dC of one step by channel lane
+  };
+};
+
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// sum over the 4 lanes that share channels
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0xB1, 0xF, 0xF, true));  // lanes 1 0 3 2
+  v += __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
+  return v;
+}
+
+template <typename T, int SP>
+__global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
+  using S = GradShape<T, SP>;
+  constexpr int Q = S::Q, C = S::C, CH = S::CH, kPairs = kSegment * CH / kWave;
+  __shared__ typename S::Lds all[S::kWavesHere];
+  const int lane = threadIdx.x & 63;
+  typename S::Lds& m = all[threadIdx.x >> 6];
+  const int64_t wave = (int64_t)blockIdx.x * S::kWavesHere + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int block = (int)(wave % p.blocks), slot = (int)(wave / p.blocks);
+  if (slot >= slots) return;
+  const int group = block / p.blocks_per_group, per_group = a.dim / a.groups;
+  const int base = (block % p.blocks_per_group) * CH;  // of the block's channels in the group
+  const int cg = lane >> 2, sg = lane & 3;             // the lane's channels cg * C.., states sg * Q..
+  // one channel a lane where a step's values are prepared and finished
+  const int own = lane % CH, own_d = group * per_group + min(base + own, per_group - 1);
+  const bool own_live = base + own < per_group;
+  const float bias = a.bias ? a.bias[own_d] : 0.0f, skip = a.skip ? a.skip[own_d] : 0.0f;
+  const bool gated = a.z != nullptr;
+
+  float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int ch = base + cg * C + c, s = sg * Q + q;
+      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(group * per_group + ch) * a.states + s] : 0.0f;
+      dA[c][q] = 0.0f;
+    }
+
+  for (int64_t item = slot; item < (int64_t)p.chunks * a.envs; item += slots) {
+    const int env = (int)(item % a.envs), piece = (int)(item / a.envs);
+    const int t0 = piece * p.chunk, t1 = min(t0 + p.chunk, a.steps);
+    float g[C][Q];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int ch = base + cg * C + c, s = sg * Q + q;
+        g[c][q] = p.chunks > 1 && ch < per_group && s < a.states ? carried[(item * a.states + s) * a.dim + group * per_group + ch] : 0.0f;
+      }
+    const T* xp = (const T*)a.x + (int64_t)env * a.x_env + own_d;
+    const T* dtp = (const T*)a.dt + (int64_t)env * a.dt_env + own_d;
+    const T* zp = (const T*)a.z + (int64_t)env * a.z_env + own_d;
+    const T* dyp = (const T*)a.dy + (int64_t)env * a.dy_env + own_d;
+    const T* bp = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
+    const T* cp = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
+
+    for (int seg = t0 + (t1 - 1 - t0) / kSegment * kSegment; seg >= t0; seg -= kSegment) {
+      const int live_steps = min(kSegment, a.steps - seg);
+      // prepare: steps past the end neither push nor decay, and nothing comes from them
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const int i = lane / CH + k * (kWave / CH), t = min(seg + i, a.steps - 1);
+        const bool live = i < live_steps;
+        const float xv = (float)xp[(int64_t)t * a.x_step];
+        float delta = (float)dtp[(int64_t)t * a.dt_step] + bias;
+        if (a.softplus) delta = softplus(delta);
+        float dv = (float)dyp[(int64_t)t * a.dy_step];
+        if (gated) {
+          const float zv = (float)zp[(int64_t)t * a.z_step];
+          dv *= zv * sigmoid(zv);
+        }
+        m.delta[i][own] = live ? delta : 0.0f;
+        m.x[i][own] = live ? xv : 0.0f;
+        m.d[i][own] = live && own_live ? dv : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < kSegment * SP / kWave; ++k) {
+        const int e = lane + k * kWave, i = e / SP, s = e % SP, t = min(seg + i, a.steps - 1);
+        const bool live = i < live_steps && s < a.states;
+        m.b[i][s] = live ? (float)bp[(int64_t)t * a.b_step + s] : 0.0f;
+        m.c[i][s] = live ? (float)cp[(int64_t)t * a.c_step + s] : 0.0f;
+      }
+      uint32_t begins = 0;
+      if (a.resets) begins = (uint32_t)__ballot(lane < live_steps && a.resets[(int64_t)min(seg + lane, a.steps - 1) * a.envs + env]);
+      float before[C][Q];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int ch = min(base + cg * C + c, per_group - 1), s = min(sg * Q + q, a.states - 1);
+          before[c][q] = a.saved[(((int64_t)(seg / kSegment) * a.envs + env) * a.states + s) * a.dim + group * per_group + ch];
+        }
+      lds_order();
+
+      float h[kSegment][C][Q];
+#pragma unroll
+      for (int i = 0; i < kSegment; ++i) {
+        float plain[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float delta = m.delta[i][cg * C + c], u = delta * m.x[i][cg * C + c];
+          plain[c] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            float prev = i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q];
+            if (begins >> i & 1u) prev = 0.0f;
+            h[i][c][q] = fmaf(prev, exp2_fast(delta * (A[c][q] * kLog2e)), u * m.b[i][sg * Q + q]);
+            plain[c] = fmaf(h[i][c][q], m.c[i][sg * Q + q], plain[c]);
+          }
+        }
+        if (gated) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const float v = quad_sum(plain[c]);
+            if (sg == 0) m.plain[i][cg * C + c] = v;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = kSegment - 1; i >= 0; --i) {
+        float db[Q], dc[Q], through[C], by[C];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) db[q] = dc[q] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float delta = m.delta[i][cg * C + c], u = delta * m.x[i][cg * C + c], dv = m.d[i][cg * C + c];
+          through[c] = by[c] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            const float gv = fmaf(m.c[i][sg * Q + q], dv, g[c][q]);
+            dc[q] = fmaf(dv, h[i][c][q], dc[q]);
+            db[q] = fmaf(gv, u, db[q]);
+            through[c] = fmaf(gv, m.b[i][sg * Q + q], through[c]);
+            float ga = gv * exp2_fast(delta * (A[c][q] * kLog2e));
+            float prev = i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q];
+            if (begins >> i & 1u) ga = prev = 0.0f;
+            g[c][q] = ga;
+            const float via = ga * prev;
+            by[c] = fmaf(via, A[c][q], by[c]);
+            dA[c][q] = fmaf(via, delta, dA[c][q]);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float v = quad_sum(through[c]), w = quad_sum(by[c]);
+          if (sg == 0) {
+            m.through[i][cg * C + c] = v;
+            m.by[i][cg * C + c] = w;
+          }
+        }
+        // dB and dC: the 16 channel lanes through LDS
+        lds_order();
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          m.cross[cg][sg * 2 * Q + q] = db[q];
+          m.cross[cg][sg * 2 * Q + Q + q] = dc[q];
+        }
+        lds_order();
+        constexpr int kOut = 2 * SP, kParts = kWave / kOut, kEach = 16 / kParts;
+        float v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kEach; ++r) v += m.cross[(lane / kOut) * kEach + r][lane % kOut];
+#pragma unroll
+        for (int k = kOut; k < kWave; k <<= 1) v += __shfl_xor(v, k, 64);
+        if (lane < kOut && i < live_steps) cross_out[(((int64_t)(seg + i) * a.envs + env) * p.blocks + block) * kOut + lane] = v;
+      }
+      lds_order();
+      // finish: one channel a lane
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const int i = lane / CH + k * (kWave / CH), t = min(seg + i, a.steps - 1);
+        if (i < live_steps && own_live) {
+          const int64_t to = ((int64_t)t * a.envs + env) * a.dim + own_d;
+          const float xv = m.x[i][own], dv = m.d[i][own], thr = m.through[i][own];
+          float ddt = fmaf(thr, xv, m.by[i][own]);
+          if (a.softplus) ddt *= sigmoid((float)dtp[(int64_t)t * a.dt_step] + bias);
+          ((T*)a.ddt)[to] = (T)ddt;
+          ((T*)a.dx)[to] = (T)fmaf(thr, m.delta[i][own], skip * dv);
+          dskip = fmaf(dv, xv, dskip);
+          dbias += ddt;
+          if (gated) {
+            const float zv = (float)zp[(int64_t)t * a.z_step], sig = sigmoid(zv);
+            const float plain = fmaf(skip, xv, m.plain[i][own]);
+            ((T*)a.dz)[to] = (T)((float)dyp[(int64_t)t * a.dy_step] * plain * sig * fmaf(zv, 1.0f - sig, 1.0f));
+          }
+        }
+      }
+      lds_order();
+    }
+  }
+  // one row of partial sums a slot: dA [dim][states], dskip [dim], dbias [dim]
+  float* row = sums_out + (int64_t)slot * a.dim * (a.states + 2);
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int ch = base + cg * C + c, s = sg * Q + q;
+      if (ch < per_group && s < a.states) row[(int64_t)(group * per_group + ch) * a.states + s] = dA[c][q];
+    }
+#pragma unroll
+  for (int k = CH; k < kWave; k <<= 1) {
+    dskip += __shfl_xor(dskip, k, 64);
+    dbias += __shfl_xor(dbias, k, 64);
+  }
+  if (lane < CH && own_live) {
+    row[(int64_t)a.dim * a.states + own_d] = dskip;
+    row[(int64_t)a.dim * (a.states + 1) + own_d] = dbias;
+  }
+}
+
+// dB and dC of a group: the sum over its channel blocks, rounded once.
+template <typename T, int SP>
+__global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, const float* cross) {
+  constexpr int Q = SP / 4;
+  const int64_t i = block_id() * 256 + threadIdx.x;
+  const int64_t row = i / (2 * SP);  // (step, env, group)
+  if (row >= (int64_t)a.steps * a.envs * a.groups) return;
+  const int o = (int)(i % (2 * SP)), s = o / (2 * Q) * Q + o % Q;
+  const float* from = cross + row * p.blocks_per_group * 2 * SP + o;
+  float v = 0.0f;
+  for (int k = 0; k < p.blocks_per_group; ++k) v += from[k * 2 * SP];
+  if (s < a.states) ((T*)(o / Q & 1 ? a.dc : a.db))[row * a.states + s] = (T)v;
+}
+
+// The sums' row, taken apart.
+__global__ __launch_bounds__(256) void split_kernel(const float* sums, int dim, int states, float* da, float* dskip, float* dbias) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < dim * states) da[i] = sums[i];
+  else if (i < dim * (states + 1)) {
+    if (dskip) dskip[i - dim * states] = sums[i];
+  } else if (i < dim * (states + 2)) {
+    if (dbias) dbias[i - dim * (states + 1)] = sums[i];
+  }
+}
+
+// One step of every env: the state is read and written once and bounds the
+// kernel.  LANES lanes share a channel, 4 states (16 bytes) each.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
+  const int64_t i = block_id() * 256 + threadIdx.x, row = i / LANES;
+  if (row >= (int64_t)a.envs * a.dim) return;
+  const int part = (int)(i % LANES), d = (int)(row % a.dim), env = (int)(row / a.dim), group = d / (a.dim / a.groups);
+  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group + part * 4;
+  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group + part * 4;
+  float4* hp = reinterpret_cast<float4*>(a.last) + i;
+  const bool begins = a.resets && a.resets[env];
+  float4 h = *hp;
+  const float4 decay = reinterpret_cast<const float4*>(a.a)[d * LANES + part];
+  float bv[4], cv[4];
+  load_row<4>(b, 4, bv);
+  load_row<4>(c, 4, cv);
+  const float x = (float)((const T*)a.x)[(int64_t)env * a.x_env + d];
+  float delta = (float)((const T*)a.dt)[(int64_t)env * a.dt_env + d] + (a.bias ? a.bias[d] : 0.0f);
+  if (a.softplus) delta = softplus(delta);
+  if (begins) h = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float u = delta * x, scaled = delta * kLog2e;
+  h.x = fmaf(h.x, exp2_fast(scaled * decay.x), u * bv[0]);
+  h.y = fmaf(h.y, exp2_fast(scaled * decay.y), u * bv[1]);
+  h.z = fmaf(h.z, exp2_fast(scaled * decay.z), u * bv[2]);
+  h.w = fmaf(h.w, exp2_fast(scaled * decay.w), u * bv[3]);
+  *hp = h;
+  float out = fmaf(h.x, cv[0], h.y * cv[1]) + fmaf(h.z, cv[2], h.w * cv[3]);
+#pragma unroll
+  for (int k = 1; k < LANES; k <<= 1) out += __shfl_xor(out, k, 64);
+  if (part == 0) {
+    if (a.skip) out = fmaf(a.skip[d], x, out);
+    if (a.z) {
+      const float zv = (float)((const T*)a.z)[(int64_t)env * a.z_env + d];
+      out *= zv * sigmoid(zv);
+    }
+    ((T*)a.y)[row] = (T)out;
+  }
+}
+// Any number of states: a lane a channel.
+template <typename T>
+__global__ __launch_bounds__(256) void scan_step_any_kernel(ScanArgs a) {
+  const int64_t row = block_id() * 256 + threadIdx.x;
+  if (row >= (int64_t)a.envs * a.dim) return;
+  const int d = (int)(row % a.dim), env = (int)(row / a.dim), group = d / (a.dim / a.groups);
+  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
+  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
+  const bool begins = a.resets && a.resets[env];
+  const float x = (float)((const T*)a.x)[(int64_t)env * a.x_env + d];
+  float delta = (float)((const T*)a.dt)[(int64_t)env * a.dt_env + d] + (a.bias ? a.bias[d] : 0.0f);
+  if (a.softplus) delta = softplus(delta);
+  float out = a.skip ? a.skip[d] * x : 0.0f;
+  for (int s = 0; s < a.states; ++s) {
+    float* hp = a.last + row * a.states + s;
+    const float h = fmaf(begins ? 0.0f : *hp, exp2_fast(delta * kLog2e * a.a[(int64_t)d * a.states + s]), delta * x * (float)b[s]);
+    *hp = h;
+    out = fmaf(h, (float)c[s], out);
+  }
+  if (a.z) {
+    const float zv = (float)((const T*)a.z)[(int64_t)env * a.z_env + d];
+    out *= zv * sigmoid(zv);
+  }
+  ((T*)a.y)[row] = (T)out;
+}
+
+template <typename F>
+void by_states(int states, F&& f) {
+  if (states <= 8) f(std::integral_constant<int, 8>{});
+  else if (states <= 16) f(std::integral_constant<int, 16>{});
+  else f(std::integral_constant<int, 32>{});
+}
+int padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : 32; }
+
+// Wavefronts below which the steps are cut into pieces, and about how many
+// there are then: 2 for each of 1,024 SIMDs.
+constexpr int64_t kFull = 1024, kWant = 4096;
+Pieces pieces_of(int steps, int envs, int dim, int groups, int channels) {
+  Pieces p;
+  p.blocks_per_group = (dim / groups + channels - 1) / channels;
+  p.blocks = groups * p.blocks_per_group;
+  const int64_t waves = (int64_t)envs * p.blocks;
+  const int64_t cuts = waves >= kFull ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kSegment - 1) / kSegment);
+  const int64_t each = (steps + cuts - 1) / cuts;
+  p.chunk = (int)((each + kSegment - 1) / kSegment * kSegment);
+  p.chunks = (steps + p.chunk - 1) / p.chunk;
+  return p;
+}
+constexpr int64_t kGradWaves = 4096;
+int grad_slots(const Pieces& p, int envs) {
+  return (int)std::min<int64_t>((int64_t)p.chunks * envs, std::max<int64_t>(1, kGradWaves / p.blocks));
+}
+int grad_channels(int states) { return 512 / padded(states); }
+
+template <typename T, int SP, int WHAT>
+void launch_scan_kernel(const ScanArgs& a, const Pieces& p, float* ends, float* sums, hipStream_t st) {
+  const int64_t waves = (int64_t)p.blocks * a.envs * p.chunks;
+  const dim3 grid = wide_grid((waves + kWaves - 1) / kWaves);
+  constexpr uint64_t e = sizeof(T);
+  const uint64_t bits = (uint64_t)(uintptr_t)a.b | (uint64_t)(uintptr_t)a.c | a.b_step * e | a.b_env * e | a.b_group * e | a.c_step * e | a.c_env * e | a.c_group * e;
+  if (a.states == SP && bits % 4 == 0) hipLaunchKernelGGL((scan_kernel<T, SP, WHAT, true>), grid, dim3(kWave * kWaves), 0, st, a, p, ends, sums);
+  else hipLaunchKernelGGL((scan_kernel<T, SP, WHAT, false>), grid, dim3(kWave * kWaves), 0, st, a, p, ends, sums);
+}
+
+}  // namespace
+
+int64_t scan_work(int steps, int envs, int dim, int groups, int states) {
+  const Pieces p = pieces_of(steps, envs, dim, groups, kWave);
+  return p.chunks > 1 ? (int64_t)p.chunks * envs * dim * (states + 1) : 0;
+}
+
+hipError_t launch_scan(const ScanArgs& a, hipStream_t st) {
+  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, kWave);
+  float *ends = a.work, *sums = a.work + (int64_t)p.chunks * a.envs * a.dim * a.states;
+  by_element(a.elem, [&](auto t) {
+    using T = decltype(t);
+    by_states(a.states, [&](auto sp) {
+      if (p.chunks > 1) {
+        launch_scan_kernel<T, sp, ENDS>(a, p, ends, sums, st);
+        const int64_t each = (int64_t)a.envs * a.states * a.dim;
+        hipLaunchKernelGGL(join_kernel<false>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
+      }
+      launch_scan_kernel<T, sp, FULL>(a, p, ends, sums, st);
+    });
+  });
+  return hipGetLastError();
+}
+
+// rows of partial sums and their sum; dB and dC by channel block; what the
+// pieces start from
+int64_t scan_grad_work(int steps, int envs, int dim, int groups, int states) {
+  const Pieces p = pieces_of(steps, envs, dim, groups, grad_channels(states));
+  int64_t n = (int64_t)(grad_slots(p, envs) + 1) * dim * (states + 2);
+  n += (int64_t)steps * envs * p.blocks * 2 * padded(states);
+  if (p.chunks > 1) n += (int64_t)p.chunks * envs * dim * (states + 1);
+  return n;
+}
+
+hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
+  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, grad_channels(a.states));
+  const int slots = grad_slots(p, a.envs), cols = a.dim * (a.states + 2);
+  float* rows = a.work;
+  float* sum = rows + (int64_t)slots * cols;
+  float* cross = sum + cols;
+  float* ends = cross + (int64_t)a.steps * a.envs * p.blocks * 2 * padded(a.states);
+  float* sums = ends + (int64_t)p.chunks * a.envs * a.dim * a.states;
+  by_element(a.elem, [&](auto t) {
+    using T = decltype(t);
+    by_states(a.states, [&](auto sp) {
+      if (p.chunks > 1) {
+        Pieces wide = p;  // the same steps, 64 channels to a wavefront
+        wide.blocks_per_group = (a.dim / a.groups + kWave - 1) / kWave;
+        wide.blocks = a.groups * wide.blocks_per_group;
+        launch_scan_kernel<T, sp, BACK>(a, wide, ends, sums, st);
+        const int64_t each = (int64_t)a.envs * a.states * a.dim;
+        hipLaunchKernelGGL(join_kernel<true>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
+      }
+      constexpr int per = GradShape<T, sp>::kWavesHere;
+      const int64_t waves = (int64_t)slots * p.blocks;
+      hipLaunchKernelGGL((scan_grad_kernel<T, sp>), dim3((unsigned)((waves + per - 1) / per)), dim3(kWave * per), 0, st, a, p, slots, (const float*)ends, cross, rows);
+      const int64_t outs = (int64_t)a.steps * a.envs * a.groups * 2 * sp;
+      hipLaunchKernelGGL((cross_sum_kernel<T, sp>), wide_grid((outs + 255) / 256), dim3(256), 0, st, a, p, (const float*)cross);
+    });
+  });
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (hipError_t e = launch_column_sum(rows, cols, slots, cols, sum, st); e != hipSuccess) return e;
+  hipLaunchKernelGGL(split_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, (const float*)sum, a.dim, a.states, a.da, a.dskip, a.dbias);
+  return hipGetLastError();
+}
+
+hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st) {
+  const int64_t channels = (int64_t)a.envs * a.dim;
+  const auto grid = [](int64_t n) { return wide_grid((n + 255) / 256); };
+  by_element(a.elem, [&](auto t) {
+    using T = decltype(t);
+    if (a.states == 4) hipLaunchKernelGGL((scan_step_kernel<T, 1>), grid(channels), dim3(256), 0, st, a);
+    else if (a.states == 8) hipLaunchKernelGGL((scan_step_kernel<T, 2>), grid(channels * 2), dim3(256), 0, st, a);
+    else if (a.states == 16) hipLaunchKernelGGL((scan_step_kernel<T, 4>), grid(channels * 4), dim3(256), 0, st, a);
+    else if (a.states == 32) hipLaunchKernelGGL((scan_step_kernel<T, 8>), grid(channels * 8), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((scan_step_any_kernel<T>), grid(channels), dim3(256), 0, st, a);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace gbx

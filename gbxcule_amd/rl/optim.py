@@ -1,0 +1,195 @@
+"""AdamW over all of a policy's tensors in a few launches.
+
+The moments of a parameter group lie in flat buffers, tensor after tensor,
+each from a multiple of 256 elements.  With ``state_bits=8`` the first moment
+is ``torch.float8_e4m3fn`` and the second ``torch.float8_e5m2``, each with a
+float32 scale for every 256 elements (the largest absolute value maps to the
+format's largest), 2 bytes an element and 1/32 more for the scales in place of
+8.  They are rounded up or down with the odds of the distance, by a hash of
+the element's place, the step and ``seed``: rounding to the nearest would hold
+a second moment still, since with beta2 = 0.999 a step changes it by less than
+half of what 8 bits resolve.  A second moment that is not zero is kept from
+rounding to zero.
+"""
+
+from __future__ import annotations
+
+import math
+from array import array
+
+import torch
+
+from .. import _lib
+from .ops import _ELEM, _call
+
+STATE_BLOCK = 256
+_GOLDEN = 0x9E3779B9
+
+
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with one pass over the data.
+
+    Parameters are CUDA tensors of one device, float32, bfloat16 or float16,
+    contiguous; gradients of the parameter's type or float32.  The update is
+    computed in 32 bits and the parameter rounded once.  ``step`` reads the
+    bias corrections on the host, so it is refused under stream capture."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0) -> None:  # fmt: skip
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not lr >= 0.0 or not eps > 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"lr and weight_decay must not be negative and eps positive, got {lr}, {weight_decay}, {eps}")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self._flat: list[dict[str, torch.Tensor]] = []
+        self._starts: list[list[int]] = []
+        super().__init__(params, {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay})
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        try:
+            self._lay_out(params)
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def _lay_out(self, params) -> None:
+        device = params[0].device
+        for p in params:
+            if p.dtype not in _ELEM or not p.is_cuda or p.device != device or not p.is_contiguous():
+                raise ValueError(f"parameters must be contiguous CUDA tensors of one device in float32, bfloat16 or "
+                                 f"float16, got {p.dtype} on {p.device}")  # fmt: skip
+        starts, total = [], 0
+        for p in params:
+            starts.append(total)
+            total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        small = self.state_bits == 8
+        kinds = (torch.float8_e4m3fn, torch.float8_e5m2) if small else (torch.float32, torch.float32)
+        flat = {}
+        for key, kind in zip(("exp_avg", "exp_avg_sq"), kinds):
+            flat[key] = torch.zeros(total * kind.itemsize, dtype=torch.uint8, device=device).view(kind)
+            if small:
+                flat[key + "_scale"] = torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=device)
+        self._flat.append(flat)
+        self._starts.append(starts)
+        for p, at in zip(params, starts):
+            state = self.state[p]
+            state["step"] = 0
+            for key, t in flat.items():
+                if key.endswith("_scale"):
+                    state[key] = t[at // STATE_BLOCK : at // STATE_BLOCK - (-p.numel() // STATE_BLOCK)]
+                else:
+                    state[key] = t[at : at + p.numel()].view(p.shape)
+
+    def flat_state(self, group: int = 0) -> dict[str, torch.Tensor]:
+        """A group's moments (and scales) as they lie: every tensor's from the
+        next multiple of 256 elements.  Views: they change with ``step``."""
+        return dict(self._flat[group])
+
+    def load_flat_state(self, step: int, state: dict[str, torch.Tensor], group: int = 0) -> None:
+        """Copies what ``flat_state`` returned, after ``step`` steps."""
+        flat = self._flat[group]
+        if set(state) != set(flat):
+            raise ValueError(f"expected {sorted(flat)}, got {sorted(state)}")
+        for key, t in state.items():
+            if t.dtype is not flat[key].dtype or t.shape != flat[key].shape:
+                raise ValueError(f"{key}: expected {flat[key].dtype} {tuple(flat[key].shape)}, got {t.dtype} {tuple(t.shape)}")
+        for key, t in state.items():
+            flat[key].copy_(t)
+        for p in self.param_groups[group]["params"]:
+            self.state[p]["step"] = int(step)
+
+    def state_dict(self):
+        """As torch's, with ``state_bits`` and ``seed``."""
+        return {**super().state_dict(), "state_bits": self.state_bits, "seed": self.seed}
+
+    def load_state_dict(self, state_dict) -> None:
+        """Copies the moments into the flat buffers; hyperparameters as torch does."""
+        groups, saved = self.param_groups, state_dict["param_groups"]
+        if state_dict.get("state_bits") != self.state_bits:
+            raise ValueError(f"a state of {state_dict.get('state_bits')} bits does not fit state_bits={self.state_bits}")
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
+            raise ValueError("the state's parameter groups are not this optimizer's")
+        plan = []
+        for g, s in zip(groups, saved):
+            for p, index in zip(g["params"], s["params"]):
+                mine, theirs = self.state[p], state_dict["state"][index]
+                for key, t in mine.items():
+                    if key != "step" and (theirs[key].shape != t.shape or theirs[key].dtype is not t.dtype):
+                        raise ValueError(f"{key} of parameter {index} has another shape or type")
+                plan.append((mine, theirs))
+        for mine, theirs in plan:
+            mine["step"] = int(theirs["step"])
+            for key, t in mine.items():
+                if key != "step":
+                    t.copy_(theirs[key])
+        for g, s in zip(groups, saved):
+            g.update({k: v for k, v in s.items() if k != "params"})
+        self.seed = int(state_dict["seed"])
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
+        """One update of every parameter that has a gradient.  ``grad_scale``
+        (float32, one element, on the device) multiplies the gradients, such as
+        a clipping factor that never leaves the GPU."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step reads its bias corrections on the host: it cannot be captured")
+        for g, group in enumerate(self.param_groups):
+            self._step_group(g, group, grad_scale)
+        return loss
+
+    def _step_group(self, g: int, group, grad_scale) -> None:
+        # tensors that one launch can take together: same types, same count of steps
+        batches: dict[tuple, tuple[list, list, list, list]] = {}
+        for p, start in zip(group["params"], self._starts[g]):
+            grad = p.grad
+            if grad is None:
+                continue
+            if grad.is_sparse or (grad.dtype is not p.dtype and grad.dtype is not torch.float32) or grad.device != p.device:
+                raise ValueError(f"a gradient of {grad.dtype} on {grad.device} does not go with {p.dtype} on {p.device}")
+            if not p.is_contiguous():
+                raise ValueError("a parameter is no longer contiguous")
+            if not grad.is_contiguous():
+                grad = grad.contiguous()
+            key = (p.dtype, grad.dtype, self.state[p]["step"])
+            batch = batches.get(key)
+            if batch is None:
+                batch = batches[key] = ([], [], [], [])
+            batch[0].append(p)
+            batch[1].append(grad)
+            batch[2].append(p.numel())
+            batch[3].append(start)
+        if not batches:
+            return
+        if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
+                                       or grad_scale.device != group["params"][0].device):  # fmt: skip
+            raise ValueError("grad_scale must be one float32 element on the parameters' device")
+        flat, (b1, b2) = self._flat[g], group["betas"]
+        lr = float(group["lr"])
+        for (kind, grad_kind, done), (params, grads, sizes, starts) in batches.items():
+            step = done + 1
+            tables = (array("Q", [p.data_ptr() for p in params]), array("Q", [t.data_ptr() for t in grads]),
+                      array("q", sizes), array("q", starts))  # fmt: skip
+            scales = (flat[k].data_ptr() if k in flat else None for k in ("exp_avg_scale", "exp_avg_sq_scale"))
+            given = _lib.AdamwIn(
+                len(params), _ELEM[kind], _ELEM[grad_kind], self.state_bits, *(_address(t) for t in tables),
+                flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), *scales,
+                None if grad_scale is None else grad_scale.data_ptr(), b1, b2, lr / (1 - b1**step),
+                1.0 / math.sqrt(1 - b2**step), group["eps"], 1 - lr * group["weight_decay"],
+                (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
+            )  # fmt: skip
+            _call("gbx_adamw", params[0], given)
+            torch.autograd.graph.increment_version(params)
+            for p in params:
+                self.state[p]["step"] = step

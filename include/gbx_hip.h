@@ -215,6 +215,98 @@ int gbx_info(gbx_ctx* ctx, int32_t key, int64_t* out);
 int gbx_set_debug(gbx_ctx* ctx, int32_t rst38, int32_t trap_pc,
                   int32_t max_instr, int32_t watch_addr);
 
+/* ---- Operators of a policy with memory -------------------------------------
+ *
+ * No context: they work on device pointers of the current device, enqueue on
+ * the stream, allocate nothing and never synchronize.  The reference has no
+ * counterpart; its learners use torch modules.  Everything is time-major:
+ * [steps][envs][channels], as rollouts are stored.  Strides are in elements;
+ * the channel stride is 1.  `resets` (uint8 [steps][envs], may be NULL) is
+ * non-zero where an episode begins: nothing from before reaches that step.
+ * Outputs without strides are contiguous.  `work` is scratch memory of the
+ * number of floats that the *_work function of the same arguments returns
+ * (negative: the arguments are out of range); it may be NULL for 0. */
+
+/* Element types. */
+enum { GBX_F32 = 0, GBX_BF16 = 1, GBX_F16 = 2 };
+
+/* out = s * rsqrt(mean(s^2) + eps) * weight, s = x + residual rounded to the
+ * element type and written to `summed` (residual and summed may be NULL).
+ * With scale NULL `out` has the element type; else it is OCP e4m3 and
+ * scale[rows][dim / group rounded up] (group 128; 0: one a row) holds what
+ * its values are multiplied by. */
+int gbx_rms_norm(int64_t rows, int32_t dim, int32_t elem, float eps, const void* x, int64_t x_stride,
+                 const void* residual, int64_t residual_stride, const float* weight, void* out,
+                 void* summed, float* scale, int32_t group, void* stream);
+/* dx (also the residual's gradient) and dweight from s, dy and the gradient of
+ * s itself (dsummed, may be NULL). */
+int64_t gbx_rms_norm_grad_work(int64_t rows, int32_t dim);
+int gbx_rms_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const void* summed,
+                      int64_t summed_stride, const void* dy, int64_t dy_stride, const void* dsummed,
+                      int64_t dsummed_stride, const float* weight, void* dx, float* dweight,
+                      float* work, void* stream);
+
+/* y[t] = act(bias + sum_j weight[width - 1 - j] * x[t - j]), width 2 to 4, act
+ * silu or nothing.  state[envs][width - 1][dim] holds the inputs before the
+ * first step (NULL: zeros), last those before the step to come. */
+int gbx_causal_conv(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu,
+                    const void* x, int64_t x_step, int64_t x_env, const float* weight, const float* bias,
+                    const void* state, const uint8_t* resets, void* y, void* last, void* stream);
+int64_t gbx_causal_conv_grad_work(int32_t steps, int32_t envs, int32_t dim, int32_t width);
+int gbx_causal_conv_grad(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu,
+                         const void* x, int64_t x_step, int64_t x_env, const float* weight, const float* bias,
+                         const void* state, const uint8_t* resets, const void* dy, int64_t dy_step,
+                         int64_t dy_env, void* dx, float* dweight, float* dbias, float* work, void* stream);
+/* One step of every env; `state` is read and moved on in place. */
+int gbx_causal_conv_step(int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu, const void* x,
+                         int64_t x_env, const float* weight, const float* bias, void* state,
+                         const uint8_t* resets, void* y, void* stream);
+
+/* Inputs of the selective scan, 1 to 32 states a channel:
+ *   delta = softplus(dt + bias) or dt + bias,
+ *   h = exp(delta a) h + delta x b,  y = (sum over states of c h + skip x) silu(z).
+ * b and c are [steps][envs][groups][states], dim a multiple of groups; z, skip
+ * and bias may be NULL. */
+typedef struct gbx_scan_in {
+  int32_t steps, envs, dim, groups, states, elem, softplus;
+  const void *x, *dt, *z, *b, *c;
+  int64_t x_step, x_env, dt_step, dt_env, z_step, z_env;
+  int64_t b_step, b_env, b_group, c_step, c_env, c_group;
+  const float *a, *skip, *bias; /* [dim][states], [dim], [dim] */
+  const uint8_t* resets;
+} gbx_scan_in;
+/* state[envs][dim][states] (NULL: zeros) before the first step, last after the
+ * last one.  saved, if not NULL, receives what the gradient starts from:
+ * [steps / 16 rounded up][envs][states][dim]. */
+int64_t gbx_selective_scan_work(const gbx_scan_in* in);
+int gbx_selective_scan(const gbx_scan_in* in, const float* state, void* y, float* last, float* saved,
+                       float* work, void* stream);
+/* Gradients; dz, dskip and dbias as z, skip and bias (NULL where those are). */
+int64_t gbx_selective_scan_grad_work(const gbx_scan_in* in);
+int gbx_selective_scan_grad(const gbx_scan_in* in, const float* saved, const void* dy, int64_t dy_step,
+                            int64_t dy_env, void* dx, void* ddt, void* dz, void* db, void* dc, float* da,
+                            float* dskip, float* dbias, float* work, void* stream);
+/* One step of every env (in->steps is 1); `state` is updated in place. */
+int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* stream);
+
+/* One AdamW step of `count` tensors (host arrays of device addresses, element
+ * counts and places of their states, multiples of 256).  state_bits 32: float
+ * moments.  8: OCP e4m3 and e5m2 with a scale for each 256 elements, rounded
+ * up or down at random by a hash of place and key.  grad_scale (device, may be
+ * NULL) multiplies the gradients.  step_size = lr / (1 - beta1^t), inv_root2 =
+ * 1 / sqrt(1 - beta2^t), keep = 1 - lr * decay. */
+typedef struct gbx_adamw_in {
+  int32_t count, elem, grad_elem, state_bits;
+  const uint64_t *params, *grads;
+  const int64_t *sizes, *starts;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  const float* grad_scale;
+  double beta1, beta2, step_size, inv_root2, eps, keep;
+  uint32_t key;
+} gbx_adamw_in;
+int gbx_adamw(const gbx_adamw_in* in, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
