@@ -119,7 +119,9 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamArgs a, Tensors ts)
       const float gi = g[i] * grad_scale;
       m[i] = m[i] * a.beta1 + gi * a.rest1;
       v[i] = v[i] * a.beta2 + gi * gi * a.rest2;
-      const float update = (m[i] * a.step_size) / (sqrtf(v[i]) * a.inv_root2 + a.eps);
+      // root and quotient to one unit in the last place: the update is added
+      // to a parameter many times its size
+      const float update = (m[i] * a.step_size) * rcp_fast(__builtin_amdgcn_sqrtf(v[i]) * a.inv_root2 + a.eps);
       p[i] = p[i] * a.keep - update;
     }
     store_row<4>((P*)t.p + e, valid, p);

@@ -72,14 +72,20 @@ __device__ __forceinline__ void lead_in(const ConvArgs& a, int env, int t0, int 
   }
 }
 
+// the weights of 8 channels lie together
 template <int W>
 __device__ __forceinline__ void load_weights(const ConvArgs& a, int c, float (&w)[W][kVec], float (&bias)[kVec]) {
+  float row[W * kVec];
+  load_row<W * kVec>(a.weight + (int64_t)c * W, (a.dim - c) * W, row);
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) {
-    const int ch = min(c + k, a.dim - 1);
+  for (int k = 0; k < kVec; ++k)
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][k] = a.weight[(int64_t)ch * W + j];
-    bias[k] = a.bias ? a.bias[ch] : 0.0f;
+    for (int j = 0; j < W; ++j) w[j][k] = row[k * W + j];
+  if (a.bias) {
+    load_row<kVec>(a.bias + c, a.dim - c, bias);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) bias[k] = 0.0f;
   }
 }
 

@@ -71,7 +71,7 @@ struct AdamArgs {
   uint32_t key;
 };
 constexpr int kStateBlock = 256;  // elements that share a scale
-constexpr int kSegment = 16;    // steps between two saved states
+constexpr int kSegment = 8;     // steps between two saved states
 constexpr int kMaxStates = 32;  // states a channel may have
 
 // out[c] = sum over rows r of in[r * stride + c], in one order

@@ -105,34 +105,59 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     }
   }
 
-  const T* x = (const T*)(WHAT == BACK ? a.dy : a.x) + (int64_t)env * (WHAT == BACK ? a.dy_env : a.x_env) + d;
-  const int64_t x_step = WHAT == BACK ? a.dy_step : a.x_step;
-  const T* dt = (const T*)a.dt + (int64_t)env * a.dt_env + d;
-  const T* z = (const T*)a.z + (int64_t)env * a.z_env + d;
-  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
-  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
-  const uint8_t* resets = a.resets + env;
-  T* y = (T*)a.y + (int64_t)env * a.dim + d;
+  // Rows of the current step: uniform addresses that move from step to step
+  // (against the steps for BACK), to which a lane adds its channel.
+  const int64_t from = WHAT == BACK ? t1 - 1 : t0, to = WHAT == BACK ? -1 : 1;
+  const uint32_t at = (uint32_t)d * sizeof(T);
+  const int64_t x_step = WHAT == BACK ? a.dy_step : a.x_step, x_env = WHAT == BACK ? a.dy_env : a.x_env;
+  const T* x = (const T*)(WHAT == BACK ? a.dy : a.x) + from * x_step + env * x_env;
+  const T* dt = (const T*)a.dt + from * a.dt_step + env * a.dt_env;
+  const T* z = (const T*)a.z + from * a.z_step + env * a.z_env;
+  const T* b = (const T*)a.b + from * a.b_step + env * a.b_env + group * a.b_group;
+  const T* c = (const T*)a.c + from * a.c_step + env * a.c_env + group * a.c_group;
+  const uint8_t* resets = a.resets + from * a.envs + env;
+  T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim;
+  float* saved = a.saved + ((int64_t)(t0 / kSegment) * a.envs + env) * a.states * a.dim;
+  auto of_lane = [&](const T* row) { return *(const T*)((const char*)row + at); };
 
   constexpr int kAhead = 4;  // steps whose loads are in flight together
   T xs[kAhead], dts[kAhead], zs[kAhead], bcs[kAhead];
   uint8_t rs[kAhead];
-  const bool lane_is_c = lane >= 32;
-  const bool lane_holds = (lane & 31) < a.states;
+  const T* row_bc = lane >= 32 ? c : b;  // without SCALAR: lanes hold B, then C
+  const int64_t row_bc_step = lane >= 32 ? to * a.c_step : to * a.b_step;
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int k = min(k0 + i, count - 1);
-      const int t = WHAT == BACK ? t1 - 1 - k : t0 + k;
-      xs[i] = x[(int64_t)t * x_step];
-      dts[i] = dt[(int64_t)t * a.dt_step];
-      if (gated && WHAT != ENDS) zs[i] = z[(int64_t)t * a.z_step];
-      if (a.resets) rs[i] = resets[(int64_t)t * a.envs];
+      const bool more = k0 + i + 1 < count;  // the last row is loaded again past the end
+      xs[i] = of_lane(x);
+      x += more ? to * x_step : 0;
+      dts[i] = of_lane(dt);
+      dt += more ? to * a.dt_step : 0;
+      if (gated && WHAT != ENDS) {
+        zs[i] = of_lane(z);
+        z += more ? to * a.z_step : 0;
+      }
+      if (a.resets) {
+        rs[i] = *resets;
+        resets += more ? to * a.envs : 0;
+      }
       if constexpr (!SCALAR) {
-        const T* row = lane_is_c ? c + (int64_t)t * a.c_step : b + (int64_t)t * a.b_step;
-        bcs[i] = lane_holds ? row[lane & 31] : (T)0.0f;
+        bcs[i] = (lane & 31) < a.states ? row_bc[lane & 31] : (T)0.0f;
+        row_bc += more ? row_bc_step : 0;
       }
     }
+  };
+  RowBits<SP, T> rb, rc;
+  if constexpr (SCALAR) {
+    if constexpr (WHAT != BACK) load_scalar(b, rb);
+    if constexpr (WHAT != ENDS) load_scalar(c, rc);
+  }
+  auto clear = [&]() {
+    // a branch, the same for all lanes: without the barrier it becomes a
+    // selection of every state at every step
+    asm volatile("");
+#pragma unroll
+    for (int s = 0; s < SP; ++s) h[s] = 0.0f;
   };
   float sum = 0.0f;
   bool began = false;
@@ -152,21 +177,24 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (k0 + i >= count) break;
-      const int t = WHAT == BACK ? t1 - 1 - k0 - i : t0 + k0 + i;
       float delta = dtv[i] + bias;
       if (a.softplus) delta = softplus(delta);
       float bv[SP], cv[SP];
       if constexpr (SCALAR) {
-        RowBits<SP, T> rb, rc;
+        // this step's rows have arrived: unpack them, then ask for the next
+        // step's (the last ones again past the end)
+        const bool more = k0 + i + 1 < count;
         if constexpr (WHAT != BACK) {
-          load_scalar(b + (int64_t)t * a.b_step, rb);
 #pragma unroll
           for (int s = 0; s < SP; ++s) bv[s] = unpack<T>(rb.w, s);
+          b += more ? to * a.b_step : 0;
+          load_scalar(b, rb);
         }
         if constexpr (WHAT != ENDS) {
-          load_scalar(c + (int64_t)t * a.c_step, rc);
 #pragma unroll
           for (int s = 0; s < SP; ++s) cv[s] = unpack<T>(rc.w, s);
+          c += more ? to * a.c_step : 0;
+          load_scalar(c, rc);
         }
       } else {
 #pragma unroll
@@ -179,38 +207,32 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
         const float dv = gated ? xv[i] * zv[i] * sigmoid(zv[i]) : xv[i];
 #pragma unroll
         for (int s = 0; s < SP; ++s) h[s] = fmaf(cv[s], dv, h[s]) * exp2_fast(delta * decay[s]);
-        if (begins[i]) {
-#pragma unroll
-          for (int s = 0; s < SP; ++s) h[s] = 0.0f;
-        }
+        if (begins[i]) clear();
         sum += delta;
         began = began || begins[i];
       } else {
-        if (begins[i]) {
-#pragma unroll
-          for (int s = 0; s < SP; ++s) h[s] = 0.0f;
-        }
+        if (begins[i]) clear();
         if constexpr (WHAT == FULL) {
-          if (a.saved && t % kSegment == 0 && live) {
-            float* to = a.saved + ((int64_t)(t / kSegment) * a.envs + env) * a.states * a.dim + d;
+          if (a.saved && (k0 + i) % kSegment == 0) {  // pieces begin at multiples of kSegment
 #pragma unroll
             for (int s = 0; s < SP; ++s)
-              if (s < a.states) to[(int64_t)s * a.dim] = h[s];
+              if (s < a.states && live) saved[(int64_t)s * a.dim + d] = h[s];
+            saved += (int64_t)a.envs * a.states * a.dim;
           }
         }
         const float u = delta * xv[i];
-        float part[2] = {skip * xv[i], 0.0f};
 #pragma unroll
-        for (int s = 0; s < SP; ++s) {
-          h[s] = fmaf(h[s], exp2_fast(delta * decay[s]), u * bv[s]);
-          if constexpr (WHAT == FULL) part[s & 1] = fmaf(h[s], cv[s], part[s & 1]);
-        }
+        for (int s = 0; s < SP; ++s) h[s] = fmaf(h[s], exp2_fast(delta * decay[s]), u * bv[s]);
         if constexpr (WHAT == FULL) {
+          float part[2] = {skip * xv[i], 0.0f};
+#pragma unroll
+          for (int s = 0; s < SP; ++s) part[s & 1] = fmaf(h[s], cv[s], part[s & 1]);
           float out = part[0] + part[1];
           if (gated) out *= zv[i] * sigmoid(zv[i]);
-          if (live) y[(int64_t)t * a.envs * a.dim] = (T)out;
+          if (live) *(T*)((char*)y + at) = (T)out;
+          y += (int64_t)a.envs * a.dim;
         } else {
-          sum = begins[i] ? delta : sum + delta;
+          sum += delta;
           began = began || begins[i];
         }
       }
@@ -268,18 +290,17 @@ __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float
 // A wavefront takes CH channels (16 lanes along channels, C of them in each
 // lane) and all states (4 lanes, Q states in each): 8 states of channels a
 // lane, so that both sums, over states within 4 lanes and over channels, are
-// cheap.  It walks the steps backwards in segments of 16: from the saved state
-// before the segment it computes the 16 states again into registers, then goes
-// back through them.  What a channel needs at a step (delta, x, d) and the
-// rows of B and C are converted once into LDS.
-template <typename T, int SP>
+// cheap.  It walks the steps backwards in segments of kSegment: from the saved
+// state before the segment it computes the segment's states again into
+// registers, then goes back through them.  What a channel needs at a step
+// (delta, x, d) and the rows of B and C are converted once into LDS.
+template <int SP>
 struct GradShape {
   static constexpr int Q = SP / 4, C = 8 / Q, CH = 16 * C, kWavesHere = 2;
   struct Lds {
     float delta[kSegment][CH], x[kSegment][CH], d[kSegment][CH];
     float through[kSegment][CH], by[kSegment][CH], plain[kSegment][CH];  // sums over states
     float b[kSegment][SP], c[kSegment][SP];
-    float cross[16][2 * SP];  // dB and dC of one step by channel lane
   };
 };
 
@@ -287,16 +308,26 @@ __device__ __forceinline__ void lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
 // sum over the 4 lanes that share channels
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0xB1, 0xF, 0xF, true));  // lanes 1 0 3 2
-  v += __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
-  return v;
+__device__ __forceinline__ float quad_sum(float v) { return add_dpp<0x4E>(add_dpp<0xB1>(v)); }  // lanes 1 0 3 2, 2 3 0 1
+// lanes 0-31: a summed over the two halves of the wavefront; lanes 32-63: b
+__device__ __forceinline__ float fold_halves(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// even rows of 16 lanes: a summed over the row and its odd neighbour; odd rows: b
+__device__ __forceinline__ float fold_rows(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 template <typename T, int SP>
-__global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
-  using S = GradShape<T, SP>;
+__global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
+  using S = GradShape<SP>;
   constexpr int Q = S::Q, C = S::C, CH = S::CH, kPairs = kSegment * CH / kWave;
   __shared__ typename S::Lds all[S::kWavesHere];
   const int lane = threadIdx.x & 63;
@@ -313,13 +344,13 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
   const float bias = a.bias ? a.bias[own_d] : 0.0f, skip = a.skip ? a.skip[own_d] : 0.0f;
   const bool gated = a.z != nullptr;
 
-  float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;
+  float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;  // A in powers of two
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int ch = base + cg * C + c, s = sg * Q + q;
-      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(group * per_group + ch) * a.states + s] : 0.0f;
+      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(group * per_group + ch) * a.states + s] * kLog2e : 0.0f;
       dA[c][q] = 0.0f;
     }
 
@@ -344,16 +375,20 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
     for (int seg = t0 + (t1 - 1 - t0) / kSegment * kSegment; seg >= t0; seg -= kSegment) {
       const int live_steps = min(kSegment, a.steps - seg);
       // prepare: steps past the end neither push nor decay, and nothing comes from them
+      T raw_dt[kPairs], raw_dy[kPairs], raw_z[kPairs];
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
         const int i = lane / CH + k * (kWave / CH), t = min(seg + i, a.steps - 1);
         const bool live = i < live_steps;
         const float xv = (float)xp[(int64_t)t * a.x_step];
-        float delta = (float)dtp[(int64_t)t * a.dt_step] + bias;
+        raw_dt[k] = dtp[(int64_t)t * a.dt_step];
+        raw_dy[k] = dyp[(int64_t)t * a.dy_step];
+        float delta = (float)raw_dt[k] + bias;
         if (a.softplus) delta = softplus(delta);
-        float dv = (float)dyp[(int64_t)t * a.dy_step];
+        float dv = (float)raw_dy[k];
         if (gated) {
-          const float zv = (float)zp[(int64_t)t * a.z_step];
+          raw_z[k] = zp[(int64_t)t * a.z_step];
+          const float zv = (float)raw_z[k];
           dv *= zv * sigmoid(zv);
         }
         m.delta[i][own] = live ? delta : 0.0f;
@@ -361,7 +396,7 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
         m.d[i][own] = live && own_live ? dv : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < kSegment * SP / kWave; ++k) {
+      for (int k = 0; k < (kSegment * SP + kWave - 1) / kWave; ++k) {
         const int e = lane + k * kWave, i = e / SP, s = e % SP, t = min(seg + i, a.steps - 1);
         const bool live = i < live_steps && s < a.states;
         m.b[i][s] = live ? (float)bp[(int64_t)t * a.b_step + s] : 0.0f;
@@ -379,77 +414,90 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
         }
       lds_order();
 
+      // (an episode's first step takes a branch of its own, the same for all
+      // lanes: selecting zeros would keep a second copy of every state)
       float h[kSegment][C][Q];
 #pragma unroll
       for (int i = 0; i < kSegment; ++i) {
-        float plain[C];
+        const bool first = begins >> i & 1u;
+        float delta[C], plain[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const float delta = m.delta[i][cg * C + c], u = delta * m.x[i][cg * C + c];
-          plain[c] = 0.0f;
+          delta[c] = m.delta[i][cg * C + c];
+          const float u = delta[c] * m.x[i][cg * C + c];
 #pragma unroll
-          for (int q = 0; q < Q; ++q) {
-            float prev = i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q];
-            if (begins >> i & 1u) prev = 0.0f;
-            h[i][c][q] = fmaf(prev, exp2_fast(delta * (A[c][q] * kLog2e)), u * m.b[i][sg * Q + q]);
-            plain[c] = fmaf(h[i][c][q], m.c[i][sg * Q + q], plain[c]);
-          }
+          for (int q = 0; q < Q; ++q) h[i][c][q] = u * m.b[i][sg * Q + q];
+        }
+        if (!first) {
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) h[i][c][q] = fmaf(i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q], exp2_fast(delta[c] * A[c][q]), h[i][c][q]);
         }
         if (gated) {
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const float v = quad_sum(plain[c]);
-            if (sg == 0) m.plain[i][cg * C + c] = v;
+            plain[c] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) plain[c] = fmaf(h[i][c][q], m.c[i][sg * Q + q], plain[c]);
+            m.plain[i][cg * C + c] = quad_sum(plain[c]);
           }
         }
       }
+      lds_order();  // the rows are read again: kept in registers they would not fit
 #pragma unroll
       for (int i = kSegment - 1; i >= 0; --i) {
-        float db[Q], dc[Q], through[C], by[C];
+        const bool first = begins >> i & 1u;
+        float db[Q], dc[Q], delta[C], through[C], by[C];
 #pragma unroll
         for (int q = 0; q < Q; ++q) db[q] = dc[q] = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const float delta = m.delta[i][cg * C + c], u = delta * m.x[i][cg * C + c], dv = m.d[i][cg * C + c];
+          delta[c] = m.delta[i][cg * C + c];
+          const float u = delta[c] * m.x[i][cg * C + c], dv = m.d[i][cg * C + c];
           through[c] = by[c] = 0.0f;
 #pragma unroll
           for (int q = 0; q < Q; ++q) {
-            const float gv = fmaf(m.c[i][sg * Q + q], dv, g[c][q]);
+            g[c][q] = fmaf(m.c[i][sg * Q + q], dv, g[c][q]);
             dc[q] = fmaf(dv, h[i][c][q], dc[q]);
-            db[q] = fmaf(gv, u, db[q]);
-            through[c] = fmaf(gv, m.b[i][sg * Q + q], through[c]);
-            float ga = gv * exp2_fast(delta * (A[c][q] * kLog2e));
-            float prev = i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q];
-            if (begins >> i & 1u) ga = prev = 0.0f;
-            g[c][q] = ga;
-            const float via = ga * prev;
-            by[c] = fmaf(via, A[c][q], by[c]);
-            dA[c][q] = fmaf(via, delta, dA[c][q]);
+            db[q] = fmaf(g[c][q], u, db[q]);
+            through[c] = fmaf(g[c][q], m.b[i][sg * Q + q], through[c]);
           }
+        }
+        if (!first) {
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+              g[c][q] *= exp2_fast(delta[c] * A[c][q]);
+              const float via = g[c][q] * (i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q]);
+              by[c] = fmaf(via, A[c][q], by[c]);
+              dA[c][q] = fmaf(via, delta[c], dA[c][q]);
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) g[c][q] = 0.0f;
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const float v = quad_sum(through[c]), w = quad_sum(by[c]);
-          if (sg == 0) {
-            m.through[i][cg * C + c] = v;
-            m.by[i][cg * C + c] = w;
-          }
+          m.through[i][cg * C + c] = quad_sum(through[c]);
+          m.by[i][cg * C + c] = quad_sum(by[c]) * kLn2;
         }
-        // dB and dC: the 16 channel lanes through LDS
-        lds_order();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          m.cross[cg][sg * 2 * Q + q] = db[q];
-          m.cross[cg][sg * 2 * Q + Q + q] = dc[q];
-        }
-        lds_order();
-        constexpr int kOut = 2 * SP, kParts = kWave / kOut, kEach = 16 / kParts;
+        // dB and dC summed over the 16 channel lanes, two sums folded into one
+        // register at a time: halves of the wavefront then hold dB and dC, odd
+        // rows of 16 lanes the upper half of the lane's states
         float v = 0.0f;
 #pragma unroll
-        for (int r = 0; r < kEach; ++r) v += m.cross[(lane / kOut) * kEach + r][lane % kOut];
-#pragma unroll
-        for (int k = kOut; k < kWave; k <<= 1) v += __shfl_xor(v, k, 64);
-        if (lane < kOut && i < live_steps) cross_out[(((int64_t)(seg + i) * a.envs + env) * p.blocks + block) * kOut + lane] = v;
+        for (int q = 0; q < Q / 2; ++q) {
+          const float w = fold_rows(fold_halves(db[q], dc[q]), fold_halves(db[q + Q / 2], dc[q + Q / 2]));
+          const float sum = add_dpp<0x124>(add_dpp<0x128>(w));  // lanes rotated by 8 and by 4 in a row of 16
+          v = (cg & 3) == q ? sum : v;
+        }
+        constexpr int kOut = 2 * SP;
+        const int o = (lane >> 5) * SP + sg * Q + (lane >> 4 & 1) * (Q / 2) + (cg & 3);
+        if ((cg & 3) < Q / 2 && i < live_steps) cross_out[(((int64_t)(seg + i) * a.envs + env) * p.blocks + block) * kOut + o] = v;
       }
       lds_order();
       // finish: one channel a lane
@@ -460,15 +508,15 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
           const int64_t to = ((int64_t)t * a.envs + env) * a.dim + own_d;
           const float xv = m.x[i][own], dv = m.d[i][own], thr = m.through[i][own];
           float ddt = fmaf(thr, xv, m.by[i][own]);
-          if (a.softplus) ddt *= sigmoid((float)dtp[(int64_t)t * a.dt_step] + bias);
+          if (a.softplus) ddt *= sigmoid((float)raw_dt[k] + bias);
           ((T*)a.ddt)[to] = (T)ddt;
           ((T*)a.dx)[to] = (T)fmaf(thr, m.delta[i][own], skip * dv);
           dskip = fmaf(dv, xv, dskip);
           dbias += ddt;
           if (gated) {
-            const float zv = (float)zp[(int64_t)t * a.z_step], sig = sigmoid(zv);
+            const float zv = (float)raw_z[k], sig = sigmoid(zv);
             const float plain = fmaf(skip, xv, m.plain[i][own]);
-            ((T*)a.dz)[to] = (T)((float)dyp[(int64_t)t * a.dy_step] * plain * sig * fmaf(zv, 1.0f - sig, 1.0f));
+            ((T*)a.dz)[to] = (T)((float)raw_dy[k] * plain * sig * fmaf(zv, 1.0f - sig, 1.0f));
           }
         }
       }
@@ -498,15 +546,14 @@ __global__ __launch_bounds__(kWave * 2) void scan_grad_kernel(ScanArgs a, Pieces
 // dB and dC of a group: the sum over its channel blocks, rounded once.
 template <typename T, int SP>
 __global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, const float* cross) {
-  constexpr int Q = SP / 4;
   const int64_t i = block_id() * 256 + threadIdx.x;
   const int64_t row = i / (2 * SP);  // (step, env, group)
   if (row >= (int64_t)a.steps * a.envs * a.groups) return;
-  const int o = (int)(i % (2 * SP)), s = o / (2 * Q) * Q + o % Q;
+  const int o = (int)(i % (2 * SP)), s = o % SP;
   const float* from = cross + row * p.blocks_per_group * 2 * SP + o;
   float v = 0.0f;
   for (int k = 0; k < p.blocks_per_group; ++k) v += from[k * 2 * SP];
-  if (s < a.states) ((T*)(o / Q & 1 ? a.dc : a.db))[row * a.states + s] = (T)v;
+  if (s < a.states) ((T*)(o < SP ? a.db : a.dc))[row * a.states + s] = (T)v;
 }
 
 // The sums' row, taken apart.
@@ -675,7 +722,7 @@ hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
         const int64_t each = (int64_t)a.envs * a.states * a.dim;
         hipLaunchKernelGGL(join_kernel<true>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
       }
-      constexpr int per = GradShape<T, sp>::kWavesHere;
+      constexpr int per = GradShape<sp>::kWavesHere;
       const int64_t waves = (int64_t)slots * p.blocks;
       hipLaunchKernelGGL((scan_grad_kernel<T, sp>), dim3((unsigned)((waves + per - 1) / per)), dim3(kWave * per), 0, st, a, p, slots, (const float*)ends, cross, rows);
       const int64_t outs = (int64_t)a.steps * a.envs * a.groups * 2 * sp;

@@ -53,5 +53,6 @@ def __getattr__(name: str):
     if name in _LAZY:
         from importlib import import_module
 
-        return getattr(import_module(f".{_LAZY[name]}", __name__), name)
+        value = globals()[name] = getattr(import_module(f".{_LAZY[name]}", __name__), name)
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

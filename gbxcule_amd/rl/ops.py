@@ -87,15 +87,22 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _call(fn: str, t: torch.Tensor, *args: Any) -> None:
-    """A launch on the current stream of ``t``'s device."""
-    lib = _lib.load()
-    if t.device.index == torch.cuda.current_device():
-        rc = getattr(lib, fn)(*args, torch.cuda.current_stream().cuda_stream)
+    """A launch on the current stream of ``t``'s device.  (The raw stream
+    getter: a ``torch.cuda.Stream`` object costs as much as the launch.)"""
+    device = t.get_device()
+    entry = getattr(_lib.load(), fn)
+    if device == torch.cuda.current_device():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(t.device):
-            rc = getattr(lib, fn)(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(device):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     if rc:
         _lib.check(rc)
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _work(count: int, like: torch.Tensor) -> torch.Tensor | None:
@@ -134,7 +141,7 @@ def _norm_operands(x, weight, residual):
 def _norm_forward(elem, x, weight, residual, eps, out, scale=None, group=0):
     rows, dim = _flat(x), x.shape[-1]
     res = None if residual is None else _flat(residual)
-    summed = None if res is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    summed = None if res is None else _empty_like(x)
     _call("gbx_rms_norm", x, rows.shape[0], dim, elem, eps, rows.data_ptr(), rows.stride(0), _ptr(res),
           0 if res is None else res.stride(0), weight.data_ptr(), out.data_ptr(), _ptr(summed), _ptr(scale), group)  # fmt: skip
     return summed
@@ -144,7 +151,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, elem):
         ctx.set_materialize_grads(False)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _empty_like(x)
         summed = _norm_forward(elem, x, weight, residual, eps, y)
         ctx.save_for_backward(x if residual is None else summed, weight)
         ctx.eps, ctx.elem, ctx.plain = eps, elem, residual is None
@@ -161,7 +168,7 @@ class _RmsNorm(torch.autograd.Function):
         rows, dy = _flat(s), _flat(dy)
         if dsummed is not None:
             dsummed = _flat(dsummed)
-        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+        dx = _empty_like(s)
         dweight = torch.empty_like(weight)
         work = _work(_lib.load().gbx_rms_norm_grad_work(rows.shape[0], dim), s)
         _call("gbx_rms_norm_grad", s, rows.shape[0], dim, ctx.elem, ctx.eps, rows.data_ptr(), rows.stride(0),
@@ -180,7 +187,7 @@ def rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
     elem, weight, residual = _norm_operands(x, weight, residual)
     if _wants_grad(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, float(eps), elem)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty_like(x)
     summed = _norm_forward(elem, x, weight, residual, float(eps), y) if x.numel() else y
     return y if residual is None else (y, summed)
 
@@ -235,7 +242,7 @@ class _CausalConv(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         steps, envs, dim = x.shape
         width = weight.shape[1]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _empty_like(x)
         last = torch.empty((envs, width - 1, dim), dtype=x.dtype, device=x.device)
         _call("gbx_causal_conv", x, steps, envs, dim, width, elem, silu, x.data_ptr(), x.stride(0), x.stride(1),
               weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(resets), y.data_ptr(), last.data_ptr())  # fmt: skip
@@ -253,7 +260,7 @@ class _CausalConv(torch.autograd.Function):
         steps, envs, dim = x.shape
         width = weight.shape[1]
         dy = _rows(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _empty_like(x)
         dweight = torch.empty_like(weight)
         dbias = None if bias is None else torch.empty_like(bias)
         work = _work(_lib.load().gbx_causal_conv_grad_work(steps, envs, dim, width), x)
@@ -298,7 +305,7 @@ def causal_conv_step(x, weight, bias, state, *, resets=None, activation: str | N
     _require(state.is_contiguous(), "state must be contiguous: it is updated in place")
     resets = _resets(resets, x, (envs,))
     silu = _silu(activation)
-    y = torch.empty((envs, dim), dtype=x.dtype, device=x.device)
+    y = _empty_like(x)
     if envs:
         _call("gbx_causal_conv_step", x, envs, dim, weight.shape[1], elem, silu, x.data_ptr(), x.stride(0),
               weight.data_ptr(), _ptr(bias), state.data_ptr(), _ptr(resets), y.data_ptr())  # fmt: skip
@@ -341,11 +348,11 @@ def _scan_in(x, dt, A, B, C, D, z, dt_bias, resets, softplus, elem) -> _lib.Scan
 def _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, resets, softplus, elem, save):
     steps, envs, dim = x.shape
     given = _scan_in(x, dt, A, B, C, D, z, dt_bias, resets, softplus, elem)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty_like(x)
     last = torch.empty((envs, dim, A.shape[1]), dtype=torch.float32, device=x.device)
     saved = None
     if save:
-        saved = torch.empty((-(-steps // 16), envs, A.shape[1], dim), dtype=torch.float32, device=x.device)
+        saved = torch.empty((-(-steps // 8), envs, A.shape[1], dim), dtype=torch.float32, device=x.device)
     work = _work(_lib.load().gbx_selective_scan_work(given), x)
     _call("gbx_selective_scan", x, given, _ptr(state), y.data_ptr(), last.data_ptr(), _ptr(saved), _ptr(work))
     return y, last, saved
@@ -369,8 +376,7 @@ class _SelectiveScan(torch.autograd.Function):
             return (None,) * 12
         given = _scan_in(x, dt, A, B, C, D, z, dt_bias, resets, ctx.softplus, ctx.elem)
         dy = _rows(dy)
-        empty = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        dx, ddt, dA, dB, dC, dD, dz, dbias = (empty(t) for t in (x, dt, A, B, C, D, z, dt_bias))
+        dx, ddt, dA, dB, dC, dD, dz, dbias = (None if t is None else _empty_like(t) for t in (x, dt, A, B, C, D, z, dt_bias))
         work = _work(_lib.load().gbx_selective_scan_grad_work(given), x)
         _call("gbx_selective_scan_grad", x, given, saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1),
               dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD),
@@ -392,7 +398,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, *, dt_bias=None, softplus: bo
     ``dt_bias`` ``[channels]``; D, z and dt_bias may be None.  ``state``
     ``[N, channels, states]`` float32 before the first step (None: zeros).
     Returns ``(y, state after the last step)``; differentiable in everything
-    but the state.  For the gradient every 16th state is kept."""
+    but the state.  For the gradient every 8th state is kept."""
     elem = _elem("x", x)
     _require(x.ndim == 3 and x.shape[2] >= 1, f"x: expected [steps, envs, channels], got {tuple(x.shape)}")
     x = _rows(x)
@@ -428,7 +434,7 @@ def selective_scan_step(x, dt, A, B, C, D=None, z=None, *, state, dt_bias=None, 
     dt, A, B, C, D, z, dt_bias, resets = _scan_operands(x, dt, A, B, C, D, z, dt_bias, resets)
     _scan_state(state, x, (*x.shape, A.shape[1]))
     _require(state.is_contiguous(), "state must be contiguous: it is updated in place")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty_like(x)
     if x.shape[0]:
         given = _scan_in(x, dt, A, B, C, D, z, dt_bias, resets, softplus, elem)
         _call("gbx_selective_scan_step", x, given, state.data_ptr(), y.data_ptr())
