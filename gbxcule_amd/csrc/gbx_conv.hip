@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
       }
     }
   }
-  // one row of partial sums a workgroup: [width][dim], then the bias
+  // one row of partial sums a workgroup: [dim][width], then the bias [dim]
   float* part = a.work + (int64_t)blockIdx.x * (W + 1) * a.dim;
 #pragma unroll
   for (int j = 0; j <= W; ++j) {
@@ -237,16 +237,9 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
       const int ch = blockIdx.y * lanes * kVec + i;
       float v = 0.0f;
       for (int r = 0; r < (kThreads >> s.shift); ++r) v += tile[(r << s.shift) + i / kVec][i % kVec];
-      if (ch < a.dim) part[(int64_t)j * a.dim + ch] = v;
+      if (ch < a.dim) part[j < W ? ch * W + j : a.dim * W + ch] = v;
     }
   }
-}
-
-// The partial sums lie [width][dim]; weights lie [dim][width].
-__global__ void conv_turn_kernel(const float* sums, int dim, int width, float* dweight, float* dbias) {
-  const int i = blockIdx.x * kThreads + threadIdx.x;
-  if (i < dim * width) dweight[i] = sums[(int64_t)(i % width) * dim + i / width];
-  if (dbias && i < dim) dbias[i] = sums[(int64_t)width * dim + i];
 }
 
 // One step of every env: reads the state once and writes it moved on.
@@ -300,9 +293,9 @@ hipError_t launch_conv(const ConvArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// partial sums of the workgroups and one row of their sums
+// the workgroups' partial sums
 int64_t conv_grad_work(int steps, int envs, int dim, int width) {
-  return ((int64_t)grid_of(shape_of(steps, envs, dim)).x + 1) * (width + 1) * dim;
+  return (int64_t)grid_of(shape_of(steps, envs, dim)).x * (width + 1) * dim;
 }
 
 hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st) {
@@ -312,11 +305,7 @@ hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st) {
     by_width(a.width, [&](auto w) { hipLaunchKernelGGL((conv_grad_kernel<decltype(t), w>), grid, dim3(kThreads), 0, st, a, s); });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  const int cols = (a.width + 1) * a.dim;
-  float* sums = a.work + (int64_t)grid.x * cols;
-  if (hipError_t e = launch_column_sum(a.work, cols, (int)grid.x, cols, sums, st); e != hipSuccess) return e;
-  hipLaunchKernelGGL(conv_turn_kernel, dim3((unsigned)((a.dim * a.width + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, sums, a.dim, a.width, a.dweight, a.dbias);
-  return hipGetLastError();
+  return launch_column_sum(a.work, (int)grid.x, SumOutputs{{a.dweight, a.dbias}, {a.dim * a.width, a.dim}}, st);
 }
 
 hipError_t launch_conv_step(const ConvArgs& a, hipStream_t st) {

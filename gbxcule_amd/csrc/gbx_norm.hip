@@ -253,14 +253,16 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
   }
 }
 
-// out[c] = sum of in[r][c] over r: 16 columns by 64 rows of a workgroup at a
-// time, so that a few columns still fill the chip's memory pipes; one order.
+// 16 columns by 64 rows of a workgroup at a time, so that a few columns still
+// keep many loads in flight.
 constexpr int kSumCols = 16, kSumRows = 64;
-__global__ __launch_bounds__(kSumCols* kSumRows) void column_sum_kernel(const float* in, int64_t stride, int rows, int cols, float* out) {
+__global__ __launch_bounds__(kSumCols* kSumRows) void column_sum_kernel(const float* in, int rows, SumOutputs to) {
   __shared__ float tile[kSumRows][kSumCols + 1];
-  const int c = blockIdx.x * kSumCols + threadIdx.x % kSumCols, r0 = threadIdx.x / kSumCols;
+  const int stride = to.cols[0] + to.cols[1] + to.cols[2];
+  int c = blockIdx.x * kSumCols + threadIdx.x % kSumCols;
+  const int r0 = threadIdx.x / kSumCols;
   float v = 0.0f;
-  if (c < cols)
+  if (c < stride)
     for (int r = r0; r < rows; r += kSumRows) v += in[(int64_t)r * stride + c];
   tile[r0][threadIdx.x % kSumCols] = v;
   __syncthreads();
@@ -269,7 +271,12 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void column_sum_kernel(const fl
     if (r0 < m) tile[r0][threadIdx.x % kSumCols] += tile[r0 + m][threadIdx.x % kSumCols];
     __syncthreads();
   }
-  if (r0 == 0 && c < cols) out[c] = tile[0][threadIdx.x];
+  if (r0 != 0) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (c >= 0 && c < to.cols[k] && to.out[k]) to.out[k][c] = tile[0][threadIdx.x];
+    c -= to.cols[k];
+  }
 }
 
 template <typename F>
@@ -297,8 +304,9 @@ int grad_blocks(int64_t rows, int dim) {
 
 }  // namespace
 
-hipError_t launch_column_sum(const float* in, int64_t stride, int rows, int cols, float* out, hipStream_t st) {
-  hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((cols + kSumCols - 1) / kSumCols)), dim3(kSumCols * kSumRows), 0, st, in, stride, rows, cols, out);
+hipError_t launch_column_sum(const float* in, int rows, const SumOutputs& to, hipStream_t st) {
+  const int cols = to.cols[0] + to.cols[1] + to.cols[2];
+  hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((cols + kSumCols - 1) / kSumCols)), dim3(kSumCols * kSumRows), 0, st, in, rows, to);
   return hipGetLastError();
 }
 
@@ -326,7 +334,7 @@ hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t st) {
     });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  return launch_column_sum(a.work, a.dim, blocks, a.dim, a.dweight, st);
+  return launch_column_sum(a.work, blocks, SumOutputs{{a.dweight}, {a.dim}}, st);
 }
 
 }  // namespace gbx

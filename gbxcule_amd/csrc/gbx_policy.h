@@ -74,8 +74,14 @@ constexpr int kStateBlock = 256;  // elements that share a scale
 constexpr int kSegment = 8;     // steps between two saved states
 constexpr int kMaxStates = 32;  // states a channel may have
 
-// out[c] = sum over rows r of in[r * stride + c], in one order
-hipError_t launch_column_sum(const float* in, int64_t stride, int rows, int cols, float* out, hipStream_t st);
+// Sums over `rows` rows of partial sums that lie one after the other, in one
+// order.  The columns are up to three outputs' in turn; those whose pointer is
+// NULL are left out.
+struct SumOutputs {
+  float* out[3];
+  int cols[3];
+};
+hipError_t launch_column_sum(const float* in, int rows, const SumOutputs& to, hipStream_t st);
 hipError_t launch_rms_norm(const NormArgs& a, hipStream_t st);
 int64_t norm_grad_work(int64_t rows, int dim);
 hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t st);

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   const T* c = (const T*)a.c + from * a.c_step + env * a.c_env + group * a.c_group;
   const uint8_t* resets = a.resets + from * a.envs + env;
   T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim;
-  float* saved = a.saved + ((int64_t)(t0 / kSegment) * a.envs + env) * a.states * a.dim;
+  float* saved = a.saved + ((int64_t)(t0 / kSegment) * a.envs + env) * a.dim * a.states;
   auto of_lane = [&](const T* row) { return *(const T*)((const char*)row + at); };
 
   constexpr int kAhead = 4;  // steps whose loads are in flight together
@@ -152,6 +152,16 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     if constexpr (WHAT != BACK) load_scalar(b, rb);
     if constexpr (WHAT != ENDS) load_scalar(c, rc);
   }
+  auto store_states = [&](float* to, const float(&v)[SP]) {
+    if (a.states == SP) {  // 16 bytes at a time
+#pragma unroll
+      for (int s = 0; s < SP; s += 4) *reinterpret_cast<float4*>(to + s) = float4{v[s], v[s + 1], v[s + 2], v[s + 3]};
+    } else {
+#pragma unroll
+      for (int s = 0; s < SP; ++s)
+        if (s < a.states) to[s] = v[s];
+    }
+  };
   auto clear = [&]() {
     // a branch, the same for all lanes: without the barrier it becomes a
     // selection of every state at every step
@@ -240,11 +250,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   }
   if (!live) return;
   if constexpr (WHAT == FULL) {
-    if (t1 == a.steps) {
-#pragma unroll
-      for (int s = 0; s < SP; ++s)
-        if (s < a.states) a.last[((int64_t)env * a.dim + d) * a.states + s] = h[s];
-    }
+    if (t1 == a.steps) store_states(a.last + ((int64_t)env * a.dim + d) * a.states, h);
   } else {
 #pragma unroll
     for (int s = 0; s < SP; ++s)
@@ -293,14 +299,18 @@ __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float
 // cheap.  It walks the steps backwards in segments of kSegment: from the saved
 // state before the segment it computes the segment's states again into
 // registers, then goes back through them.  What a channel needs at a step
-// (delta, x, d) and the rows of B and C are converted once into LDS.
+// (delta, x, d) and the rows of B and C are converted once into LDS.  The
+// wavefronts of a workgroup take neighbouring channels of the same steps and
+// add their dB and dC in LDS at the end of a segment.
+constexpr int kGradWaves = 4;  // wavefronts of a workgroup at most
 template <int SP>
 struct GradShape {
-  static constexpr int Q = SP / 4, C = 8 / Q, CH = 16 * C, kWavesHere = 2;
+  static constexpr int Q = SP / 4, C = 8 / Q, CH = 16 * C;
   struct Lds {
     float delta[kSegment][CH], x[kSegment][CH], d[kSegment][CH];
     float through[kSegment][CH], by[kSegment][CH], plain[kSegment][CH];  // sums over states
     float b[kSegment][SP], c[kSegment][SP];
+    float cross[2][kSegment][2 * SP];  // dB, dC; two segments in turn
   };
 };
 
@@ -326,34 +336,34 @@ __device__ __forceinline__ float fold_rows(float a, float b) {
 }
 
 template <typename T, int SP>
-__global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
+__global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
   using S = GradShape<SP>;
-  constexpr int Q = S::Q, C = S::C, CH = S::CH, kPairs = kSegment * CH / kWave;
-  __shared__ typename S::Lds all[S::kWavesHere];
-  const int lane = threadIdx.x & 63;
-  typename S::Lds& m = all[threadIdx.x >> 6];
-  const int64_t wave = (int64_t)blockIdx.x * S::kWavesHere + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int block = (int)(wave % p.blocks), slot = (int)(wave / p.blocks);
-  if (slot >= slots) return;
-  const int group = block / p.blocks_per_group, per_group = a.dim / a.groups;
-  const int base = (block % p.blocks_per_group) * CH;  // of the block's channels in the group
-  const int cg = lane >> 2, sg = lane & 3;             // the lane's channels cg * C.., states sg * Q..
+  constexpr int Q = S::Q, C = S::C, CH = S::CH, kApart = kWave / CH, kPairs = kSegment / kApart;
+  extern __shared__ __align__(16) char lds[];
+  typename S::Lds* all = reinterpret_cast<typename S::Lds*>(lds);
+  const int lane = threadIdx.x & 63, which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
+  typename S::Lds& m = all[which];
+  const int block = blockIdx.x % p.blocks, slot = blockIdx.x / p.blocks;
+  const int group = block / p.blocks_per_group, per_group = a.dim / a.groups, first_d = group * per_group;
+  const int base = (block % p.blocks_per_group * waves + which) * CH;  // of the wavefront's channels in the group
+  const int cg = lane >> 2, sg = lane & 3;                             // the lane's channels cg * C.., states sg * Q..
   // one channel a lane where a step's values are prepared and finished
-  const int own = lane % CH, own_d = group * per_group + min(base + own, per_group - 1);
-  const bool own_live = base + own < per_group;
+  const int own = lane % CH, own_i = lane / CH, own_d = first_d + min(base + own, per_group - 1);
+  const bool own_live = base + own < per_group, gated = a.z != nullptr;
   const float bias = a.bias ? a.bias[own_d] : 0.0f, skip = a.skip ? a.skip[own_d] : 0.0f;
-  const bool gated = a.z != nullptr;
 
   float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;  // A in powers of two
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int c = 0; c < C; ++c) {
+    const int ch = base + cg * C + c;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int ch = base + cg * C + c, s = sg * Q + q;
-      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(group * per_group + ch) * a.states + s] * kLog2e : 0.0f;
+      const int s = sg * Q + q;
+      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(first_d + ch) * a.states + s] * kLog2e : 0.0f;
       dA[c][q] = 0.0f;
     }
-
+  }
+  int turn = 0;
   for (int64_t item = slot; item < (int64_t)p.chunks * a.envs; item += slots) {
     const int env = (int)(item % a.envs), piece = (int)(item / a.envs);
     const int t0 = piece * p.chunk, t1 = min(t0 + p.chunk, a.steps);
@@ -363,55 +373,81 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int ch = base + cg * C + c, s = sg * Q + q;
-        g[c][q] = p.chunks > 1 && ch < per_group && s < a.states ? carried[(item * a.states + s) * a.dim + group * per_group + ch] : 0.0f;
+        g[c][q] = p.chunks > 1 && ch < per_group && s < a.states ? carried[(item * a.states + s) * a.dim + first_d + ch] : 0.0f;
       }
-    const T* xp = (const T*)a.x + (int64_t)env * a.x_env + own_d;
-    const T* dtp = (const T*)a.dt + (int64_t)env * a.dt_env + own_d;
-    const T* zp = (const T*)a.z + (int64_t)env * a.z_env + own_d;
-    const T* dyp = (const T*)a.dy + (int64_t)env * a.dy_env + own_d;
-    const T* bp = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
-    const T* cp = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
+    // a lane's part of the addresses; the steps' part is the same for all
+    const T* xp = (const T*)a.x + env * a.x_env + own_i * a.x_step + own_d;
+    const T* dtp = (const T*)a.dt + env * a.dt_env + own_i * a.dt_step + own_d;
+    const T* zp = (const T*)a.z + env * a.z_env + own_i * a.z_step + own_d;
+    const T* dyp = (const T*)a.dy + env * a.dy_env + own_i * a.dy_step + own_d;
+    const int row_i = lane / SP, row_s = lane % SP;
+    const T* bp = (const T*)a.b + env * a.b_env + group * a.b_group + row_i * a.b_step + row_s;
+    const T* cp = (const T*)a.c + env * a.c_env + group * a.c_group + row_i * a.c_step + row_s;
+    const int64_t out_step = (int64_t)a.envs * a.dim, out = (int64_t)env * a.dim + own_i * out_step + own_d;
 
-    for (int seg = t0 + (t1 - 1 - t0) / kSegment * kSegment; seg >= t0; seg -= kSegment) {
+    // A segment's inputs as they lie in memory; the next segment's are on
+    // their way while this one is worked on.
+    constexpr int kRows = kWave / SP, kRowLoads = kSegment / kRows;
+    struct Inputs {
+      T x[kPairs], dt[kPairs], dy[kPairs], z[kPairs], b[kRowLoads], c[kRowLoads];
+      uint8_t begins;
+      float before[C][Q];
+    } in, next;
+    auto fetch = [&](int seg, Inputs& to) {
       const int live_steps = min(kSegment, a.steps - seg);
-      // prepare: steps past the end neither push nor decay, and nothing comes from them
-      T raw_dt[kPairs], raw_dy[kPairs], raw_z[kPairs];
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
-        const int i = lane / CH + k * (kWave / CH), t = min(seg + i, a.steps - 1);
-        const bool live = i < live_steps;
-        const float xv = (float)xp[(int64_t)t * a.x_step];
-        raw_dt[k] = dtp[(int64_t)t * a.dt_step];
-        raw_dy[k] = dyp[(int64_t)t * a.dy_step];
-        float delta = (float)raw_dt[k] + bias;
+        const int64_t t = seg + k * kApart;
+        to.x[k] = to.dt[k] = to.dy[k] = to.z[k] = (T)0.0f;
+        if (own_i + k * kApart < live_steps) {
+          to.x[k] = xp[t * a.x_step];
+          to.dt[k] = dtp[t * a.dt_step];
+          to.dy[k] = dyp[t * a.dy_step];
+          if (gated) to.z[k] = zp[t * a.z_step];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRowLoads; ++k) {
+        const int64_t t = seg + k * kRows;
+        to.b[k] = to.c[k] = (T)0.0f;
+        if (row_i + k * kRows < live_steps && row_s < a.states) {
+          to.b[k] = bp[t * a.b_step];
+          to.c[k] = cp[t * a.c_step];
+        }
+      }
+      to.begins = a.resets && lane < live_steps ? a.resets[(int64_t)(seg + lane) * a.envs + env] : 0;
+      const float* saved = a.saved + ((int64_t)(seg / kSegment) * a.envs + env) * a.dim * a.states;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int s = min(sg * Q + q, a.states - 1), ch = base + cg * C;
+        float row[C];
+        load_row<C>(saved + (int64_t)s * a.dim + first_d + ch, per_group - ch, row);
+#pragma unroll
+        for (int c = 0; c < C; ++c) to.before[c][q] = row[c];
+      }
+    };
+    const int last_seg = t0 + (t1 - 1 - t0) / kSegment * kSegment;
+    fetch(last_seg, next);
+    for (int seg = last_seg; seg >= t0; seg -= kSegment) {
+      const int live_steps = min(kSegment, a.steps - seg);
+      in = next;
+      const uint32_t begins = (uint32_t)__ballot(in.begins != 0);
+      // prepare: steps past the end neither push nor decay, and nothing comes from them
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const int i = own_i + k * kApart;
+        float delta = (float)in.dt[k] + bias, dv = (float)in.dy[k];
         if (a.softplus) delta = softplus(delta);
-        float dv = (float)raw_dy[k];
-        if (gated) {
-          raw_z[k] = zp[(int64_t)t * a.z_step];
-          const float zv = (float)raw_z[k];
-          dv *= zv * sigmoid(zv);
-        }
-        m.delta[i][own] = live ? delta : 0.0f;
-        m.x[i][own] = live ? xv : 0.0f;
-        m.d[i][own] = live && own_live ? dv : 0.0f;
+        if (gated) dv *= (float)in.z[k] * sigmoid((float)in.z[k]);
+        m.delta[i][own] = i < live_steps ? delta : 0.0f;
+        m.x[i][own] = (float)in.x[k];
+        m.d[i][own] = own_live ? dv : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < (kSegment * SP + kWave - 1) / kWave; ++k) {
-        const int e = lane + k * kWave, i = e / SP, s = e % SP, t = min(seg + i, a.steps - 1);
-        const bool live = i < live_steps && s < a.states;
-        m.b[i][s] = live ? (float)bp[(int64_t)t * a.b_step + s] : 0.0f;
-        m.c[i][s] = live ? (float)cp[(int64_t)t * a.c_step + s] : 0.0f;
+      for (int k = 0; k < kRowLoads; ++k) {
+        m.b[row_i + k * kRows][row_s] = (float)in.b[k];
+        m.c[row_i + k * kRows][row_s] = (float)in.c[k];
       }
-      uint32_t begins = 0;
-      if (a.resets) begins = (uint32_t)__ballot(lane < live_steps && a.resets[(int64_t)min(seg + lane, a.steps - 1) * a.envs + env]);
-      float before[C][Q];
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int ch = min(base + cg * C + c, per_group - 1), s = min(sg * Q + q, a.states - 1);
-          before[c][q] = a.saved[(((int64_t)(seg / kSegment) * a.envs + env) * a.states + s) * a.dim + group * per_group + ch];
-        }
       lds_order();
 
       // (an episode's first step takes a branch of its own, the same for all
@@ -432,7 +468,7 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int q = 0; q < Q; ++q) h[i][c][q] = fmaf(i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q], exp2_fast(delta[c] * A[c][q]), h[i][c][q]);
+            for (int q = 0; q < Q; ++q) h[i][c][q] = fmaf(i == 0 ? in.before[c][q] : h[i == 0 ? 0 : i - 1][c][q], exp2_fast(delta[c] * A[c][q]), h[i][c][q]);
         }
         if (gated) {
 #pragma unroll
@@ -444,13 +480,12 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
           }
         }
       }
+      if (seg > t0) fetch(seg - kSegment, next);
       lds_order();  // the rows are read again: kept in registers they would not fit
 #pragma unroll
       for (int i = kSegment - 1; i >= 0; --i) {
         const bool first = begins >> i & 1u;
         float db[Q], dc[Q], delta[C], through[C], by[C];
-#pragma unroll
-        for (int q = 0; q < Q; ++q) db[q] = dc[q] = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           delta[c] = m.delta[i][cg * C + c];
@@ -459,8 +494,8 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
           for (int q = 0; q < Q; ++q) {
             g[c][q] = fmaf(m.c[i][sg * Q + q], dv, g[c][q]);
-            dc[q] = fmaf(dv, h[i][c][q], dc[q]);
-            db[q] = fmaf(g[c][q], u, db[q]);
+            dc[q] = c == 0 ? dv * h[i][c][q] : fmaf(dv, h[i][c][q], dc[q]);
+            db[q] = c == 0 ? g[c][q] * u : fmaf(g[c][q], u, db[q]);
             through[c] = fmaf(g[c][q], m.b[i][sg * Q + q], through[c]);
           }
         }
@@ -470,11 +505,12 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
               g[c][q] *= exp2_fast(delta[c] * A[c][q]);
-              const float via = g[c][q] * (i == 0 ? before[c][q] : h[i == 0 ? 0 : i - 1][c][q]);
+              const float via = g[c][q] * (i == 0 ? in.before[c][q] : h[i == 0 ? 0 : i - 1][c][q]);
               by[c] = fmaf(via, A[c][q], by[c]);
               dA[c][q] = fmaf(via, delta[c], dA[c][q]);
             }
         } else {
+          asm volatile("");  // (stays a branch)
 #pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -483,44 +519,53 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           m.through[i][cg * C + c] = quad_sum(through[c]);
-          m.by[i][cg * C + c] = quad_sum(by[c]) * kLn2;
+          m.by[i][cg * C + c] = quad_sum(by[c]);
         }
         // dB and dC summed over the 16 channel lanes, two sums folded into one
         // register at a time: halves of the wavefront then hold dB and dC, odd
         // rows of 16 lanes the upper half of the lane's states
-        float v = 0.0f;
 #pragma unroll
         for (int q = 0; q < Q / 2; ++q) {
           const float w = fold_rows(fold_halves(db[q], dc[q]), fold_halves(db[q + Q / 2], dc[q + Q / 2]));
-          const float sum = add_dpp<0x124>(add_dpp<0x128>(w));  // lanes rotated by 8 and by 4 in a row of 16
-          v = (cg & 3) == q ? sum : v;
+          // lanes rotated by 8 and by 4 in a row of 16: four lanes write the same sum
+          m.cross[turn][i][(lane >> 5) * SP + sg * Q + (lane >> 4 & 1) * (Q / 2) + q] = add_dpp<0x124>(add_dpp<0x128>(w));
         }
-        constexpr int kOut = 2 * SP;
-        const int o = (lane >> 5) * SP + sg * Q + (lane >> 4 & 1) * (Q / 2) + (cg & 3);
-        if ((cg & 3) < Q / 2 && i < live_steps) cross_out[(((int64_t)(seg + i) * a.envs + env) * p.blocks + block) * kOut + o] = v;
       }
       lds_order();
       // finish: one channel a lane
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
-        const int i = lane / CH + k * (kWave / CH), t = min(seg + i, a.steps - 1);
+        const int i = own_i + k * kApart;
         if (i < live_steps && own_live) {
-          const int64_t to = ((int64_t)t * a.envs + env) * a.dim + own_d;
-          const float xv = m.x[i][own], dv = m.d[i][own], thr = m.through[i][own];
-          float ddt = fmaf(thr, xv, m.by[i][own]);
-          if (a.softplus) ddt *= sigmoid((float)raw_dt[k] + bias);
+          const int64_t to = out + (seg + k * kApart) * out_step;
+          const float xv = (float)in.x[k], dv = m.d[i][own], thr = m.through[i][own];
+          float ddt = fmaf(thr, xv, m.by[i][own] * kLn2);
+          if (a.softplus) ddt *= sigmoid((float)in.dt[k] + bias);
           ((T*)a.ddt)[to] = (T)ddt;
           ((T*)a.dx)[to] = (T)fmaf(thr, m.delta[i][own], skip * dv);
           dskip = fmaf(dv, xv, dskip);
           dbias += ddt;
           if (gated) {
-            const float zv = (float)raw_z[k], sig = sigmoid(zv);
+            const float zv = (float)in.z[k], sig = sigmoid(zv);
             const float plain = fmaf(skip, xv, m.plain[i][own]);
-            ((T*)a.dz)[to] = (T)((float)raw_dy[k] * plain * sig * fmaf(zv, 1.0f - sig, 1.0f));
+            ((T*)a.dz)[to] = (T)((float)in.dy[k] * plain * sig * fmaf(zv, 1.0f - sig, 1.0f));
           }
         }
       }
-      lds_order();
+      // dB and dC of the workgroup's channels; the wavefronts that are still
+      // here write the other half of `cross` in the next segment
+      __syncthreads();
+      for (int e = threadIdx.x; e < kSegment * 2 * SP; e += blockDim.x) {
+        const int i = e / (2 * SP), o = e % (2 * SP), s = o % SP;
+        float v = 0.0f;
+        for (int w = 0; w < waves; ++w) v += all[w].cross[turn][i][o];
+        if (i < live_steps) {
+          const int64_t row = (int64_t)(seg + i) * a.envs + env;
+          if (p.blocks_per_group > 1) cross_out[(row * p.blocks + block) * (2 * SP) + o] = v;
+          else if (s < a.states) ((T*)(o < SP ? a.db : a.dc))[(row * a.groups + group) * a.states + s] = (T)v;
+        }
+      }
+      turn ^= 1;
     }
   }
   // one row of partial sums a slot: dA [dim][states], dskip [dim], dbias [dim]
@@ -530,7 +575,7 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int ch = base + cg * C + c, s = sg * Q + q;
-      if (ch < per_group && s < a.states) row[(int64_t)(group * per_group + ch) * a.states + s] = dA[c][q];
+      if (ch < per_group && s < a.states) row[(int64_t)(first_d + ch) * a.states + s] = dA[c][q];
     }
 #pragma unroll
   for (int k = CH; k < kWave; k <<= 1) {
@@ -543,7 +588,7 @@ __global__ __launch_bounds__(kWave * 2, 2) void scan_grad_kernel(ScanArgs a, Pie
   }
 }
 
-// dB and dC of a group: the sum over its channel blocks, rounded once.
+// dB and dC of a group of several channel blocks: their sum, rounded once.
 template <typename T, int SP>
 __global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, const float* cross) {
   const int64_t i = block_id() * 256 + threadIdx.x;
@@ -554,17 +599,6 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, co
   float v = 0.0f;
   for (int k = 0; k < p.blocks_per_group; ++k) v += from[k * 2 * SP];
   if (s < a.states) ((T*)(o < SP ? a.db : a.dc))[row * a.states + s] = (T)v;
-}
-
-// The sums' row, taken apart.
-__global__ __launch_bounds__(256) void split_kernel(const float* sums, int dim, int states, float* da, float* dskip, float* dbias) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < dim * states) da[i] = sums[i];
-  else if (i < dim * (states + 1)) {
-    if (dskip) dskip[i - dim * states] = sums[i];
-  } else if (i < dim * (states + 2)) {
-    if (dbias) dbias[i - dim * (states + 1)] = sums[i];
-  }
 }
 
 // One step of every env: the state is read and written once and bounds the
@@ -642,22 +676,33 @@ int padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : 32; }
 // Wavefronts below which the steps are cut into pieces, and about how many
 // there are then: 2 for each of 1,024 SIMDs.
 constexpr int64_t kFull = 1024, kWant = 4096;
-Pieces pieces_of(int steps, int envs, int dim, int groups, int channels) {
+Pieces pieces_of(int steps, int envs, int dim, int groups, int channels, int waves_of_block) {
   Pieces p;
-  p.blocks_per_group = (dim / groups + channels - 1) / channels;
+  p.blocks_per_group = (dim / groups + channels * waves_of_block - 1) / (channels * waves_of_block);
   p.blocks = groups * p.blocks_per_group;
-  const int64_t waves = (int64_t)envs * p.blocks;
+  const int64_t waves = (int64_t)envs * p.blocks * waves_of_block;
   const int64_t cuts = waves >= kFull ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kSegment - 1) / kSegment);
   const int64_t each = (steps + cuts - 1) / cuts;
   p.chunk = (int)((each + kSegment - 1) / kSegment * kSegment);
   p.chunks = (steps + p.chunk - 1) / p.chunk;
   return p;
 }
-constexpr int64_t kGradWaves = 4096;
-int grad_slots(const Pieces& p, int envs) {
-  return (int)std::min<int64_t>((int64_t)p.chunks * envs, std::max<int64_t>(1, kGradWaves / p.blocks));
+// The gradient's workgroups: up to kGradWaves wavefronts of 512 / padded
+// channels each, and rows of partial sums for about 4,096 wavefronts.
+int grad_waves(int dim, int groups, int states) {
+  const int each = 512 / padded(states), blocks = (dim / groups + each - 1) / each;
+  return blocks > 2 ? kGradWaves : blocks;
 }
-int grad_channels(int states) { return 512 / padded(states); }
+int grad_slots(const Pieces& p, int envs, int waves) {
+  return (int)std::min<int64_t>((int64_t)p.chunks * envs, std::max<int64_t>(1, 4096 / (p.blocks * waves)));
+}
+Pieces grad_pieces(int steps, int envs, int dim, int groups, int states) {
+  return pieces_of(steps, envs, dim, groups, 512 / padded(states), grad_waves(dim, groups, states));
+}
+// dB and dC by channel block, where a group has several
+int64_t cross_floats(const Pieces& p, int steps, int envs, int states) {
+  return p.blocks_per_group > 1 ? (int64_t)steps * envs * p.blocks * 2 * padded(states) : 0;
+}
 
 template <typename T, int SP, int WHAT>
 void launch_scan_kernel(const ScanArgs& a, const Pieces& p, float* ends, float* sums, hipStream_t st) {
@@ -672,12 +717,12 @@ void launch_scan_kernel(const ScanArgs& a, const Pieces& p, float* ends, float* 
 }  // namespace
 
 int64_t scan_work(int steps, int envs, int dim, int groups, int states) {
-  const Pieces p = pieces_of(steps, envs, dim, groups, kWave);
+  const Pieces p = pieces_of(steps, envs, dim, groups, kWave, 1);
   return p.chunks > 1 ? (int64_t)p.chunks * envs * dim * (states + 1) : 0;
 }
 
 hipError_t launch_scan(const ScanArgs& a, hipStream_t st) {
-  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, kWave);
+  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, kWave, 1);
   float *ends = a.work, *sums = a.work + (int64_t)p.chunks * a.envs * a.dim * a.states;
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
@@ -693,23 +738,21 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// rows of partial sums and their sum; dB and dC by channel block; what the
-// pieces start from
+// rows of partial sums; dB and dC by channel block; what the pieces start from
 int64_t scan_grad_work(int steps, int envs, int dim, int groups, int states) {
-  const Pieces p = pieces_of(steps, envs, dim, groups, grad_channels(states));
-  int64_t n = (int64_t)(grad_slots(p, envs) + 1) * dim * (states + 2);
-  n += (int64_t)steps * envs * p.blocks * 2 * padded(states);
+  const Pieces p = grad_pieces(steps, envs, dim, groups, states);
+  int64_t n = (int64_t)grad_slots(p, envs, grad_waves(dim, groups, states)) * dim * (states + 2);
+  n += cross_floats(p, steps, envs, states);
   if (p.chunks > 1) n += (int64_t)p.chunks * envs * dim * (states + 1);
   return n;
 }
 
 hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
-  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, grad_channels(a.states));
-  const int slots = grad_slots(p, a.envs), cols = a.dim * (a.states + 2);
+  const Pieces p = grad_pieces(a.steps, a.envs, a.dim, a.groups, a.states);
+  const int waves = grad_waves(a.dim, a.groups, a.states), slots = grad_slots(p, a.envs, waves), cols = a.dim * (a.states + 2);
   float* rows = a.work;
-  float* sum = rows + (int64_t)slots * cols;
-  float* cross = sum + cols;
-  float* ends = cross + (int64_t)a.steps * a.envs * p.blocks * 2 * padded(a.states);
+  float* cross = rows + (int64_t)slots * cols;
+  float* ends = cross + cross_floats(p, a.steps, a.envs, a.states);
   float* sums = ends + (int64_t)p.chunks * a.envs * a.dim * a.states;
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
@@ -722,17 +765,16 @@ hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
         const int64_t each = (int64_t)a.envs * a.states * a.dim;
         hipLaunchKernelGGL(join_kernel<true>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
       }
-      constexpr int per = GradShape<sp>::kWavesHere;
-      const int64_t waves = (int64_t)slots * p.blocks;
-      hipLaunchKernelGGL((scan_grad_kernel<T, sp>), dim3((unsigned)((waves + per - 1) / per)), dim3(kWave * per), 0, st, a, p, slots, (const float*)ends, cross, rows);
-      const int64_t outs = (int64_t)a.steps * a.envs * a.groups * 2 * sp;
-      hipLaunchKernelGGL((cross_sum_kernel<T, sp>), wide_grid((outs + 255) / 256), dim3(256), 0, st, a, p, (const float*)cross);
+      const size_t lds = sizeof(typename GradShape<sp>::Lds) * waves;
+      hipLaunchKernelGGL((scan_grad_kernel<T, sp>), dim3((unsigned)(slots * p.blocks)), dim3(kWave * waves), lds, st, a, p, slots, (const float*)ends, cross, rows);
+      if (p.blocks_per_group > 1) {
+        const int64_t outs = (int64_t)a.steps * a.envs * a.groups * 2 * sp;
+        hipLaunchKernelGGL((cross_sum_kernel<T, sp>), wide_grid((outs + 255) / 256), dim3(256), 0, st, a, p, (const float*)cross);
+      }
     });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (hipError_t e = launch_column_sum(rows, cols, slots, cols, sum, st); e != hipSuccess) return e;
-  hipLaunchKernelGGL(split_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, st, (const float*)sum, a.dim, a.states, a.da, a.dskip, a.dbias);
-  return hipGetLastError();
+  return launch_column_sum(rows, slots, SumOutputs{{a.da, a.dskip, a.dbias}, {a.dim * a.states, a.dim, a.dim}}, st);
 }
 
 hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st) {

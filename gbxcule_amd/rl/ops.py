@@ -352,7 +352,7 @@ def _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, resets, softplus, elem, 
     last = torch.empty((envs, dim, A.shape[1]), dtype=torch.float32, device=x.device)
     saved = None
     if save:
-        saved = torch.empty((-(-steps // 8), envs, A.shape[1], dim), dtype=torch.float32, device=x.device)
+        saved = torch.empty((-(-steps // 8), envs, dim, A.shape[1]), dtype=torch.float32, device=x.device)
     work = _work(_lib.load().gbx_selective_scan_work(given), x)
     _call("gbx_selective_scan", x, given, _ptr(state), y.data_ptr(), last.data_ptr(), _ptr(saved), _ptr(work))
     return y, last, saved

@@ -277,7 +277,7 @@ typedef struct gbx_scan_in {
 } gbx_scan_in;
 /* state[envs][dim][states] (NULL: zeros) before the first step, last after the
  * last one.  saved, if not NULL, receives what the gradient starts from:
- * [steps / 8 rounded up][envs][states][dim]. */
+ * [steps / 8 rounded up][envs][dim][states]. */
 int64_t gbx_selective_scan_work(const gbx_scan_in* in);
 int gbx_selective_scan(const gbx_scan_in* in, const float* state, void* y, float* last, float* saved,
                        float* work, void* stream);
