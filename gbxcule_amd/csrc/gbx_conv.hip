@@ -14,48 +14,63 @@
 namespace gbx {
 namespace {
 
-constexpr int kThreads = 256, kVec = 8;
-constexpr int kMinSteps = 16;  // of a piece of the steps: its lead-in of up to 7 is read twice
-// Lanes that keep the memory busy: 2,048 for each of 256 CUs.  Rows of fewer
-// lanes are cut along the steps.
-constexpr int64_t kBusyLanes = 256 * 2048;
+constexpr int kThreads = 256;
+constexpr int kMinSteps = 16;  // of a piece of the steps: its lead-in of up to 3 is read twice
+// Lanes that keep the memory busy, times the channels of each: rows of fewer
+// are cut along the steps.
+constexpr int64_t kBusy = 256 * 2048 * 8;
 
-// Shape of the launch: a workgroup is `lanes` pieces of 8 channels by
-// 256 / lanes rows; a row is one env and one piece of the steps.
+// Shape of the launch: a workgroup is `lanes` groups of V neighbouring channels
+// by 256 / lanes rows; a row is one env and one piece of the steps.
 struct Shape {
-  int pieces, shift, chunk, chunks;  // 8-channel pieces; log2 of lanes in a row; steps of a piece, pieces
+  int groups, shift, chunk, chunks;  // groups of channels; log2 of lanes in a row; steps of a piece, pieces
   int64_t rows;
 };
-Shape shape_of(int steps, int envs, int dim) {
+Shape shape_of(int steps, int envs, int dim, int v) {
   Shape s;
-  s.pieces = (dim + kVec - 1) / kVec;
+  s.groups = (dim + v - 1) / v;
   s.shift = 0;
-  while (s.shift < 5 && (1 << s.shift) < s.pieces) ++s.shift;
-  const int64_t lanes = (int64_t)envs * s.pieces;
-  const int64_t want = std::max<int64_t>(1, kBusyLanes / lanes);
+  while (s.shift < 5 && (1 << s.shift) < s.groups) ++s.shift;
+  const int64_t want = std::max<int64_t>(1, kBusy / ((int64_t)envs * s.groups * v));
   s.chunk = (int)std::max<int64_t>(kMinSteps, (steps + want - 1) / want);
   s.chunks = (steps + s.chunk - 1) / s.chunk;
   s.rows = (int64_t)envs * s.chunks;
   return s;
 }
 
-// The inputs before step t0 of one env and 8 channels, oldest first, zero
-// where an episode begins between them and step t0 - 1.
-template <int W, typename T>
-__device__ __forceinline__ void lead_in(const ConvArgs& a, int env, int t0, int c, float (&win)[W - 1][kVec], int& age) {
+// Neighbouring channels of a row, as they lie.  WHOLE: every group has V.
+template <typename T, int V>
+struct Packed {
+  T v[V];
+};
+template <bool WHOLE, typename T, int V>
+__device__ __forceinline__ void fetch_row(const T* p, int n, Packed<T, V>& r) {
+  if (WHOLE || n >= V) {
+    __builtin_memcpy(&r, p, sizeof(r));
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = k < n ? p[k] : (T)0.0f;
+  }
+}
+
+// The inputs before step t0 of one env and V channels, oldest first, zero where
+// an episode begins between them and step t0 - 1; `age`: steps since the
+// episode began, no more than W.
+template <int W, int V, typename T>
+__device__ __forceinline__ void lead_in(const ConvArgs& a, int env, int t0, int c, float (&win)[W - 1][V], int& age) {
   const int n = a.dim - c;
-  age = W;  // steps since the episode began, no more than W
+  age = W;
 #pragma unroll
   for (int i = 0; i < W - 1; ++i) {
     const int t = t0 - (W - 1) + i;
     if (t < 0) {
-      if (a.state) load_row<kVec>((const T*)a.state + ((int64_t)env * (W - 1) + (t + W - 1)) * a.dim + c, n, win[i]);
+      if (a.state) load_row<V>((const T*)a.state + ((int64_t)env * (W - 1) + (t + W - 1)) * a.dim + c, n, win[i]);
       else {
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) win[i][k] = 0.0f;
+        for (int k = 0; k < V; ++k) win[i][k] = 0.0f;
       }
     } else {
-      load_row<kVec>((const T*)a.x + (int64_t)t * a.x_step + (int64_t)env * a.x_env + c, n, win[i]);
+      load_row<V>((const T*)a.x + (int64_t)t * a.x_step + (int64_t)env * a.x_env + c, n, win[i]);
     }
   }
   if (a.resets) {
@@ -67,78 +82,118 @@ __device__ __forceinline__ void lead_in(const ConvArgs& a, int env, int t0, int 
 #pragma unroll
       for (int j = 0; j < i; ++j)
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) win[j][k] = begins ? 0.0f : win[j][k];
+        for (int k = 0; k < V; ++k) win[j][k] = begins ? 0.0f : win[j][k];
     }
   }
 }
 
-// the weights of 8 channels lie together
-template <int W>
-__device__ __forceinline__ void load_weights(const ConvArgs& a, int c, float (&w)[W][kVec], float (&bias)[kVec]) {
-  float row[W * kVec];
-  load_row<W * kVec>(a.weight + (int64_t)c * W, (a.dim - c) * W, row);
+// the weights of neighbouring channels lie together
+template <int W, int V>
+__device__ __forceinline__ void load_weights(const ConvArgs& a, int c, float (&w)[W][V], float (&bias)[V]) {
+  float row[W * V];
+  load_row<W * V>(a.weight + (int64_t)c * W, (a.dim - c) * W, row);
 #pragma unroll
-  for (int k = 0; k < kVec; ++k)
+  for (int k = 0; k < V; ++k)
 #pragma unroll
     for (int j = 0; j < W; ++j) w[j][k] = row[k * W + j];
   if (a.bias) {
-    load_row<kVec>(a.bias + c, a.dim - c, bias);
+    load_row<V>(a.bias + c, a.dim - c, bias);
   } else {
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) bias[k] = 0.0f;
+    for (int k = 0; k < V; ++k) bias[k] = 0.0f;
   }
 }
 
-template <typename T, int W>
+// Where an episode begins in some lane, that lane's older inputs become zero.
+// A branch that most wavefronts skip: selections would cost each step as much
+// as the products do.
+template <int N, int V>
+__device__ __forceinline__ void forget(bool begins, float (&win)[N][V]) {
+  if (__ballot(begins)) {
+    asm volatile("");
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) win[j][k] = begins ? 0.0f : win[j][k];
+  }
+}
+template <int W, int V>
+__device__ __forceinline__ float convolve(const float (&w)[W][V], const float (&win)[W - 1][V], float in, float bias, int k) {
+  float pre = bias;
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) pre = fmaf(w[j][k], win[j][k], pre);
+  return fmaf(w[W - 1][k], in, pre);
+}
+template <int W, int V>
+__device__ __forceinline__ void move_on(float (&win)[W - 1][V], float in, int k) {
+#pragma unroll
+  for (int j = 0; j + 1 < W - 1; ++j) win[j][k] = win[j + 1][k];
+  win[W - 2][k] = in;
+}
+
+constexpr int kForward = 8, kBackward = 4;  // channels of a lane: 16 or 8 bytes of a 16-bit type
+
+template <typename T, int W, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
+  constexpr int V = kForward, kAhead = 4;  // steps whose loads are in flight while four others are worked on
   const int lanes = 1 << s.shift;
-  const int piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+  const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
   const int64_t row = (int64_t)blockIdx.x * (kThreads >> s.shift) + (threadIdx.x >> s.shift);
-  if (piece >= s.pieces || row >= s.rows) return;
+  if (group >= s.groups || row >= s.rows) return;
   const int env = (int)(row % a.envs), part = (int)(row / a.envs);
-  const int c = piece * kVec, n = a.dim - c;
+  const int c = group * V, n = a.dim - c;
   const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
-  float w[W][kVec], bias[kVec], win[W - 1][kVec];
+  const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env + c;
+  const uint8_t* resets = a.resets + (int64_t)t0 * a.envs + env;
+  T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim + c;
+  Packed<T, V> next[kAhead];
+  uint8_t next_begins[kAhead];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int on = t + i + 1 < t1;  // the last row is loaded again past the end
+      fetch_row<WHOLE>(x, n, next[i]);
+      x += on ? a.x_step : 0;
+      next_begins[i] = 0;
+      if (a.resets) {
+        next_begins[i] = *resets;
+        resets += on ? a.envs : 0;
+      }
+    }
+  };
+  fetch(t0);
+  float w[W][V], bias[V], win[W - 1][V];
   int age;
   load_weights<W>(a, c, w, bias);
-  lead_in<W, T>(a, env, t0, c, win, age);
-  const T* x = (const T*)a.x + (int64_t)env * a.x_env + c;
-  T* y = (T*)a.y + (int64_t)env * a.dim + c;
-  constexpr int kAhead = 4;  // steps whose loads are in flight together
+  lead_in<W, V, T>(a, env, t0, c, win, age);
   for (int t = t0; t < t1; t += kAhead) {
-    float in[kAhead][kVec];
+    Packed<T, V> in[kAhead];
     bool begins[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int ti = min(t + i, t1 - 1);
-      load_row<kVec>(x + (int64_t)ti * a.x_step, n, in[i]);
-      begins[i] = a.resets && a.resets[(int64_t)ti * a.envs + env];
+      in[i] = next[i];
+      begins[i] = next_begins[i] != 0;
     }
+    if (t + kAhead < t1) fetch(t + kAhead);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (t + i >= t1) break;
-      float out[kVec];
+      forget(begins[i], win);
+      float out[V];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        float pre = bias[k];
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-          win[j][k] = begins[i] ? 0.0f : win[j][k];
-          pre = fmaf(w[j][k], win[j][k], pre);
-        }
-        pre = fmaf(w[W - 1][k], in[i][k], pre);
+      for (int k = 0; k < V; ++k) {
+        const float v = (float)in[i].v[k], pre = convolve<W, V>(w, win, v, bias[k], k);
         out[k] = a.silu ? pre * sigmoid(pre) : pre;
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j) win[j][k] = win[j + 1][k];
-        win[W - 2][k] = in[i][k];
+        move_on<W, V>(win, v, k);
       }
-      store_row<kVec>(y + (int64_t)(t + i) * a.envs * a.dim, n, out);
+      store_row<V>(y, WHOLE ? V : n, out);
+      y += (int64_t)a.envs * a.dim;
     }
   }
   if (t1 == a.steps) {
     T* last = (T*)a.last + (int64_t)env * (W - 1) * a.dim + c;
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_row<kVec>(last + (int64_t)j * a.dim, n, win[j]);
+    for (int j = 0; j < W - 1; ++j) store_row<V>(last + (int64_t)j * a.dim, n, win[j]);
   }
 }
 
@@ -149,79 +204,117 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
 // inputs; a piece of the steps goes width - 1 steps past its end to finish
 // its own.  dweight and dbias of a workgroup's rows are added in LDS and
 // written as one row of partial sums.
-template <typename T, int W>
+template <typename T, int W, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s) {
-  __shared__ float tile[kThreads][kVec];
+  constexpr int V = kBackward, kAhead = 4;
+  __shared__ float tile[kThreads][V];
   const int lanes = 1 << s.shift;
-  const int piece = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+  const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
   const int64_t row = (int64_t)blockIdx.x * (kThreads >> s.shift) + (threadIdx.x >> s.shift);
-  const int c = piece * kVec, n = a.dim - c;
-  float dw[W][kVec], db[kVec];
+  const int c = group * V, n = a.dim - c;
+  float dw[W][V], db[V];
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) {
+  for (int k = 0; k < V; ++k) {
     db[k] = 0.0f;
 #pragma unroll
     for (int j = 0; j < W; ++j) dw[j][k] = 0.0f;
   }
-  if (piece < s.pieces && row < s.rows) {
+  if (group < s.groups && row < s.rows) {
     const int env = (int)(row % a.envs), part = (int)(row / a.envs);
     const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
-    float w[W][kVec], bias[kVec], win[W - 1][kVec], acc[W][kVec];  // acc[i]: dx of step t - (W - 1) + i
+    const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env + c;
+    const T* dy = (const T*)a.dy + (int64_t)t0 * a.dy_step + (int64_t)env * a.dy_env + c;
+    const uint8_t* resets = a.resets + (int64_t)t0 * a.envs + env;
+    T* dx = (T*)a.dx + ((int64_t)t0 * a.envs + env) * a.dim + c;
+    Packed<T, V> next_x[kAhead], next_d[kAhead];
+    uint8_t next_begins[kAhead];
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int on = t + i + 1 < a.steps;
+        fetch_row<WHOLE>(x, n, next_x[i]);
+        x += on ? a.x_step : 0;
+        fetch_row<WHOLE>(dy, n, next_d[i]);
+        dy += on ? a.dy_step : 0;
+        next_begins[i] = 0;
+        if (a.resets) {
+          next_begins[i] = *resets;
+          resets += on ? a.envs : 0;
+        }
+      }
+    };
+    fetch(t0);
+    float w[W][V], bias[V], win[W - 1][V], acc[W][V];  // acc[i]: dx of step t - (W - 1) + i
     int age;
     load_weights<W>(a, c, w, bias);
-    lead_in<W, T>(a, env, t0, c, win, age);
+    lead_in<W, V, T>(a, env, t0, c, win, age);
 #pragma unroll
     for (int j = 0; j < W; ++j)
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) acc[j][k] = 0.0f;
-    const T* x = (const T*)a.x + (int64_t)env * a.x_env + c;
-    const T* dy = (const T*)a.dy + (int64_t)env * a.dy_env + c;
-    T* dx = (T*)a.dx + (int64_t)env * a.dim + c;
-    constexpr int kAhead = 4;
-    for (int t = t0; t < t1 + W - 1; t += kAhead) {
-      float in[kAhead][kVec], d[kAhead][kVec];
+      for (int k = 0; k < V; ++k) acc[j][k] = 0.0f;
+    const int end = t1 + W - 1;
+    for (int t = t0; t < end; t += kAhead) {
+      Packed<T, V> xs[kAhead], ds[kAhead];
       bool begins[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int ti = min(t + i, a.steps - 1);
-        load_row<kVec>(x + (int64_t)ti * a.x_step, n, in[i]);
-        load_row<kVec>(dy + (int64_t)ti * a.dy_step, n, d[i]);
-        begins[i] = a.resets && a.resets[(int64_t)ti * a.envs + env];
+        xs[i] = next_x[i];
+        ds[i] = next_d[i];
+        begins[i] = next_begins[i] != 0;
       }
+      if (t + kAhead < end) fetch(t + kAhead);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int ti = t + i;
-        if (ti >= t1 + W - 1) break;
+        if (ti >= end) break;
+        forget(begins[i], win);
         age = begins[i] ? 0 : min(age + 1, W);
-        const bool mine = ti < t1, any = ti < a.steps;
+        float d[V];
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          float pre = bias[k], dk = any ? d[i][k] : 0.0f;
-#pragma unroll
-          for (int j = 0; j < W - 1; ++j) {
-            win[j][k] = begins[i] ? 0.0f : win[j][k];
-            pre = fmaf(w[j][k], win[j][k], pre);
-          }
-          pre = fmaf(w[W - 1][k], in[i][k], pre);
+        for (int k = 0; k < V; ++k) {
+          const float v = (float)xs[i].v[k];
+          d[k] = (float)ds[i].v[k];
           if (a.silu) {
-            const float sig = sigmoid(pre);
-            dk *= sig * fmaf(pre, 1.0f - sig, 1.0f);
+            const float pre = convolve<W, V>(w, win, v, bias[k], k), sig = sigmoid(pre);
+            d[k] *= sig * fmaf(pre, 1.0f - sig, 1.0f);
           }
-          // acc moves one step on; its last slot begins with this step
-#pragma unroll
-          for (int j = 0; j < W - 1; ++j) acc[j][k] = W - 1 - j <= age ? fmaf(w[j][k], dk, acc[j + 1][k]) : acc[j + 1][k];
-          acc[W - 1][k] = w[W - 1][k] * dk;
-          const float own = mine ? dk : 0.0f;
-          db[k] += own;
-#pragma unroll
-          for (int j = 0; j < W - 1; ++j) dw[j][k] = fmaf(own, win[j][k], dw[j][k]);
-          dw[W - 1][k] = fmaf(own, in[i][k], dw[W - 1][k]);
-#pragma unroll
-          for (int j = 0; j + 1 < W - 1; ++j) win[j][k] = win[j + 1][k];
-          win[W - 2][k] = in[i][k];
         }
-        const int done = ti - (W - 1);
-        if (done >= t0 && done < t1) store_row<kVec>(dx + (int64_t)done * a.envs * a.dim, n, acc[0]);
+        if (ti < t1) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            db[k] += d[k];
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j) dw[j][k] = fmaf(d[k], win[j][k], dw[j][k]);
+            dw[W - 1][k] = fmaf(d[k], (float)xs[i].v[k], dw[W - 1][k]);
+          }
+        }
+        // acc moves one step on; its last slot begins with this step.  Steps
+        // before the episode's first get nothing, and nothing comes from past the end.
+        const bool any = ti < a.steps;
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[j][k] = acc[j + 1][k];
+        if (__ballot(age < W - 1 || !any)) {
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[j][k] = any && W - 1 - j <= age ? fmaf(w[j][k], d[k], acc[j][k]) : acc[j][k];
+        } else {
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[j][k] = fmaf(w[j][k], d[k], acc[j][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          acc[W - 1][k] = w[W - 1][k] * d[k];
+          move_on<W, V>(win, (float)xs[i].v[k], k);
+        }
+        if (ti - (W - 1) >= t0) {
+          store_row<V>(dx, WHOLE ? V : n, acc[0]);
+          dx += (int64_t)a.envs * a.dim;
+        }
       }
     }
   }
@@ -231,12 +324,12 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
   for (int j = 0; j <= W; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) tile[threadIdx.x][k] = j < W ? dw[j < W ? j : 0][k] : db[k];
+    for (int k = 0; k < V; ++k) tile[threadIdx.x][k] = j < W ? dw[j < W ? j : 0][k] : db[k];
     __syncthreads();
-    for (int i = threadIdx.x; i < lanes * kVec; i += kThreads) {
-      const int ch = blockIdx.y * lanes * kVec + i;
+    for (int i = threadIdx.x; i < lanes * V; i += kThreads) {
+      const int ch = blockIdx.y * lanes * V + i;
       float v = 0.0f;
-      for (int r = 0; r < (kThreads >> s.shift); ++r) v += tile[(r << s.shift) + i / kVec][i % kVec];
+      for (int r = 0; r < (kThreads >> s.shift); ++r) v += tile[(r << s.shift) + i / V][i % V];
       if (ch < a.dim) part[j < W ? ch * W + j : a.dim * W + ch] = v;
     }
   }
@@ -245,6 +338,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
 // One step of every env: reads the state once and writes it moved on.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a, int pieces) {
+  constexpr int kVec = kForward;
   const int64_t i = block_id() * kThreads + threadIdx.x;
   const int64_t env = i / pieces;
   const int c = (int)(i % pieces) * kVec, n = a.dim - c;
@@ -258,13 +352,9 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a, int pie
   load_weights<W>(a, c, w, bias);
 #pragma unroll
   for (int k = 0; k < kVec; ++k) {
-    float pre = bias[k];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-      win[j][k] = begins ? 0.0f : win[j][k];
-      pre = fmaf(w[j][k], win[j][k], pre);
-    }
-    pre = fmaf(w[W - 1][k], in[k], pre);
+    for (int j = 0; j < W - 1; ++j) win[j][k] = begins ? 0.0f : win[j][k];
+    const float pre = convolve<W, kVec>(w, win, in[k], bias[k], k);
     out[k] = a.silu ? pre * sigmoid(pre) : pre;
   }
   store_row<kVec>((T*)a.y + env * a.dim + c, n, out);
@@ -280,36 +370,44 @@ void by_width(int width, F&& f) {
 }
 dim3 grid_of(const Shape& s) {
   const int per = kThreads >> s.shift;
-  return dim3((unsigned)((s.rows + per - 1) / per), (unsigned)((s.pieces + (1 << s.shift) - 1) >> s.shift));
+  return dim3((unsigned)((s.rows + per - 1) / per), (unsigned)((s.groups + (1 << s.shift) - 1) >> s.shift));
 }
 
 }  // namespace
 
 hipError_t launch_conv(const ConvArgs& a, hipStream_t st) {
-  const Shape s = shape_of(a.steps, a.envs, a.dim);
+  const Shape s = shape_of(a.steps, a.envs, a.dim, kForward);
   by_element(a.elem, [&](auto t) {
-    by_width(a.width, [&](auto w) { hipLaunchKernelGGL((conv_kernel<decltype(t), w>), grid_of(s), dim3(kThreads), 0, st, a, s); });
+    using T = decltype(t);
+    by_width(a.width, [&](auto w) {
+      if (a.dim % kForward == 0) hipLaunchKernelGGL((conv_kernel<T, w, true>), grid_of(s), dim3(kThreads), 0, st, a, s);
+      else hipLaunchKernelGGL((conv_kernel<T, w, false>), grid_of(s), dim3(kThreads), 0, st, a, s);
+    });
   });
   return hipGetLastError();
 }
 
 // the workgroups' partial sums
 int64_t conv_grad_work(int steps, int envs, int dim, int width) {
-  return (int64_t)grid_of(shape_of(steps, envs, dim)).x * (width + 1) * dim;
+  return (int64_t)grid_of(shape_of(steps, envs, dim, kBackward)).x * (width + 1) * dim;
 }
 
 hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st) {
-  const Shape s = shape_of(a.steps, a.envs, a.dim);
+  const Shape s = shape_of(a.steps, a.envs, a.dim, kBackward);
   const dim3 grid = grid_of(s);
   by_element(a.elem, [&](auto t) {
-    by_width(a.width, [&](auto w) { hipLaunchKernelGGL((conv_grad_kernel<decltype(t), w>), grid, dim3(kThreads), 0, st, a, s); });
+    using T = decltype(t);
+    by_width(a.width, [&](auto w) {
+      if (a.dim % kBackward == 0) hipLaunchKernelGGL((conv_grad_kernel<T, w, true>), grid, dim3(kThreads), 0, st, a, s);
+      else hipLaunchKernelGGL((conv_grad_kernel<T, w, false>), grid, dim3(kThreads), 0, st, a, s);
+    });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   return launch_column_sum(a.work, (int)grid.x, SumOutputs{{a.dweight, a.dbias}, {a.dim * a.width, a.dim}}, st);
 }
 
 hipError_t launch_conv_step(const ConvArgs& a, hipStream_t st) {
-  const int pieces = (a.dim + kVec - 1) / kVec;
+  const int pieces = (a.dim + kForward - 1) / kForward;
   const dim3 grid = wide_grid(((int64_t)a.envs * pieces + kThreads - 1) / kThreads);
   by_element(a.elem, [&](auto t) {
     by_width(a.width, [&](auto w) { hipLaunchKernelGGL((conv_step_kernel<decltype(t), w>), grid, dim3(kThreads), 0, st, a, pieces); });
