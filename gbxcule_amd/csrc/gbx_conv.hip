@@ -30,7 +30,7 @@ Shape shape_of(int steps, int envs, int dim, int v) {
   Shape s;
   s.groups = (dim + v - 1) / v;
   s.shift = 0;
-  while (s.shift < 5 && (1 << s.shift) < s.groups) ++s.shift;
+  while (s.shift < 6 && (1 << s.shift) < s.groups) ++s.shift;
   const int64_t want = std::max<int64_t>(1, kBusy / ((int64_t)envs * s.groups * v));
   s.chunk = (int)std::max<int64_t>(kMinSteps, (steps + want - 1) / want);
   s.chunks = (steps + s.chunk - 1) / s.chunk;
@@ -133,26 +133,34 @@ __device__ __forceinline__ void move_on(float (&win)[W - 1][V], float in, int k)
 
 constexpr int kForward = 8, kBackward = 4;  // channels of a lane: 16 or 8 bytes of a 16-bit type
 
-template <typename T, int W, bool WHOLE>
+// A row's place: its first channel group's lane, env and piece of the steps.
+// WIDE: a wavefront is one row, and what depends on the row alone is scalar.
+template <bool WIDE>
+__device__ __forceinline__ int64_t row_of(const Shape& s) {
+  const int in = threadIdx.x >> s.shift;
+  return (int64_t)blockIdx.x * (kThreads >> s.shift) + (WIDE ? __builtin_amdgcn_readfirstlane(in) : in);
+}
+
+template <typename T, int W, bool WHOLE, bool WIDE>
 __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
   constexpr int V = kForward, kAhead = 4;  // steps whose loads are in flight while four others are worked on
   const int lanes = 1 << s.shift;
   const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
-  const int64_t row = (int64_t)blockIdx.x * (kThreads >> s.shift) + (threadIdx.x >> s.shift);
+  const int64_t row = row_of<WIDE>(s);
   if (group >= s.groups || row >= s.rows) return;
   const int env = (int)(row % a.envs), part = (int)(row / a.envs);
   const int c = group * V, n = a.dim - c;
   const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
-  const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env + c;
+  const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env;
   const uint8_t* resets = a.resets + (int64_t)t0 * a.envs + env;
-  T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim + c;
+  T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim;
   Packed<T, V> next[kAhead];
   uint8_t next_begins[kAhead];
   auto fetch = [&](int t) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int on = t + i + 1 < t1;  // the last row is loaded again past the end
-      fetch_row<WHOLE>(x, n, next[i]);
+      fetch_row<WHOLE>(x + c, n, next[i]);
       x += on ? a.x_step : 0;
       next_begins[i] = 0;
       if (a.resets) {
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       in[i] = next[i];
-      begins[i] = next_begins[i] != 0;
+      begins[i] = (WIDE ? __builtin_amdgcn_readfirstlane((int)next_begins[i]) : (int)next_begins[i]) != 0;
     }
     if (t + kAhead < t1) fetch(t + kAhead);
 #pragma unroll
@@ -186,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
         out[k] = a.silu ? pre * sigmoid(pre) : pre;
         move_on<W, V>(win, v, k);
       }
-      store_row<V>(y, WHOLE ? V : n, out);
+      store_row<V>(y + c, WHOLE ? V : n, out);
       y += (int64_t)a.envs * a.dim;
     }
   }
@@ -204,13 +212,13 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
 // inputs; a piece of the steps goes width - 1 steps past its end to finish
 // its own.  dweight and dbias of a workgroup's rows are added in LDS and
 // written as one row of partial sums.
-template <typename T, int W, bool WHOLE>
+template <typename T, int W, bool WHOLE, bool WIDE>
 __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s) {
   constexpr int V = kBackward, kAhead = 4;
   __shared__ float tile[kThreads][V];
   const int lanes = 1 << s.shift;
   const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
-  const int64_t row = (int64_t)blockIdx.x * (kThreads >> s.shift) + (threadIdx.x >> s.shift);
+  const int64_t row = row_of<WIDE>(s);
   const int c = group * V, n = a.dim - c;
   float dw[W][V], db[V];
 #pragma unroll
@@ -222,19 +230,19 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
   if (group < s.groups && row < s.rows) {
     const int env = (int)(row % a.envs), part = (int)(row / a.envs);
     const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
-    const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env + c;
-    const T* dy = (const T*)a.dy + (int64_t)t0 * a.dy_step + (int64_t)env * a.dy_env + c;
+    const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env;
+    const T* dy = (const T*)a.dy + (int64_t)t0 * a.dy_step + (int64_t)env * a.dy_env;
     const uint8_t* resets = a.resets + (int64_t)t0 * a.envs + env;
-    T* dx = (T*)a.dx + ((int64_t)t0 * a.envs + env) * a.dim + c;
+    T* dx = (T*)a.dx + ((int64_t)t0 * a.envs + env) * a.dim;
     Packed<T, V> next_x[kAhead], next_d[kAhead];
     uint8_t next_begins[kAhead];
     auto fetch = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int on = t + i + 1 < a.steps;
-        fetch_row<WHOLE>(x, n, next_x[i]);
+        fetch_row<WHOLE>(x + c, n, next_x[i]);
         x += on ? a.x_step : 0;
-        fetch_row<WHOLE>(dy, n, next_d[i]);
+        fetch_row<WHOLE>(dy + c, n, next_d[i]);
         dy += on ? a.dy_step : 0;
         next_begins[i] = 0;
         if (a.resets) {
@@ -260,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
       for (int i = 0; i < kAhead; ++i) {
         xs[i] = next_x[i];
         ds[i] = next_d[i];
-        begins[i] = next_begins[i] != 0;
+        begins[i] = (WIDE ? __builtin_amdgcn_readfirstlane((int)next_begins[i]) : (int)next_begins[i]) != 0;
       }
       if (t + kAhead < end) fetch(t + kAhead);
 #pragma unroll
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
           move_on<W, V>(win, (float)xs[i].v[k], k);
         }
         if (ti - (W - 1) >= t0) {
-          store_row<V>(dx, WHOLE ? V : n, acc[0]);
+          store_row<V>(dx + c, WHOLE ? V : n, acc[0]);
           dx += (int64_t)a.envs * a.dim;
         }
       }
@@ -380,8 +388,11 @@ hipError_t launch_conv(const ConvArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_width(a.width, [&](auto w) {
-      if (a.dim % kForward == 0) hipLaunchKernelGGL((conv_kernel<T, w, true>), grid_of(s), dim3(kThreads), 0, st, a, s);
-      else hipLaunchKernelGGL((conv_kernel<T, w, false>), grid_of(s), dim3(kThreads), 0, st, a, s);
+      const bool wide = s.shift == 6;
+      if (a.dim % kForward == 0 && wide) hipLaunchKernelGGL((conv_kernel<T, w, true, true>), grid_of(s), dim3(kThreads), 0, st, a, s);
+      else if (a.dim % kForward == 0) hipLaunchKernelGGL((conv_kernel<T, w, true, false>), grid_of(s), dim3(kThreads), 0, st, a, s);
+      else if (wide) hipLaunchKernelGGL((conv_kernel<T, w, false, true>), grid_of(s), dim3(kThreads), 0, st, a, s);
+      else hipLaunchKernelGGL((conv_kernel<T, w, false, false>), grid_of(s), dim3(kThreads), 0, st, a, s);
     });
   });
   return hipGetLastError();
@@ -398,8 +409,11 @@ hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_width(a.width, [&](auto w) {
-      if (a.dim % kBackward == 0) hipLaunchKernelGGL((conv_grad_kernel<T, w, true>), grid, dim3(kThreads), 0, st, a, s);
-      else hipLaunchKernelGGL((conv_grad_kernel<T, w, false>), grid, dim3(kThreads), 0, st, a, s);
+      const bool wide = s.shift == 6;
+      if (a.dim % kBackward == 0 && wide) hipLaunchKernelGGL((conv_grad_kernel<T, w, true, true>), grid, dim3(kThreads), 0, st, a, s);
+      else if (a.dim % kBackward == 0) hipLaunchKernelGGL((conv_grad_kernel<T, w, true, false>), grid, dim3(kThreads), 0, st, a, s);
+      else if (wide) hipLaunchKernelGGL((conv_grad_kernel<T, w, false, true>), grid, dim3(kThreads), 0, st, a, s);
+      else hipLaunchKernelGGL((conv_grad_kernel<T, w, false, false>), grid, dim3(kThreads), 0, st, a, s);
     });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
