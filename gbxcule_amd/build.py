@@ -21,21 +21,21 @@ SOURCES = (
     "gbx_step.hip", "gbx_aux.hip", "gbx_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_adamw.hip", "gbx_api.hip",
 )  # fmt: skip
 ARCH = os.environ.get("GBX_OFFLOAD_ARCH", "gfx950")
-# -O2 with the iterative ILP machine scheduler: on the step kernel's hot
-# loop this schedules the dependent loads earlier than -O3 with the default
-# occupancy-first scheduler (same-box A/B: 16K-env CPU-step workload +2.4%,
-# 131K-env banked cart +2.5%, RL rollout shape unchanged).
 DEVICE_FLAGS = (
     "-O2",
     f"--offload-arch={ARCH}",
     "-std=c++17",
-    "-mllvm",
-    "-amdgpu-sched-strategy=iterative-ilp",
     "-Xclang",
     "-target-feature",
     "-Xclang",
     "-packed-fp32-ops",
 )
+# The emulator's sources: the iterative ILP machine scheduler.  On the step
+# kernel's hot loop this schedules the dependent loads earlier than -O3 with
+# the default occupancy-first scheduler (same-box A/B: 16K-env CPU-step
+# workload +2.4%, 131K-env banked cart +2.5%, RL rollout shape unchanged).
+ILP_FLAGS = ("-mllvm", "-amdgpu-sched-strategy=iterative-ilp")
+ILP_SOURCES = ("gbx_step.hip", "gbx_aux.hip", "gbx_api.hip")
 
 
 def hipcc() -> str:
@@ -53,8 +53,9 @@ def build(verbose: bool = False) -> Path:
     include = ["-I", str(PKG.parent / "include")]
     objects = [LIB_DIR / f"{Path(s).stem}.o" for s in SOURCES]
     commands = [
-        [hipcc(), *DEVICE_FLAGS, "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)] for s, o in zip(SOURCES, objects)
-    ]
+        [hipcc(), *DEVICE_FLAGS, *(ILP_FLAGS if s in ILP_SOURCES else ()), "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)]
+        for s, o in zip(SOURCES, objects)
+    ]  # fmt: skip
     with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
         done = list(pool.map(lambda cmd: subprocess.run(cmd, capture_output=True, text=True), commands))
     link = [hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", str(tmp), *map(str, objects)]

@@ -14,16 +14,15 @@ namespace gbx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlock = kStateBlock;       // 256: a wavefront, 4 elements a lane
-constexpr int kTileBlocks = 16;           // of a workgroup's tile
-constexpr int kTile = kTileBlocks * kBlock;
+constexpr int kBlock = kStateBlock;
+constexpr int kTile = 4096;  // elements of a workgroup
 
 struct Tensor {
   void* p;
   const void* g;
   int64_t n;
   uint32_t start;  // first block of its states
-  uint32_t tile;   // first tile of the launch
+  uint32_t tile;   // first tile
 };
 constexpr int kTensors = 100;  // of a launch: they travel as kernel arguments, 4 KB at most
 struct Tensors {
@@ -41,117 +40,150 @@ __device__ __forceinline__ uint32_t noise_of(uint32_t index, uint32_t key) {
   return h ^ (h >> 15);
 }
 
-// v rounded to MANTISSA bits, up with the odds of its distance from the value
-// below (16 random bits), so that a running mean moves even where each change
-// is less than half a step of the format.  LEAST: the smallest normal value.
+// `mag` >= 0 rounded to MANTISSA bits, up with the odds of its distance from the
+// value below (16 random bits), so that a running mean moves even where each
+// change is less than half a step of the format: the random bits are added
+// below the last kept bit and the rest is cut off.  Values below the smallest
+// normal one, LEAST, have the spacing of [LEAST, 2 LEAST) and are rounded there.
 template <int MANTISSA>
-__device__ __forceinline__ float round_8(float v, uint32_t noise16, float least) {
+__device__ __forceinline__ float round_8(float mag, uint32_t noise16, float least) {
   constexpr int kCut = 23 - MANTISSA;
-  const float mag = fabsf(v);
-  const uint32_t bits = __float_as_uint(mag) + (noise16 << (kCut - 16));
-  const float normal = __uint_as_float(bits & ~((1u << kCut) - 1u));
-  const float quantum = least / (float)(1 << MANTISSA), steps = mag * (1.0f / quantum), whole = floorf(steps);
-  const float small = (whole + floorf((steps - whole) + (float)noise16 * 0x1p-16f)) * quantum;
-  return copysignf(mag < least ? small : normal, v);
+  const float lift = mag < least ? least : 0.0f;
+  const uint32_t bits = __float_as_uint(mag + lift) + (noise16 << (kCut - 16));
+  return __uint_as_float(bits & ~((1u << kCut) - 1u)) - lift;
 }
 
-// Largest bit pattern (absolute values order as their bits do, NaN above all)
-// of the wavefront.
-__device__ __forceinline__ float wave_most(uint32_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
-    v = o > v ? o : v;
-  }
-  return __uint_as_float(v);
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+  return o > v ? o : v;
 }
-__device__ __forceinline__ uint32_t most4(const float (&v)[4]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-    m = b > m ? b : m;
-  }
-  return m;
+// Largest bit patterns of two values over 32 lanes (patterns of absolute values
+// order as the values do, NaN above all).  Rows of 16 lanes: the first swap
+// leaves a's in even rows and b's in odd ones, the second gives both to all.
+__device__ __forceinline__ void most_of_both(uint32_t& a, uint32_t& b) {
+  const auto folded = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  uint32_t v = folded[0] > folded[1] ? folded[0] : folded[1];
+  v = max_dpp<0x121>(max_dpp<0x122>(max_dpp<0x124>(max_dpp<0x128>(v))));  // rotated by 8, 4, 2, 1
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  a = both[0];
+  b = both[1];
 }
 constexpr float kScaleFloor = 1e-30f, kE4m3Max = 448.0f, kE5m2Max = 57344.0f;
 
-template <typename P, typename G, bool SMALL>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamArgs a, Tensors ts) {
-#pragma clang fp contract(off)  // each operation rounds, as in the formula
-  // the workgroup's tensor: the last one whose first tile is not beyond it
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// One element's update; `m` and `v` come in multiplied by beta1 and beta2.
+// Root and reciprocal are right to one unit in the last place: what they make
+// is added to a parameter many times its size.
+__device__ __forceinline__ float update(const AdamArgs& a, float p, float g, float rest1, float rest2, float& m, float& v) {
+  m = fmaf(g, rest1, m);
+  v = fmaf(g * g, rest2, v);
+  const float root = fmaf(__builtin_amdgcn_sqrtf(v), a.inv_root2, a.eps);
+  return fmaf(-m * a.step_size, rcp_fast(root), p * a.keep);
+}
+
+// The workgroup's tensor: the last one whose first tile is not beyond it.
+__device__ __forceinline__ Tensor tensor_of(const Tensors& ts) {
+  const int lane = threadIdx.x & 63;
   int which = -1;
 #pragma unroll
   for (int k = 0; k < kTensors; k += 64) {
     const bool has = k + lane < ts.count && ts.t[min(k + lane, kTensors - 1)].tile <= blockIdx.x;
     which += __popcll(__ballot(has));
   }
-  const Tensor t = ts.t[__builtin_amdgcn_readfirstlane(which)];
-  const float grad_scale = a.grad_scale ? *a.grad_scale : 1.0f;
+  return ts.t[__builtin_amdgcn_readfirstlane(which)];
+}
+
+template <typename P, typename G>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamArgs a, Tensors ts) {
+  const Tensor t = tensor_of(ts);
+  const float scale = a.grad_scale ? *a.grad_scale : 1.0f, rest1 = a.rest1 * scale, rest2 = a.rest2 * scale * scale;
   const int64_t first = (int64_t)(blockIdx.x - t.tile) * kTile;
+  float* exp_avg = (float*)a.exp_avg + (int64_t)t.start * kBlock;
+  float* exp_avg_sq = (float*)a.exp_avg_sq + (int64_t)t.start * kBlock;
 #pragma unroll
-  for (int k = 0; k < kTileBlocks / 4; ++k) {
-    const int64_t at = first + (int64_t)(k * 4 + wave) * kBlock, e = at + lane * 4;  // in the tensor
-    if (at >= t.n) return;
-    const int64_t block = t.start + at / kBlock, s = block * kBlock + lane * 4;  // in the states
-    const int valid = (int)min<int64_t>(4, max<int64_t>(0, t.n - e));
+  for (int k = 0; k < kTile / (4 * kThreads); ++k) {
+    const int64_t e = first + (k * kThreads + threadIdx.x) * 4;
+    if (e >= t.n) return;
+    const int valid = (int)min<int64_t>(4, t.n - e);
     float p[4], g[4], m[4], v[4];
     load_row<4>((const P*)t.p + e, valid, p);
     load_row<4>((const G*)t.g + e, valid, g);
-    if constexpr (SMALL) {
-      const uint32_t mq = *(const uint32_t*)((const uint8_t*)a.exp_avg + s), vq = *(const uint32_t*)((const uint8_t*)a.exp_avg_sq + s);
-      const float ms = a.exp_avg_scale[block], vs = a.exp_avg_sq_scale[block];
-      m[0] = __builtin_amdgcn_cvt_f32_fp8((int)mq, 0) * ms;
-      m[1] = __builtin_amdgcn_cvt_f32_fp8((int)mq, 1) * ms;
-      m[2] = __builtin_amdgcn_cvt_f32_fp8((int)mq, 2) * ms;
-      m[3] = __builtin_amdgcn_cvt_f32_fp8((int)mq, 3) * ms;
-      v[0] = __builtin_amdgcn_cvt_f32_bf8((int)vq, 0) * vs;
-      v[1] = __builtin_amdgcn_cvt_f32_bf8((int)vq, 1) * vs;
-      v[2] = __builtin_amdgcn_cvt_f32_bf8((int)vq, 2) * vs;
-      v[3] = __builtin_amdgcn_cvt_f32_bf8((int)vq, 3) * vs;
-    } else {
-      load_row<4>((const float*)a.exp_avg + s, 4, m);
-      load_row<4>((const float*)a.exp_avg_sq + s, 4, v);
-    }
+    load_row<4>(exp_avg + e, 4, m);
+    load_row<4>(exp_avg_sq + e, 4, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float gi = g[i] * grad_scale;
-      m[i] = m[i] * a.beta1 + gi * a.rest1;
-      v[i] = v[i] * a.beta2 + gi * gi * a.rest2;
-      // root and quotient to one unit in the last place: the update is added
-      // to a parameter many times its size
-      const float update = (m[i] * a.step_size) * rcp_fast(__builtin_amdgcn_sqrtf(v[i]) * a.inv_root2 + a.eps);
-      p[i] = p[i] * a.keep - update;
+      m[i] *= a.beta1;
+      v[i] *= a.beta2;
+      p[i] = update(a, p[i], g[i], rest1, rest2, m[i], v[i]);
     }
     store_row<4>((P*)t.p + e, valid, p);
-    if constexpr (SMALL) {
-      const float most_m = wave_most(most4(m)), most_v = wave_most(most4(v));
-      const float top_m = most_m < kScaleFloor ? kScaleFloor : most_m, top_v = most_v < kScaleFloor ? kScaleFloor : most_v;
-      const float inv_m = kE4m3Max / top_m, inv_v = kE5m2Max / top_v;
+    store_row<4>(exp_avg + e, 4, m);
+    store_row<4>(exp_avg_sq + e, 4, v);
+  }
+}
+
+// 8-bit states: 32 lanes hold a block of 256, 8 elements each.
+template <typename P, typename G>
+__global__ __launch_bounds__(kThreads) void adamw_8_kernel(AdamArgs a, Tensors ts) {
+  const Tensor t = tensor_of(ts);
+  const float scale = a.grad_scale ? *a.grad_scale : 1.0f, rest1 = a.rest1 * scale, rest2 = a.rest2 * scale * scale;
+  const int64_t first = (int64_t)(blockIdx.x - t.tile) * kTile;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t noise = noise_of((uint32_t)(s + i), a.key);
-        float x = m[i] * inv_m, y = v[i] * inv_v;
-        x = fabsf(x) > kE4m3Max ? copysignf(kE4m3Max, x) : x;
-        y = y > kE5m2Max ? kE5m2Max : y;
-        m[i] = round_8<3>(x, noise & 0xFFFFu, 0x1p-6f);
-        const float q = round_8<2>(y, noise >> 16, 0x1p-14f);
-        v[i] = y > 0.0f && q < 0x1p-16f ? 0x1p-16f : q;  // a second moment that is not zero stays so
+  for (int k = 0; k < kTile / (8 * kThreads); ++k) {
+    const int64_t e = first + (k * kThreads + threadIdx.x) * 8;  // in the tensor
+    if (e / kBlock * kBlock >= t.n) return;                      // all 32 lanes of a block together
+    const int64_t block = t.start + e / kBlock, s = (int64_t)t.start * kBlock + e;
+    const int valid = (int)min<int64_t>(8, max<int64_t>(0, t.n - e));
+    float p[8], g[8], m[8], v[8];
+    load_row<8>((const P*)t.p + e, valid, p);
+    load_row<8>((const G*)t.g + e, valid, g);
+    const uint2 mq = *(const uint2*)((const uint8_t*)a.exp_avg + s), vq = *(const uint2*)((const uint8_t*)a.exp_avg_sq + s);
+    const float ms = a.exp_avg_scale[block] * a.beta1, vs = a.exp_avg_sq_scale[block] * a.beta2;
+    auto widen = [](uint32_t q, float by, float* to, auto bf8) {
+      if constexpr (bf8.value) {
+        to[0] = __builtin_amdgcn_cvt_f32_bf8((int)q, 0) * by, to[1] = __builtin_amdgcn_cvt_f32_bf8((int)q, 1) * by;
+        to[2] = __builtin_amdgcn_cvt_f32_bf8((int)q, 2) * by, to[3] = __builtin_amdgcn_cvt_f32_bf8((int)q, 3) * by;
+      } else {
+        to[0] = __builtin_amdgcn_cvt_f32_fp8((int)q, 0) * by, to[1] = __builtin_amdgcn_cvt_f32_fp8((int)q, 1) * by;
+        to[2] = __builtin_amdgcn_cvt_f32_fp8((int)q, 2) * by, to[3] = __builtin_amdgcn_cvt_f32_fp8((int)q, 3) * by;
       }
-      int mq = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false);
-      mq = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], mq, true);
-      int vq = __builtin_amdgcn_cvt_pk_bf8_f32(v[0], v[1], 0, false);
-      vq = __builtin_amdgcn_cvt_pk_bf8_f32(v[2], v[3], vq, true);
-      *(uint32_t*)((uint8_t*)a.exp_avg + s) = (uint32_t)mq;
-      *(uint32_t*)((uint8_t*)a.exp_avg_sq + s) = (uint32_t)vq;
-      if (lane == 0) {
-        a.exp_avg_scale[block] = top_m / kE4m3Max;
-        a.exp_avg_sq_scale[block] = top_v / kE5m2Max;
-      }
-    } else {
-      store_row<4>((float*)a.exp_avg + s, 4, m);
-      store_row<4>((float*)a.exp_avg_sq + s, 4, v);
+    };
+    widen(mq.x, ms, m, std::false_type{});
+    widen(mq.y, ms, m + 4, std::false_type{});
+    widen(vq.x, vs, v, std::true_type{});
+    widen(vq.y, vs, v + 4, std::true_type{});
+    uint32_t most_m = 0, most_v = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = update(a, p[i], g[i], rest1, rest2, m[i], v[i]);
+      const uint32_t bm = __float_as_uint(m[i]) & 0x7FFFFFFFu, bv = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+      most_m = bm > most_m ? bm : most_m;
+      most_v = bv > most_v ? bv : most_v;
+    }
+    store_row<8>((P*)t.p + e, valid, p);
+    most_of_both(most_m, most_v);
+    const float fm = __uint_as_float(most_m), fv = __uint_as_float(most_v);
+    const float top_m = fm < kScaleFloor ? kScaleFloor : fm, top_v = fv < kScaleFloor ? kScaleFloor : fv;
+    // (a unit or two above the formats' largest values is cut off below)
+    const float inv_m = kE4m3Max * rcp_fast(top_m), inv_v = kE5m2Max * rcp_fast(top_v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t noise = noise_of((uint32_t)s + i, a.key);
+      m[i] *= inv_m;
+      v[i] *= inv_v;
+      m[i] = copysignf(round_8<3>(fabsf(m[i]), noise & 0xFFFFu, 0x1p-6f), m[i]);
+      const float q = round_8<2>(v[i], noise >> 16, 0x1p-14f);
+      v[i] = v[i] > 0.0f ? fmaxf(q, 0x1p-16f) : q;  // a second moment that is not zero stays so
+    }
+    auto narrow = [](const float* v, auto bf8) {
+      if constexpr (bf8.value) return (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(v[2], v[3], __builtin_amdgcn_cvt_pk_bf8_f32(v[0], v[1], 0, false), true);
+      else return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), true);
+    };
+    *(uint2*)((uint8_t*)a.exp_avg + s) = uint2{narrow(m, std::false_type{}), narrow(m + 4, std::false_type{})};
+    *(uint2*)((uint8_t*)a.exp_avg_sq + s) = uint2{narrow(v, std::true_type{}), narrow(v + 4, std::true_type{})};
+    if ((threadIdx.x & 31u) == 0u) {
+      a.exp_avg_scale[block] = top_m * (1.0f / kE4m3Max);
+      a.exp_avg_sq_scale[block] = top_v * (1.0f / kE5m2Max);
     }
   }
 }
@@ -176,8 +208,8 @@ hipError_t launch_adamw(const AdamArgs& a, hipStream_t st) {
       using P = decltype(p);
       auto go = [&](auto g) {
         using G = decltype(g);
-        if (a.small) hipLaunchKernelGGL((adamw_kernel<P, G, true>), grid, block, 0, st, a, ts);
-        else hipLaunchKernelGGL((adamw_kernel<P, G, false>), grid, block, 0, st, a, ts);
+        if (a.small) hipLaunchKernelGGL((adamw_8_kernel<P, G>), grid, block, 0, st, a, ts);
+        else hipLaunchKernelGGL((adamw_kernel<P, G>), grid, block, 0, st, a, ts);
       };
       if (a.grad_elem == a.elem) go(P{});
       else go(float{});

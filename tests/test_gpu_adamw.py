@@ -69,8 +69,9 @@ def _round_8(t, noise16, mantissa, least, kind):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_8_bit_states(dtype):
-    """Every operation is rounded as in torch on the CPU, so the states agree
-    but for values a rounding away from where they turn: fewer than 1 in 1,000."""
+    """The same rounding of the same numbers, which differ by a few units in the
+    last place of 32 bits: the states agree but for values that near to where
+    they turn, fewer than 1 in 1,000."""
     from gbxcule_amd.rl import AdamW
 
     gen = torch.Generator(device="cuda").manual_seed(2)
