@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamArgs a, Tensors ts)
   for (int k = 0; k < kTile / (4 * kThreads); ++k) {
     const int64_t e = first + (k * kThreads + threadIdx.x) * 4;
     if (e >= t.n) return;
-    const int valid = (int)min<int64_t>(4, t.n - e);
+    const int valid = (int)least(4, t.n - e);
     float p[4], g[4], m[4], v[4];
     load_row<4>((const P*)t.p + e, valid, p);
     load_row<4>((const G*)t.g + e, valid, g);
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void adamw_8_kernel(AdamArgs a, Tensors t
     const int64_t e = first + (k * kThreads + threadIdx.x) * 8;  // in the tensor
     if (e / kBlock * kBlock >= t.n) return;                      // all 32 lanes of a block together
     const int64_t block = t.start + e / kBlock, s = (int64_t)t.start * kBlock + e;
-    const int valid = (int)min<int64_t>(8, max<int64_t>(0, t.n - e));
+    const int valid = t.n > e ? (int)least(8, t.n - e) : 0;
     float p[8], g[8], m[8], v[8];
     load_row<8>((const P*)t.p + e, valid, p);
     load_row<8>((const G*)t.g + e, valid, g);

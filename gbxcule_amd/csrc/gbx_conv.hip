@@ -24,7 +24,7 @@ constexpr int64_t kBusy = 256 * 2048 * 8;
 // by 256 / lanes rows; a row is one env and one piece of the steps.
 struct Shape {
   int groups, shift, chunk, chunks;  // groups of channels; log2 of lanes in a row; steps of a piece, pieces
-  int64_t rows;
+  uint32_t rows;                     // below 2^28: only rows of few lanes are cut
 };
 Shape shape_of(int steps, int envs, int dim, int v) {
   Shape s;
@@ -34,7 +34,7 @@ Shape shape_of(int steps, int envs, int dim, int v) {
   const int64_t want = std::max<int64_t>(1, kBusy / ((int64_t)envs * s.groups * v));
   s.chunk = (int)std::max<int64_t>(kMinSteps, (steps + want - 1) / want);
   s.chunks = (steps + s.chunk - 1) / s.chunk;
-  s.rows = (int64_t)envs * s.chunks;
+  s.rows = (uint32_t)((int64_t)envs * s.chunks);
   return s;
 }
 
@@ -136,9 +136,9 @@ constexpr int kForward = 8, kBackward = 4;  // channels of a lane: 16 or 8 bytes
 // A row's place: its first channel group's lane, env and piece of the steps.
 // WIDE: a wavefront is one row, and what depends on the row alone is scalar.
 template <bool WIDE>
-__device__ __forceinline__ int64_t row_of(const Shape& s) {
+__device__ __forceinline__ uint32_t row_of(const Shape& s) {
   const int in = threadIdx.x >> s.shift;
-  return (int64_t)blockIdx.x * (kThreads >> s.shift) + (WIDE ? __builtin_amdgcn_readfirstlane(in) : in);
+  return blockIdx.x * (kThreads >> s.shift) + (WIDE ? __builtin_amdgcn_readfirstlane(in) : in);
 }
 
 template <typename T, int W, bool WHOLE, bool WIDE>
@@ -146,9 +146,9 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
   constexpr int V = kForward, kAhead = 4;  // steps whose loads are in flight while four others are worked on
   const int lanes = 1 << s.shift;
   const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
-  const int64_t row = row_of<WIDE>(s);
+  const uint32_t row = row_of<WIDE>(s);
   if (group >= s.groups || row >= s.rows) return;
-  const int env = (int)(row % a.envs), part = (int)(row / a.envs);
+  const int env = (int)(row % (uint32_t)a.envs), part = (int)(row / (uint32_t)a.envs);
   const int c = group * V, n = a.dim - c;
   const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
   const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env;
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
   __shared__ float tile[kThreads][V];
   const int lanes = 1 << s.shift;
   const int group = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
-  const int64_t row = row_of<WIDE>(s);
+  const uint32_t row = row_of<WIDE>(s);
   const int c = group * V, n = a.dim - c;
   float dw[W][V], db[V];
 #pragma unroll
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
     for (int j = 0; j < W; ++j) dw[j][k] = 0.0f;
   }
   if (group < s.groups && row < s.rows) {
-    const int env = (int)(row % a.envs), part = (int)(row / a.envs);
+    const int env = (int)(row % (uint32_t)a.envs), part = (int)(row / (uint32_t)a.envs);
     const int t0 = part * s.chunk, t1 = min(t0 + s.chunk, a.steps);
     const T* x = (const T*)a.x + (int64_t)t0 * a.x_step + (int64_t)env * a.x_env;
     const T* dy = (const T*)a.dy + (int64_t)t0 * a.dy_step + (int64_t)env * a.dy_env;
@@ -344,30 +344,43 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(ConvArgs a, Shape s
 }
 
 // One step of every env: reads the state once and writes it moved on.
-template <typename T, int W>
-__global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a, int pieces) {
-  constexpr int kVec = kForward;
-  const int64_t i = block_id() * kThreads + threadIdx.x;
-  const int64_t env = i / pieces;
-  const int c = (int)(i % pieces) * kVec, n = a.dim - c;
-  if (env >= a.envs) return;
-  const bool begins = a.resets && a.resets[env];
-  T* state = (T*)a.last + env * (W - 1) * a.dim + c;
-  float w[W][kVec], bias[kVec], win[W - 1][kVec], in[kVec], out[kVec];
+template <typename T, int W, int EACH, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a) {
+  constexpr int V = kForward;
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V, n = a.dim - c;
+  const int64_t env0 = first_env<EACH>();
+  if (env0 >= a.envs || n <= 0) return;
+  Packed<T, V> in[EACH], past[EACH][W - 1];
+  uint8_t begins[EACH];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) load_row<kVec>(state + (int64_t)j * a.dim, n, win[j]);
-  load_row<kVec>((const T*)a.x + env * a.x_env + c, n, in);
+  for (int e = 0; e < EACH; ++e) {
+    const int64_t env = least(env0 + e * blockDim.y, a.envs - 1);
+    const T* state = (const T*)a.last + env * (W - 1) * a.dim + c;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) fetch_row<WHOLE>(state + (int64_t)j * a.dim, n, past[e][j]);
+    fetch_row<WHOLE>((const T*)a.x + env * a.x_env + c, n, in[e]);
+    begins[e] = a.resets ? a.resets[env] : 0;
+  }
+  float w[W][V], bias[V];
   load_weights<W>(a, c, w, bias);
 #pragma unroll
-  for (int k = 0; k < kVec; ++k) {
+  for (int e = 0; e < EACH; ++e) {
+    const int64_t env = env0 + e * blockDim.y;
+    if (env >= a.envs) break;
+    T* state = (T*)a.last + env * (W - 1) * a.dim + c;
+    float win[W - 1][V], x[V], out[V];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) win[j][k] = begins ? 0.0f : win[j][k];
-    const float pre = convolve<W, kVec>(w, win, in[k], bias[k], k);
-    out[k] = a.silu ? pre * sigmoid(pre) : pre;
+    for (int k = 0; k < V; ++k) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) win[j][k] = begins[e] ? 0.0f : (float)past[e][j].v[k];
+      x[k] = (float)in[e].v[k];
+      const float pre = convolve<W, V>(w, win, x[k], bias[k], k);
+      out[k] = a.silu ? pre * sigmoid(pre) : pre;
+    }
+    store_row<V>((T*)a.y + env * a.dim + c, WHOLE ? V : n, out);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) store_row<V>(state + (int64_t)j * a.dim, WHOLE ? V : n, j + 1 < W - 1 ? win[j + 1 < W - 1 ? j + 1 : 0] : x);
   }
-  store_row<kVec>((T*)a.y + env * a.dim + c, n, out);
-#pragma unroll
-  for (int j = 0; j < W - 1; ++j) store_row<kVec>(state + (int64_t)j * a.dim, n, j + 1 < W - 1 ? win[j + 1 < W - 1 ? j + 1 : 0] : in);
 }
 
 template <typename F>
@@ -421,10 +434,16 @@ hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_conv_step(const ConvArgs& a, hipStream_t st) {
-  const int pieces = (a.dim + kForward - 1) / kForward;
-  const dim3 grid = wide_grid(((int64_t)a.envs * pieces + kThreads - 1) / kThreads);
+  const StepShape s = step_shape((a.dim + kForward - 1) / kForward, a.envs);
   by_element(a.elem, [&](auto t) {
-    by_width(a.width, [&](auto w) { hipLaunchKernelGGL((conv_step_kernel<decltype(t), w>), grid, dim3(kThreads), 0, st, a, pieces); });
+    using T = decltype(t);
+    by_width(a.width, [&](auto w) {
+      const bool whole = a.dim % kForward == 0;
+      if (s.each == 4 && whole) hipLaunchKernelGGL((conv_step_kernel<T, w, 4, true>), s.grid(), s.block(), 0, st, a);
+      else if (s.each == 4) hipLaunchKernelGGL((conv_step_kernel<T, w, 4, false>), s.grid(), s.block(), 0, st, a);
+      else if (whole) hipLaunchKernelGGL((conv_step_kernel<T, w, 1, true>), s.grid(), s.block(), 0, st, a);
+      else hipLaunchKernelGGL((conv_step_kernel<T, w, 1, false>), s.grid(), s.block(), 0, st, a);
+    });
   });
   return hipGetLastError();
 }

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float
   const int d = (int)(i % a.dim), s = (int)(i / a.dim % a.states), env = (int)(i / a.dim / a.states);
   const float decay = a.a[(int64_t)d * a.states + s] * kLog2e;
   float h = !BACKWARD && a.state ? a.state[((int64_t)env * a.dim + d) * a.states + s] : 0.0f;
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 16;  // pieces whose loads are in flight together
   for (int k0 = 0; k0 < chunks; k0 += kAhead) {
     float e[kAhead], sum[kAhead];
 #pragma unroll
@@ -603,66 +603,78 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, co
 
 // One step of every env: the state is read and written once and bounds the
 // kernel.  LANES lanes share a channel, 4 states (16 bytes) each.
-template <typename T, int LANES>
+template <typename T, int LANES, int EACH>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
-  const int64_t i = block_id() * 256 + threadIdx.x, row = i / LANES;
-  if (row >= (int64_t)a.envs * a.dim) return;
-  const int part = (int)(i % LANES), d = (int)(row % a.dim), env = (int)(row / a.dim), group = d / (a.dim / a.groups);
-  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group + part * 4;
-  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group + part * 4;
-  float4* hp = reinterpret_cast<float4*>(a.last) + i;
-  const bool begins = a.resets && a.resets[env];
-  float4 h = *hp;
-  const float4 decay = reinterpret_cast<const float4*>(a.a)[d * LANES + part];
-  float bv[4], cv[4];
-  load_row<4>(b, 4, bv);
-  load_row<4>(c, 4, cv);
-  const float x = (float)((const T*)a.x)[(int64_t)env * a.x_env + d];
-  float delta = (float)((const T*)a.dt)[(int64_t)env * a.dt_env + d] + (a.bias ? a.bias[d] : 0.0f);
-  if (a.softplus) delta = softplus(delta);
-  if (begins) h = float4{0.0f, 0.0f, 0.0f, 0.0f};
-  const float u = delta * x, scaled = delta * kLog2e;
-  h.x = fmaf(h.x, exp2_fast(scaled * decay.x), u * bv[0]);
-  h.y = fmaf(h.y, exp2_fast(scaled * decay.y), u * bv[1]);
-  h.z = fmaf(h.z, exp2_fast(scaled * decay.z), u * bv[2]);
-  h.w = fmaf(h.w, exp2_fast(scaled * decay.w), u * bv[3]);
-  *hp = h;
-  float out = fmaf(h.x, cv[0], h.y * cv[1]) + fmaf(h.z, cv[2], h.w * cv[3]);
+  const int i = blockIdx.x * blockDim.x + threadIdx.x, d = i / LANES, part = i % LANES;
+  const int64_t env0 = first_env<EACH>();
+  if (env0 >= a.envs || d >= a.dim) return;
+  const int group = a.groups == 1 ? 0 : d / (a.dim / a.groups);
+  const T* b = (const T*)a.b + group * a.b_group + part * 4;
+  const T* c = (const T*)a.c + group * a.c_group + part * 4;
+  float4 h[EACH];
+  float bv[EACH][4], cv[EACH][4];
+  T x[EACH], dt[EACH], z[EACH];
+  uint8_t begins[EACH];
 #pragma unroll
-  for (int k = 1; k < LANES; k <<= 1) out += __shfl_xor(out, k, 64);
-  if (part == 0) {
-    if (a.skip) out = fmaf(a.skip[d], x, out);
-    if (a.z) {
-      const float zv = (float)((const T*)a.z)[(int64_t)env * a.z_env + d];
-      out *= zv * sigmoid(zv);
-    }
-    ((T*)a.y)[row] = (T)out;
+  for (int k = 0; k < EACH; ++k) {
+    const int64_t env = least(env0 + k * blockDim.y, a.envs - 1);
+    h[k] = reinterpret_cast<const float4*>(a.last)[env * a.dim * LANES + i];
+    load_row<4>(b + env * a.b_env, 4, bv[k]);
+    load_row<4>(c + env * a.c_env, 4, cv[k]);
+    x[k] = ((const T*)a.x)[env * a.x_env + d];
+    dt[k] = ((const T*)a.dt)[env * a.dt_env + d];
+    z[k] = a.z ? ((const T*)a.z)[env * a.z_env + d] : (T)0.0f;
+    begins[k] = a.resets ? a.resets[env] : 0;
+  }
+  const float4 decay = reinterpret_cast<const float4*>(a.a)[i];
+  const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int64_t env = env0 + k * blockDim.y;
+    float delta = (float)dt[k] + bias;
+    if (a.softplus) delta = softplus(delta);
+    if (begins[k]) h[k] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float u = delta * (float)x[k], scaled = delta * kLog2e;
+    h[k].x = fmaf(h[k].x, exp2_fast(scaled * decay.x), u * bv[k][0]);
+    h[k].y = fmaf(h[k].y, exp2_fast(scaled * decay.y), u * bv[k][1]);
+    h[k].z = fmaf(h[k].z, exp2_fast(scaled * decay.z), u * bv[k][2]);
+    h[k].w = fmaf(h[k].w, exp2_fast(scaled * decay.w), u * bv[k][3]);
+    float out = fmaf(h[k].x, cv[k][0], h[k].y * cv[k][1]) + fmaf(h[k].z, cv[k][2], h[k].w * cv[k][3]);
+    if constexpr (LANES > 1) out = add_dpp<0xB1>(out);
+    if constexpr (LANES > 2) out = add_dpp<0x4E>(out);
+    if constexpr (LANES > 4) out += __shfl_xor(out, 4, 64);
+    if (env >= a.envs) break;
+    reinterpret_cast<float4*>(a.last)[env * a.dim * LANES + i] = h[k];
+    out = fmaf(skip, (float)x[k], out);
+    if (a.z) out *= (float)z[k] * sigmoid((float)z[k]);
+    if (part == 0) ((T*)a.y)[env * a.dim + d] = (T)out;
   }
 }
 // Any number of states: a lane a channel.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_step_any_kernel(ScanArgs a) {
-  const int64_t row = block_id() * 256 + threadIdx.x;
-  if (row >= (int64_t)a.envs * a.dim) return;
-  const int d = (int)(row % a.dim), env = (int)(row / a.dim), group = d / (a.dim / a.groups);
-  const T* b = (const T*)a.b + (int64_t)env * a.b_env + (int64_t)group * a.b_group;
-  const T* c = (const T*)a.c + (int64_t)env * a.c_env + (int64_t)group * a.c_group;
+  const int64_t env = first_env<1>();
+  const int d = blockIdx.x * blockDim.x + threadIdx.x;
+  if (env >= a.envs || d >= a.dim) return;
+  const int group = a.groups == 1 ? 0 : d / (a.dim / a.groups);
+  const T* b = (const T*)a.b + env * a.b_env + group * a.b_group;
+  const T* c = (const T*)a.c + env * a.c_env + group * a.c_group;
   const bool begins = a.resets && a.resets[env];
-  const float x = (float)((const T*)a.x)[(int64_t)env * a.x_env + d];
-  float delta = (float)((const T*)a.dt)[(int64_t)env * a.dt_env + d] + (a.bias ? a.bias[d] : 0.0f);
+  const float x = (float)((const T*)a.x)[env * a.x_env + d];
+  float delta = (float)((const T*)a.dt)[env * a.dt_env + d] + (a.bias ? a.bias[d] : 0.0f);
   if (a.softplus) delta = softplus(delta);
   float out = a.skip ? a.skip[d] * x : 0.0f;
+  float* hp = a.last + (env * a.dim + d) * a.states;
   for (int s = 0; s < a.states; ++s) {
-    float* hp = a.last + row * a.states + s;
-    const float h = fmaf(begins ? 0.0f : *hp, exp2_fast(delta * kLog2e * a.a[(int64_t)d * a.states + s]), delta * x * (float)b[s]);
-    *hp = h;
+    const float h = fmaf(begins ? 0.0f : hp[s], exp2_fast(delta * kLog2e * a.a[(int64_t)d * a.states + s]), delta * x * (float)b[s]);
+    hp[s] = h;
     out = fmaf(h, (float)c[s], out);
   }
   if (a.z) {
-    const float zv = (float)((const T*)a.z)[(int64_t)env * a.z_env + d];
+    const float zv = (float)((const T*)a.z)[env * a.z_env + d];
     out *= zv * sigmoid(zv);
   }
-  ((T*)a.y)[row] = (T)out;
+  ((T*)a.y)[env * a.dim + d] = (T)out;
 }
 
 template <typename F>
@@ -778,15 +790,24 @@ hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st) {
-  const int64_t channels = (int64_t)a.envs * a.dim;
-  const auto grid = [](int64_t n) { return wide_grid((n + 255) / 256); };
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
-    if (a.states == 4) hipLaunchKernelGGL((scan_step_kernel<T, 1>), grid(channels), dim3(256), 0, st, a);
-    else if (a.states == 8) hipLaunchKernelGGL((scan_step_kernel<T, 2>), grid(channels * 2), dim3(256), 0, st, a);
-    else if (a.states == 16) hipLaunchKernelGGL((scan_step_kernel<T, 4>), grid(channels * 4), dim3(256), 0, st, a);
-    else if (a.states == 32) hipLaunchKernelGGL((scan_step_kernel<T, 8>), grid(channels * 8), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((scan_step_any_kernel<T>), grid(channels), dim3(256), 0, st, a);
+    auto go = [&](auto lanes) {
+      const StepShape s = step_shape((int64_t)a.dim * lanes, a.envs);
+      if (s.each == 4) hipLaunchKernelGGL((scan_step_kernel<T, lanes, 4>), s.grid(), s.block(), 0, st, a);
+      else hipLaunchKernelGGL((scan_step_kernel<T, lanes, 1>), s.grid(), s.block(), 0, st, a);
+    };
+    if (a.states == 4) go(std::integral_constant<int, 1>{});
+    else if (a.states == 8) go(std::integral_constant<int, 2>{});
+    else if (a.states == 16) go(std::integral_constant<int, 4>{});
+    else if (a.states == 32) go(std::integral_constant<int, 8>{});
+    else {
+      StepShape s = step_shape(a.dim, 1);
+      const int64_t blocks = ((int64_t)a.envs + s.rows - 1) / s.rows;
+      s.grid_.y = (unsigned)std::min<int64_t>(blocks, kEnvRow);
+      s.grid_.z = (unsigned)((blocks + kEnvRow - 1) / kEnvRow);
+      hipLaunchKernelGGL(scan_step_any_kernel<T>, s.grid(), s.block(), 0, st, a);
+    }
   });
   return hipGetLastError();
 }
