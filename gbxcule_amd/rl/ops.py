@@ -50,7 +50,7 @@ def _elem(name: str, t: torch.Tensor) -> int:
 
 def _like(name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple[int, ...]) -> torch.Tensor:
     """``t`` of ``like``'s type and device and the given shape, last dimension contiguous."""
-    if t.dtype is not like.dtype or t.device != like.device:
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -65,17 +65,19 @@ def _param(name: str, t: torch.Tensor | None, like: torch.Tensor, shape: tuple[i
     """A parameter in 32 bits (the cast is differentiable), contiguous."""
     if t is None:
         return None
-    if t.device != like.device or not t.is_floating_point():
+    if t.get_device() != like.get_device() or not t.is_floating_point():
         raise ValueError(f"{name}: expected a floating-point tensor on {like.device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    return (t if t.dtype is torch.float32 else t.float()).contiguous()
+    if t.dtype is not torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _resets(t: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...]) -> torch.Tensor | None:
     if t is None:
         return None
-    if t.dtype not in (torch.bool, torch.uint8) or t.device != like.device:
+    if t.dtype not in (torch.bool, torch.uint8) or t.get_device() != like.get_device():
         raise ValueError(f"resets: expected bool or uint8 on {like.device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"resets: expected shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -417,7 +419,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, *, dt_bias=None, softplus: bo
 
 
 def _scan_state(state, x, shape):
-    if state.dtype is not torch.float32 or state.device != x.device or state.shape != shape:
+    if state.dtype is not torch.float32 or state.get_device() != x.get_device() or state.shape != shape:
         raise ValueError(f"state: expected float32 {shape} on {x.device}, got {state.dtype} {tuple(state.shape)} on {state.device}")
     return state
 

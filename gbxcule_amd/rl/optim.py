@@ -26,10 +26,6 @@ STATE_BLOCK = 256
 _GOLDEN = 0x9E3779B9
 
 
-def _address(a: array) -> int:
-    return a.buffer_info()[0]
-
-
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with one pass over the data.
 
@@ -48,7 +44,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         self.state_bits, self.seed = int(state_bits), int(seed)
         self._flat: list[dict[str, torch.Tensor]] = []
+        # by parameter group: where each tensor's states start, its elements, its state
         self._starts: list[list[int]] = []
+        self._sizes: list[list[int]] = []
+        self._states: list[list[dict]] = []
         super().__init__(params, {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay})
 
     def add_param_group(self, param_group) -> None:
@@ -79,8 +78,9 @@ class AdamW(torch.optim.Optimizer):
                 flat[key + "_scale"] = torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=device)
         self._flat.append(flat)
         self._starts.append(starts)
-        for p, at in zip(params, starts):
-            state = self.state[p]
+        self._sizes.append([p.numel() for p in params])
+        self._states.append([self.state[p] for p in params])
+        for p, at, state in zip(params, starts, self._states[-1]):
             state["step"] = 0
             for key, t in flat.items():
                 if key.endswith("_scale"):
@@ -134,7 +134,6 @@ class AdamW(torch.optim.Optimizer):
             g.update({k: v for k, v in s.items() if k != "params"})
         self.seed = int(state_dict["seed"])
 
-    @torch.no_grad()
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
         """One update of every parameter that has a gradient.  ``grad_scale``
         (float32, one element, on the device) multiplies the gradients, such as
@@ -150,46 +149,47 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, g: int, group, grad_scale) -> None:
-        # tensors that one launch can take together: same types, same count of steps
-        batches: dict[tuple, tuple[list, list, list, list]] = {}
-        for p, start in zip(group["params"], self._starts[g]):
-            grad = p.grad
-            if grad is None:
-                continue
-            if grad.is_sparse or (grad.dtype is not p.dtype and grad.dtype is not torch.float32) or grad.device != p.device:
-                raise ValueError(f"a gradient of {grad.dtype} on {grad.device} does not go with {p.dtype} on {p.device}")
-            if not p.is_contiguous():
-                raise ValueError("a parameter is no longer contiguous")
-            if not grad.is_contiguous():
-                grad = grad.contiguous()
-            key = (p.dtype, grad.dtype, self.state[p]["step"])
-            batch = batches.get(key)
-            if batch is None:
-                batch = batches[key] = ([], [], [], [])
-            batch[0].append(p)
-            batch[1].append(grad)
-            batch[2].append(p.numel())
-            batch[3].append(start)
-        if not batches:
-            return
+        params, sizes = group["params"], self._sizes[g]
+        device = self._flat[g]["exp_avg"].get_device()
+        if [p.numel() for p in params] != sizes or not all(p.is_contiguous() and p.get_device() == device for p in params):
+            raise ValueError("a parameter has another size, layout or device than when the optimizer was made")
         if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
-                                       or grad_scale.device != group["params"][0].device):  # fmt: skip
+                                       or grad_scale.get_device() != device):  # fmt: skip
             raise ValueError("grad_scale must be one float32 element on the parameters' device")
-        flat, (b1, b2) = self._flat[g], group["betas"]
-        lr = float(group["lr"])
-        for (kind, grad_kind, done), (params, grads, sizes, starts) in batches.items():
-            step = done + 1
-            tables = (array("Q", [p.data_ptr() for p in params]), array("Q", [t.data_ptr() for t in grads]),
-                      array("q", sizes), array("q", starts))  # fmt: skip
-            scales = (flat[k].data_ptr() if k in flat else None for k in ("exp_avg_scale", "exp_avg_sq_scale"))
-            given = _lib.AdamwIn(
-                len(params), _ELEM[kind], _ELEM[grad_kind], self.state_bits, *(_address(t) for t in tables),
-                flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), *scales,
-                None if grad_scale is None else grad_scale.data_ptr(), b1, b2, lr / (1 - b1**step),
-                1.0 / math.sqrt(1 - b2**step), group["eps"], 1 - lr * group["weight_decay"],
-                (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
-            )  # fmt: skip
-            _call("gbx_adamw", params[0], given)
-            torch.autograd.graph.increment_version(params)
-            for p in params:
-                self.state[p]["step"] = step
+        grads, states = [p.grad for p in params], self._states[g]
+        kind, done = params[0].dtype, states[0]["step"]
+        if all(t is not None and t.dtype is kind and p.dtype is kind and not t.is_sparse and s["step"] == done
+               for p, t, s in zip(params, grads, states)):  # fmt: skip
+            self._launch(g, group, grad_scale, params, grads, sizes, self._starts[g], states)
+            return
+        # tensors that a launch can take together: same types, same count of steps
+        batches: dict[tuple, tuple[list, ...]] = {}
+        for p, t, s, size, start in zip(params, grads, states, sizes, self._starts[g]):
+            if t is None:
+                continue
+            if t.is_sparse or p.dtype not in _ELEM or t.dtype not in (p.dtype, torch.float32):
+                raise ValueError(f"a {'sparse ' if t.is_sparse else ''}gradient of {t.dtype} does not go with {p.dtype}")
+            batch = batches.setdefault((p.dtype, t.dtype, s["step"]), ([], [], [], [], []))
+            for to, v in zip(batch, (p, t, size, start, s)):
+                to.append(v)
+        for batch in batches.values():
+            self._launch(g, group, grad_scale, *batch)
+
+    def _launch(self, g, group, grad_scale, params, grads, sizes, starts, states) -> None:
+        grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
+        step, flat, lr = states[0]["step"] + 1, self._flat[g], float(group["lr"])
+        b1, b2 = group["betas"]
+        tables = (array("Q", [p.data_ptr() for p in params]), array("Q", [t.data_ptr() for t in grads]),
+                  array("q", sizes), array("q", starts))  # fmt: skip
+        scales = (flat["exp_avg_scale"].data_ptr(), flat["exp_avg_sq_scale"].data_ptr()) if self.state_bits == 8 else (None, None)
+        given = _lib.AdamwIn(
+            len(params), _ELEM[params[0].dtype], _ELEM[grads[0].dtype], self.state_bits,
+            *[t.buffer_info()[0] for t in tables], flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), *scales,
+            None if grad_scale is None else grad_scale.data_ptr(), b1, b2, lr / (1 - b1**step),
+            1.0 / math.sqrt(1 - b2**step), group["eps"], 1 - lr * group["weight_decay"],
+            (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
+        )  # fmt: skip
+        _call("gbx_adamw", params[0], given)
+        torch.autograd.graph.increment_version(params)
+        for s in states:
+            s["step"] = step
