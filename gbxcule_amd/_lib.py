@@ -39,8 +39,6 @@ BUF_MEM, BUF_PIX, BUF_PIX_PACKED, BUF_OBS, BUF_REWARD, BUF_ACTIONS, BUF_CART_RAM
     INFO_STEP_WAVES,
 ) = range(12)
 
-F32, BF16, F16 = range(3)
-
 _vp, _i32, _i64, _f32, _f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 

@@ -1,4 +1,5 @@
-"""Build the HIP shared library ``gbxcule_amd/lib/libgbx_hip.so`` for gfx950.
+"""Build the HIP shared library ``gbxcule_amd/lib/libgbx_hip.so`` for gfx950 and
+``gbxcule_amd/lib/gbx_torch.so``, the binding of its policy operators to torch.
 
 ``hipcc`` cross-compiles for gfx950 without a GPU present.  All HIP sources are
 compiled with packed FP32 instructions disabled (``-packed-fp32-ops``).
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -17,6 +19,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libgbx_hip.so"
+EXT_PATH = LIB_DIR / "gbx_torch.so"
+EXT_SOURCE = "gbx_torch.cpp"
 SOURCES = (
     "gbx_step.hip", "gbx_aux.hip", "gbx_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_adamw.hip", "gbx_api.hip",
 )  # fmt: skip
@@ -45,32 +49,54 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found; the HIP library cannot be built")
 
 
-def build(verbose: bool = False) -> Path:
-    """Compile every HIP source and link the shared library (always rebuilds).
-    The sources compile side by side."""
-    LIB_DIR.mkdir(exist_ok=True)
-    tmp = LIB_DIR / "libgbx_hip.so.tmp"
-    include = ["-I", str(PKG.parent / "include")]
-    objects = [LIB_DIR / f"{Path(s).stem}.o" for s in SOURCES]
-    commands = [
-        [hipcc(), *DEVICE_FLAGS, *(ILP_FLAGS if s in ILP_SOURCES else ()), "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)]
-        for s, o in zip(SOURCES, objects)
+def _extension_command(out: Path) -> list[str]:
+    """Host code only: g++ against torch's headers and libraries."""
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    system = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
+    return [
+        shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        "-DTORCH_EXTENSION_NAME=gbx_torch", "-I", str(PKG.parent / "include"),
+        *[flag for path in system for flag in ("-isystem", path)], str(CSRC / EXT_SOURCE), "-o", str(out),
+        "-L", str(lib), "-L", str(LIB_DIR), "-lgbx_hip", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python",
+        "-Wl,-rpath,$ORIGIN",
     ]  # fmt: skip
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+
+
+def _run(commands: list[list[str]], verbose: bool) -> None:
+    """The commands side by side; the first that fails is reported."""
+    with ThreadPoolExecutor(max_workers=len(commands)) as pool:
         done = list(pool.map(lambda cmd: subprocess.run(cmd, capture_output=True, text=True), commands))
-    link = [hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", str(tmp), *map(str, objects)]
-    if all(res.returncode == 0 for res in done):
-        commands.append(link)
-        done.append(subprocess.run(link, capture_output=True, text=True))
     for cmd, res in zip(commands, done):
         if verbose:
             print(" ".join(cmd), flush=True)
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
-            raise RuntimeError(f"hipcc failed: {cmd[-3]}" if cmd is not link else "hipcc failed linking libgbx_hip.so")
+            raise RuntimeError(f"build failed: {' '.join(cmd)}")
+
+
+def build(verbose: bool = False) -> Path:
+    """Compile every source and link both libraries (always rebuilds)."""
+    LIB_DIR.mkdir(exist_ok=True)
+    objects = [LIB_DIR / f"{Path(s).stem}.o" for s in SOURCES]
+    include = ["-I", str(PKG.parent / "include")]
+    _run(
+        [
+            [hipcc(), *DEVICE_FLAGS, *(ILP_FLAGS if s in ILP_SOURCES else ()), "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)]
+            for s, o in zip(SOURCES, objects)
+        ],
+        verbose,
+    )  # fmt: skip
+    tmp = LIB_DIR / "libgbx_hip.so.tmp"
+    _run([[hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-Wl,-soname,libgbx_hip.so", "-o", str(tmp), *map(str, objects)]], verbose)
     for o in objects:
         o.unlink()
     os.replace(tmp, LIB_PATH)
+    tmp = LIB_DIR / "gbx_torch.so.tmp"
+    _run([_extension_command(tmp)], verbose)
+    os.replace(tmp, EXT_PATH)
     return LIB_PATH
 
 

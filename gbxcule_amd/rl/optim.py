@@ -15,14 +15,13 @@ rounding to zero.
 from __future__ import annotations
 
 import math
-from array import array
 
 import torch
 
-from .. import _lib
-from .ops import _ELEM, _call
+from .._torch_ops import ext
 
 STATE_BLOCK = 256
+KINDS = (torch.float32, torch.bfloat16, torch.float16)
 _GOLDEN = 0x9E3779B9
 
 
@@ -44,10 +43,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         self.state_bits, self.seed = int(state_bits), int(seed)
         self._flat: list[dict[str, torch.Tensor]] = []
-        # by parameter group: where each tensor's states start, its elements, its state
-        self._starts: list[list[int]] = []
-        self._sizes: list[list[int]] = []
-        self._states: list[list[dict]] = []
+        self._plans: list = []  # by parameter group, as self._flat
+        self._states: list[list[dict]] = []  # self.state of a group's parameters
         super().__init__(params, {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay})
 
     def add_param_group(self, param_group) -> None:
@@ -62,7 +59,7 @@ class AdamW(torch.optim.Optimizer):
     def _lay_out(self, params) -> None:
         device = params[0].device
         for p in params:
-            if p.dtype not in _ELEM or not p.is_cuda or p.device != device or not p.is_contiguous():
+            if p.dtype not in KINDS or not p.is_cuda or p.device != device or not p.is_contiguous():
                 raise ValueError(f"parameters must be contiguous CUDA tensors of one device in float32, bfloat16 or "
                                  f"float16, got {p.dtype} on {p.device}")  # fmt: skip
         starts, total = [], 0
@@ -77,8 +74,8 @@ class AdamW(torch.optim.Optimizer):
             if small:
                 flat[key + "_scale"] = torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=device)
         self._flat.append(flat)
-        self._starts.append(starts)
-        self._sizes.append([p.numel() for p in params])
+        keys = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+        self._plans.append(ext.AdamwPlan([p.numel() for p in params], starts, *(flat.get(k) for k in keys)))
         self._states.append([self.state[p] for p in params])
         for p, at, state in zip(params, starts, self._states[-1]):
             state["step"] = 0
@@ -149,47 +146,26 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, g: int, group, grad_scale) -> None:
-        params, sizes = group["params"], self._sizes[g]
-        device = self._flat[g]["exp_avg"].get_device()
-        if [p.numel() for p in params] != sizes or not all(p.is_contiguous() and p.get_device() == device for p in params):
-            raise ValueError("a parameter has another size, layout or device than when the optimizer was made")
-        if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
-                                       or grad_scale.get_device() != device):  # fmt: skip
-            raise ValueError("grad_scale must be one float32 element on the parameters' device")
-        grads, states = [p.grad for p in params], self._states[g]
-        kind, done = params[0].dtype, states[0]["step"]
-        if all(t is not None and t.dtype is kind and p.dtype is kind and not t.is_sparse and s["step"] == done
-               for p, t, s in zip(params, grads, states)):  # fmt: skip
-            self._launch(g, group, grad_scale, params, grads, sizes, self._starts[g], states)
+        states = self._states[g]
+        done = states[0]["step"]
+        if all(s["step"] == done for s in states) and self._launch(g, group, grad_scale, (), done + 1):
+            for s in states:
+                s["step"] = done + 1
             return
         # tensors that a launch can take together: same types, same count of steps
-        batches: dict[tuple, tuple[list, ...]] = {}
-        for p, t, s, size, start in zip(params, grads, states, sizes, self._starts[g]):
-            if t is None:
-                continue
-            if t.is_sparse or p.dtype not in _ELEM or t.dtype not in (p.dtype, torch.float32):
-                raise ValueError(f"a {'sparse ' if t.is_sparse else ''}gradient of {t.dtype} does not go with {p.dtype}")
-            batch = batches.setdefault((p.dtype, t.dtype, s["step"]), ([], [], [], [], []))
-            for to, v in zip(batch, (p, t, size, start, s)):
-                to.append(v)
-        for batch in batches.values():
-            self._launch(g, group, grad_scale, *batch)
+        batches: dict[tuple, list[int]] = {}
+        for i, (p, s) in enumerate(zip(group["params"], states)):
+            if p.grad is not None:
+                batches.setdefault((p.dtype, p.grad.dtype, s["step"]), []).append(i)
+        for (_, _, done), which in batches.items():
+            if not self._launch(g, group, grad_scale, which, done + 1):
+                raise RuntimeError("a gradient changed during the step")
+            for i in which:
+                states[i]["step"] = done + 1
 
-    def _launch(self, g, group, grad_scale, params, grads, sizes, starts, states) -> None:
-        grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
-        step, flat, lr = states[0]["step"] + 1, self._flat[g], float(group["lr"])
-        b1, b2 = group["betas"]
-        tables = (array("Q", [p.data_ptr() for p in params]), array("Q", [t.data_ptr() for t in grads]),
-                  array("q", sizes), array("q", starts))  # fmt: skip
-        scales = (flat["exp_avg_scale"].data_ptr(), flat["exp_avg_sq_scale"].data_ptr()) if self.state_bits == 8 else (None, None)
-        given = _lib.AdamwIn(
-            len(params), _ELEM[params[0].dtype], _ELEM[grads[0].dtype], self.state_bits,
-            *[t.buffer_info()[0] for t in tables], flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), *scales,
-            None if grad_scale is None else grad_scale.data_ptr(), b1, b2, lr / (1 - b1**step),
-            1.0 / math.sqrt(1 - b2**step), group["eps"], 1 - lr * group["weight_decay"],
-            (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
+    def _launch(self, g: int, group, grad_scale, which, step: int) -> bool:
+        (b1, b2), lr = group["betas"], float(group["lr"])
+        return self._plans[g].step(
+            group["params"], which, grad_scale, b1, b2, lr / (1 - b1**step), 1.0 / math.sqrt(1 - b2**step),
+            group["eps"], 1 - lr * group["weight_decay"], (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
         )  # fmt: skip
-        _call("gbx_adamw", params[0], given)
-        torch.autograd.graph.increment_version(params)
-        for s in states:
-            s["step"] = step
