@@ -58,25 +58,25 @@ __device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
   const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
   return o > v ? o : v;
 }
-// Largest bit patterns of two values over 32 lanes (patterns of absolute values
-// order as the values do, NaN above all).  Rows of 16 lanes: the first swap
-// leaves a's in even rows and b's in odd ones, the second gives both to all.
-__device__ __forceinline__ void most_of_both(uint32_t& a, uint32_t& b) {
+// Largest bit pattern over 32 lanes of `a` in the even rows of 16 lanes and of
+// `b` in the odd ones (patterns of absolute values order as the values do, NaN
+// above all).
+__device__ __forceinline__ uint32_t most_of_rows(uint32_t a, uint32_t b) {
   const auto folded = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-  uint32_t v = folded[0] > folded[1] ? folded[0] : folded[1];
-  v = max_dpp<0x121>(max_dpp<0x122>(max_dpp<0x124>(max_dpp<0x128>(v))));  // rotated by 8, 4, 2, 1
-  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  a = both[0];
-  b = both[1];
+  const uint32_t v = folded[0] > folded[1] ? folded[0] : folded[1];
+  return max_dpp<0x121>(max_dpp<0x122>(max_dpp<0x124>(max_dpp<0x128>(v))));  // rotated by 8, 4, 2, 1
 }
 constexpr float kScaleFloor = 1e-30f, kE4m3Max = 448.0f, kE5m2Max = 57344.0f;
 
-// One element's update; `m` and `v` come in multiplied by beta1 and beta2.
-// Root and reciprocal are right to one unit in the last place: what they make
-// is added to a parameter many times its size.
+// One element's update.  The moments round at each operation, as written: in 8
+// bits a unit in the last place decides which way a value turns, and the same
+// formula elsewhere should turn the same way.  Root and reciprocal are right
+// to one unit in the last place: what they make is added to a parameter many
+// times its size.
 __device__ __forceinline__ float update(const AdamArgs& a, float p, float g, float rest1, float rest2, float& m, float& v) {
-  m = fmaf(g, rest1, m);
-  v = fmaf(g * g, rest2, v);
+#pragma clang fp contract(off)
+  m = m * a.beta1 + g * rest1;
+  v = v * a.beta2 + g * g * rest2;
   const float root = fmaf(__builtin_amdgcn_sqrtf(v), a.inv_root2, a.eps);
   return fmaf(-m * a.step_size, rcp_fast(root), p * a.keep);
 }
@@ -112,8 +112,6 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamArgs a, Tensors ts)
     load_row<4>(exp_avg_sq + e, 4, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      m[i] *= a.beta1;
-      v[i] *= a.beta2;
       p[i] = update(a, p[i], g[i], rest1, rest2, m[i], v[i]);
     }
     store_row<4>((P*)t.p + e, valid, p);
@@ -138,7 +136,7 @@ __global__ __launch_bounds__(kThreads) void adamw_8_kernel(AdamArgs a, Tensors t
     load_row<8>((const P*)t.p + e, valid, p);
     load_row<8>((const G*)t.g + e, valid, g);
     const uint2 mq = *(const uint2*)((const uint8_t*)a.exp_avg + s), vq = *(const uint2*)((const uint8_t*)a.exp_avg_sq + s);
-    const float ms = a.exp_avg_scale[block] * a.beta1, vs = a.exp_avg_sq_scale[block] * a.beta2;
+    const float ms = a.exp_avg_scale[block], vs = a.exp_avg_sq_scale[block];
     auto widen = [](uint32_t q, float by, float* to, auto bf8) {
       if constexpr (bf8.value) {
         to[0] = __builtin_amdgcn_cvt_f32_bf8((int)q, 0) * by, to[1] = __builtin_amdgcn_cvt_f32_bf8((int)q, 1) * by;
@@ -161,11 +159,14 @@ __global__ __launch_bounds__(kThreads) void adamw_8_kernel(AdamArgs a, Tensors t
       most_v = bv > most_v ? bv : most_v;
     }
     store_row<8>((P*)t.p + e, valid, p);
-    most_of_both(most_m, most_v);
-    const float fm = __uint_as_float(most_m), fv = __uint_as_float(most_v);
-    const float top_m = fm < kScaleFloor ? kScaleFloor : fm, top_v = fv < kScaleFloor ? kScaleFloor : fv;
+    // one reciprocal for both: the first moment's in even rows of 16 lanes
+    const bool second = threadIdx.x & 16u;
+    const float limit = second ? kE5m2Max : kE4m3Max, most = __uint_as_float(most_of_rows(most_m, most_v));
+    const float top = most < kScaleFloor ? kScaleFloor : most, inv = (1.0f / top) * limit;
+    if ((threadIdx.x & 15u) == 0u) (second ? a.exp_avg_sq_scale : a.exp_avg_scale)[block] = top * (second ? 1.0f / kE5m2Max : 1.0f / kE4m3Max);
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(inv), __float_as_uint(inv), false, false);
     // (a unit or two above the formats' largest values is cut off below)
-    const float inv_m = kE4m3Max * rcp_fast(top_m), inv_v = kE5m2Max * rcp_fast(top_v);
+    const float inv_m = __uint_as_float(both[0]), inv_v = __uint_as_float(both[1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t noise = noise_of((uint32_t)s + i, a.key);
@@ -181,10 +182,6 @@ __global__ __launch_bounds__(kThreads) void adamw_8_kernel(AdamArgs a, Tensors t
     };
     *(uint2*)((uint8_t*)a.exp_avg + s) = uint2{narrow(m, std::false_type{}), narrow(m + 4, std::false_type{})};
     *(uint2*)((uint8_t*)a.exp_avg_sq + s) = uint2{narrow(v, std::true_type{}), narrow(v + 4, std::true_type{})};
-    if ((threadIdx.x & 31u) == 0u) {
-      a.exp_avg_scale[block] = top_m * (1.0f / kE4m3Max);
-      a.exp_avg_sq_scale[block] = top_v * (1.0f / kE5m2Max);
-    }
   }
 }
 

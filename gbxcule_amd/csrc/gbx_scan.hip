@@ -685,15 +685,19 @@ void by_states(int states, F&& f) {
 }
 int padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : 32; }
 
-// Wavefronts below which the steps are cut into pieces, and about how many
-// there are then: 2 for each of 1,024 SIMDs.
-constexpr int64_t kFull = 1024, kWant = 4096;
+// Wavefronts below which the steps are cut into pieces, about how many there
+// are then (4 for each of 1,024 SIMDs), and the fewest steps of a piece: two
+// more launches take as long as some 40 steps (one row of 16,384 steps: 2,048
+// wavefronts 220 us, 4,096 192, 8,192 208; 4,096 steps of two rows in pieces
+// of at least 8 steps 92 us, 16 67; 40 steps of 16 rows in pieces of 16 30 us,
+// 32 38).
+constexpr int64_t kFull = 1024, kWant = 4096, kLeastPiece = 16;
 Pieces pieces_of(int steps, int envs, int dim, int groups, int channels, int waves_of_block) {
   Pieces p;
   p.blocks_per_group = (dim / groups + channels * waves_of_block - 1) / (channels * waves_of_block);
   p.blocks = groups * p.blocks_per_group;
   const int64_t waves = (int64_t)envs * p.blocks * waves_of_block;
-  const int64_t cuts = waves >= kFull ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kSegment - 1) / kSegment);
+  const int64_t cuts = waves >= kFull ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kLeastPiece - 1) / kLeastPiece);
   const int64_t each = (steps + cuts - 1) / cuts;
   p.chunk = (int)((each + kSegment - 1) / kSegment * kSegment);
   p.chunks = (steps + p.chunk - 1) / p.chunk;
