@@ -21,25 +21,28 @@ LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libgbx_hip.so"
 EXT_PATH = LIB_DIR / "gbx_torch.so"
 EXT_SOURCE = "gbx_torch.cpp"
-SOURCES = (
-    "gbx_step.hip", "gbx_aux.hip", "gbx_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_adamw.hip", "gbx_api.hip",
-)  # fmt: skip
 ARCH = os.environ.get("GBX_OFFLOAD_ARCH", "gfx950")
+# -O2 with the iterative ILP machine scheduler: on the step kernel's hot
+# loop this schedules the dependent loads earlier than -O3 with the default
+# occupancy-first scheduler (same-box A/B: 16K-env CPU-step workload +2.4%,
+# 131K-env banked cart +2.5%, RL rollout shape unchanged).
 DEVICE_FLAGS = (
     "-O2",
     f"--offload-arch={ARCH}",
     "-std=c++17",
+    "-mllvm",
+    "-amdgpu-sched-strategy=iterative-ilp",
     "-Xclang",
     "-target-feature",
     "-Xclang",
     "-packed-fp32-ops",
 )
-# The emulator's sources: the iterative ILP machine scheduler.  On the step
-# kernel's hot loop this schedules the dependent loads earlier than -O3 with
-# the default occupancy-first scheduler (same-box A/B: 16K-env CPU-step
-# workload +2.4%, 131K-env banked cart +2.5%, RL rollout shape unchanged).
-ILP_FLAGS = ("-mllvm", "-amdgpu-sched-strategy=iterative-ilp")
-ILP_SOURCES = ("gbx_step.hip", "gbx_aux.hip", "gbx_api.hip")
+# The policy operators: the default scheduler.  The other one leaves the
+# gradient of the scan more spilled registers, and its register allocation
+# crashes on the 8-bit AdamW kernel.
+POLICY_SOURCES = ("gbx_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_adamw.hip")
+SOURCES = ("gbx_step.hip", "gbx_aux.hip", *POLICY_SOURCES, "gbx_api.hip")
+POLICY_FLAGS = tuple(f for f in DEVICE_FLAGS if f != "-mllvm" and "sched-strategy" not in f)
 
 
 def hipcc() -> str:
@@ -84,7 +87,7 @@ def build(verbose: bool = False) -> Path:
     include = ["-I", str(PKG.parent / "include")]
     _run(
         [
-            [hipcc(), *DEVICE_FLAGS, *(ILP_FLAGS if s in ILP_SOURCES else ()), "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)]
+            [hipcc(), *(POLICY_FLAGS if s in POLICY_SOURCES else DEVICE_FLAGS), "-fPIC", *include, "-c", str(CSRC / s), "-o", str(o)]
             for s, o in zip(SOURCES, objects)
         ],
         verbose,

@@ -602,15 +602,17 @@ __global__ __launch_bounds__(256) void cross_sum_kernel(ScanArgs a, Pieces p, co
 }
 
 // One step of every env: the state is read and written once and bounds the
-// kernel.  LANES lanes share a channel, 4 states (16 bytes) each.
+// kernel.  LANES lanes share a channel, 4 states (16 bytes) each; where a
+// channel has no power of two of them, the last lanes have none.
 template <typename T, int LANES, int EACH>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x, d = i / LANES, part = i % LANES;
+  const int i = blockIdx.x * blockDim.x + threadIdx.x, d = i / LANES, part = i % LANES, parts = a.states / 4;
   const int64_t env0 = first_env<EACH>();
   if (env0 >= a.envs || d >= a.dim) return;
-  const int group = a.groups == 1 ? 0 : d / (a.dim / a.groups);
-  const T* b = (const T*)a.b + group * a.b_group + part * 4;
-  const T* c = (const T*)a.c + group * a.c_group + part * 4;
+  const bool holds = part < parts;
+  const int group = a.groups == 1 ? 0 : d / (a.dim / a.groups), place = d * parts + (holds ? part : 0);
+  const T* b = (const T*)a.b + group * a.b_group + (holds ? part : 0) * 4;
+  const T* c = (const T*)a.c + group * a.c_group + (holds ? part : 0) * 4;
   float4 h[EACH];
   float bv[EACH][4], cv[EACH][4];
   T x[EACH], dt[EACH], z[EACH];
@@ -618,7 +620,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
     const int64_t env = least(env0 + k * blockDim.y, a.envs - 1);
-    h[k] = reinterpret_cast<const float4*>(a.last)[env * a.dim * LANES + i];
+    h[k] = reinterpret_cast<const float4*>(a.last)[env * a.dim * parts + place];
     load_row<4>(b + env * a.b_env, 4, bv[k]);
     load_row<4>(c + env * a.c_env, 4, cv[k]);
     x[k] = ((const T*)a.x)[env * a.x_env + d];
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     z[k] = a.z ? ((const T*)a.z)[env * a.z_env + d] : (T)0.0f;
     begins[k] = a.resets ? a.resets[env] : 0;
   }
-  const float4 decay = reinterpret_cast<const float4*>(a.a)[i];
+  const float4 decay = reinterpret_cast<const float4*>(a.a)[place];
   const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
@@ -640,17 +642,18 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     h[k].z = fmaf(h[k].z, exp2_fast(scaled * decay.z), u * bv[k][2]);
     h[k].w = fmaf(h[k].w, exp2_fast(scaled * decay.w), u * bv[k][3]);
     float out = fmaf(h[k].x, cv[k][0], h[k].y * cv[k][1]) + fmaf(h[k].z, cv[k][2], h[k].w * cv[k][3]);
+    if (!holds) out = 0.0f;
     if constexpr (LANES > 1) out = add_dpp<0xB1>(out);
     if constexpr (LANES > 2) out = add_dpp<0x4E>(out);
     if constexpr (LANES > 4) out += __shfl_xor(out, 4, 64);
     if (env >= a.envs) break;
-    reinterpret_cast<float4*>(a.last)[env * a.dim * LANES + i] = h[k];
+    if (holds) reinterpret_cast<float4*>(a.last)[env * a.dim * parts + place] = h[k];
     out = fmaf(skip, (float)x[k], out);
     if (a.z) out *= (float)z[k] * sigmoid((float)z[k]);
     if (part == 0) ((T*)a.y)[env * a.dim + d] = (T)out;
   }
 }
-// Any number of states: a lane a channel.
+// No multiple of 4 states: a lane a channel.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_step_any_kernel(ScanArgs a) {
   const int64_t env = first_env<1>();
@@ -801,17 +804,16 @@ hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st) {
       if (s.each == 4) hipLaunchKernelGGL((scan_step_kernel<T, lanes, 4>), s.grid(), s.block(), 0, st, a);
       else hipLaunchKernelGGL((scan_step_kernel<T, lanes, 1>), s.grid(), s.block(), 0, st, a);
     };
-    if (a.states == 4) go(std::integral_constant<int, 1>{});
-    else if (a.states == 8) go(std::integral_constant<int, 2>{});
-    else if (a.states == 16) go(std::integral_constant<int, 4>{});
-    else if (a.states == 32) go(std::integral_constant<int, 8>{});
-    else {
+    if (a.states % 4) {
       StepShape s = step_shape(a.dim, 1);
       const int64_t blocks = ((int64_t)a.envs + s.rows - 1) / s.rows;
       s.grid_.y = (unsigned)std::min<int64_t>(blocks, kEnvRow);
       s.grid_.z = (unsigned)((blocks + kEnvRow - 1) / kEnvRow);
       hipLaunchKernelGGL(scan_step_any_kernel<T>, s.grid(), s.block(), 0, st, a);
-    }
+    } else if (a.states == 4) go(std::integral_constant<int, 1>{});
+    else if (a.states == 8) go(std::integral_constant<int, 2>{});
+    else if (a.states <= 16) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
   });
   return hipGetLastError();
 }
