@@ -8,20 +8,41 @@
 namespace gbx {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kVec = 8;  // channels a lane takes at a time: 16 bytes of a 16-bit type
+constexpr int threads_of(int lanes) { return lanes > 256 ? lanes : 256; }
 
-// Sum (or, of bit patterns of absolute values, maximum) over LANES
-// neighbouring lanes; 256 lanes are the whole workgroup.
+// Where rows end.  WHOLE: with a piece of 8 channels.  LAPPED: inside one; the
+// last piece then begins 8 channels before the end and shares some with the
+// piece before it.  Both compute and write the same values there, and sums
+// leave the shared ones out: without it the one lane with a part of a piece
+// would load and store it element by element (131,072 rows of 255 channels
+// forward and backward 565 us).  TINY: rows shorter than a piece.
+enum Ends { WHOLE, LAPPED, TINY };
+struct Piece {
+  int c, valid, skip;  // first channel; channels from there on (8 or more: a whole piece); shared ones
+};
+template <int ENDS>
+__device__ __forceinline__ Piece piece_of(int k, int dim) {
+  const int c = k * kVec;
+  if constexpr (ENDS == LAPPED) {
+    if (c < dim) return {c < dim - kVec ? c : dim - kVec, kVec, c < dim - kVec ? 0 : c - (dim - kVec)};
+  }
+  return {c, ENDS == TINY ? dim - c : c < dim ? kVec : 0, 0};
+}
+
+// Sum (or, of bit patterns of absolute values, maximum) over LANES neighbouring
+// lanes; more than 64 are the whole workgroup.
 template <int LANES>
 __device__ __forceinline__ float sum_over(float v, float* lds) {
 #pragma unroll
   for (int m = 1; m < (LANES < 64 ? LANES : 64); m <<= 1) v += __shfl_xor(v, m, 64);
-  if constexpr (LANES == 256) {
+  if constexpr (LANES > 64) {
     __syncthreads();  // the last use of lds has been read
     if ((threadIdx.x & 63u) == 0u) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) v += lds[w];
   }
   return v;
 }
@@ -32,13 +53,13 @@ __device__ __forceinline__ uint32_t max_over(uint32_t v, float* lds) {
     const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
     v = o > v ? o : v;
   }
-  if constexpr (LANES == 256) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(lds);
+  if constexpr (LANES > 64) {
+    uint32_t* all = reinterpret_cast<uint32_t*>(lds);
     __syncthreads();
-    if ((threadIdx.x & 63u) == 0u) w[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63u) == 0u) all[threadIdx.x >> 6] = v;
     __syncthreads();
-    const uint32_t a = w[0] > w[1] ? w[0] : w[1], b = w[2] > w[3] ? w[2] : w[3];
-    v = a > b ? a : b;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) v = all[w] > v ? all[w] : v;
   }
   return v;
 }
@@ -52,10 +73,10 @@ constexpr float kScaleFloor = 1e-30f;  // keeps the scale of an all-zero group p
 // LANES lanes hold one row, kVec * NV channels each, in registers: x and the
 // residual are read once, y and s written once.  NV = 0 takes rows of any
 // length in steps of the workgroup and reads the row a second time.
-template <typename T, int LANES, int NV, bool FP8>
-__global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
-  constexpr int kRows = kThreads / LANES, kHeld = NV ? NV : 1;
-  __shared__ float lds[4];
+template <typename T, int LANES, int NV, int ENDS, bool FP8>
+__global__ __launch_bounds__(threads_of(LANES)) void norm_kernel(NormArgs a) {
+  constexpr int kRows = threads_of(LANES) / LANES, kHeld = NV ? NV : 1;
+  __shared__ float lds[16];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, dim = a.dim;
   const int rounds = NV ? NV : (dim + kVec * LANES - 1) / (kVec * LANES);
   const float inv_dim = 1.0f / (float)dim;
@@ -63,8 +84,8 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
   if constexpr (NV > 0) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * LANES + lane) * kVec;
-      load_row<kVec>(a.weight + c, dim - c, w[k]);
+      const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
+      load_row<kVec>(a.weight + e.c, e.valid, w[k]);
     }
   }
   for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.rows; row += (int64_t)gridDim.x * kRows) {
@@ -75,39 +96,40 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
     float s[kHeld][kVec], ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < rounds; ++k) {
-      const int c = (k * LANES + lane) * kVec;
+      const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
       float(&v)[kVec] = s[NV ? k : 0];
-      load_row<kVec>(x + c, dim - c, v);
+      load_row<kVec>(x + e.c, e.valid, v);
       if (a.residual) {
         float o[kVec];
-        load_row<kVec>(r + c, dim - c, o);
+        load_row<kVec>(r + e.c, e.valid, o);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) v[i] = (float)(T)(v[i] + o[i]);
-        store_row<kVec>(summed + c, dim - c, v);
+        store_row<kVec>(summed + e.c, e.valid, v);
       }
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) ss = fmaf(v[i], v[i], ss);
+      for (int i = 0; i < kVec; ++i) ss = ENDS == LAPPED && i < e.skip ? ss : fmaf(v[i], v[i], ss);
     }
     const float rstd = rsqrtf(fmaf(sum_over<LANES>(ss, lds), inv_dim, a.eps));
     auto normed = [&](int k, float (&y)[kVec]) {
-      const int c = (k * LANES + lane) * kVec;
       if constexpr (NV > 0) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) y[i] = s[k][i] * rstd * w[k][i];
       } else {
+        const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
         float wk[kVec];
-        load_row<kVec>(a.residual ? summed + c : x + c, dim - c, y);
-        load_row<kVec>(a.weight + c, dim - c, wk);
+        load_row<kVec>((a.residual ? summed : x) + e.c, e.valid, y);
+        load_row<kVec>(a.weight + e.c, e.valid, wk);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) y[i] *= rstd * wk[i];
       }
     };
-    auto most = [](const float (&y)[kVec], uint32_t m) {
+    auto most = [&](int k, const float (&y)[kVec], uint32_t m) {
       // bit patterns of absolute values order as the values do, NaN above all
+      const int skip = piece_of<ENDS>(k * LANES + lane, dim).skip;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         const uint32_t b = __float_as_uint(y[i]) & 0x7FFFFFFFu;
-        m = b > m ? b : m;
+        m = b > m && !(ENDS == LAPPED && i < skip) ? b : m;
       }
       return m;
     };
@@ -118,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
         for (int k = 0; k < rounds; ++k) {
           float y[kVec];
           normed(k, y);
-          row_most = most(y, row_most);
+          row_most = most(k, y, row_most);
         }
         row_most = max_over<LANES>(row_most, lds);
       }
@@ -126,11 +148,12 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
       const int groups = a.group ? (dim + 127) / 128 : 1;
 #pragma unroll
       for (int k = 0; k < rounds; ++k) {
-        const int c = (k * LANES + lane) * kVec;
+        const int c = (k * LANES + lane) * kVec;  // without the shared channels, whose scale may be another one
+        const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
         float y[kVec];
         normed(k, y);
         // 128 channels are 16 neighbouring lanes
-        const uint32_t m = a.group ? max_over<16>(most(y, 0u), lds) : row_most;
+        const uint32_t m = a.group ? max_over<16>(most(k, y, 0u), lds) : row_most;
         const float top = m > 0x7F800000u ? __uint_as_float(m) : fmaxf(__uint_as_float(m), kScaleFloor);
         const float inv = kE4m3Max / top;
         if (a.group ? (lane % 16 == 0 && c < dim) : (lane == 0 && k == 0)) a.scale[row * groups + (a.group ? c / 128 : 0)] = top / kE4m3Max;
@@ -139,21 +162,21 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
         int hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * inv, y[5] * inv, 0, false);
         hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * inv, y[7] * inv, hi, true);
         const uint64_t both = (uint32_t)lo | (uint64_t)(uint32_t)hi << 32;
-        if (dim - c >= kVec) {
-          __builtin_memcpy(q + c, &both, 8);
+        if (e.valid >= kVec && e.skip == 0) {
+          __builtin_memcpy(q + e.c, &both, 8);
         } else {
 #pragma unroll
           for (int i = 0; i < kVec; ++i)
-            if (i < dim - c) q[c + i] = (uint8_t)(both >> (8 * i));
+            if (i < e.valid && i >= e.skip) q[e.c + i] = (uint8_t)(both >> (8 * i));
         }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < rounds; ++k) {
-        const int c = (k * LANES + lane) * kVec;
+        const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
         float y[kVec];
         normed(k, y);
-        store_row<kVec>(out + c, dim - c, y);
+        store_row<kVec>(out + e.c, e.valid, y);
       }
     }
   }
@@ -165,10 +188,10 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
 // one pass, so nothing but s itself has to be kept from the forward.  A
 // workgroup sums dweight over its rows in registers, then over its row slots
 // in LDS, and writes one row of partial sums: no atomics, one order.
-template <typename T, int LANES, int NV>
-__global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
-  constexpr int kRows = kThreads / LANES, kHeld = NV ? NV : 1;
-  __shared__ float lds[4];
+template <typename T, int LANES, int NV, int ENDS>
+__global__ __launch_bounds__(threads_of(LANES)) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kThreads = threads_of(LANES), kRows = kThreads / LANES, kHeld = NV ? NV : 1;
+  __shared__ float lds[16];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, dim = a.dim;
   const int rounds = NV ? NV : (dim + kVec * LANES - 1) / (kVec * LANES);
   const float inv_dim = 1.0f / (float)dim;
@@ -177,8 +200,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
   if constexpr (NV > 0) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * LANES + lane) * kVec;
-      load_row<kVec>(a.weight + c, dim - c, w[k]);
+      const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
+      load_row<kVec>(a.weight + e.c, e.valid, w[k]);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) dw[k][i] = 0.0f;
     }
@@ -192,29 +215,32 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
     float s[kHeld][kVec], dy[kHeld][kVec], ss = 0.0f, gs = 0.0f;
 #pragma unroll
     for (int k = 0; k < rounds; ++k) {
-      const int c = (k * LANES + lane) * kVec, h = NV ? k : 0;
-      load_row<kVec>(sp + c, dim - c, s[h]);
-      load_row<kVec>(dyp + c, dim - c, dy[h]);
-      if constexpr (NV == 0) load_row<kVec>(a.weight + c, dim - c, w[0]);
+      const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
+      const int h = NV ? k : 0;
+      load_row<kVec>(sp + e.c, e.valid, s[h]);
+      load_row<kVec>(dyp + e.c, e.valid, dy[h]);
+      if constexpr (NV == 0) load_row<kVec>(a.weight + e.c, e.valid, w[0]);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        ss = fmaf(s[h][i], s[h][i], ss);
-        gs = fmaf(s[h][i], dy[h][i] * w[h][i], gs);
+        const bool mine = ENDS != LAPPED || i >= e.skip;
+        ss = mine ? fmaf(s[h][i], s[h][i], ss) : ss;
+        gs = mine ? fmaf(s[h][i], dy[h][i] * w[h][i], gs) : gs;
       }
     }
     const float rstd = rsqrtf(fmaf(sum_over<LANES>(ss, lds), inv_dim, a.eps));
     const float pull = sum_over<LANES>(gs, lds) * inv_dim * rstd * rstd;
 #pragma unroll
     for (int k = 0; k < rounds; ++k) {
-      const int c = (k * LANES + lane) * kVec, h = NV ? k : 0;
+      const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
+      const int h = NV ? k : 0;
       if constexpr (NV == 0) {
-        load_row<kVec>(sp + c, dim - c, s[0]);
-        load_row<kVec>(dyp + c, dim - c, dy[0]);
-        load_row<kVec>(a.weight + c, dim - c, w[0]);
+        load_row<kVec>(sp + e.c, e.valid, s[0]);
+        load_row<kVec>(dyp + e.c, e.valid, dy[0]);
+        load_row<kVec>(a.weight + e.c, e.valid, w[0]);
       }
       float dx[kVec];
       if (a.dsummed) {
-        load_row<kVec>(dsp + c, dim - c, dx);
+        load_row<kVec>(dsp + e.c, e.valid, dx);
       } else {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) dx[i] = 0.0f;
@@ -224,18 +250,21 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
         dx[i] = fmaf(rstd, fmaf(-s[h][i], pull, dy[h][i] * w[h][i]), dx[i]);
         const float grow = dy[h][i] * (s[h][i] * rstd);
         if constexpr (NV > 0) dw[k][i] += grow;
-        else if (c + i < dim) part[c + i] = row == first ? grow : part[c + i] + grow;
+        else if (i >= e.skip && i < e.valid) part[e.c + i] = row == first ? grow : part[e.c + i] + grow;
       }
-      store_row<kVec>(dxp + c, dim - c, dx);
+      store_row<kVec>(dxp + e.c, e.valid, dx);
     }
   }
   if constexpr (NV > 0) {
     if constexpr (kRows > 1) {
       __shared__ float tile[kThreads * NV * kVec];
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
+      for (int k = 0; k < NV; ++k) {
+        const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) tile[sub * (LANES * NV * kVec) + (k * LANES + lane) * kVec + i] = dw[k][i];
+        for (int i = 0; i < kVec; ++i)
+          if (i < e.valid) tile[sub * (LANES * NV * kVec) + e.c + i] = dw[k][i];
+      }
       __syncthreads();
       for (int c = threadIdx.x; c < dim; c += kThreads) {
         float v = 0.0f;
@@ -246,8 +275,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * LANES + lane) * kVec;
-        store_row<kVec>(part + c, dim - c, dw[k]);
+        const Piece e = piece_of<ENDS>(k * LANES + lane, dim);
+        store_row<kVec>(part + e.c, e.valid, dw[k]);
       }
     }
   }
@@ -279,26 +308,34 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void column_sum_kernel(const fl
   }
 }
 
+// f(lanes of a row, 8-channel pieces of a lane): the fewest that hold it.
 template <typename F>
 void by_row_length(int dim, F&& f) {
-  // lanes of a row and 8-channel pieces of a lane: the fewest that hold it
-  if (dim <= 128) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-  else if (dim <= 256) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
-  else if (dim <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-  else if (dim <= 1024) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-  else if (dim <= 2048) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  else if (dim <= 4096) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-  else if (dim <= 8192) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-  else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
+  auto go = [&](auto lanes, auto pieces) { f(lanes, pieces); };
+  using std::integral_constant;
+  if (dim <= 128) go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (dim <= 256) go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  else if (dim <= 512) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (dim <= 1024) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (dim <= 2048) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (dim <= 4096) go(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+  else if (dim <= 8192) go(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else go(integral_constant<int, 256>{}, integral_constant<int, 0>{});
 }
-int lanes_of(int dim) {
-  int lanes = 0;
-  by_row_length(dim, [&](auto l, auto) { lanes = l; });
-  return lanes;
+int rows_of_block(int dim) {
+  int rows = 0;
+  by_row_length(dim, [&](auto lanes, auto) { rows = threads_of(lanes) / lanes; });
+  return rows;
+}
+template <typename F>
+void by_ends(int dim, F&& f) {
+  if (dim % kVec == 0) f(std::integral_constant<int, WHOLE>{});
+  else if (dim > kVec) f(std::integral_constant<int, LAPPED>{});
+  else f(std::integral_constant<int, TINY>{});
 }
 constexpr int kGradBlocks = 1024;  // workgroups of the gradient, each a row of partial sums
 int grad_blocks(int64_t rows, int dim) {
-  const int per = kThreads / lanes_of(dim);
+  const int per = rows_of_block(dim);
   return (int)std::min<int64_t>((rows + per - 1) / per, kGradBlocks);
 }
 
@@ -311,13 +348,17 @@ hipError_t launch_column_sum(const float* in, int rows, const SumOutputs& to, hi
 }
 
 hipError_t launch_rms_norm(const NormArgs& a, hipStream_t st) {
+  const int64_t per = rows_of_block(a.dim);
+  const dim3 grid((unsigned)std::min<int64_t>((a.rows + per - 1) / per, 1 << 16));
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_row_length(a.dim, [&](auto lanes, auto nv) {
-      const int64_t per = kThreads / lanes;
-      const dim3 grid((unsigned)std::min<int64_t>((a.rows + per - 1) / per, 1 << 16));
-      if (a.scale) hipLaunchKernelGGL((norm_kernel<T, lanes, nv, true>), grid, dim3(kThreads), 0, st, a);
-      else hipLaunchKernelGGL((norm_kernel<T, lanes, nv, false>), grid, dim3(kThreads), 0, st, a);
+      by_ends(a.dim, [&](auto ends) {
+        if constexpr (ends != TINY || lanes == 16) {
+          if (a.scale) hipLaunchKernelGGL((norm_kernel<T, lanes, nv, ends, true>), grid, dim3(threads_of(lanes)), 0, st, a);
+          else hipLaunchKernelGGL((norm_kernel<T, lanes, nv, ends, false>), grid, dim3(threads_of(lanes)), 0, st, a);
+        }
+      });
     });
   });
   return hipGetLastError();
@@ -330,7 +371,9 @@ hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_row_length(a.dim, [&](auto lanes, auto nv) {
-      hipLaunchKernelGGL((norm_grad_kernel<T, lanes, nv>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
+      by_ends(a.dim, [&](auto ends) {
+        if constexpr (ends != TINY || lanes == 16) hipLaunchKernelGGL((norm_grad_kernel<T, lanes, nv, ends>), dim3((unsigned)blocks), dim3(threads_of(lanes)), 0, st, a);
+      });
     });
   });
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
