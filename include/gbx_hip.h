@@ -223,7 +223,8 @@ int gbx_set_debug(gbx_ctx* ctx, int32_t rst38, int32_t trap_pc,
  * [steps][envs][channels], as rollouts are stored.  Strides are in elements;
  * the channel stride is 1.  `resets` (uint8 [steps][envs], may be NULL) is
  * non-zero where an episode begins: nothing from before reaches that step.
- * Outputs without strides are contiguous.  `work` is scratch memory of the
+ * Outputs without strides are contiguous; outputs and inputs do not overlap.
+ * `work` is scratch memory of the
  * number of floats that the *_work function of the same arguments returns
  * (negative: the arguments are out of range); it may be NULL for 0. */
 
@@ -277,7 +278,7 @@ typedef struct gbx_scan_in {
 } gbx_scan_in;
 /* state[envs][dim][states] (NULL: zeros) before the first step, last after the
  * last one.  saved, if not NULL, receives what the gradient starts from:
- * [steps / 8 rounded up][envs][dim][states]. */
+ * [steps / 8 rounded up][envs][states][dim]. */
 int64_t gbx_selective_scan_work(const gbx_scan_in* in);
 int gbx_selective_scan(const gbx_scan_in* in, const float* state, void* y, float* last, float* saved,
                        float* work, void* stream);
