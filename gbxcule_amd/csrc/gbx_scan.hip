@@ -271,9 +271,8 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
 
 // Runs over the pieces, first to last (BACKWARD: last to first), and leaves in
 // `ends` what each piece starts from.  A lane is one env, state and channel, and
-// waits for its loads: 256 pieces of 1,024 channels x 16 states 27 us, the 5
-// pieces of 37 envs x 200 channels 4 us.  (Runs of pieces joined through LDS
-// gain a tenth at most at 256 pieces and lose a third at tens of them.)
+// waits for its loads, 16 pieces at a time: the 5 pieces of 37 envs x 200
+// channels x 8 states take 4 us.
 template <bool BACKWARD>
 __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float* ends, const float* sums) {
   const int64_t i = block_id() * 256 + threadIdx.x, each = (int64_t)a.envs * a.states * a.dim;
@@ -296,6 +295,68 @@ __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float
       const int piece = BACKWARD ? chunks - 1 - k0 - k : k0 + k;
       ends[piece * each + i] = h;
       h = sum[k] == __builtin_inff() ? e[k] : fmaf(h, exp2_fast(sum[k] * decay), e[k]);
+    }
+  }
+}
+
+// The same for many pieces.  A workgroup is 64 channels of one env and state by
+// 16 runs of up to 16 pieces: each lane composes its run, the runs are joined
+// through LDS, and the lane goes through its run again from what comes before
+// it.  256 pieces of 1,024 channels x 16 states take 13 us (join_kernel 27), 64
+// of 512 channels as long as there, but 32 pieces of 16 envs 40 us longer.
+constexpr int kRuns = 16, kRun = 16, kManyPieces = 64;
+template <bool BACKWARD>
+__global__ __launch_bounds__(kWave* kRuns) void join_runs_kernel(ScanArgs a, int chunks, float* ends, const float* sums) {
+  __shared__ float last[kRuns][kWave], through[kRuns][kWave];  // of a run: its end from zero; what it lets through
+  const int lane = threadIdx.x % kWave, run = threadIdx.x / kWave, blocks = (a.dim + kWave - 1) / kWave;
+  const int64_t row = block_id() / blocks;  // env and state
+  if (row >= (int64_t)a.envs * a.states) return;
+  const int d0 = (int)(block_id() % blocks) * kWave + lane, d = min(d0, a.dim - 1);
+  const int s = (int)(row % a.states), env = (int)(row / a.states);
+  const float decay = a.a[(int64_t)d * a.states + s] * kLog2e;
+  float h = !BACKWARD && a.state ? a.state[((int64_t)env * a.dim + d) * a.states + s] : 0.0f;
+  // (an episode that begins in a piece lets nothing through, whatever lies before)
+  constexpr float kNothing = -1.0f;
+  const auto pass = [&](float from, float by, float end) { return by < 0.0f ? end : fmaf(from, by, end); };
+  for (int first = 0; first < chunks; first += kRuns * kRun) {
+    const int count = min(kRuns * kRun, chunks - first), per = (count + kRuns - 1) / kRuns;
+    const int mine = max(0, min(per, count - run * per));
+    const auto piece_of = [&](int k) {
+      const int j = first + run * per + min(k, mine - 1);
+      return (int64_t)(BACKWARD ? chunks - 1 - j : j) * a.envs + env;
+    };
+    float e[kRun], by[kRun], end = 0.0f, all = 1.0f;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      e[k] = by[k] = 0.0f;
+      if (mine > 0) {
+        e[k] = ends[(piece_of(k) * a.states + s) * a.dim + d];
+        by[k] = sums[piece_of(k) * a.dim + d];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) by[k] = by[k] == __builtin_inff() ? kNothing : exp2_fast(by[k] * decay);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      if (k >= mine) break;
+      end = pass(end, by[k], e[k]);
+      all = by[k] < 0.0f || all < 0.0f ? kNothing : all * by[k];
+    }
+    last[run][lane] = end;
+    through[run][lane] = all;
+    __syncthreads();
+    float start = h;
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      start = r == run ? h : start;
+      h = pass(h, through[r][lane], last[r][lane]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      if (k >= mine) break;
+      if (d0 < a.dim) ends[(piece_of(k) * a.states + s) * a.dim + d] = start;
+      start = pass(start, by[k], e[k]);
     }
   }
 }
@@ -744,6 +805,17 @@ int64_t cross_floats(const Pieces& p, int steps, int envs, int states) {
   return p.blocks_per_group > 1 ? (int64_t)steps * envs * p.blocks * 2 * padded(states) : 0;
 }
 
+template <bool BACKWARD>
+void launch_join(const ScanArgs& a, const Pieces& p, float* ends, const float* sums, hipStream_t st) {
+  const int64_t rows = (int64_t)a.envs * a.states;
+  if (p.chunks >= kManyPieces) {
+    const dim3 grid = wide_grid(rows * ((a.dim + kWave - 1) / kWave));
+    hipLaunchKernelGGL(join_runs_kernel<BACKWARD>, grid, dim3(kWave * kRuns), 0, st, a, p.chunks, ends, sums);
+  } else {
+    hipLaunchKernelGGL(join_kernel<BACKWARD>, wide_grid((rows * a.dim + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, sums);
+  }
+}
+
 template <typename T, int SP, int WHAT>
 void launch_scan_kernel(const ScanArgs& a, const Pieces& p, float* ends, float* sums, hipStream_t st) {
   const int64_t waves = (int64_t)p.blocks * a.envs * p.chunks;
@@ -769,8 +841,7 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t st) {
     by_states(a.states, [&](auto sp) {
       if (p.chunks > 1) {
         launch_scan_kernel<T, sp, ENDS>(a, p, ends, sums, st);
-        const int64_t each = (int64_t)a.envs * a.states * a.dim;
-        hipLaunchKernelGGL(join_kernel<false>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
+        launch_join<false>(a, p, ends, sums, st);
       }
       launch_scan_kernel<T, sp, FULL>(a, p, ends, sums, st);
     });
@@ -802,8 +873,7 @@ hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st) {
         wide.blocks_per_group = (a.dim / a.groups + kWave - 1) / kWave;
         wide.blocks = a.groups * wide.blocks_per_group;
         launch_scan_kernel<T, sp, BACK>(a, wide, ends, sums, st);
-        const int64_t each = (int64_t)a.envs * a.states * a.dim;
-        hipLaunchKernelGGL(join_kernel<true>, wide_grid((each + 255) / 256), dim3(256), 0, st, a, p.chunks, ends, (const float*)sums);
+        launch_join<true>(a, p, ends, sums, st);
       }
       const size_t lds = sizeof(typename GradShape<sp>::Lds) * waves;
       hipLaunchKernelGGL((scan_grad_kernel<T, sp>), dim3((unsigned)(slots * p.blocks)), dim3(kWave * waves), lds, st, a, p, slots, (const float*)ends, cross, rows);

@@ -297,6 +297,33 @@ def test_scan_pieces_join_as_one():
     ref.check(end, last, 256, "state")
 
 
+@pytest.mark.parametrize("case", [
+    (1100, 1, 70, 16, 1, F32, 0.004, True, True, True, True, True),
+    (1537, 2, 65, 8, 1, BF16, 0.01, True, True, True, True, True),
+    (4801, 1, 33, 4, 1, F32, 0.0, False, True, True, True, True),
+], ids=str)  # fmt: skip
+def test_scan_of_many_pieces(case):
+    """One long row: 64 pieces and more than 256, which are joined by runs."""
+    from gbxcule_amd.rl import selective_scan
+
+    steps, envs, dim, states, groups, dtype = case[:6]
+    gen, t, state, resets = _scan_inputs(case)
+    leaf = dict(zip(NAMES, _leaf(*(t[k] for k in NAMES))))
+    y, last = selective_scan(*(leaf[k] for k in NAMES[:7]), dt_bias=leaf["dt_bias"], state=state, resets=resets)
+    wide = {k: ref.f64(leaf[k]) for k in NAMES}
+    want, want_last = ref.selective_scan(*(wide[k] for k in NAMES), True, ref.f64(state), None if resets is None else resets.cpu())
+    # the roundings that a state carries are those of the steps that its decay reaches, joins of pieces among them
+    n = 512
+    ref.check(y, want, n, "y")
+    ref.check(last, want_last, n, "state")
+    dy = _randn(gen, steps, envs, dim, dtype=dtype)
+    names = [k for k in NAMES if leaf[k] is not None]
+    got = torch.autograd.grad(y, [leaf[k] for k in names], dy)
+    exact = torch.autograd.grad(want, [wide[k] for k in names], ref.f64(dy))
+    for g, v, name in zip(got, exact, names):
+        ref.check(g, v, 2 * n + (steps * envs if name in ("A", "D", "dt_bias") else dim), f"gradient of {name}")
+
+
 @pytest.mark.parametrize("steps", [40, 400])
 def test_scan_ignores_what_lies_before_an_episode(steps):
     from gbxcule_amd.rl import selective_scan, selective_scan_step
