@@ -74,12 +74,12 @@ enum { FULL, ENDS, BACK };  // what scan_kernel computes
 //
 // Bound by the vector units: a state takes an exponential at half rate and four
 // products a step in FULL, three in ENDS.  128 steps x 1,024 envs x 512 channels
-// x 16 states (1.07 G state steps) take 378 us with the states for the gradient
-// written, 2.8 T state steps/s where six issue slots each would allow 6; 16,384
-// steps of one env x 1,024 channels x 16 states 100 us in FULL, 75 in ENDS.
+// x 16 states (1.07 G state steps) take 325 us with the states for the gradient
+// written, 3.3 T state steps/s where six issue slots each would allow 6; 16,384
+// steps of one env x 1,024 channels x 16 states 85 us in FULL, 64 in ENDS.
 // All states in a lane: no sum across lanes, and delta, softplus and the gate
 // once a channel.  More wavefronts by launch bounds are slower (8 a SIMD: 823
-// us, 6: 590 us).
+// us, 6: 590).
 template <typename T, int SP, int WHAT, bool SCALAR>
 __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces p, float* ends, float* sums) {
   const int lane = threadIdx.x & 63;
@@ -94,11 +94,12 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   const int d = group * per_group + min(in_group, per_group - 1);
   const int t0 = piece * p.chunk, t1 = min(t0 + p.chunk, a.steps), count = t1 - t0;
   const bool gated = a.z != nullptr;
+  const int states = SCALAR ? SP : a.states;
 
   float decay[SP], h[SP];  // A in powers of two; the states, or their gradient
 #pragma unroll
   for (int s = 0; s < SP; ++s) {
-    decay[s] = s < a.states ? a.a[(int64_t)d * a.states + s] * kLog2e : 0.0f;
+    decay[s] = s < states ? a.a[(int64_t)d * states + s] * kLog2e : 0.0f;
     h[s] = 0.0f;
   }
   const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
@@ -106,11 +107,11 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     if (p.chunks > 1) {
 #pragma unroll
       for (int s = 0; s < SP; ++s)
-        if (s < a.states) h[s] = ends[((int64_t)item * a.states + s) * a.dim + d];
+        if (s < states) h[s] = ends[((int64_t)item * states + s) * a.dim + d];
     } else if (a.state) {
 #pragma unroll
       for (int s = 0; s < SP; ++s)
-        if (s < a.states) h[s] = a.state[((int64_t)env * a.dim + d) * a.states + s];
+        if (s < states) h[s] = a.state[((int64_t)env * a.dim + d) * states + s];
     }
   }
 
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   const T* c = (const T*)a.c + from * a.c_step + env * a.c_env + group * a.c_group;
   const uint8_t* resets = a.resets + from * a.envs + env;
   T* y = (T*)a.y + ((int64_t)t0 * a.envs + env) * a.dim;
-  float* saved = a.saved + ((int64_t)(t0 / kSegment) * a.envs + env) * a.dim * a.states;
+  float* saved = a.saved + ((int64_t)(t0 / kSegment) * a.envs + env) * a.dim * states;
   auto of_lane = [&](const T* row) { return *(const T*)((const char*)row + at); };
 
   constexpr int kAhead = 4;  // steps whose loads are in flight together
@@ -135,26 +136,32 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   const T* row_bc = lane >= 32 ? c : b;  // without SCALAR: lanes hold B, then C
   const int64_t row_bc_step = lane >= 32 ? to * a.c_step : to * a.b_step;
   auto fetch = [&](int k0) {
+    // the last row is loaded again past the end
+    const auto rows = [&](auto&& load) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const bool more = k0 + i + 1 < count;  // the last row is loaded again past the end
+      for (int i = 0; i < kAhead; ++i) load(i, k0 + i + 1 < count ? to : 0);
+    };
+    rows([&](int i, int64_t on) {
       xs[i] = of_lane(x);
-      x += more ? to * x_step : 0;
+      x += on * x_step;
       dts[i] = of_lane(dt);
-      dt += more ? to * a.dt_step : 0;
-      if (gated && WHAT != ENDS) {
+      dt += on * a.dt_step;
+    });
+    if (gated && WHAT != ENDS)
+      rows([&](int i, int64_t on) {
         zs[i] = of_lane(z);
-        z += more ? to * a.z_step : 0;
-      }
-      if (a.resets) {
+        z += on * a.z_step;
+      });
+    if (a.resets)
+      rows([&](int i, int64_t on) {
         rs[i] = *resets;
-        resets += more ? to * a.envs : 0;
-      }
-      if constexpr (!SCALAR) {
-        bcs[i] = (lane & 31) < a.states ? row_bc[lane & 31] : (T)0.0f;
-        row_bc += more ? row_bc_step : 0;
-      }
-    }
+        resets += on * a.envs;
+      });
+    if constexpr (!SCALAR)
+      rows([&](int i, int64_t on) {
+        bcs[i] = (lane & 31) < states ? row_bc[lane & 31] : (T)0.0f;
+        row_bc += on ? row_bc_step : 0;
+      });
   };
   RowBits<SP, T> rb, rc;
   if constexpr (SCALAR) {
@@ -162,13 +169,13 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     if constexpr (WHAT != ENDS) load_scalar(c, rc);
   }
   auto store_states = [&](float* to, const float(&v)[SP]) {
-    if (a.states == SP) {  // 16 bytes at a time
+    if (states == SP) {  // 16 bytes at a time
 #pragma unroll
       for (int s = 0; s < SP; s += 4) *reinterpret_cast<float4*>(to + s) = float4{v[s], v[s + 1], v[s + 2], v[s + 3]};
     } else {
 #pragma unroll
       for (int s = 0; s < SP; ++s)
-        if (s < a.states) to[s] = v[s];
+        if (s < states) to[s] = v[s];
     }
   };
   auto clear = [&]() {
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   float sum = 0.0f;
   bool began = false;
   fetch(0);
-  for (int k0 = 0; k0 < count; k0 += kAhead) {
+  auto four = [&](int k0, auto whole) {
     float xv[kAhead], dtv[kAhead], zv[kAhead], bcv[kAhead];
     bool begins[kAhead];
 #pragma unroll
@@ -195,7 +202,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     if (k0 + kAhead < count) fetch(k0 + kAhead);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (k0 + i >= count) break;
+      if (!whole && k0 + i >= count) break;
       float delta = dtv[i] + bias;
       if (a.softplus) delta = softplus(delta);
       float bv[SP], cv[SP];
@@ -233,10 +240,12 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
         if (begins[i]) clear();
         if constexpr (WHAT == FULL) {
           if (a.saved && (k0 + i) % kSegment == 0) {  // pieces begin at multiples of kSegment
+            if (live) {
 #pragma unroll
-            for (int s = 0; s < SP; ++s)
-              if (s < a.states && live) saved[(int64_t)s * a.dim + d] = h[s];
-            saved += (int64_t)a.envs * a.states * a.dim;
+              for (int s = 0; s < SP; ++s)
+                if (s < states) saved[(int64_t)s * a.dim + d] = h[s];
+            }
+            saved += (int64_t)a.envs * states * a.dim;
           }
         }
         const float u = delta * xv[i];
@@ -256,14 +265,19 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
         }
       }
     }
-  }
+  };
+  // (an exit after each of the four would keep copies of the states for it:
+  // 377 us where this takes 325)
+  int k0 = 0;
+  for (; k0 + kAhead <= count; k0 += kAhead) four(k0, std::true_type{});
+  if (k0 < count) four(k0, std::false_type{});
   if (!live) return;
   if constexpr (WHAT == FULL) {
-    if (t1 == a.steps) store_states(a.last + ((int64_t)env * a.dim + d) * a.states, h);
+    if (t1 == a.steps) store_states(a.last + ((int64_t)env * a.dim + d) * states, h);
   } else {
 #pragma unroll
     for (int s = 0; s < SP; ++s)
-      if (s < a.states) ends[((int64_t)item * a.states + s) * a.dim + d] = h[s];
+      if (s < states) ends[((int64_t)item * states + s) * a.dim + d] = h[s];
     // an episode that begins inside lets nothing through: infinity says so
     sums[(int64_t)item * a.dim + d] = began ? __builtin_inff() : sum;
   }
