@@ -399,6 +399,11 @@ constexpr int kGradWaves = 4;  // wavefronts of a workgroup at most
 template <int SP>
 struct GradShape {
   static constexpr int Q = SP / 4, C = 8 / Q, CH = 16 * C;
+  // Last steps of a segment whose decays stay in registers from the way forward
+  // to the way back; the others' are computed twice.  16 states 1,397 us with
+  // none, 1,371 with 2, 1,360 with 4, 1,838 with 8, which spill; 8 states 886,
+  // 877, 987, 1,472 (forward and backward of the rollout above).
+  static constexpr int kKept = SP == 8 ? 2 : 4;
   struct Lds {
     float delta[kSegment][CH], x[kSegment][CH], d[kSegment][CH];
     float through[kSegment][CH], by[kSegment][CH], plain[kSegment][CH];  // sums over states
@@ -431,7 +436,7 @@ __device__ __forceinline__ float fold_rows(float a, float b) {
 template <typename T, int SP>
 __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArgs a, Pieces p, int slots, const float* carried, float* cross_out, float* sums_out) {
   using S = GradShape<SP>;
-  constexpr int Q = S::Q, C = S::C, CH = S::CH, kApart = kWave / CH, kPairs = kSegment / kApart;
+  constexpr int Q = S::Q, C = S::C, CH = S::CH, kOnce = kSegment - S::kKept, kApart = kWave / CH, kPairs = kSegment / kApart;
   extern __shared__ __align__(16) char lds[];
   typename S::Lds* all = reinterpret_cast<typename S::Lds*>(lds);
   const int lane = threadIdx.x & 63, which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
@@ -545,7 +550,7 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
 
       // (an episode's first step takes a branch of its own, the same for all
       // lanes: selecting zeros would keep a second copy of every state)
-      float h[kSegment][C][Q];
+      float h[kSegment][C][Q], kept[S::kKept][C][Q];
 #pragma unroll
       for (int i = 0; i < kSegment; ++i) {
         const bool first = begins >> i & 1u;
@@ -561,7 +566,11 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
 #pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int q = 0; q < Q; ++q) h[i][c][q] = fmaf(i == 0 ? in.before[c][q] : h[i == 0 ? 0 : i - 1][c][q], exp2_fast(delta[c] * A[c][q]), h[i][c][q]);
+            for (int q = 0; q < Q; ++q) {
+              const float decay = exp2_fast(delta[c] * A[c][q]);
+              if (i >= kOnce) kept[i >= kOnce ? i - kOnce : 0][c][q] = decay;
+              h[i][c][q] = fmaf(i == 0 ? in.before[c][q] : h[i == 0 ? 0 : i - 1][c][q], decay, h[i][c][q]);
+            }
         }
         if (gated) {
 #pragma unroll
@@ -597,7 +606,7 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
           for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-              g[c][q] *= exp2_fast(delta[c] * A[c][q]);
+              g[c][q] *= i >= kOnce ? kept[i >= kOnce ? i - kOnce : 0][c][q] : exp2_fast(delta[c] * A[c][q]);
               const float via = g[c][q] * (i == 0 ? in.before[c][q] : h[i == 0 ? 0 : i - 1][c][q]);
               by[c] = fmaf(via, A[c][q], by[c]);
               dA[c][q] = fmaf(via, delta[c], dA[c][q]);
