@@ -57,6 +57,19 @@ struct Pieces {
   int chunk, chunks;             // steps of a piece, pieces
 };
 
+// Up to 8 pieces are joined by FULL itself, each going over those before its
+// own: as a launch between, join_kernel is another 4 us and the host's time for
+// it (forward of 77 steps of 37 envs x 200 channels x 8 states in 5 pieces 21.5
+// -> 18.8 us, 128 of 16 x 512 x 16 in 8 28.6 -> 24.5, 128 of 64 x 512 x 32 in 2
+// 93 -> 85).  The gradient's kernel has no registers left for it.
+constexpr int kFewPieces = 8;
+// What a piece ends with, from the state it starts with (or the gradient,
+// against the steps): `end` from zero and its decay.  An episode that begins
+// inside lets nothing through: its sum of step sizes is given as infinity.
+__device__ __forceinline__ float through_piece(float from, float sum, float decay, float end) {
+  return sum == __builtin_inff() ? end : fmaf(from, exp2_fast(sum * decay), end);
+}
+
 enum { FULL, ENDS, BACK };  // what scan_kernel computes
 
 // A lane is a channel and holds its states; B and C are the same for all lanes
@@ -68,8 +81,8 @@ enum { FULL, ENDS, BACK };  // what scan_kernel computes
 // the steps are cut: ENDS computes, for each piece, the state that it ends
 // with when it starts from zero and the sum of its step sizes, whose decay
 // carries any start state across the piece (h_end = exp(A * sum) * h_start +
-// ends); join_kernel runs over the pieces; FULL then starts each piece from
-// its own state.  BACK is ENDS for the gradient, against the steps: the
+// ends); join_kernel runs over them where they are many; FULL then starts each
+// piece from its own state.  BACK is ENDS for the gradient, against the steps: the
 // gradient of the state before a piece when nothing flows into its end.
 //
 // Bound by the vector units: a state takes an exponential at half rate and four
@@ -104,14 +117,23 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
   }
   const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.skip ? a.skip[d] : 0.0f;
   if constexpr (WHAT == FULL) {
-    if (p.chunks > 1) {
+    if (p.chunks > kFewPieces) {
 #pragma unroll
       for (int s = 0; s < SP; ++s)
         if (s < states) h[s] = ends[((int64_t)item * states + s) * a.dim + d];
-    } else if (a.state) {
+    } else {
+      if (a.state) {
 #pragma unroll
-      for (int s = 0; s < SP; ++s)
-        if (s < states) h[s] = a.state[((int64_t)env * a.dim + d) * states + s];
+        for (int s = 0; s < SP; ++s)
+          if (s < states) h[s] = a.state[((int64_t)env * a.dim + d) * states + s];
+      }
+      for (int j = 0; j < piece; ++j) {
+        const int64_t of = (int64_t)j * a.envs + env;
+        const float sum = sums[of * a.dim + d];
+#pragma unroll
+        for (int s = 0; s < SP; ++s)
+          if (s < states) h[s] = through_piece(h[s], sum, decay[s], ends[(of * states + s) * a.dim + d]);
+      }
     }
   }
 
@@ -278,15 +300,13 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
 #pragma unroll
     for (int s = 0; s < SP; ++s)
       if (s < states) ends[((int64_t)item * states + s) * a.dim + d] = h[s];
-    // an episode that begins inside lets nothing through: infinity says so
     sums[(int64_t)item * a.dim + d] = began ? __builtin_inff() : sum;
   }
 }
 
 // Runs over the pieces, first to last (BACKWARD: last to first), and leaves in
 // `ends` what each piece starts from.  A lane is one env, state and channel, and
-// waits for its loads, 16 pieces at a time: the 5 pieces of 37 envs x 200
-// channels x 8 states take 4 us.
+// waits for its loads, 16 pieces at a time.
 template <bool BACKWARD>
 __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float* ends, const float* sums) {
   const int64_t i = block_id() * 256 + threadIdx.x, each = (int64_t)a.envs * a.states * a.dim;
@@ -308,7 +328,7 @@ __global__ __launch_bounds__(256) void join_kernel(ScanArgs a, int chunks, float
       if (k0 + k >= chunks) break;
       const int piece = BACKWARD ? chunks - 1 - k0 - k : k0 + k;
       ends[piece * each + i] = h;
-      h = sum[k] == __builtin_inff() ? e[k] : fmaf(h, exp2_fast(sum[k] * decay), e[k]);
+      h = through_piece(h, sum[k], decay, e[k]);
     }
   }
 }
@@ -831,6 +851,7 @@ int64_t cross_floats(const Pieces& p, int steps, int envs, int states) {
 template <bool BACKWARD>
 void launch_join(const ScanArgs& a, const Pieces& p, float* ends, const float* sums, hipStream_t st) {
   const int64_t rows = (int64_t)a.envs * a.states;
+  if (!BACKWARD && p.chunks <= kFewPieces) return;
   if (p.chunks >= kManyPieces) {
     const dim3 grid = wide_grid(rows * ((a.dim + kWave - 1) / kWave));
     hipLaunchKernelGGL(join_runs_kernel<BACKWARD>, grid, dim3(kWave * kRuns), 0, st, a, p.chunks, ends, sums);
