@@ -17,6 +17,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
 
 from .._torch_ops import ext
 
@@ -134,7 +135,19 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
         """One update of every parameter that has a gradient.  ``grad_scale``
         (float32, one element, on the device) multiplies the gradients, such as
-        a clipping factor that never leaves the GPU."""
+        a clipping factor that never leaves the GPU.
+
+        Hooks on the step run, and a profiler sees it, as with torch's own
+        optimizers.  Torch's wrapper for both is called only where there are
+        any: it takes as long as the rest of a small policy's step on the host."""
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_optimizer_pre_hooks
+                or _global_optimizer_post_hooks or torch.autograd._profiler_enabled()):  # fmt: skip
+            return _hooked_step(self, closure, grad_scale=grad_scale)
+        return self._step(closure, grad_scale=grad_scale)
+
+    step.hooked = True  # or torch would wrap it for every call
+
+    def _step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -169,3 +182,6 @@ class AdamW(torch.optim.Optimizer):
             group["params"], which, grad_scale, b1, b2, lr / (1 - b1**step), 1.0 / math.sqrt(1 - b2**step),
             group["eps"], 1 - lr * group["weight_decay"], (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
         )  # fmt: skip
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

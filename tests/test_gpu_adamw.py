@@ -255,3 +255,43 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="captured"):
         with torch.cuda.graph(graph):
             opt.step()
+
+
+def test_hooks_and_profiler():
+    """Hooks on the step run once, before and after it, whether the optimizer's
+    own or for all optimizers; a profiler sees the step; a scheduler counts it."""
+    from torch.optim.optimizer import register_optimizer_step_post_hook, register_optimizer_step_pre_hook
+
+    from gbxcule_amd.rl import AdamW
+
+    p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    opt = AdamW([p], lr=0.5)
+    p.grad = torch.ones_like(p)
+    seen = []
+    note = lambda name: lambda o, args, kwargs: seen.append((name, o is opt, opt.state[p]["step"]))  # noqa: E731
+    opt.step()
+    handles = [opt.register_step_pre_hook(note("pre"))]
+    opt.step()
+    assert seen == [("pre", True, 1)]
+    handles.append(opt.register_step_post_hook(note("post")))
+    opt.step()
+    assert seen[1:] == [("pre", True, 2), ("post", True, 3)]
+    for h in handles:
+        h.remove()
+    seen.clear()
+    handles = [register_optimizer_step_pre_hook(note("all pre")), register_optimizer_step_post_hook(note("all post"))]
+    try:
+        opt.step(lambda: seen.append("closure"))
+    finally:
+        for h in handles:
+            h.remove()
+    assert seen == [("all pre", True, 3), "closure", ("all post", True, 4)]
+    opt.step()
+    assert len(seen) == 3 and opt.state[p]["step"] == 5
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any(e.key.startswith("Optimizer.step#AdamW") for e in prof.key_averages())
+    schedule = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.1)
+    opt.step()
+    schedule.step()
+    assert opt.state[p]["step"] == 7 and opt.param_groups[0]["lr"] == pytest.approx(0.05)
