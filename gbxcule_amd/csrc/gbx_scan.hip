@@ -57,12 +57,13 @@ struct Pieces {
   int chunk, chunks;             // steps of a piece, pieces
 };
 
-// Up to 8 pieces are joined by FULL itself, each going over those before its
+// Up to 16 pieces are joined by FULL itself, each going over those before its
 // own: as a launch between, join_kernel is another 4 us and the host's time for
 // it (forward of 77 steps of 37 envs x 200 channels x 8 states in 5 pieces 21.5
-// -> 18.8 us, 128 of 16 x 512 x 16 in 8 28.6 -> 24.5, 128 of 64 x 512 x 32 in 2
-// 93 -> 85).  The gradient's kernel has no registers left for it.
-constexpr int kFewPieces = 8;
+// -> 18.8 us, 128 of 16 x 512 x 16 in 8 28.6 -> 24.5, 256 of them in 16 37.0 ->
+// 34.4, but 512 of 8 x 512 x 16 in 32 36.8 -> 39.0).  The gradient's kernel has
+// no registers left for it.
+constexpr int kFewPieces = 16;
 // What a piece ends with, from the state it starts with (or the gradient,
 // against the steps): `end` from zero and its decay.  An episode that begins
 // inside lets nothing through: its sum of step sizes is given as infinity.
@@ -410,9 +411,9 @@ __global__ __launch_bounds__(kWave* kRuns) void join_runs_kernel(ScanArgs a, int
 // wavefronts of a workgroup take neighbouring channels of the same steps and
 // add their dB and dC in LDS at the end of a segment.
 //
-// Bound by the vector units: 26 instructions a state step, two of them
+// Bound by the vector units: 25 instructions a state step, three in two of them
 // exponentials, which are active three quarters of the time.  128 steps x 1,024
-// envs x 512 channels x 16 states in bf16: 1,075 us, 1.0 T state steps/s.  8
+// envs x 512 channels x 16 states in bf16: 1,030 us, 1.0 T state steps/s.  8
 // elements a lane and 8 steps a segment fill the registers of two wavefronts a
 // SIMD; three spill (2,284 us).
 constexpr int kGradWaves = 4;  // wavefronts of a workgroup at most
