@@ -819,14 +819,17 @@ int padded(int states) { return states <= 8 ? 8 : states <= 16 ? 16 : 32; }
 // more launches take as long as some 40 steps (one row of 16,384 steps: 2,048
 // wavefronts 220 us, 4,096 192, 8,192 208; 4,096 steps of two rows in pieces
 // of at least 8 steps 92 us, 16 67; 40 steps of 16 rows in pieces of 16 30 us,
-// 32 38).
-constexpr int64_t kFull = 1024, kWant = 4096, kLeastPiece = 16;
-Pieces pieces_of(int steps, int envs, int dim, int groups, int channels, int waves_of_block) {
+// 32 38).  A wavefront for each SIMD is not enough up to 16 states (1,024 of
+// them, 128 envs x 512 channels: 128 steps x 16 states 87 us whole, 78 in pieces,
+// 8 states 67 and 54, 1,024 steps x 16 states 670 and 506; 1,504 102 and 104),
+// with 32 it is (122 and 132).
+constexpr int64_t kFull = 1280, kFull32 = 1024, kWant = 4096, kLeastPiece = 16;
+Pieces pieces_of(int steps, int envs, int dim, int groups, int states, int channels, int waves_of_block) {
   Pieces p;
   p.blocks_per_group = (dim / groups + channels * waves_of_block - 1) / (channels * waves_of_block);
   p.blocks = groups * p.blocks_per_group;
   const int64_t waves = (int64_t)envs * p.blocks * waves_of_block;
-  const int64_t cuts = waves >= kFull ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kLeastPiece - 1) / kLeastPiece);
+  const int64_t cuts = waves >= (states <= 16 ? kFull : kFull32) ? 1 : std::min<int64_t>((kWant + waves - 1) / waves, (steps + kLeastPiece - 1) / kLeastPiece);
   const int64_t each = (steps + cuts - 1) / cuts;
   p.chunk = (int)((each + kSegment - 1) / kSegment * kSegment);
   p.chunks = (steps + p.chunk - 1) / p.chunk;
@@ -842,7 +845,7 @@ int grad_slots(const Pieces& p, int envs, int waves) {
   return (int)std::min<int64_t>((int64_t)p.chunks * envs, std::max<int64_t>(1, 4096 / (p.blocks * waves)));
 }
 Pieces grad_pieces(int steps, int envs, int dim, int groups, int states) {
-  return pieces_of(steps, envs, dim, groups, 512 / padded(states), grad_waves(dim, groups, states));
+  return pieces_of(steps, envs, dim, groups, states, 512 / padded(states), grad_waves(dim, groups, states));
 }
 // dB and dC by channel block, where a group has several
 int64_t cross_floats(const Pieces& p, int steps, int envs, int states) {
@@ -874,12 +877,12 @@ void launch_scan_kernel(const ScanArgs& a, const Pieces& p, float* ends, float* 
 }  // namespace
 
 int64_t scan_work(int steps, int envs, int dim, int groups, int states) {
-  const Pieces p = pieces_of(steps, envs, dim, groups, kWave, 1);
+  const Pieces p = pieces_of(steps, envs, dim, groups, states, kWave, 1);
   return p.chunks > 1 ? (int64_t)p.chunks * envs * dim * (states + 1) : 0;
 }
 
 hipError_t launch_scan(const ScanArgs& a, hipStream_t st) {
-  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, kWave, 1);
+  const Pieces p = pieces_of(a.steps, a.envs, a.dim, a.groups, a.states, kWave, 1);
   float *ends = a.work, *sums = a.work + (int64_t)p.chunks * a.envs * a.dim * a.states;
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
