@@ -534,7 +534,9 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
           to.c[k] = cp[t * a.c_step];
         }
       }
-      to.begins = a.resets && lane < live_steps ? a.resets[(int64_t)(seg + lane) * a.envs + env] : 0;
+      // steps past the end are cut off as an episode's first is: what the last
+      // state holds, finite or not, reaches no sum through them
+      to.begins = lane >= live_steps ? 1 : a.resets ? a.resets[(int64_t)(seg + lane) * a.envs + env] : 0;
       const float* saved = a.saved + ((int64_t)(seg / kSegment) * a.envs + env) * a.dim * a.states;
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
       const int live_steps = min(kSegment, a.steps - seg);
       in = next;
       const uint32_t begins = (uint32_t)__ballot(in.begins != 0);
-      // prepare: steps past the end neither push nor decay, and nothing comes from them
+      // prepare: steps past the end push nothing, and nothing comes from them
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
         const int i = own_i + k * kApart;
