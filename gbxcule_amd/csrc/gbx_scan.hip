@@ -471,14 +471,17 @@ __global__ __launch_bounds__(kWave* kGradWaves, 2) void scan_grad_kernel(ScanArg
   const bool own_live = base + own < per_group, gated = a.z != nullptr;
   const float bias = a.bias ? a.bias[own_d] : 0.0f, skip = a.skip ? a.skip[own_d] : 0.0f;
 
-  float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;  // A in powers of two
+  // A in powers of two.  Lanes past the last channel or state hold its rate, so
+  // that a step of infinite size makes a zero of their decay too; with a rate of
+  // zero it would be NaN, and sums over lanes with it.
+  float A[C][Q], dA[C][Q], dskip = 0.0f, dbias = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int ch = base + cg * C + c;
+    const int ch = min(base + cg * C + c, per_group - 1);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int s = sg * Q + q;
-      A[c][q] = ch < per_group && s < a.states ? a.a[(int64_t)(first_d + ch) * a.states + s] * kLog2e : 0.0f;
+      const int s = min(sg * Q + q, a.states - 1);
+      A[c][q] = a.a[(int64_t)(first_d + ch) * a.states + s] * kLog2e;
       dA[c][q] = 0.0f;
     }
   }

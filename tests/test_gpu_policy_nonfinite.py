@@ -44,3 +44,29 @@ def test_scan_gradient_of_a_last_step_that_is_left_out(steps, states, dtype, bad
     assert torch.equal(got["A"], want["A"])  # the last state decays into nothing
     for k in ("x", "dt", "B", "C", "z"):
         assert torch.equal(got[k][fine], want[k][fine]), k
+
+
+@pytest.mark.parametrize("states", [8, 12, 20])
+def test_scan_gradient_of_an_infinite_step_size_that_is_left_out(states):
+    """One channel forgets everything in a step of infinite size, as it does in
+    one of size 300 (e^-300 is zero in 32 bits); that step is left out of the
+    loss and an episode begins after it.  33 channels leave lanes of the kernel
+    without one, 12 and 20 states without a state."""
+    case = (24, 2, 33, states, 1, F32, 0.0, True, True, True, True, True)
+    gen, t, state, _ = _scan_inputs(case)
+    t["A"] = -1.0 - torch.rand(33, states, device="cuda", generator=gen)
+    resets = torch.zeros(24, 2, dtype=torch.bool, device="cuda")
+    resets[12, 0] = True
+    dy = _randn(gen, 24, 2, 33)
+    dy[11, 0] = 0
+    got = {}
+    for size in (300.0, float("inf")):
+        t["dt"] = t["dt"].clone()
+        t["dt"][11, 0, 32] = size
+        got[size] = _gradients(t, dy, state, resets)
+    fine = torch.ones(24, 2, dtype=torch.bool, device="cuda")
+    fine[11, 0] = False
+    for k in ("x", "dt", "B", "C", "z"):
+        assert torch.isfinite(got[300.0][k]).all()
+        assert torch.equal(got[float("inf")][k][fine], got[300.0][k][fine]), k
+    assert torch.equal(got[float("inf")]["A"][:32], got[300.0]["A"][:32])
