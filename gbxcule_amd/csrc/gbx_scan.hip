@@ -66,9 +66,11 @@ struct Pieces {
 constexpr int kFewPieces = 16;
 // What a piece ends with, from the state it starts with (or the gradient,
 // against the steps): `end` from zero and its decay.  An episode that begins
-// inside lets nothing through: its sum of step sizes is given as infinity.
+// inside lets nothing through: its sum of step sizes is given as infinity.  A
+// start of zero adds nothing, also where the growth over a piece (rates or step
+// sizes of the other sign) passes 32 bits.
 __device__ __forceinline__ float through_piece(float from, float sum, float decay, float end) {
-  return sum == __builtin_inff() ? end : fmaf(from, exp2_fast(sum * decay), end);
+  return sum == __builtin_inff() || from == 0.0f ? end : fmaf(from, exp2_fast(sum * decay), end);
 }
 
 enum { FULL, ENDS, BACK };  // what scan_kernel computes
@@ -350,9 +352,10 @@ __global__ __launch_bounds__(kWave* kRuns) void join_runs_kernel(ScanArgs a, int
   const int s = (int)(row % a.states), env = (int)(row / a.states);
   const float decay = a.a[(int64_t)d * a.states + s] * kLog2e;
   float h = !BACKWARD && a.state ? a.state[((int64_t)env * a.dim + d) * a.states + s] : 0.0f;
-  // (an episode that begins in a piece lets nothing through, whatever lies before)
+  // (as through_piece: an episode that begins in a piece lets nothing through,
+  // whatever lies before, and zero adds nothing)
   constexpr float kNothing = -1.0f;
-  const auto pass = [&](float from, float by, float end) { return by < 0.0f ? end : fmaf(from, by, end); };
+  const auto pass = [&](float from, float by, float end) { return by < 0.0f || from == 0.0f ? end : fmaf(from, by, end); };
   for (int first = 0; first < chunks; first += kRuns * kRun) {
     const int count = min(kRuns * kRun, chunks - first), per = (count + kRuns - 1) / kRuns;
     const int mine = max(0, min(per, count - run * per));

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from . import _policy_ref as ref
 from .conftest import require_gpu
 from .test_gpu_policy_ops import BF16, F32, NAMES, _gen, _leaf, _randn, _scan_inputs
 
@@ -70,3 +71,29 @@ def test_scan_gradient_of_an_infinite_step_size_that_is_left_out(states):
         assert torch.isfinite(got[300.0][k]).all()
         assert torch.equal(got[float("inf")][k][fine], got[300.0][k][fine]), k
     assert torch.equal(got[float("inf")]["A"][:32], got[300.0]["A"][:32])
+
+
+@pytest.mark.parametrize("steps", [64, 300, 1100])  # 4, 19 and 69 pieces: joined by the pass itself, in a row and in runs
+def test_growth_of_nothing_is_nothing(steps):
+    """States that grow by e^8 a step hold nothing until the last two steps
+    push: over 16 steps the growth alone is e^128, beyond 32 bits.  The same
+    against the steps for the gradient, where only the first two count."""
+    from gbxcule_amd.rl import selective_scan
+
+    gen = _gen(steps)
+    x, b, c = _randn(gen, steps, 1, 40), _randn(gen, steps, 1, 16), _randn(gen, steps, 1, 16)
+    x[:-2] = 0
+    dt = torch.ones_like(x)
+    rate = torch.full((40, 16), 8.0, device="cuda")
+    dy = _randn(gen, steps, 1, 40)
+    dy[2:] = 0
+    x, dt, rate, b, c = _leaf(x, dt, rate, b, c)
+    y, last = selective_scan(x, dt, rate, b, c, softplus=False)
+    wide = [ref.f64(v) for v in (x, dt, rate, b.unsqueeze(2), c.unsqueeze(2))]
+    want, want_last = ref.selective_scan(*wide, None, None, None, False, None, None)
+    ref.check(y, want, 128, "y")
+    ref.check(last, want_last, 128, "state")
+    got = torch.autograd.grad(y, (x, dt, rate, b, c), dy)
+    exact = torch.autograd.grad(want, wide, ref.f64(dy))
+    for g, v, name in zip(got, exact, ("x", "dt", "A", "B", "C")):
+        ref.check(g, v.view(g.shape), 256, f"gradient of {name}")
