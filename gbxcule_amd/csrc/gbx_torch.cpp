@@ -84,6 +84,11 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 const Tensor* opt(const Maybe& t) { return t ? &*t : nullptr; }
+// (a tangent would be dropped where no autograd function is called: a derivative
+// of zero)
+void no_tangent(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }  // undefined: not given
 // (autograd's functions take what is not given as no argument, not as an undefined tensor)
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
@@ -169,6 +174,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 
 std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& weight, const Maybe& residual, double eps) {
   const int elem = input("x", x);
+  no_tangent("rms_norm", {&x, &weight, opt(residual)});
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x: expected [..., channels], got ", x.sizes());
   const Tensor w = param("weight", weight, x, {x.size(-1)}), r = given(like("residual", residual, x, x.sizes()));
   if (wants_grad({&x, &w, &r})) return RmsNorm::apply(x, w, maybe(r), eps, (int64_t)elem);
@@ -179,6 +185,7 @@ std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& weight, const Maybe&
 std::vector<Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const Maybe& residual, double eps, int64_t group) {
   const int elem = input("x", x);
   no_grad("rms_norm_fp8", {&x, &weight, opt(residual)});
+  no_tangent("rms_norm_fp8", {&x, &weight, opt(residual)});
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x: expected [..., channels], got ", x.sizes());
   const Tensor w = param("weight", weight, x, {x.size(-1)}), r = given(like("residual", residual, x, x.sizes()));
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
@@ -223,6 +230,7 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
 
 std::vector<Tensor> causal_conv(const Tensor& x_, const Tensor& weight, const Maybe& bias, const Maybe& state, const Maybe& resets, bool silu) {
   const int elem = input("x", x_);
+  no_tangent("causal_conv", {&x_, &weight, opt(bias), opt(state)});
   TORCH_CHECK_VALUE(x_.dim() == 3 && x_.size(2) >= 1, "x: expected [steps, envs, channels], got ", x_.sizes());
   check_width(weight);
   const Tensor x = rows(x_);
@@ -241,6 +249,7 @@ std::vector<Tensor> causal_conv(const Tensor& x_, const Tensor& weight, const Ma
 Tensor causal_conv_step(const Tensor& x_, const Tensor& weight, const Maybe& bias, const Tensor& state, const Maybe& resets, bool silu) {
   const int elem = input("x", x_);
   no_grad("causal_conv_step", {&x_, &weight, opt(bias), &state});
+  no_tangent("causal_conv_step", {&x_, &weight, opt(bias), &state});
   TORCH_CHECK_VALUE(x_.dim() == 2 && x_.size(1) >= 1, "x: expected [envs, channels], got ", x_.sizes());
   check_width(weight);
   const Tensor x = rows(x_);
@@ -329,6 +338,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
 std::vector<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor& b, const Tensor& c, const Maybe& skip, const Maybe& z, const Maybe& bias, bool softplus,
                                    const Maybe& state, const Maybe& resets) {
   const int elem = input("x", x);
+  no_tangent("selective_scan", {&x, &dt, &a, &b, &c, opt(skip), opt(z), opt(bias), opt(state)});
   TORCH_CHECK_VALUE(x.dim() == 3 && x.size(2) >= 1, "x: expected [steps, envs, channels], got ", x.sizes());
   const Scan s = scan_operands(x, dt, a, b, c, skip, z, bias, resets);
   TORCH_CHECK_VALUE(!wants_grad({opt(state)}), "state carries no gradient: detach it");
@@ -345,6 +355,7 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, c
                            bool softplus, const Maybe& resets) {
   const int elem = input("x", x);
   no_grad("selective_scan_step", {&x, &dt, &a, &b, &c, opt(skip), opt(z), &state, opt(bias)});
+  no_tangent("selective_scan_step", {&x, &dt, &a, &b, &c, opt(skip), opt(z), &state, opt(bias)});
   TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= 1, "x: expected [envs, channels], got ", x.sizes());
   const Scan s = scan_operands(x, dt, a, b, c, skip, z, bias, resets);
   state_of(state, x, at::kFloat, {x.size(0), x.size(1), s.a.size(1)});

@@ -8,9 +8,10 @@ of N envs.  ``resets`` (bool or uint8 ``[T, N]``) is set where an env begins an
 episode at that step: nothing from before reaches it, whatever it holds, so
 episodes of any length lie one after the other in a row.
 
-The whole-rollout forms are differentiable, once (the learner); the carried
-state is not: gradients stop where a rollout begins.  ``*_step`` is the actor's
-form, one step of every env with the state updated in place.
+The whole-rollout forms are differentiable, once and in reverse (the learner); a
+tangent of forward mode raises ``NotImplementedError``.  The carried state is
+not differentiable: gradients stop where a rollout begins.  ``*_step`` is the
+actor's form, one step of every env with the state updated in place.
 
 Inputs are CUDA tensors of float32, bfloat16 or float16 whose last dimension
 is contiguous (others are copied); other dimensions may have any stride, so
