@@ -118,6 +118,9 @@ Tensor work(const Tensor& x, int64_t count) {
   check(count);
   return count ? floats(x, {count}) : Tensor();
 }
+// Tells autograd that t changes in place; before the launch, since it raises
+// where t may not (an inference tensor outside inference mode).
+void will_change(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the policy operators are differentiable once: no create_graph"); }
 
 // ------------------------------------------------------------------ the norm
@@ -260,8 +263,8 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& weight, const Maybe& bia
   const Tensor begins = given(starts(resets, x, {envs})), y = blank(x);
   if (envs) {
     const c10::DeviceGuard guard(x.device());
+    will_change(state);
     check(gbx_causal_conv_step(narrow("envs", envs), narrow("channels", dim), (int)width, elem, silu, in(x), x.stride(0), fin(w), fin(b), out(state), bytes(begins), out(y), stream(x)));
-    state.unsafeGetTensorImpl()->bump_version();
   }
   return y;
 }
@@ -364,8 +367,8 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, c
   if (x.size(0)) {
     const c10::DeviceGuard guard(x.device());
     const gbx_scan_in g = scan_in(s, softplus, elem);
+    will_change(state);
     check(gbx_selective_scan_step(&g, fout(state), out(y), stream(x)));
-    state.unsafeGetTensorImpl()->bump_version();
   }
   return y;
 }
@@ -419,8 +422,8 @@ struct AdamwPlan {
     a.exp_avg = out(exp_avg), a.exp_avg_sq = out(exp_avg_sq), a.exp_avg_scale = fout(exp_avg_scale), a.exp_avg_sq_scale = fout(exp_avg_sq_scale);
     a.grad_scale = grad_scale ? fin(*grad_scale) : nullptr;
     a.beta1 = beta1, a.beta2 = beta2, a.step_size = step_size, a.inv_root2 = inv_root2, a.eps = eps, a.keep = keep, a.key = key;
+    for (size_t k = 0; k < count; ++k) will_change(params[which.empty() ? k : (size_t)which[k]]);
     check(gbx_adamw(&a, stream(exp_avg)));
-    for (size_t k = 0; k < count; ++k) params[which.empty() ? k : (size_t)which[k]].unsafeGetTensorImpl()->bump_version();
     return true;
   }
 };

@@ -49,3 +49,22 @@ def test_forward_mode_is_refused(which, grad):
                 call(*tensors[:k], dual, *tensors[k + 1 :])
         assert torch.equal(tensors[-1], kept), (name, k)
     call(*tensors)
+
+
+def test_a_state_that_may_not_be_changed_is_not():
+    """torch refuses to change an inference tensor outside inference mode."""
+    for name, call, tensors in _calls():
+        if not name.endswith("_step"):
+            continue
+        with torch.inference_mode():
+            state = tensors[-1].clone()
+            kept = state.clone()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="inference"):
+            call(*tensors[:-1], state)
+        torch.cuda.synchronize()
+        assert torch.equal(state, kept), name
+        with torch.inference_mode():
+            y = call(*tensors[:-1], state)
+        mine = tensors[-1].clone()
+        version = mine._version
+        assert torch.equal(call(*tensors[:-1], mine), y) and torch.equal(mine, state) and mine._version > version, name
