@@ -113,6 +113,9 @@ const uint8_t* bytes(const Tensor& t) { return (const uint8_t*)in(t); }
 void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 Tensor floats(const Tensor& x, IntArrayRef shape) { return at::empty(shape, x.options().dtype(at::kFloat)); }
 Tensor blank(const Tensor& t) { return t.defined() ? at::empty(t.sizes(), t.options()) : Tensor(); }
+Tensor zeros(const Tensor& t) { return t.defined() ? at::zeros(t.sizes(), t.options()) : Tensor(); }
+// after no steps: what was there before, or zeros
+Tensor unmoved(const Tensor& state, const Tensor& like) { return state.defined() ? state.clone() : zeros(like); }
 // scratch memory, from the caching allocator like the outputs
 Tensor work(const Tensor& x, int64_t count) {
   check(count);
@@ -205,9 +208,14 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     const Tensor bias = given(bias_), state = given(state_), resets = given(resets_);
     ctx->set_materialize_grads(false);
     const c10::DeviceGuard guard(x.device());
-    const Tensor y = blank(x), last = at::empty({x.size(1), weight.size(1) - 1, x.size(2)}, x.options());
-    check(gbx_causal_conv(narrow("steps", x.size(0)), narrow("envs", x.size(1)), narrow("channels", x.size(2)), (int)weight.size(1), (int)elem, (int)silu, in(x),
-                          x.stride(0), x.stride(1), fin(weight), fin(bias), in(state), bytes(resets), out(y), out(last), stream(x)));
+    const Tensor y = blank(x);
+    Tensor last = at::empty({x.size(1), weight.size(1) - 1, x.size(2)}, x.options());
+    if (x.numel() == 0) {
+      last = unmoved(state, last);
+    } else {
+      check(gbx_causal_conv(narrow("steps", x.size(0)), narrow("envs", x.size(1)), narrow("channels", x.size(2)), (int)weight.size(1), (int)elem, (int)silu, in(x),
+                            x.stride(0), x.stride(1), fin(weight), fin(bias), in(state), bytes(resets), out(y), out(last), stream(x)));
+    }
     ctx->save_for_backward({x, weight, bias, state, resets});
     ctx->saved_data["silu"] = silu;
     ctx->saved_data["elem"] = elem;
@@ -221,6 +229,10 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &resets = saved[4];
     const c10::DeviceGuard guard(x.device());
+    if (x.numel() == 0) {
+      for (int i = 0; i < 3; ++i) result[i] = zeros(saved[i]);
+      return result;
+    }
     const int32_t steps = (int32_t)x.size(0), envs = (int32_t)x.size(1), dim = (int32_t)x.size(2), width = (int32_t)weight.size(1);
     const Tensor dy = rows(grads[0]), dx = blank(x), dweight = blank(weight), dbias = blank(bias);
     const Tensor scratch = work(x, gbx_causal_conv_grad_work(steps, envs, dim, width));
@@ -242,10 +254,6 @@ std::vector<Tensor> causal_conv(const Tensor& x_, const Tensor& weight, const Ma
   TORCH_CHECK_VALUE(!wants_grad({opt(state)}), "state carries no gradient: detach it");
   const Tensor before = state ? state_of(*state, x, x.scalar_type(), {envs, width - 1, dim}).contiguous() : Tensor();
   const Tensor begins = given(starts(resets, x, {steps, envs}));
-  if (x.numel() == 0) {
-    const Tensor last = state ? before.clone() : at::zeros({envs, width - 1, dim}, x.options());
-    return {x * w.sum().to(x.scalar_type()), last};  // empty, with the inputs' graph
-  }
   return CausalConv::apply(x, w, maybe(b), maybe(before), maybe(begins), (int64_t)silu, (int64_t)elem);
 }
 
@@ -302,8 +310,9 @@ Scan scan_operands(const Tensor& x_, const Tensor& dt, const Tensor& a, const Te
 variable_list scan_forward(const Scan& s, const Tensor& state, bool softplus, int elem, bool save) {
   const c10::DeviceGuard guard(s.x.device());
   const int64_t steps = s.x.size(0), envs = s.x.size(1), dim = s.x.size(2), states = s.a.size(1);
-  const gbx_scan_in g = scan_in(s, softplus, elem);
   const Tensor y = blank(s.x), last = floats(s.x, {envs, dim, states}), saved = save ? floats(s.x, {(steps + 7) / 8, envs, states, dim}) : Tensor();
+  if (s.x.numel() == 0) return {y, unmoved(state, last), saved};
+  const gbx_scan_in g = scan_in(s, softplus, elem);
   const Tensor scratch = work(s.x, gbx_selective_scan_work(&g));
   check(gbx_selective_scan(&g, fin(state), out(y), fout(last), fout(saved), fout(scratch), stream(s.x)));
   return {y, last, saved};
@@ -328,6 +337,10 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
     const auto v = ctx->get_saved_variables();
     const Scan s{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8]};
     const c10::DeviceGuard guard(s.x.device());
+    if (s.x.numel() == 0) {
+      for (int i = 0; i < 8; ++i) result[i] = zeros(v[i]);
+      return result;
+    }
     const gbx_scan_in g = scan_in(s, ctx->saved_data["softplus"].toBool(), (int)ctx->saved_data["elem"].toInt());
     const Tensor dy = rows(grads[0]);
     for (int i = 0; i < 8; ++i) result[i] = blank(v[i]);
@@ -347,7 +360,6 @@ std::vector<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Tens
   TORCH_CHECK_VALUE(!wants_grad({opt(state)}), "state carries no gradient: detach it");
   const std::vector<int64_t> kept{x.size(1), x.size(2), s.a.size(1)};
   const Tensor before = state ? state_of(*state, x, at::kFloat, kept).contiguous() : Tensor();
-  if (x.numel() == 0) return {s.x * 0, state ? before.clone() : at::zeros(kept, x.options().dtype(at::kFloat))};
   if (wants_grad({&s.x, &s.dt, &s.a, &s.b, &s.c, &s.skip, &s.z, &s.bias}))
     return SelectiveScan::apply(s.x, s.dt, s.a, s.b, s.c, maybe(s.skip), maybe(s.z), maybe(s.bias), maybe(before), maybe(s.resets), softplus, (int64_t)elem);
   const variable_list r = scan_forward(s, before, softplus, elem, false);

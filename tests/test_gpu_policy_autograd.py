@@ -7,7 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 from .conftest import require_gpu
-from .test_gpu_policy_ops import _gen, _randn
+from .test_gpu_policy_ops import BF16, F32, _gen, _leaf, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,37 @@ def test_a_state_that_may_not_be_changed_is_not():
         mine = tensors[-1].clone()
         version = mine._version
         assert torch.equal(call(*tensors[:-1], mine), y) and torch.equal(mine, state) and mine._version > version, name
+
+
+@pytest.mark.parametrize("steps, envs", [(0, 3), (4, 0), (0, 0)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_empty_rollouts_keep_their_graph(steps, envs, dtype):
+    """As with torch's operators: gradients of the inputs' shapes, zero for parameters."""
+    from gbxcule_amd.rl import causal_conv, rms_norm, selective_scan
+
+    g = _gen(2)
+    rows = lambda d: _randn(g, steps, envs, d, dtype=dtype)  # noqa: E731
+    resets = torch.zeros(steps, envs, dtype=torch.bool, device="cuda")
+    window, h = _randn(g, envs, 3, 16, dtype=dtype), _randn(g, envs, 16, 8)
+    norm = _leaf(rows(16), _randn(g, 16), rows(16))
+    conv = _leaf(rows(16), _randn(g, 16, 4, dtype=BF16), _randn(g, 16))
+    scan = _leaf(rows(16), rows(16), _randn(g, 16, 8), rows(8), rows(8), _randn(g, 16), rows(16), _randn(g, 16))
+    for state in (True, False):
+        results = [
+            (norm, rms_norm(*norm)[0]),
+            (conv, *causal_conv(*conv, state=window if state else None, resets=resets)),
+            (scan, *selective_scan(*scan[:7], dt_bias=scan[7], state=h if state else None, resets=resets)),
+        ]
+        for (leaves, y, *last), kept in zip(results, (None, window, h)):
+            assert y.shape == (steps, envs, 16) and y.dtype is dtype and y.requires_grad
+            if last:
+                assert last[0].shape == kept.shape and last[0].dtype is kept.dtype and not last[0].requires_grad
+                assert torch.equal(last[0], kept if state else torch.zeros_like(kept)) and (envs == 0 or last[0].data_ptr() != kept.data_ptr())
+            for v, t in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), leaves):
+                assert v.shape == t.shape and v.dtype is t.dtype and not v.any()
+    # a parameter alone wants a gradient
+    for k in (2, 5, 7):
+        one = [t.detach() for t in scan]
+        one[k].requires_grad_()
+        selective_scan(*one[:7], dt_bias=one[7])[0].sum().backward()
+        assert one[k].grad is not None and not one[k].grad.any()
