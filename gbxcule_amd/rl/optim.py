@@ -15,6 +15,7 @@ rounding to zero.
 from __future__ import annotations
 
 import math
+from collections import defaultdict
 
 import torch
 from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
@@ -104,6 +105,22 @@ class AdamW(torch.optim.Optimizer):
         for p in self.param_groups[group]["params"]:
             self.state[p]["step"] = int(step)
 
+    def __getstate__(self):
+        # (pickle takes 8-bit moments as bytes only)
+        plain = lambda t: t.view(torch.uint8) if torch.is_tensor(t) and t.itemsize == 1 else t  # noqa: E731
+        state = {p: {key: plain(t) for key, t in s.items()} for p, s in self.state.items()}
+        return {**super().__getstate__(), "state": state, "state_bits": self.state_bits, "seed": self.seed}
+
+    def __setstate__(self, state) -> None:
+        """Copies (``copy.deepcopy``, pickle) get flat buffers of their own."""
+        super().__setstate__(state)
+        kept, self.state = self.state, defaultdict(dict)
+        self._flat, self._plans, self._states = [], [], []
+        for group in self.param_groups:
+            self._lay_out(group["params"])
+            for p, mine in zip(group["params"], self._states[-1]):
+                _copy_state(mine, {key: kept[p][key] if key == "step" else kept[p][key].view(t.dtype) for key, t in mine.items()})
+
     def state_dict(self):
         """As torch's, with ``state_bits`` and ``seed``."""
         return {**super().state_dict(), "state_bits": self.state_bits, "seed": self.seed}
@@ -124,10 +141,7 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"{key} of parameter {index} has another shape or type")
                 plan.append((mine, theirs))
         for mine, theirs in plan:
-            mine["step"] = int(theirs["step"])
-            for key, t in mine.items():
-                if key != "step":
-                    t.copy_(theirs[key])
+            _copy_state(mine, theirs)
         for g, s in zip(groups, saved):
             g.update({k: v for k, v in s.items() if k != "params"})
         self.seed = int(state_dict["seed"])
@@ -182,6 +196,14 @@ class AdamW(torch.optim.Optimizer):
             group["params"], which, grad_scale, b1, b2, lr / (1 - b1**step), 1.0 / math.sqrt(1 - b2**step),
             group["eps"], 1 - lr * group["weight_decay"], (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
         )  # fmt: skip
+
+
+def _copy_state(mine: dict, theirs: dict) -> None:
+    """A parameter's step and moments, into the views of the flat buffers."""
+    for key, t in mine.items():
+        if key != "step":
+            t.copy_(theirs[key])
+    mine["step"] = int(theirs["step"])
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

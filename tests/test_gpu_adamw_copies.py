@@ -1,0 +1,94 @@
+"""AdamW as torch's optimizers are used beside ``step``: copied, pickled,
+loaded with hooks, over parameters of several types and in several groups."""
+
+from __future__ import annotations
+
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from .conftest import require_gpu
+from .test_gpu_adamw import BF16, F32, _params
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    require_gpu()
+
+
+def _gradients(params, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    for p in params:
+        p.grad = torch.randn(p.shape, device="cuda", generator=gen).to(p.dtype)
+
+
+def _two_groups(bits, seed=4):
+    from gbxcule_amd.rl import AdamW
+
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    params = _params(gen, F32) + _params(gen, BF16, [(300,), (7, 9)])
+    groups = [{"params": params[:5], "lr": 0.01}, {"params": params[5:], "weight_decay": 0.2}]
+    return params, AdamW(groups, lr=0.003, betas=(0.8, 0.95), state_bits=bits, seed=seed)
+
+
+def _all(opt):
+    return [p for g in opt.param_groups for p in g["params"]]
+
+
+def _pickled(opt):
+    return pickle.loads(pickle.dumps(opt))
+
+
+def _saved(opt):
+    file = io.BytesIO()
+    torch.save(opt, file)
+    file.seek(0)
+    return torch.load(file, weights_only=False)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("way", [copy.deepcopy, _pickled, _saved])
+def test_a_copy_steps_as_the_original_does(bits, way):
+    params, one = _two_groups(bits)
+    for t in range(3):
+        _gradients(params, t)
+        one.step()
+    two = way(one)
+    assert type(two) is type(one) and two.state_bits == bits and two.seed == 4
+    assert all(p is not q and torch.equal(p, q) for p, q in zip(_all(one), _all(two)))
+    for g in range(2):
+        for (k, a), b in zip(one.flat_state(g).items(), two.flat_state(g).values()):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) and a.data_ptr() != b.data_ptr(), k
+    before = [p.detach().clone() for p in params]
+    _gradients(_all(two), 3)
+    two.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, before))  # the original's are its own
+    assert all(s["step"] == 3 for s in one.state.values()) and all(s["step"] == 4 for s in two.state.values())
+    _gradients(params, 3)
+    one.step()
+    for p, q in zip(_all(one), _all(two)):
+        assert torch.equal(p, q)
+        for k, v in one.state[p].items():
+            mine = two.state[q][k]
+            assert v == mine if k == "step" else torch.equal(v.float(), mine.float()), k
+    two.load_state_dict(one.state_dict())
+    two.add_param_group({"params": [torch.nn.Parameter(torch.ones(5, device="cuda"))]})
+    _gradients(_all(two), 4)
+    two.step()
+
+
+def test_a_shallow_copy_leaves_the_original_alone():
+    params, one = _two_groups(32)
+    _gradients(params, 0)
+    one.step()
+    copy.copy(one)
+    moments = [one.state[p]["exp_avg"].clone() for p in params]
+    one.step()
+    for p, m in zip(params, moments):
+        if p.numel():
+            assert not torch.equal(one.state[p]["exp_avg"], m)
