@@ -126,7 +126,12 @@ class AdamW(torch.optim.Optimizer):
         return {**super().state_dict(), "state_bits": self.state_bits, "seed": self.seed}
 
     def load_state_dict(self, state_dict) -> None:
-        """Copies the moments into the flat buffers; hyperparameters as torch does."""
+        """Copies the moments into the flat buffers; hyperparameters and the
+        hooks on loading as torch does."""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups, saved = self.param_groups, state_dict["param_groups"]
         if state_dict.get("state_bits") != self.state_bits:
             raise ValueError(f"a state of {state_dict.get('state_bits')} bits does not fit state_bits={self.state_bits}")
@@ -145,6 +150,8 @@ class AdamW(torch.optim.Optimizer):
         for g, s in zip(groups, saved):
             g.update({k: v for k, v in s.items() if k != "params"})
         self.seed = int(state_dict["seed"])
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
         """One update of every parameter that has a gradient.  ``grad_scale``

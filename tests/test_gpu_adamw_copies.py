@@ -92,3 +92,20 @@ def test_a_shallow_copy_leaves_the_original_alone():
     for p, m in zip(params, moments):
         if p.numel():
             assert not torch.equal(one.state[p]["exp_avg"], m)
+
+
+def test_load_hooks_run():
+    params, one = _two_groups(32)
+    _gradients(params, 0)
+    one.step()
+    kept = one.state_dict()
+    seen = []
+
+    def faster(opt, state):
+        seen.append(("pre", opt is one, state is not kept))
+        return {**state, "param_groups": [{**g, "lr": 9.0} for g in state["param_groups"]]}
+
+    one.register_load_state_dict_pre_hook(faster)
+    one.register_load_state_dict_post_hook(lambda opt: seen.append(("post", opt is one, opt.param_groups[0]["lr"])))
+    one.load_state_dict(kept)
+    assert seen == [("pre", True, True), ("post", True, 9.0)] and kept["param_groups"][0]["lr"] == 0.01
