@@ -127,21 +127,27 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """Copies the moments into the flat buffers; hyperparameters and the
-        hooks on loading as torch does."""
+        hooks on loading as torch does.  A state that does not fit raises
+        ``ValueError`` and changes nothing."""
         state_dict = dict(state_dict)
         for hook in self._optimizer_load_state_dict_pre_hooks.values():
             changed = hook(self, state_dict)
             state_dict = state_dict if changed is None else changed
+        absent = {"param_groups", "state", "state_bits", "seed"} - set(state_dict)
+        if absent:
+            raise ValueError(f"the state has no {', '.join(sorted(absent))}")
         groups, saved = self.param_groups, state_dict["param_groups"]
-        if state_dict.get("state_bits") != self.state_bits:
-            raise ValueError(f"a state of {state_dict.get('state_bits')} bits does not fit state_bits={self.state_bits}")
+        if state_dict["state_bits"] != self.state_bits:
+            raise ValueError(f"a state of {state_dict['state_bits']} bits does not fit state_bits={self.state_bits}")
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("the state's parameter groups are not this optimizer's")
         plan = []
         for g, s in zip(groups, saved):
             for p, index in zip(g["params"], s["params"]):
-                mine, theirs = self.state[p], state_dict["state"][index]
+                mine, theirs = self.state[p], state_dict["state"].get(index, {})
                 for key, t in mine.items():
+                    if key not in theirs:
+                        raise ValueError(f"the state has no {key} of parameter {index}")
                     if key != "step" and (theirs[key].shape != t.shape or theirs[key].dtype is not t.dtype):
                         raise ValueError(f"{key} of parameter {index} has another shape or type")
                 plan.append((mine, theirs))

@@ -109,3 +109,23 @@ def test_load_hooks_run():
     one.register_load_state_dict_post_hook(lambda opt: seen.append(("post", opt is one, opt.param_groups[0]["lr"])))
     one.load_state_dict(kept)
     assert seen == [("pre", True, True), ("post", True, 9.0)] and kept["param_groups"][0]["lr"] == 0.01
+
+
+def test_a_state_with_something_missing_is_refused_whole():
+    params, one = _two_groups(8)
+    _gradients(params, 0)
+    one.step()
+    kept = copy.deepcopy(one.state_dict())
+    _gradients(params, 1)
+    one.step()
+    now = {k: v.float().clone() for k, v in one.flat_state().items()}
+    for spoil in (lambda s: s["state"].pop(3), lambda s: s["state"][2].pop("exp_avg_scale"), lambda s: s["state"][2].pop("step"), lambda s: s.pop("seed"),
+                  lambda s: s["state"][12].update(exp_avg=torch.zeros(2)), lambda s: s.pop("state"), lambda s: s.pop("param_groups")):  # fmt: skip
+        bad = copy.deepcopy(kept)
+        spoil(bad)
+        with pytest.raises(ValueError):
+            one.load_state_dict(bad)
+        assert all(s["step"] == 2 for s in one.state.values())
+        assert all(torch.equal(v.float(), now[k]) for k, v in one.flat_state().items())
+    one.load_state_dict(kept)
+    assert all(s["step"] == 1 for s in one.state.values())
