@@ -6,10 +6,10 @@ is ``torch.float8_e4m3fn`` and the second ``torch.float8_e5m2``, each with a
 float32 scale for every 256 elements (the largest absolute value maps to the
 format's largest), 2 bytes an element and 1/32 more for the scales in place of
 8.  They are rounded up or down with the odds of the distance, by a hash of
-the element's place, the step and ``seed``: rounding to the nearest would hold
-a second moment still, since with beta2 = 0.999 a step changes it by less than
-half of what 8 bits resolve.  A second moment that is not zero is kept from
-rounding to zero.
+the element's group and place, the step and ``seed``: rounding to the nearest
+would hold a second moment still, since with beta2 = 0.999 a step changes it by
+less than half of what 8 bits resolve.  A second moment that is not zero is kept
+from rounding to zero.
 """
 
 from __future__ import annotations
@@ -24,7 +24,9 @@ from .._torch_ops import ext
 
 STATE_BLOCK = 256
 KINDS = (torch.float32, torch.bfloat16, torch.float16)
-_GOLDEN = 0x9E3779B9
+# between the rounding keys of two steps, and of two groups' equal places: the
+# fractions of the golden ratio and of the square root of 3
+_GOLDEN, _ROOT3 = 0x9E3779B9, 0xBB67AE85
 
 
 class AdamW(torch.optim.Optimizer):
@@ -207,7 +209,7 @@ class AdamW(torch.optim.Optimizer):
         (b1, b2), lr = group["betas"], float(group["lr"])
         return self._plans[g].step(
             group["params"], which, grad_scale, b1, b2, lr / (1 - b1**step), 1.0 / math.sqrt(1 - b2**step),
-            group["eps"], 1 - lr * group["weight_decay"], (self.seed + step * _GOLDEN) & 0xFFFFFFFF,
+            group["eps"], 1 - lr * group["weight_decay"], (self.seed + step * _GOLDEN + g * _ROOT3) & 0xFFFFFFFF,
         )  # fmt: skip
 
 

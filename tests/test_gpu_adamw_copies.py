@@ -129,3 +129,21 @@ def test_a_state_with_something_missing_is_refused_whole():
         assert all(torch.equal(v.float(), now[k]) for k, v in one.flat_state().items())
     one.load_state_dict(kept)
     assert all(s["step"] == 1 for s in one.state.values())
+
+
+def test_groups_round_apart():
+    """Equal parameters and gradients in three groups: the moments' roundings
+    fall by odds of their own, and about a third of 4,096 elements turn another way."""
+    from gbxcule_amd.rl import AdamW
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    params = [torch.nn.Parameter(torch.zeros(4096, device="cuda")) for _ in range(3)]
+    opt = AdamW([{"params": [p]} for p in params], state_bits=8)
+    grad = torch.randn(4096, device="cuda", generator=gen)
+    for p in params:
+        p.grad = grad.clone()
+    opt.step()
+    for key in ("exp_avg", "exp_avg_sq"):
+        a, b, c = (opt.flat_state(g)[key].float() for g in range(3))
+        for u, v in ((a, b), (a, c), (b, c)):
+            assert 0.1 < float((u != v).float().mean()) < 0.9, key
