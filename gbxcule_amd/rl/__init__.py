@@ -17,7 +17,8 @@ from .packed import (
 )
 from .rollout import RolloutBuffer
 
-# loaded on first use: these modules import torch, the others only where they run
+# Loaded on first use: these modules import torch and the operators' libraries,
+# the others only where they run.  Not in __all__, which a star import would load.
 _LAZY = {
     "AdamW": "optim",
     "causal_conv": "ops",
@@ -29,22 +30,15 @@ _LAZY = {
 }
 
 __all__ = [
-    "AdamW",
     "AsyncPPOBufferManager",
     "AsyncPPOBufferState",
     "PackedPixelEnv",
     "RolloutBuffer",
-    "causal_conv",
-    "causal_conv_step",
     "collect_rollout",
     "get_diff_lut",
     "get_unpack_lut",
     "pack_2bpp_u8",
     "packed_l1_distance",
-    "rms_norm",
-    "rms_norm_fp8",
-    "selective_scan",
-    "selective_scan_step",
     "unpack_2bpp_u8",
 ]
 
@@ -56,3 +50,7 @@ def __getattr__(name: str):
         value = globals()[name] = getattr(import_module(f".{_LAZY[name]}", __name__), name)
         return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__() -> list[str]:
+    return sorted({*globals(), *_LAZY})
