@@ -1,5 +1,6 @@
 """Build the HIP shared library ``gbxcule_amd/lib/libgbx_hip.so`` for gfx950 and
-``gbxcule_amd/lib/gbx_torch.so``, the binding of its policy operators to torch.
+``gbxcule_amd/lib/gbx_torch.so``, the binding of its policy operators to torch
+(where torch is installed: the library alone serves users of the C ABI).
 
 ``hipcc`` cross-compiles for gfx950 without a GPU present.  All HIP sources are
 compiled with packed FP32 instructions disabled (``-packed-fp32-ops``).
@@ -7,6 +8,7 @@ compiled with packed FP32 instructions disabled (``-packed-fp32-ops``).
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -53,14 +55,15 @@ def hipcc() -> str:
 
 
 def _extension_command(out: Path) -> list[str]:
-    """Host code only: g++ against torch's headers and libraries."""
+    """Host code only, against torch's headers and libraries: g++, or ROCm's
+    compiler where there is none."""
     import torch
     from torch.utils import cpp_extension
 
     lib = Path(torch.__file__).resolve().parent / "lib"
     system = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
     return [
-        shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        shutil.which("g++") or str(Path(hipcc()).parent / "amdclang++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         "-DTORCH_EXTENSION_NAME=gbx_torch", "-I", str(PKG.parent / "include"),
         *[flag for path in system for flag in ("-isystem", path)], str(CSRC / EXT_SOURCE), "-o", str(out),
         "-L", str(lib), "-L", str(LIB_DIR), "-lgbx_hip", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python",
@@ -97,6 +100,9 @@ def build(verbose: bool = False) -> Path:
     for o in objects:
         o.unlink()
     os.replace(tmp, LIB_PATH)
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: gbx_torch.so, which binds the policy operators to it, is not built", file=sys.stderr)
+        return LIB_PATH
     tmp = LIB_DIR / "gbx_torch.so.tmp"
     _run([_extension_command(tmp)], verbose)
     os.replace(tmp, EXT_PATH)
