@@ -10,8 +10,9 @@ import pickle
 import pytest
 import torch
 
+from . import _policy_ref as ref
 from .conftest import require_gpu
-from .test_gpu_adamw import BF16, F32, _params
+from .test_gpu_adamw import BF16, F16, F32, _formula, _params
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +148,24 @@ def test_groups_round_apart():
         a, b, c = (opt.flat_state(g)[key].float() for g in range(3))
         for u, v in ((a, b), (a, c), (b, c)):
             assert 0.1 < float((u != v).float().mean()) < 0.9, key
+
+
+def test_parameters_of_several_types():
+    """As a policy of 16-bit matrices and 32-bit vectors has them."""
+    from gbxcule_amd.rl import AdamW
+
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    kinds = [F32, BF16, F16] * 4
+    params = [_params(gen, kind, [shape])[0] for kind, shape in zip(kinds, [(3,), (40, 30), (257,), (256,), (1,), (5, 5), (0,), (70, 7), (9,), (4097,), (2,), (64,)])]
+    opt = AdamW(params, lr=0.01, betas=(0.8, 0.99), eps=1e-6, weight_decay=0.1)
+    state = [[torch.zeros(p.shape, dtype=torch.float64) for _ in range(2)] for p in params]
+    for t in range(1, 4):
+        before = [p.detach().cpu().double() for p in params]
+        _gradients(params, t)
+        opt.step()
+        for i, p in enumerate(params):
+            want, *state[i] = _formula(before[i], p.grad.cpu().double(), *state[i], t, 0.01, 0.8, 0.99, 1e-6, 0.1)
+            ref.check(p, want, 32, f"parameter {i} after step {t}")
+            ref.check(opt.state[p]["exp_avg"], state[i][0], 8 * t, f"first moment {i}")
+            ref.check(opt.state[p]["exp_avg_sq"], state[i][1], 8 * t, f"second moment {i}")
+            assert opt.state[p]["step"] == t

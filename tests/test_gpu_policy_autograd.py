@@ -51,6 +51,18 @@ def test_forward_mode_is_refused(which, grad):
     call(*tensors)
 
 
+def test_no_second_derivative():
+    for name, call, tensors in _calls():
+        if name not in ("rms_norm", "causal_conv", "selective_scan"):
+            continue
+        x = tensors[0].clone().requires_grad_()
+        out = call(x, *tensors[1:])
+        (g,) = torch.autograd.grad(out[0].sum(), x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(out[0].sum(), x, create_graph=True)
+        assert torch.equal(g, torch.autograd.grad(out[0].sum(), x)[0])
+
+
 def test_a_state_that_may_not_be_changed_is_not():
     """torch refuses to change an inference tensor outside inference mode."""
     for name, call, tensors in _calls():
