@@ -152,8 +152,9 @@ __device__ __forceinline__ uint32_t row_of(const Shape& s) {
 }
 
 // Bound by memory: 128 steps x 1,024 envs x 1,024 channels in bf16 with episodes
-// that begin in one step of a hundred move 537 MB in 110 us (4.9 TB/s, as a copy
-// does).  Pieces of the steps are long where there are many rows (the lead-in is
+// that begin in one step of a hundred move 537 MB in 113 us (4.7 TB/s; a copy
+// reaches 4.9), 4 steps of 131,072 envs x 512 with a carried state 1.88 GB in 366
+// us (5.1).  Pieces of the steps are long where there are many rows (the lead-in is
 // read twice) and no shorter than 16 steps where there are few.
 template <typename T, int W, bool WHOLE, bool WIDE>
 __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
@@ -227,9 +228,12 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(ConvArgs a, Shape s) {
 // its own.  dweight and dbias of a workgroup's rows are added in LDS and
 // written as one row of partial sums.
 //
-// 128 steps x 1,024 envs x 1,024 channels in bf16 move 805 MB in 206 us (3.9
+// 128 steps x 1,024 envs x 1,024 channels in bf16 move 805 MB in 191 us (4.2
 // TB/s): memory and the vector units (127 us of issue) take turns, with 4
-// channels in a lane.
+// channels in a lane.  The partial sums grow with the rows: where an env has few
+// steps they and their sum are much of the work (4 steps of 131,072 envs x 512
+// channels: 336 MB of them beside 1.6 GB, forward and backward 1,321 us, 2.2
+// times what their own bytes take).
 // 8 channels a lane took the same time with half the wavefronts, and more
 // wavefronts by launch bounds spill (427 us).
 template <typename T, int W, bool WHOLE, bool WIDE>

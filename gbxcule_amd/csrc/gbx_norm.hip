@@ -75,8 +75,8 @@ constexpr float kScaleFloor = 1e-30f;  // keeps the scale of an all-zero group p
 // length in steps of the workgroup and reads the row a second time.
 //
 // Bound by memory: 131,072 rows of 512 channels in bf16 with a residual move
-// 537 MB in 91 us (5.9 TB/s; a copy reaches 4.9), 20,011 rows of 1,024 to 8
-// bits 144 MB in 27 us (5.3 TB/s).  64 rows take 3 us, a launch's least.
+// 537 MB in 89 us (6.0 TB/s; a copy reaches 4.9), 20,011 rows of 1,024 to 8
+// bits 144 MB in 27 us (5.4 TB/s).  64 rows take 3 us, a launch's least.
 template <typename T, int LANES, int NV, int ENDS, bool FP8>
 __global__ __launch_bounds__(threads_of(LANES)) void norm_kernel(NormArgs a) {
   constexpr int kRows = threads_of(LANES) / LANES, kHeld = NV ? NV : 1;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_kernel(NormArgs a) {
 // in LDS, and writes one row of partial sums: no atomics, one order.
 //
 // Bound by memory: 131,072 rows of 512 channels in bf16 with the sum's gradient
-// move 537 MB in 109 us (4.9 TB/s); twice the workgroups are slower, since each
+// move 537 MB in 106 us (5.1 TB/s); twice the workgroups are slower, since each
 // has a row of partial sums to write and to have added.
 template <typename T, int LANES, int NV, int ENDS>
 __global__ __launch_bounds__(threads_of(LANES)) void norm_grad_kernel(NormGradArgs a) {

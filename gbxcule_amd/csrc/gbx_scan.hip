@@ -88,11 +88,21 @@ enum { FULL, ENDS, BACK };  // what scan_kernel computes
 // piece from its own state.  BACK is ENDS for the gradient, against the steps: the
 // gradient of the state before a piece when nothing flows into its end.
 //
-// Bound by the vector units: a state takes an exponential at half rate and four
-// products a step in FULL, three in ENDS.  128 steps x 1,024 envs x 512 channels
-// x 16 states (1.07 G state steps) take 325 us with the states for the gradient
-// written, 3.3 T state steps/s where six issue slots each would allow 6; 16,384
-// steps of one env x 1,024 channels x 16 states 85 us in FULL, 64 in ENDS.
+// Bound by the vector units: a state takes an exponential and four products a
+// step in FULL, three in ENDS; with what a channel needs once a step, the loop of
+// FULL has 8 vector instructions a state step, an eighth of them exponentials.
+// 128 steps x 1,024 envs x 512 channels x 16 states (1.07 G state steps, 1.07 GB
+// with the states for the gradient, half of it those) take 318 us, 3.4 T state
+// steps/s; as whole calls 330 us, 276 without those states, whose stores are half
+// hidden.  16,384 steps of one env x 1,024 channels x 16 states take 77 us in
+// FULL, 58 in ENDS.
+//
+// States are padded to 8, 16 or 32 (by_states), and a group's last wavefront to 64
+// channels.  Without SCALAR two lane reads come to each state step: 128 steps x
+// 512 envs x 512 channels x 16 states 149 us, 12 states 185, 24 states 328, 32
+// states 285; 1,000 channels whose 16-bit rows of B start on odd elements 340 us,
+// 992 whose do not 266.  128 steps x 1,024 envs x 128 channels in one or two groups
+// 99 us, in 4 of 32 channels 145, in 8 of 16 251.
 // All states in a lane: no sum across lanes, and delta, softplus and the gate
 // once a channel.  More wavefronts by launch bounds are slower (8 a SIMD: 823
 // us, 6: 590).
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(kWave* kWaves) void scan_kernel(ScanArgs a, Pieces 
     }
   };
   // (an exit after each of the four would keep copies of the states for it:
-  // 377 us where this takes 325)
+  // 377 us where this took 325)
   int k0 = 0;
   for (; k0 + kAhead <= count; k0 += kAhead) four(k0, std::true_type{});
   if (k0 < count) four(k0, std::false_type{});
@@ -414,9 +424,9 @@ __global__ __launch_bounds__(kWave* kRuns) void join_runs_kernel(ScanArgs a, int
 // wavefronts of a workgroup take neighbouring channels of the same steps and
 // add their dB and dC in LDS at the end of a segment.
 //
-// Bound by the vector units: 25 instructions a state step, three in two of them
-// exponentials, which are active three quarters of the time.  128 steps x 1,024
-// envs x 512 channels x 16 states in bf16: 1,030 us, 1.0 T state steps/s.  8
+// Bound by the vector units, which are active three quarters of the time: about
+// 25 instructions a state step, one and a half of them exponentials.  128 steps x 1,024
+// envs x 512 channels x 16 states in bf16: 1,008 us, 1.07 T state steps/s.  8
 // elements a lane and 8 steps a segment fill the registers of two wavefronts a
 // SIMD; three spill (2,284 us).
 constexpr int kGradWaves = 4;  // wavefronts of a workgroup at most
@@ -787,7 +797,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     if (part == 0) ((T*)a.y)[env * a.dim + d] = (T)out;
   }
 }
-// No multiple of 4 states: a lane a channel.
+// No multiple of 4 states: a lane a channel, whose states lie apart from its
+// neighbours'.  16,384 envs x 512 channels x 15 states 861 us (16 states: 220).
 template <typename T>
 __global__ __launch_bounds__(256) void scan_step_any_kernel(ScanArgs a) {
   const int64_t env = first_env<1>();

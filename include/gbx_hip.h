@@ -291,9 +291,10 @@ int gbx_selective_scan_grad(const gbx_scan_in* in, const float* saved, const voi
 int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* stream);
 
 /* One AdamW step of `count` tensors (host arrays of device addresses, element
- * counts and places of their states, multiples of 256).  state_bits 32: float
- * moments.  8: OCP e4m3 and e5m2 with a scale for each 256 elements, rounded
- * up or down at random by a hash of place and key.  grad_scale (device, may be
+ * counts and places of their states, multiples of 256).  A tensor's states
+ * take whole blocks of 256 elements: what lies past its end in its last block
+ * is written too.  state_bits 32: float moments.  8: OCP e4m3 and e5m2 with a
+ * scale for each block, rounded up or down at random by a hash of place and key.  grad_scale (device, may be
  * NULL) multiplies the gradients.  step_size = lr / (1 - beta1^t), inv_root2 =
  * 1 / sqrt(1 - beta2^t), keep = 1 - lr * decay. */
 typedef struct gbx_adamw_in {
