@@ -105,6 +105,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_rms_norm_grad_work": (_i64, [_i64, _i32]),
     "gbx_rms_norm_grad": (
         ctypes.c_int, [_i64, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "gbx_layer_norm": (ctypes.c_int, [_i64, _i32, _i32, _f32, _vp, _i64, _vp, _i64, *[_vp] * 5]),
+    "gbx_layer_norm_grad_work": (_i64, [_i64, _i32]),
+    "gbx_layer_norm_grad": (
+        ctypes.c_int, [_i64, _i32, _i32, _f32, _vp, _i64, _vp, _i64, _vp, _i64, *[_vp] * 6]),
     "gbx_causal_conv": (ctypes.c_int, [*[_i32] * 6, _vp, _i64, _i64, *[_vp] * 7]),
     "gbx_causal_conv_grad_work": (_i64, [_i32] * 4),
     "gbx_causal_conv_grad": (ctypes.c_int, [*[_i32] * 6, _vp, _i64, _i64, *[_vp] * 5, _i64, _i64, *[_vp] * 5]),

@@ -870,6 +870,32 @@ int gbx_rms_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const 
   return GBX_OK;
 }
 
+int gbx_layer_norm(int64_t rows, int32_t dim, int32_t elem, float eps, const void* x, int64_t x_stride,
+                   const void* residual, int64_t residual_stride, const float* weight, const float* bias, void* out,
+                   void* summed, void* stream) {
+  if (int e = check_norm(rows, dim, elem)) return e;
+  if (rows == 0) return GBX_OK;
+  if (!x || !weight || !out) return fail(GBX_E_INVALID, "x, weight or out is NULL");
+  if (!residual != !summed) return fail(GBX_E_INVALID, "residual and summed go together");
+  LayerNormArgs a{rows, dim, elem, eps, x, residual, x_stride, residual_stride, weight, bias, out, summed};
+  HIP_TRY(launch_layer_norm(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int64_t gbx_layer_norm_grad_work(int64_t rows, int32_t dim) {
+  if (int e = check_norm(rows, dim, GBX_F32)) return e;
+  return layer_norm_grad_work(rows, dim);
+}
+int gbx_layer_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const void* summed, int64_t summed_stride,
+                        const void* dy, int64_t dy_stride, const void* dsummed, int64_t dsummed_stride,
+                        const float* weight, void* dx, float* dweight, float* dbias, float* work, void* stream) {
+  if (int e = check_norm(rows, dim, elem)) return e;
+  if (rows == 0) return fail(GBX_E_INVALID, "no rows");
+  if (!summed || !dy || !weight || !dx || !dweight || !work) return fail(GBX_E_INVALID, "an argument is NULL");
+  LayerNormGradArgs a{rows, dim, elem, eps, summed, dy, dsummed, summed_stride, dy_stride, dsummed_stride, weight, dx, dweight, dbias, work};
+  HIP_TRY(launch_layer_norm_grad(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
 int gbx_causal_conv(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t elem, int32_t silu, const void* x,
                     int64_t x_step, int64_t x_env, const float* weight, const float* bias, const void* state,
                     const uint8_t* resets, void* y, void* last, void* stream) {

@@ -30,6 +30,25 @@ struct NormGradArgs {
   void* dx;
   float *dweight, *work;
 };
+struct LayerNormArgs {
+  int64_t rows;
+  int dim, elem;
+  float eps;
+  const void *x, *residual;  // residual may be NULL
+  int64_t x_stride, residual_stride;
+  const float *weight, *bias;  // bias may be NULL
+  void *out, *summed;          // contiguous; summed NULL without a residual
+};
+struct LayerNormGradArgs {
+  int64_t rows;
+  int dim, elem;
+  float eps;
+  const void *summed, *dy, *dsummed;  // dsummed may be NULL
+  int64_t summed_stride, dy_stride, dsummed_stride;
+  const float* weight;
+  void* dx;
+  float *dweight, *dbias, *work;  // dbias may be NULL
+};
 struct ConvArgs {
   int steps, envs, dim, width, elem, silu;
   const void* x;
@@ -85,6 +104,9 @@ hipError_t launch_column_sum(const float* in, int rows, const SumOutputs& to, hi
 hipError_t launch_rms_norm(const NormArgs& a, hipStream_t st);
 int64_t norm_grad_work(int64_t rows, int dim);
 hipError_t launch_rms_norm_grad(const NormGradArgs& a, hipStream_t st);
+hipError_t launch_layer_norm(const LayerNormArgs& a, hipStream_t st);
+int64_t layer_norm_grad_work(int64_t rows, int dim);
+hipError_t launch_layer_norm_grad(const LayerNormGradArgs& a, hipStream_t st);
 hipError_t launch_conv(const ConvArgs& a, hipStream_t st);
 int64_t conv_grad_work(int steps, int envs, int dim, int width);
 hipError_t launch_conv_grad(const ConvArgs& a, hipStream_t st);

@@ -201,6 +201,66 @@ std::vector<Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const Ma
   return residual ? std::vector<Tensor>{q, scale, summed} : std::vector<Tensor>{q, scale};
 }
 
+// -------------------------------------------------------------- the layer norm
+
+std::vector<Tensor> layer_norm_forward(int elem, const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, double eps) {
+  const c10::DeviceGuard guard(x.device());
+  const Tensor y = blank(x), summed = residual.defined() ? blank(x) : Tensor();
+  if (x.numel() != 0) {
+    const Tensor xr = flat(x), rr = residual.defined() ? flat(residual) : Tensor();
+    check(gbx_layer_norm(xr.size(0), narrow("channels", x.size(-1)), elem, (float)eps, in(xr), xr.stride(0), in(rr), rr.defined() ? rr.stride(0) : 0, fin(weight), fin(bias), out(y), out(summed),
+                         stream(x)));
+  }
+  return residual.defined() ? std::vector<Tensor>{y, summed} : std::vector<Tensor>{y};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& bias_, const Maybe& residual_, double eps, int64_t elem) {
+    const Tensor bias = given(bias_), residual = given(residual_);
+    ctx->set_materialize_grads(false);
+    const variable_list r = layer_norm_forward((int)elem, x, weight, bias, residual, eps);
+    ctx->save_for_backward({residual.defined() ? r[1] : x, weight});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["elem"] = elem;
+    ctx->saved_data["plain"] = !residual.defined();
+    ctx->saved_data["bias"] = bias.defined();
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &s = saved[0], &weight = saved[1];
+    const bool plain = ctx->saved_data["plain"].toBool(), biased = ctx->saved_data["bias"].toBool();
+    const Tensor dsummed = plain ? Tensor() : grads[1];
+    Tensor dx, dweight, dbias;
+    if (!grads[0].defined() || s.numel() == 0) {  // the sum alone was used, or there are no rows
+      dx = dsummed.defined() ? dsummed : at::zeros_like(s);
+      dweight = at::zeros_like(weight);
+      if (biased) dbias = at::zeros_like(weight);
+    } else {
+      const c10::DeviceGuard guard(s.device());
+      const int32_t dim = (int32_t)s.size(-1);
+      const Tensor sr = flat(s), dy = flat(grads[0]), ds = dsummed.defined() ? flat(dsummed) : Tensor();
+      dx = blank(s);
+      dweight = blank(weight);
+      if (biased) dbias = blank(weight);
+      const Tensor scratch = work(s, gbx_layer_norm_grad_work(sr.size(0), dim));
+      check(gbx_layer_norm_grad(sr.size(0), dim, (int)ctx->saved_data["elem"].toInt(), (float)ctx->saved_data["eps"].toDouble(), in(sr), sr.stride(0), in(dy), dy.stride(0), in(ds),
+                                ds.defined() ? ds.stride(0) : 0, fin(weight), out(dx), fout(dweight), fout(dbias), fout(scratch), stream(s)));
+    }
+    return {dx, dweight, dbias, plain ? Tensor() : dx, Tensor(), Tensor()};
+  }
+};
+
+std::vector<Tensor> layer_norm(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, double eps) {
+  const int elem = input("x", x);
+  no_tangent("layer_norm", {&x, &weight, opt(bias), opt(residual)});
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x: expected [..., channels], got ", x.sizes());
+  const Tensor w = param("weight", weight, x, {x.size(-1)}), b = given(param("bias", bias, x, {x.size(-1)})), r = given(like("residual", residual, x, x.sizes()));
+  if (wants_grad({&x, &w, &b, &r})) return LayerNorm::apply(x, w, maybe(b), maybe(r), eps, (int64_t)elem);
+  return layer_norm_forward(elem, x, w, b, r, eps);
+}
+
 // ----------------------------------------------------- the causal convolution
 
 struct CausalConv : torch::autograd::Function<CausalConv> {
@@ -454,6 +514,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("rms_norm", &rms_norm, Unlocked());
   m.def("rms_norm_fp8", &rms_norm_fp8, Unlocked());
+  m.def("layer_norm", &layer_norm, Unlocked());
   m.def("causal_conv", &causal_conv, Unlocked());
   m.def("causal_conv_step", &causal_conv_step, Unlocked());
   m.def("selective_scan", &selective_scan, Unlocked());

@@ -23,6 +23,7 @@ _LAZY = {
     "AdamW": "optim",
     "causal_conv": "ops",
     "causal_conv_step": "ops",
+    "layer_norm": "ops",
     "rms_norm": "ops",
     "rms_norm_fp8": "ops",
     "selective_scan": "ops",

@@ -47,6 +47,16 @@ def rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
     return out[0] if residual is None else tuple(out)
 
 
+def layer_norm(x, weight, bias=None, residual=None, *, eps: float = 1e-5):
+    """``(s - mean(s)) * rsqrt(mean((s - mean(s))**2) + eps) * weight + bias``
+    over the last dimension; ``bias`` may be None.
+
+    s, ``residual`` and the result are as in ``rms_norm``: y, or ``(y, s)``.
+    Differentiable in x, weight, bias and residual."""
+    out = ext.layer_norm(x, weight, bias, residual, eps)
+    return out[0] if residual is None else tuple(out)
+
+
 def rms_norm_fp8(x, weight, residual=None, *, eps: float = 1e-6, group: int | None = None):
     """``rms_norm`` with y in 8 bits: ``(q, scale)`` or ``(q, scale, s)``.
 

@@ -247,6 +247,19 @@ int gbx_rms_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const 
                       int64_t dsummed_stride, const float* weight, void* dx, float* dweight,
                       float* work, void* stream);
 
+/* out = (s - mean(s)) * rsqrt(mean((s - mean(s))^2) + eps) * weight + bias, s
+ * as above; bias may be NULL. */
+int gbx_layer_norm(int64_t rows, int32_t dim, int32_t elem, float eps, const void* x, int64_t x_stride,
+                   const void* residual, int64_t residual_stride, const float* weight,
+                   const float* bias, void* out, void* summed, void* stream);
+/* dx (also the residual's gradient), dweight and dbias (may be NULL) from s,
+ * dy and the gradient of s itself (dsummed, may be NULL). */
+int64_t gbx_layer_norm_grad_work(int64_t rows, int32_t dim);
+int gbx_layer_norm_grad(int64_t rows, int32_t dim, int32_t elem, float eps, const void* summed,
+                        int64_t summed_stride, const void* dy, int64_t dy_stride, const void* dsummed,
+                        int64_t dsummed_stride, const float* weight, void* dx, float* dweight,
+                        float* dbias, float* work, void* stream);
+
 /* y[t] = act(bias + sum_j weight[width - 1 - j] * x[t - j]), width 2 to 4, act
  * silu or nothing.  state[envs][width - 1][dim] holds the inputs before the
  * first step (NULL: zeros), last those before the step to come. */
