@@ -54,6 +54,20 @@ class ScanIn(ctypes.Structure):
     ]
 
 
+class DeltaIn(ctypes.Structure):
+    """``gbx_delta_in``."""
+
+    _fields_ = [
+        *((k, _i32) for k in ("steps", "envs", "heads", "share", "keys", "values", "elem", "normalize")),
+        ("scale", _f32),
+        *((k, _vp) for k in ("q", "k", "v")),
+        *((f"{k}_{d}", _i64) for k in ("q", "k", "v") for d in ("step", "env", "head")),
+        *((k, _vp) for k in ("gate", "beta")),
+        *((k, _i64) for k in ("gate_step", "gate_env", "beta_step", "beta_env")),
+        ("resets", _vp),
+    ]
+
+
 class AdamwIn(ctypes.Structure):
     """``gbx_adamw_in``."""
 
@@ -118,6 +132,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_selective_scan_grad_work": (_i64, [ctypes.POINTER(ScanIn)]),
     "gbx_selective_scan_grad": (ctypes.c_int, [ctypes.POINTER(ScanIn), _vp, _vp, _i64, _i64, *[_vp] * 10]),
     "gbx_selective_scan_step": (ctypes.c_int, [ctypes.POINTER(ScanIn), *[_vp] * 3]),
+    "gbx_delta_rule_work": (_i64, [ctypes.POINTER(DeltaIn)]),
+    "gbx_delta_rule": (ctypes.c_int, [ctypes.POINTER(DeltaIn), *[_vp] * 6]),
+    "gbx_delta_rule_grad_work": (_i64, [ctypes.POINTER(DeltaIn)]),
+    "gbx_delta_rule_grad": (ctypes.c_int, [ctypes.POINTER(DeltaIn), _vp, _vp, *[_i64] * 3, *[_vp] * 7]),
+    "gbx_delta_rule_step": (ctypes.c_int, [ctypes.POINTER(DeltaIn), *[_vp] * 3]),
     "gbx_adamw": (ctypes.c_int, [ctypes.POINTER(AdamwIn), _vp]),
 }
 

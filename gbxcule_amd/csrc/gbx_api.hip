@@ -260,6 +260,28 @@ int check_conv(int32_t steps, int32_t envs, int32_t dim, int32_t width, int32_t 
   if (width < 2 || width > 4) return fail(GBX_E_INVALID, "width must be 2, 3 or 4");
   return GBX_OK;
 }
+int delta_args(const gbx_delta_in* in, DeltaArgs& a) {
+  if (!in) return fail(GBX_E_INVALID, "in is NULL");
+  if (int e = check_rows(in->steps, in->envs)) return e;
+  if (in->heads < 1 || in->heads > 1 << 16) return fail(GBX_E_INVALID, "head count out of range");
+  if (in->share < 1 || in->heads % in->share) return fail(GBX_E_INVALID, "heads must be a multiple of share");
+  if (in->keys < 1 || in->keys > kMaxHeadDim || in->values < 1 || in->values > kMaxHeadDim)
+    return fail(GBX_E_INVALID, "1 to 128 keys and values a head are supported");
+  if (in->elem < GBX_F32 || in->elem > GBX_F16) return fail(GBX_E_INVALID, "bad element type");
+  // every index of a workgroup, and of a head's state, stays in its type
+  if ((int64_t)in->envs * in->heads > (int64_t)1 << 31) return fail(GBX_E_INVALID, "envs times heads out of range");
+  if (!in->q || !in->k || !in->v || !in->gate || !in->beta) return fail(GBX_E_INVALID, "q, k, v, gate or beta is NULL");
+  a = DeltaArgs{};
+  a.steps = in->steps, a.envs = in->envs, a.heads = in->heads, a.share = in->share, a.keys = in->keys, a.values = in->values;
+  a.elem = in->elem, a.normalize = in->normalize, a.scale = in->scale;
+  a.q = in->q, a.k = in->k, a.v = in->v;
+  a.q_step = in->q_step, a.q_env = in->q_env, a.q_head = in->q_head;
+  a.k_step = in->k_step, a.k_env = in->k_env, a.k_head = in->k_head;
+  a.v_step = in->v_step, a.v_env = in->v_env, a.v_head = in->v_head;
+  a.gate = in->gate, a.beta = in->beta, a.gate_step = in->gate_step, a.gate_env = in->gate_env;
+  a.beta_step = in->beta_step, a.beta_env = in->beta_env, a.resets = in->resets;
+  return GBX_OK;
+}
 int scan_args(const gbx_scan_in* in, ScanArgs& a) {
   if (!in) return fail(GBX_E_INVALID, "in is NULL");
   if (int e = check_rows(in->steps, in->envs)) return e;
@@ -977,6 +999,46 @@ int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* 
   if (!state || !y) return fail(GBX_E_INVALID, "state or y is NULL");
   a.last = state, a.y = y;
   HIP_TRY(launch_scan_step(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
+int64_t gbx_delta_rule_work(const gbx_delta_in* in) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  return delta_work(a);
+}
+int gbx_delta_rule(const gbx_delta_in* in, const float* state, void* y, float* last, float* saved, float* work, void* stream) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  if (!y || !last) return fail(GBX_E_INVALID, "y or last is NULL");
+  if (!work && delta_work(a) > 0) return fail(GBX_E_INVALID, "work is NULL");
+  a.state = state, a.y = y, a.last = last, a.saved = saved, a.work = work;
+  HIP_TRY(launch_delta(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int64_t gbx_delta_rule_grad_work(const gbx_delta_in* in) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  return delta_grad_work(a);
+}
+int gbx_delta_rule_grad(const gbx_delta_in* in, const float* saved, const void* dy, int64_t dy_step, int64_t dy_env,
+                        int64_t dy_head, void* dq, void* dk, void* dv, float* dgate, float* dbeta, float* work, void* stream) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  if (!saved || !dy || !dq || !dk || !dv || !dgate || !dbeta) return fail(GBX_E_INVALID, "an argument is NULL");
+  if (!work && delta_grad_work(a) > 0) return fail(GBX_E_INVALID, "work is NULL");
+  a.saved = const_cast<float*>(saved), a.dy = dy, a.dy_step = dy_step, a.dy_env = dy_env, a.dy_head = dy_head;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.dgate = dgate, a.dbeta = dbeta, a.work = work;
+  HIP_TRY(launch_delta_grad(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+int gbx_delta_rule_step(const gbx_delta_in* in, float* state, void* y, void* stream) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  if (a.steps != 1) return fail(GBX_E_INVALID, "steps must be 1");
+  if (!state || !y) return fail(GBX_E_INVALID, "state or y is NULL");
+  a.last = state, a.y = y;
+  HIP_TRY(launch_delta_step(a, (hipStream_t)stream));
   return GBX_OK;
 }
 

@@ -79,6 +79,23 @@ struct ScanArgs {
   void *dx, *ddt, *dz, *db, *dc;  // contiguous
   float *da, *dskip, *dbias;
 };
+struct DeltaArgs {
+  int steps, envs, heads, share, keys, values, elem, normalize;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_step, q_env, q_head, k_step, k_env, k_head, v_step, v_env, v_head;
+  const float *gate, *beta;  // the head stride is 1
+  int64_t gate_step, gate_env, beta_step, beta_env;
+  const float* state;     // [envs][heads][keys][values] or NULL
+  const uint8_t* resets;  // [steps][envs] or NULL
+  void* y;                // contiguous
+  float *last, *saved;    // saved: [chunks][envs][heads][keys][values] or NULL
+  float* work;
+  const void* dy;  // the rest: gradient only
+  int64_t dy_step, dy_env, dy_head;
+  void *dq, *dk, *dv;
+  float *dgate, *dbeta;
+};
 struct AdamArgs {
   int count, elem, grad_elem, small;  // small: 8-bit states
   const uint64_t *params, *grads;     // host: device addresses
@@ -92,6 +109,8 @@ struct AdamArgs {
 constexpr int kStateBlock = 256;  // elements that share a scale
 constexpr int kSegment = 8;     // steps between two saved states
 constexpr int kMaxStates = 32;  // states a channel may have
+constexpr int kDeltaChunk = 16;   // steps of the delta rule that are solved together
+constexpr int kMaxHeadDim = 128;  // channels of its keys and of its values
 
 // Sums over `rows` rows of partial sums that lie one after the other, in one
 // order.  The columns are up to three outputs' in turn; those whose pointer is
@@ -116,6 +135,11 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t st);
 int64_t scan_grad_work(int steps, int envs, int dim, int groups, int states);
 hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st);
 hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st);
+int64_t delta_work(const DeltaArgs& a);
+hipError_t launch_delta(const DeltaArgs& a, hipStream_t st);
+int64_t delta_grad_work(const DeltaArgs& a);
+hipError_t launch_delta_grad(const DeltaArgs& a, hipStream_t st);
+hipError_t launch_delta_step(const DeltaArgs& a, hipStream_t st);
 hipError_t launch_adamw(const AdamArgs& a, hipStream_t st);
 
 // A grid has fewer than 2^32 threads: more workgroups than 2^22 go to its

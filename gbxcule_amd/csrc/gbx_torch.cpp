@@ -8,6 +8,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -445,6 +446,125 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, c
   return y;
 }
 
+// ------------------------------------------------------- the gated delta rule
+
+struct Delta {  // checked operands; undefined: not given
+  Tensor q, k, v, gate, beta, resets;
+};
+// gates in 32 bits (autograd sees the cast), heads next to each other
+Tensor gates(const char* name, const Tensor& t, const Tensor& x, IntArrayRef shape) {
+  TORCH_CHECK_VALUE(t.is_floating_point(), name, ": expected a floating-point tensor, got ", t.scalar_type());
+  same_place(name, t, x, shape);
+  return rows(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat));
+}
+Delta delta_operands(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, const Maybe& resets) {
+  const int64_t heads = v.size(-2);
+  TORCH_CHECK_VALUE(heads >= 1 && v.size(-1) >= 1 && v.size(-1) <= 128, "v: expected [..., heads, 1 to 128 values], got ", v.sizes());
+  TORCH_CHECK_VALUE(q.dim() == v.dim() && q.size(-1) >= 1 && q.size(-1) <= 128 && q.size(-2) >= 1 && heads % q.size(-2) == 0,
+                    "q: expected [..., heads, 1 to 128 keys] with heads dividing ", heads, ", got ", q.sizes());
+  const std::vector<int64_t> lead(v.sizes().begin(), v.sizes().end() - 2);
+  std::vector<int64_t> each = lead, shared = lead;
+  each.push_back(heads);
+  shared.push_back(q.size(-2));
+  shared.push_back(q.size(-1));
+  return {like("q", q, v, shared), like("k", k, v, shared), rows(v), gates("g", gate, v, each), gates("beta", beta, v, each), given(starts(resets, v, lead))};
+}
+gbx_delta_in delta_in(const Delta& d, double scale, bool normalize, int elem) {
+  const bool one = d.v.dim() == 3;  // a single step
+  const auto step = [&](const Tensor& t) { return one ? 0 : t.stride(0); };
+  const auto env = [&](const Tensor& t) { return t.stride(one ? 0 : 1); };
+  gbx_delta_in g{};
+  g.steps = one ? 1 : narrow("steps", d.v.size(0)), g.envs = narrow("envs", d.v.size(-3)), g.heads = narrow("heads", d.v.size(-2));
+  g.share = (int32_t)(d.v.size(-2) / d.q.size(-2)), g.keys = (int32_t)d.q.size(-1), g.values = (int32_t)d.v.size(-1);
+  g.elem = elem, g.normalize = normalize, g.scale = (float)scale;
+  g.q = in(d.q), g.k = in(d.k), g.v = in(d.v);
+  g.q_step = step(d.q), g.q_env = env(d.q), g.q_head = d.q.stride(-2), g.k_step = step(d.k), g.k_env = env(d.k), g.k_head = d.k.stride(-2);
+  g.v_step = step(d.v), g.v_env = env(d.v), g.v_head = d.v.stride(-2);
+  g.gate = fin(d.gate), g.beta = fin(d.beta);
+  g.gate_step = step(d.gate), g.gate_env = env(d.gate), g.beta_step = step(d.beta), g.beta_env = env(d.beta), g.resets = bytes(d.resets);
+  return g;
+}
+variable_list delta_forward(const Delta& d, const Tensor& state, double scale, bool normalize, int elem, bool save) {
+  const c10::DeviceGuard guard(d.v.device());
+  const int64_t steps = d.v.size(0), envs = d.v.size(1), heads = d.v.size(2), values = d.v.size(3), keys = d.q.size(3);
+  const Tensor y = blank(d.v), last = floats(d.v, {envs, heads, keys, values}), saved = save ? floats(d.v, {(steps + 15) / 16, envs, heads, keys, values}) : Tensor();
+  if (d.v.numel() == 0) return {y, unmoved(state, last), saved};
+  const gbx_delta_in g = delta_in(d, scale, normalize, elem);
+  const Tensor scratch = work(d.v, gbx_delta_rule_work(&g));
+  check(gbx_delta_rule(&g, fin(state), out(y), fout(last), fout(saved), fout(scratch), stream(d.v)));
+  return {y, last, saved};
+}
+
+struct DeltaRule : torch::autograd::Function<DeltaRule> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, const Maybe& state, const Maybe& resets_,
+                               double scale, bool normalize, int64_t elem) {
+    const Tensor resets = given(resets_);
+    ctx->set_materialize_grads(false);
+    const variable_list r = delta_forward({q, k, v, gate, beta, resets}, given(state), scale, normalize, (int)elem, true);
+    ctx->save_for_backward({q, k, v, gate, beta, resets, r[2]});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["elem"] = elem;
+    ctx->mark_non_differentiable({r[1]});
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    variable_list result(10);
+    if (!grads[0].defined()) return result;
+    const auto s = ctx->get_saved_variables();
+    const Delta d{s[0], s[1], s[2], s[3], s[4], s[5]};
+    const c10::DeviceGuard guard(d.v.device());
+    if (d.v.numel() == 0) {
+      for (int i = 0; i < 5; ++i) result[i] = zeros(s[i]);
+      return result;
+    }
+    const gbx_delta_in g = delta_in(d, ctx->saved_data["scale"].toDouble(), ctx->saved_data["normalize"].toBool(), (int)ctx->saved_data["elem"].toInt());
+    const Tensor dy = rows(grads[0]);
+    for (int i = 0; i < 5; ++i) result[i] = blank(s[i]);
+    const Tensor scratch = work(d.v, gbx_delta_rule_grad_work(&g));
+    check(gbx_delta_rule_grad(&g, fin(s[6]), in(dy), dy.stride(0), dy.stride(1), dy.stride(2), out(result[0]), out(result[1]), out(result[2]), fout(result[3]), fout(result[4]), fout(scratch),
+                              stream(d.v)));
+    return result;
+  }
+};
+
+std::vector<Tensor> delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, std::optional<double> scale_, bool normalize, const Maybe& state,
+                               const Maybe& resets) {
+  const int elem = input("v", v);
+  no_tangent("delta_rule", {&q, &k, &v, &gate, &beta, opt(state)});
+  TORCH_CHECK_VALUE(v.dim() == 4, "v: expected [steps, envs, heads, values], got ", v.sizes());
+  const Delta d = delta_operands(q, k, v, gate, beta, resets);
+  TORCH_CHECK_VALUE(!wants_grad({opt(state)}), "state carries no gradient: detach it");
+  const int64_t keys = q.size(-1);
+  const Tensor before = state ? state_of(*state, v, at::kFloat, {v.size(1), v.size(2), keys, v.size(3)}).contiguous() : Tensor();
+  const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)keys);
+  if (wants_grad({&d.q, &d.k, &d.v, &d.gate, &d.beta}))
+    return DeltaRule::apply(d.q, d.k, d.v, d.gate, d.beta, maybe(before), maybe(d.resets), scale, normalize, (int64_t)elem);
+  const variable_list r = delta_forward(d, before, scale, normalize, elem, false);
+  return {r[0], r[1]};
+}
+
+Tensor delta_rule_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gate, const Tensor& beta, const Tensor& state, std::optional<double> scale_, bool normalize,
+                       const Maybe& resets) {
+  const int elem = input("v", v);
+  no_grad("delta_rule_step", {&q, &k, &v, &gate, &beta, &state});
+  no_tangent("delta_rule_step", {&q, &k, &v, &gate, &beta, &state});
+  TORCH_CHECK_VALUE(v.dim() == 3, "v: expected [envs, heads, values], got ", v.sizes());
+  const Delta d = delta_operands(q, k, v, gate, beta, resets);
+  const int64_t keys = q.size(-1);
+  state_of(state, v, at::kFloat, {v.size(0), v.size(1), keys, v.size(2)});
+  TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is updated in place");
+  const Tensor y = blank(v);
+  if (v.size(0)) {
+    const c10::DeviceGuard guard(v.device());
+    const gbx_delta_in g = delta_in(d, scale_ ? *scale_ : 1.0 / std::sqrt((double)keys), normalize, elem);
+    will_change(state);
+    check(gbx_delta_rule_step(&g, fout(state), out(y), stream(v)));
+  }
+  return y;
+}
+
 // --------------------------------------------------------------------- AdamW
 
 // What does not change from step to step of a parameter group.
@@ -519,6 +639,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("causal_conv_step", &causal_conv_step, Unlocked());
   m.def("selective_scan", &selective_scan, Unlocked());
   m.def("selective_scan_step", &selective_scan_step, Unlocked());
+  m.def("delta_rule", &delta_rule, Unlocked());
+  m.def("delta_rule_step", &delta_rule_step, Unlocked());
   py::class_<AdamwPlan>(m, "AdamwPlan")
       .def(py::init<std::vector<int64_t>, std::vector<int64_t>, const Tensor&, const Tensor&, const Maybe&, const Maybe&>())
       .def("step", &AdamwPlan::step, Unlocked());

@@ -23,6 +23,8 @@ _LAZY = {
     "AdamW": "optim",
     "causal_conv": "ops",
     "causal_conv_step": "ops",
+    "delta_rule": "ops",
+    "delta_rule_step": "ops",
     "layer_norm": "ops",
     "rms_norm": "ops",
     "rms_norm_fp8": "ops",

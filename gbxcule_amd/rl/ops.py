@@ -113,3 +113,31 @@ def selective_scan_step(x, dt, A, B, C, D=None, z=None, *, state, dt_bias=None, 
     ``[N, channels]``; ``state`` ``[N, channels, states]`` float32 is updated in
     place (where ``resets`` ``[N]`` is set, from zeros).  No gradient."""
     return ext.selective_scan_step(x, dt, A, B, C, D, z, state, dt_bias, softplus, resets)
+
+
+def delta_rule(q, k, v, g, beta, *, scale: float | None = None, normalize: bool = True, state=None, resets=None):
+    """Gated delta rule along the steps: a matrix S for each head, corrected
+    towards what its key should recall::
+
+        S = exp(g) * S                          (S = 0 before a step where an episode begins)
+        S = S + k (beta * (v - S^T k))^T
+        y = scale * S^T q
+
+    ``q``, ``k`` ``[T, N, heads / share, keys]``, each of their heads shared by
+    ``share`` neighbouring heads of ``v`` ``[T, N, heads, values]``; up to 128
+    keys and values.  ``g`` (the logarithm of the decay, mostly below 0; below
+    -104 it clears the state as an episode's start does) and ``beta`` ``[T, N,
+    heads]`` are taken in 32 bits.  ``normalize``: q and k are divided by
+    ``sqrt(sum of squares + 1e-6)``.  ``scale=None``: ``keys ** -0.5``.
+    ``state`` ``[N, heads, keys, values]`` float32 before the first step (None:
+    zeros).  Returns ``(y, state after the last step)``; differentiable in
+    everything but the state.  For the gradient every 16th state is kept."""
+    return tuple(ext.delta_rule(q, k, v, g, beta, scale, normalize, state, resets))
+
+
+def delta_rule_step(q, k, v, g, beta, *, state, scale: float | None = None, normalize: bool = True, resets=None):
+    """One step of ``delta_rule``: ``q``, ``k`` ``[N, heads / share, keys]``,
+    ``v`` ``[N, heads, values]``, ``g``, ``beta`` ``[N, heads]`` -> y ``[N, heads,
+    values]``; ``state`` ``[N, heads, keys, values]`` float32 is updated in place
+    (where ``resets`` ``[N]`` is set, from zeros).  No gradient."""
+    return ext.delta_rule_step(q, k, v, g, beta, state, scale, normalize, resets)

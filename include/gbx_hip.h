@@ -303,6 +303,37 @@ int gbx_selective_scan_grad(const gbx_scan_in* in, const float* saved, const voi
 /* One step of every env (in->steps is 1); `state` is updated in place. */
 int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* stream);
 
+/* Inputs of the gated delta rule, a matrix state a head:
+ *   S = exp(gate) S,  e = beta (v - S^T k),  S += k e^T,  y = scale S^T q.
+ * q and k are [steps][envs][heads / share][keys], v [steps][envs][heads][values],
+ * keys and values 1 to 128; each head of q and k is shared by `share`
+ * neighbouring heads.  gate and beta are [steps][envs][heads]; their head
+ * stride is 1.  normalize: q and k are divided by sqrt(their squared length +
+ * 1e-6).  A gate below -104, whose exp is zero in 32 bits, clears the state as
+ * an episode's start does. */
+typedef struct gbx_delta_in {
+  int32_t steps, envs, heads, share, keys, values, elem, normalize;
+  float scale;
+  const void *q, *k, *v;
+  int64_t q_step, q_env, q_head, k_step, k_env, k_head, v_step, v_env, v_head;
+  const float *gate, *beta;
+  int64_t gate_step, gate_env, beta_step, beta_env;
+  const uint8_t* resets;
+} gbx_delta_in;
+/* state[envs][heads][keys][values] (NULL: zeros) before the first step, last
+ * after the last one.  saved, if not NULL, receives what the gradient starts
+ * from: [steps / 16 rounded up][envs][heads][keys][values]. */
+int64_t gbx_delta_rule_work(const gbx_delta_in* in);
+int gbx_delta_rule(const gbx_delta_in* in, const float* state, void* y, float* last, float* saved,
+                   float* work, void* stream);
+/* Gradients, of the shapes of q, k, v, gate and beta. */
+int64_t gbx_delta_rule_grad_work(const gbx_delta_in* in);
+int gbx_delta_rule_grad(const gbx_delta_in* in, const float* saved, const void* dy, int64_t dy_step,
+                        int64_t dy_env, int64_t dy_head, void* dq, void* dk, void* dv, float* dgate,
+                        float* dbeta, float* work, void* stream);
+/* One step of every env (in->steps is 1); `state` is updated in place. */
+int gbx_delta_rule_step(const gbx_delta_in* in, float* state, void* y, void* stream);
+
 /* One AdamW step of `count` tensors (host arrays of device addresses, element
  * counts and places of their states, multiples of 256).  A tensor's states
  * take whole blocks of 256 elements: what lies past its end in its last block
