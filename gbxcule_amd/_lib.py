@@ -68,6 +68,20 @@ class DeltaIn(ctypes.Structure):
     ]
 
 
+class SampleIn(ctypes.Structure):
+    """``gbx_sample_in``."""
+
+    _fields_ = [
+        ("rows", _i64),
+        *((k, _i32) for k in ("actions", "elem")),
+        ("logits", _vp),
+        ("stride", _i64),
+        *((k, _vp) for k in ("uniform", "temperatures", "top_ps", "min_ps", "top_ks")),
+        *((k, _f64) for k in ("temperature", "top_p", "min_p")),
+        ("top_k", _i32),
+    ]
+
+
 class AdamwIn(ctypes.Structure):
     """``gbx_adamw_in``."""
 
@@ -137,6 +151,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_delta_rule_grad_work": (_i64, [ctypes.POINTER(DeltaIn)]),
     "gbx_delta_rule_grad": (ctypes.c_int, [ctypes.POINTER(DeltaIn), _vp, _vp, *[_i64] * 3, *[_vp] * 7]),
     "gbx_delta_rule_step": (ctypes.c_int, [ctypes.POINTER(DeltaIn), *[_vp] * 3]),
+    "gbx_sample_actions": (ctypes.c_int, [ctypes.POINTER(SampleIn), *[_vp] * 3]),
     "gbx_adamw": (ctypes.c_int, [ctypes.POINTER(AdamwIn), _vp]),
 }
 

@@ -42,7 +42,7 @@ DEVICE_FLAGS = (
 # The policy operators: the default scheduler.  The other one leaves the
 # gradient of the scan more spilled registers, and its register allocation
 # crashes on the 8-bit AdamW kernel.
-POLICY_SOURCES = ("gbx_norm.hip", "gbx_layer_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_delta.hip", "gbx_delta_grad.hip",
+POLICY_SOURCES = ("gbx_norm.hip", "gbx_layer_norm.hip", "gbx_conv.hip", "gbx_scan.hip", "gbx_delta.hip", "gbx_delta_grad.hip", "gbx_sample.hip",
                   "gbx_adamw.hip")  # fmt: skip
 SOURCES = ("gbx_step.hip", "gbx_aux.hip", *POLICY_SOURCES, "gbx_api.hip")
 POLICY_FLAGS = tuple(f for f in DEVICE_FLAGS if f != "-mllvm" and "sched-strategy" not in f)

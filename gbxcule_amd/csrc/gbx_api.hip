@@ -1042,6 +1042,20 @@ int gbx_delta_rule_step(const gbx_delta_in* in, float* state, void* y, void* str
   return GBX_OK;
 }
 
+int gbx_sample_actions(const gbx_sample_in* in, int32_t* action, float* logp, void* stream) {
+  if (!in) return fail(GBX_E_INVALID, "in is NULL");
+  if (int e = check_norm(in->rows, in->actions, in->elem)) return e;
+  if (in->rows == 0) return GBX_OK;
+  if (!in->logits || !in->uniform || !action || !logp) return fail(GBX_E_INVALID, "logits, uniform, action or logp is NULL");
+  if (!in->temperatures && !(in->temperature >= 0.0)) return fail(GBX_E_INVALID, "temperature must be 0 or more");
+  if (!in->top_ps && !(in->top_p > 0.0)) return fail(GBX_E_INVALID, "top_p must be more than 0");
+  if (!in->min_ps && !(in->min_p <= 1.0)) return fail(GBX_E_INVALID, "min_p must be 1 or less");
+  SampleArgs a{in->rows, in->actions, in->elem, in->logits, in->stride, in->uniform, in->temperatures, in->top_ps, in->min_ps,
+               in->top_ks, in->temperature, in->top_p, in->min_p, in->top_k, action, logp};
+  HIP_TRY(launch_sample(a, (hipStream_t)stream));
+  return GBX_OK;
+}
+
 int gbx_adamw(const gbx_adamw_in* in, void* stream) {
   if (!in || in->count < 0) return fail(GBX_E_INVALID, "in is NULL or its count negative");
   if (in->count == 0) return GBX_OK;

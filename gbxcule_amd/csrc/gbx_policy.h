@@ -96,6 +96,20 @@ struct DeltaArgs {
   void *dq, *dk, *dv;
   float *dgate, *dbeta;
 };
+struct SampleArgs {
+  int64_t rows;
+  int actions, elem;
+  const void* logits;
+  int64_t stride;
+  const float* uniform;
+  // one a row, or NULL: the same for all
+  const float *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  double temperature, top_p, min_p;
+  int top_k;
+  int32_t* action;
+  float* logp;
+};
 struct AdamArgs {
   int count, elem, grad_elem, small;  // small: 8-bit states
   const uint64_t *params, *grads;     // host: device addresses
@@ -140,6 +154,7 @@ hipError_t launch_delta(const DeltaArgs& a, hipStream_t st);
 int64_t delta_grad_work(const DeltaArgs& a);
 hipError_t launch_delta_grad(const DeltaArgs& a, hipStream_t st);
 hipError_t launch_delta_step(const DeltaArgs& a, hipStream_t st);
+hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
 hipError_t launch_adamw(const AdamArgs& a, hipStream_t st);
 
 // A grid has fewer than 2^32 threads: more workgroups than 2^22 go to its

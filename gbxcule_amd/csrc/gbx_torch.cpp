@@ -8,9 +8,11 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
+#include <variant>
 #include <vector>
 
 #include "gbx_hip.h"
@@ -565,6 +567,35 @@ Tensor delta_rule_step(const Tensor& q, const Tensor& k, const Tensor& v, const 
   return y;
 }
 
+// ------------------------------------------------------------------ sampling
+
+// options: each a number or a tensor with one for each row
+std::vector<Tensor> sample_actions(const Tensor& logits, const Tensor& uniform, const std::variant<double, Tensor>& temperature, const std::variant<int64_t, Tensor>& top_k,
+                                   const std::variant<double, Tensor>& top_p, const std::variant<double, Tensor>& min_p) {
+  const int elem = input("logits", logits);
+  no_grad("sample_actions", {&logits});
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits: expected [..., actions], got ", logits.sizes());
+  const IntArrayRef lead(logits.sizes().data(), logits.dim() - 1);
+  const auto row = [&](const char* name, const Tensor& t, at::ScalarType kind) {
+    TORCH_CHECK_VALUE(t.scalar_type() == kind, name, ": expected ", kind, ", got ", t.scalar_type());
+    same_place(name, t, logits, lead);
+    return t.contiguous();
+  };
+  const auto option = [&](const char* name, const auto& o, at::ScalarType kind) { return std::holds_alternative<Tensor>(o) ? row(name, std::get<Tensor>(o), kind) : Tensor(); };
+  const Tensor u = row("uniform", uniform, at::kFloat), t = option("temperature", temperature, at::kFloat), k = option("top_k", top_k, at::kInt);
+  const Tensor p = option("top_p", top_p, at::kFloat), m = option("min_p", min_p, at::kFloat);
+  const Tensor action = at::empty(lead, logits.options().dtype(at::kInt)), logp = floats(logits, lead);
+  const c10::DeviceGuard guard(logits.device());
+  const Tensor x = flat(logits);
+  gbx_sample_in g{};
+  g.rows = action.numel(), g.actions = narrow("actions", x.size(1)), g.elem = elem, g.logits = in(x), g.stride = x.stride(0), g.uniform = fin(u);
+  g.temperatures = fin(t), g.top_ps = fin(p), g.min_ps = fin(m), g.top_ks = (const int32_t*)in(k);
+  g.temperature = t.defined() ? 0.0 : std::get<double>(temperature), g.top_p = p.defined() ? 0.0 : std::get<double>(top_p), g.min_p = m.defined() ? 0.0 : std::get<double>(min_p);
+  g.top_k = k.defined() ? 0 : (int32_t)std::clamp<int64_t>(std::get<int64_t>(top_k), 0, INT32_MAX);
+  check(gbx_sample_actions(&g, (int32_t*)out(action), fout(logp), stream(logits)));
+  return {action, logp};
+}
+
 // --------------------------------------------------------------------- AdamW
 
 // What does not change from step to step of a parameter group.
@@ -641,6 +672,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("selective_scan_step", &selective_scan_step, Unlocked());
   m.def("delta_rule", &delta_rule, Unlocked());
   m.def("delta_rule_step", &delta_rule_step, Unlocked());
+  m.def("sample_actions", &sample_actions, Unlocked());
   py::class_<AdamwPlan>(m, "AdamwPlan")
       .def(py::init<std::vector<int64_t>, std::vector<int64_t>, const Tensor&, const Tensor&, const Maybe&, const Maybe&>())
       .def("step", &AdamwPlan::step, Unlocked());

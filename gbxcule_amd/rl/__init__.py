@@ -28,6 +28,7 @@ _LAZY = {
     "layer_norm": "ops",
     "rms_norm": "ops",
     "rms_norm_fp8": "ops",
+    "sample_actions": "ops",
     "selective_scan": "ops",
     "selective_scan_step": "ops",
 }

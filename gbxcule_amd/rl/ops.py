@@ -141,3 +141,22 @@ def delta_rule_step(q, k, v, g, beta, *, state, scale: float | None = None, norm
     values]``; ``state`` ``[N, heads, keys, values]`` float32 is updated in place
     (where ``resets`` ``[N]`` is set, from zeros).  No gradient."""
     return ext.delta_rule_step(q, k, v, g, beta, state, scale, normalize, resets)
+
+
+def sample_actions(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Actions drawn from ``logits`` ``[..., actions]`` with the random numbers
+    ``uniform`` ``[...]`` (float32, from 0 to below 1): ``(action int32 [...],
+    logp float32 [...])``.
+
+    Weights are ``exp(logits / temperature)``; temperature 0 takes the largest
+    logit.  From the likeliest action on, the lowest index first among equals, a
+    row keeps its first ``top_k`` (0: all), of those the fewest that hold
+    ``top_p`` of their weight (1: all), of those all with at least ``min_p`` of the
+    largest weight, and always one.  ``action`` is the first index at which the
+    running sum of the kept weights passes ``uniform`` times their sum, and
+    ``logp`` the logarithm of the probability it was drawn with.  Each option is a
+    number or a tensor ``[...]`` with one for each row (float32, ``top_k`` int32).
+
+    NaN and -infinity are never drawn; a row of nothing else has action -1 and
+    logp NaN.  Weights and sums are in 64 bits.  No gradient."""
+    return tuple(ext.sample_actions(logits, uniform, temperature, top_k, top_p, min_p))

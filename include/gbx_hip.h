@@ -334,6 +334,28 @@ int gbx_delta_rule_grad(const gbx_delta_in* in, const float* saved, const void* 
 /* One step of every env (in->steps is 1); `state` is updated in place. */
 int gbx_delta_rule_step(const gbx_delta_in* in, float* state, void* y, void* stream);
 
+/* Actions drawn from logits[rows][actions], 1 to 2^20 actions, with the random
+ * numbers uniform[rows], 0 <= u < 1.  Weights are exp(logit / temperature)
+ * (temperature 0: the largest logit alone).  From the likeliest on, the lowest
+ * index first among equals, a row keeps its first top_k (0 or less: all), of those the
+ * fewest that hold top_p of their weight (1 or more: all), of those all with at
+ * least min_p of the largest weight, and always one.  The action is the first at which the
+ * running sum of what is kept, by index, passes u times its sum; logp is the
+ * logarithm of its share of that sum.  NaN and -infinity are never drawn; a row of
+ * nothing else has action -1 and logp NaN.  Several +infinities share evenly.
+ * The arrays hold one option a row, NULL: the number is all rows'. */
+typedef struct gbx_sample_in {
+  int64_t rows;
+  int32_t actions, elem;
+  const void* logits;
+  int64_t stride; /* of rows */
+  const float *uniform, *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  double temperature, top_p, min_p;
+  int32_t top_k;
+} gbx_sample_in;
+int gbx_sample_actions(const gbx_sample_in* in, int32_t* action, float* logp, void* stream);
+
 /* One AdamW step of `count` tensors (host arrays of device addresses, element
  * counts and places of their states, multiples of 256).  A tensor's states
  * take whole blocks of 256 elements: what lies past its end in its last block
