@@ -146,6 +146,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gbx_selective_scan_grad_work": (_i64, [ctypes.POINTER(ScanIn)]),
     "gbx_selective_scan_grad": (ctypes.c_int, [ctypes.POINTER(ScanIn), _vp, _vp, _i64, _i64, *[_vp] * 10]),
     "gbx_selective_scan_step": (ctypes.c_int, [ctypes.POINTER(ScanIn), *[_vp] * 3]),
+    "gbx_delta_rule_saved": (_i64, [ctypes.POINTER(DeltaIn)]),
     "gbx_delta_rule_work": (_i64, [ctypes.POINTER(DeltaIn)]),
     "gbx_delta_rule": (ctypes.c_int, [ctypes.POINTER(DeltaIn), *[_vp] * 6]),
     "gbx_delta_rule_grad_work": (_i64, [ctypes.POINTER(DeltaIn)]),

@@ -1002,6 +1002,11 @@ int gbx_selective_scan_step(const gbx_scan_in* in, float* state, void* y, void* 
   return GBX_OK;
 }
 
+int64_t gbx_delta_rule_saved(const gbx_delta_in* in) {
+  DeltaArgs a;
+  if (int e = delta_args(in, a)) return e;
+  return delta_saved(a);
+}
 int64_t gbx_delta_rule_work(const gbx_delta_in* in) {
   DeltaArgs a;
   if (int e = delta_args(in, a)) return e;

@@ -42,24 +42,235 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr float kClosed = -104.0f;
 constexpr float kUnitEps = 1e-6f;  // added to a squared length before its root
 
-// d += a b, 16 x 16 x 16 in 32 bits
+__device__ __forceinline__ f4 zero4() { return f4{0.0f, 0.0f, 0.0f, 0.0f}; }
+
+// Factors of a product, four places of the summed index a lane.
+//
+// Whole: 32 bits, on the 32-bit matrix instructions, which take eight times as
+// long for half as many places as the 16-bit ones.  Parts: a sum of N bfloat16
+// values, each what the ones before leave; an input's bfloat16 is one part, a
+// float16 exactly two.  A product of two sums is their terms' products, added in
+// 32 bits, two of them in an instruction that sums 32 places.
+struct Whole {
+  f4 v;
+};
+typedef uint32_t w2 __attribute__((ext_vector_type(2)));
+typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+template <int N>
+struct Parts {
+  w2 p[N];
+};
+// two bfloat16 in a word, and back
+__device__ __forceinline__ uint32_t narrow2(float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, b2));
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ f4 wide(w2 w) { return f4{low(w[0]), high(w[0]), low(w[1]), high(w[1])}; }
+template <int N>
+__device__ __forceinline__ Parts<N> parts_of(f4 x) {
+  Parts<N> r;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    r.p[n] = w2{narrow2(x[0], x[1]), narrow2(x[2], x[3])};
+    if (n + 1 < N) x -= wide(r.p[n]);
+  }
+  return r;
+}
+
+// d += a b, 16 x 16 x 16
 __device__ __forceinline__ f4 mma(f4 a, f4 b, f4 d) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], d, 0, 0, 0);
   return d;
 }
-__device__ __forceinline__ f4 zero4() { return f4{0.0f, 0.0f, 0.0f, 0.0f}; }
+__device__ __forceinline__ f4 mma(Whole a, Whole b, f4 d) { return mma(a.v, b.v, d); }
+// (All 16-bit products are of this one shape: a chain of 16 and 32 places through
+// the same sum has come out without some of its terms.)
+__device__ __forceinline__ f4 two_terms(w2 a, w2 b, w2 a2, w2 b2, f4 d) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, w4{a[0], a[1], a2[0], a2[1]}), __builtin_bit_cast(b8, w4{b[0], b[1], b2[0], b2[1]}), d, 0, 0, 0);
+}
+__device__ __forceinline__ f4 one_term(w2 a, w2 b, f4 d) { return two_terms(a, b, a, w2{0u, 0u}, d); }
+// Terms whose places add up to more than the longer sum's last are below its
+// rounding and left out, but where an instruction has room for one.
+template <int A, int B>
+__device__ __forceinline__ f4 mma(const Parts<A>& a, const Parts<B>& b, f4 d) {
+  if constexpr (A > B) {
+    if constexpr (A == 2) return two_terms(a.p[0], b.p[0], a.p[1], b.p[0], d);
+    else if constexpr (B == 1) return two_terms(a.p[0], b.p[0], a.p[1], b.p[0], one_term(a.p[2], b.p[0], d));
+    else return two_terms(a.p[0], b.p[0], a.p[0], b.p[1], two_terms(a.p[1], b.p[0], a.p[1], b.p[1], two_terms(a.p[2], b.p[0], a.p[2], b.p[1], d)));
+  } else if constexpr (A == 1) {
+    if constexpr (B == 1) return one_term(a.p[0], b.p[0], d);
+    else if constexpr (B == 2) return two_terms(a.p[0], b.p[0], a.p[0], b.p[1], d);
+    else return two_terms(a.p[0], b.p[0], a.p[0], b.p[1], one_term(a.p[0], b.p[2], d));
+  } else if constexpr (B == 2) {
+    return two_terms(a.p[0], b.p[0], a.p[1], b.p[0], two_terms(a.p[0], b.p[1], a.p[1], b.p[1], d));
+  } else if constexpr (A == 2) {
+    return two_terms(a.p[0], b.p[0], a.p[1], b.p[0], two_terms(a.p[0], b.p[1], a.p[1], b.p[1], two_terms(a.p[0], b.p[2], a.p[1], b.p[2], d)));
+  } else {
+    return two_terms(a.p[0], b.p[0], a.p[0], b.p[1], two_terms(a.p[1], b.p[0], a.p[1], b.p[1], two_terms(a.p[2], b.p[0], a.p[0], b.p[2], d)));
+  }
+}
+
+// Inputs in words as they lie in memory.
+template <typename T, int COUNT>
+struct Words {
+  static constexpr int kWords = (COUNT * (int)sizeof(T) + 3) / 4;
+  uint32_t w[kWords];
+};
+// A value of which the compiler does not know that it is the same every time:
+// what is made from it inside a loop is made there, not before.  (Hundreds of
+// masks and addresses of rows that may end inside a tile, kept through a loop over
+// chunks, leave no registers.)
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// COUNT elements.
+template <int COUNT, typename T>
+__device__ __forceinline__ Words<T, COUNT> load_whole(const T* p) {
+  Words<T, COUNT> r{};
+  __builtin_memcpy(r.w, p, COUNT * sizeof(T));
+  return r;
+}
+// Zeros where `has` does not hold.
+template <int COUNT, typename T>
+__device__ __forceinline__ void mask(Words<T, COUNT>& r, bool has) {
+#pragma unroll
+  for (int i = 0; i < r.kWords; ++i) r.w[i] = has ? r.w[i] : 0u;
+}
+// COUNT elements, zero from `valid` on.  (Zeros and loads meet in whole words:
+// where they met in 16-bit elements, each took a register.)
+template <int COUNT, typename T>
+__device__ __forceinline__ Words<T, COUNT> load_words(const T* p, int valid) {
+  Words<T, COUNT> r{};
+  valid = opaque(valid);
+  if (valid >= COUNT) {
+    __builtin_memcpy(r.w, p, COUNT * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        if (i < valid) __builtin_memcpy(&r.w[i], p + i, 4);
+      } else {
+        uint16_t h = 0;
+        if (i < valid) __builtin_memcpy(&h, p + i, 2);
+        r.w[i / 2] |= (uint32_t)h << (16 * (i & 1));
+      }
+    }
+  }
+  return r;
+}
+// elements I and J of 16 bits as one word
+template <int I, int J>
+__device__ __forceinline__ uint32_t pick(const uint32_t* p, const uint32_t* q) {
+  return __builtin_amdgcn_perm(q[J / 2], p[I / 2], ((J & 1) ? 0x07060000u : 0x05040000u) | ((I & 1) ? 0x0302u : 0x0100u));
+}
+
+// How the products take the inputs, of type T, and values computed from them.
+#ifndef GBX_PARTS
+#define GBX_PARTS 3
+#endif
+#ifndef GBX_BIG
+#define GBX_BIG 3
+#endif
+constexpr int kParts = GBX_PARTS, kStateParts = GBX_BIG;
+template <typename T>
+struct Factor {
+  using Raw = Parts<1>;
+  using Fine = Parts<kParts>;
+  using Big = Parts<kStateParts>;
+  // elements I, J, K and L of four rows of words
+  template <int I, int J, int K, int L>
+  static __device__ __forceinline__ Raw raw(const uint32_t* x, const uint32_t* y, const uint32_t* z, const uint32_t* v) {
+    return {{w2{pick<I, J>(x, y), pick<K, L>(z, v)}}};
+  }
+  static __device__ __forceinline__ f4 wide(const Raw& x) { return gbx::wide(x.p[0]); }
+  static __device__ __forceinline__ Fine fine(f4 x) { return parts_of<kParts>(x); }
+  static __device__ __forceinline__ Big big(f4 x) { return parts_of<kStateParts>(x); }
+};
+template <>
+struct Factor<_Float16> {
+  using Raw = Parts<2>;
+  using Fine = Parts<kParts>;
+  using Big = Parts<kStateParts>;
+  static __device__ __forceinline__ float half(const uint32_t* x, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(x[i / 2] >> (16 * (i & 1)))); }
+  template <int I, int J, int K, int L>
+  static __device__ __forceinline__ Raw raw(const uint32_t* x, const uint32_t* y, const uint32_t* z, const uint32_t* v) {
+    return parts_of<2>(f4{half(x, I), half(y, J), half(z, K), half(v, L)});
+  }
+  static __device__ __forceinline__ f4 wide(const Raw& x) { return gbx::wide(x.p[0]) + gbx::wide(x.p[1]); }
+  static __device__ __forceinline__ Fine fine(f4 x) { return parts_of<kParts>(x); }
+  static __device__ __forceinline__ Big big(f4 x) { return parts_of<kStateParts>(x); }
+};
+template <>
+struct Factor<float> {
+  using Raw = Whole;
+  using Fine = Whole;
+  using Big = Whole;
+  template <int I, int J, int K, int L>
+  static __device__ __forceinline__ Raw raw(const uint32_t* x, const uint32_t* y, const uint32_t* z, const uint32_t* v) {
+    return {f4{__uint_as_float(x[I]), __uint_as_float(y[J]), __uint_as_float(z[K]), __uint_as_float(v[L])}};
+  }
+  static __device__ __forceinline__ f4 wide(const Raw& x) { return x.v; }
+  static __device__ __forceinline__ Fine fine(f4 x) { return {x}; }
+  static __device__ __forceinline__ Big big(f4 x) { return {x}; }
+};
+template <typename T>
+using Raw = typename Factor<T>::Raw;
+template <typename T>
+using Fine = typename Factor<T>::Fine;
 
 struct Lane {
   int c, g;  // place among 16 lanes (a row or column), group of 16 (four places of the other index)
   __device__ __forceinline__ int in(int j) const { return 4 * g + j; }
 };
+__device__ __forceinline__ Lane again(Lane l) { return {opaque(l.c), opaque(l.g)}; }
+
+// Another of the 16 lanes' value, zero past their ends.
+template <int CONTROL>
+__device__ __forceinline__ float row_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xF, 0xF, true));
+}
+template <int CONTROL>
+__device__ __forceinline__ double row_lane(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CONTROL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CONTROL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int kQuad = 0x55, kLeft = 0x100, kRight = 0x110, kTurn = 0x120, kOf = 0x150;  // times a lane; by n lanes; lane n's
+// sum over the 16 lanes, in all of them
+__device__ __forceinline__ float row_sum(float v) {
+  v += row_lane<kTurn + 8>(v);
+  v += row_lane<kTurn + 4>(v);
+  v += row_lane<kTurn + 2>(v);
+  return v + row_lane<kTurn + 1>(v);
+}
+// sums over the lanes up to this one, and from this one on
+template <typename V>
+__device__ __forceinline__ V sum_up_to(V v) {
+  v += row_lane<kRight + 1>(v);
+  v += row_lane<kRight + 2>(v);
+  v += row_lane<kRight + 4>(v);
+  return v + row_lane<kRight + 8>(v);
+}
+__device__ __forceinline__ float sum_from(float v) {
+  v += row_lane<kLeft + 1>(v);
+  v += row_lane<kLeft + 2>(v);
+  v += row_lane<kLeft + 4>(v);
+  return v + row_lane<kLeft + 8>(v);
+}
+__device__ __forceinline__ float from_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_ds_bpermute(4 * lane, __float_as_int(v))); }
 
 // A lane's value of the row in(j), given each row's in the lanes c.
 __device__ __forceinline__ f4 across(float own, Lane l) {
   f4 v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = __shfl(own, l.in(j), 16);
+  for (int j = 0; j < 4; ++j) v[j] = from_lane(own, 20 * l.g + j);
   return v;
 }
 
@@ -69,39 +280,72 @@ struct Span {
   __device__ __forceinline__ bool has(int t) const { return t >= lo && t < hi; }
 };
 
-// Rows of q or k: 4 * NT channels of step c each, tile r's place in(j) channel
-// NT * in(j) + r.
-template <int NT, typename T>
-__device__ __forceinline__ void load_rows(const T* p, int64_t step, int channels, Span s, Lane l, f4 (&v)[NT]) {
-  float x[4 * NT];
-  load_row<4 * NT>(p + l.c * step + 4 * NT * l.g, s.has(l.c) ? channels - 4 * NT * l.g : 0, x);
-#pragma unroll
-  for (int r = 0; r < NT; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[r][j] = x[NT * j + r];
-}
-// Columns: NT channels from NT * c on of each step in(j); of q, k, v or dy.
-template <int NT, typename T>
-__device__ __forceinline__ void load_cols(const T* p, int64_t step, int channels, Span s, Lane l, f4 (&v)[NT]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float x[NT];
-    load_row<NT>(p + l.in(j) * step + NT * l.c, s.has(l.in(j)) ? channels - NT * l.c : 0, x);
-#pragma unroll
-    for (int r = 0; r < NT; ++r) v[r][j] = x[r];
+// f(std::integral_constant) for 0 to N - 1
+template <int N, typename F, int I = 0>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, F, I + 1>((F&&)f);
   }
 }
 
-// 1 / length of row c, which the four groups hold a quarter each of.
-template <int NT>
-__device__ __forceinline__ float unit_of(const f4 (&row)[NT], bool normalize) {
-  float ss = 0.0f;
+// A tensor's steps of one head of an env, read as rows (4 * NT channels of step
+// c each, tile r's place in(j) channel NT * in(j) + r) or as columns (NT channels
+// from NT * c on of each step in(j)).
+//
+// FULL: there are as many channels as the tiles have.  Steps outside of the span
+// then read the span's first: loads without branches, which all go out
+// together.  They come out as zeros, or, where nothing is made of them, as they are (KEEP).
+template <typename T, int NT, bool FULL>
+struct Steps {
+  const T* p;  // of the first step, the same in all lanes
+  int64_t step, row, col;
+  int channels;
+  __device__ __forceinline__ Steps(const T* p_, int64_t step_, int channels_, Lane l)
+      : p(p_), step(step_), row(l.c * step_ + 4 * NT * l.g), col(4 * l.g * step_ + NT * l.c), channels(channels_) {}
+  template <bool KEEP = false>
+  __device__ __forceinline__ void rows(int t0, Span s, Lane l, Raw<T> (&v)[NT]) const {
+    Words<T, 4 * NT> x;
+    const bool has = s.has(l.c);
+    if constexpr (FULL) {
+      x = load_whole<4 * NT>(p + t0 * step + (has ? row : s.lo * step + 4 * NT * l.g));
+      if constexpr (!KEEP) mask(x, has);
+    } else {
+      x = load_words<4 * NT>(p + t0 * step + row, has ? channels - 4 * NT * l.g : 0);
+    }
+    each<NT>([&](auto r) { v[r] = Factor<T>::template raw<r, NT + r, 2 * NT + r, 3 * NT + r>(x.w, x.w, x.w, x.w); });
+  }
+  template <bool KEEP = false>
+  __device__ __forceinline__ void cols(int t0, Span s, Lane l, Raw<T> (&v)[NT]) const {
+    Words<T, NT> x[4];
 #pragma unroll
-  for (int r = 0; r < NT; ++r)
+    for (int j = 0; j < 4; ++j) {
+      const bool has = s.has(l.in(j));
+      if constexpr (FULL) {
+        x[j] = load_whole<NT>(p + t0 * step + (has ? j * step + col : s.lo * step + NT * l.c));
+        if constexpr (!KEEP) mask(x[j], has);
+      } else {
+        x[j] = load_words<NT>(p + (t0 + j) * step + col, has ? channels - NT * l.c : 0);
+      }
+    }
+    each<NT>([&](auto r) { v[r] = Factor<T>::template raw<r, r, r, r>(x[0].w, x[1].w, x[2].w, x[3].w); });
+  }
+};
+
+// Inner products of the rows with each other: row c, places in(j), or the other way round.
+template <int NT, typename R>
+__device__ __forceinline__ f4 square_of(const R (&row)[NT]) {
+  f4 x = zero4();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ss = fmaf(row[r][j], row[r][j], ss);
-  ss += __shfl_xor(ss, 16, 64);
-  ss += __shfl_xor(ss, 32, 64);
+  for (int r = 0; r < NT; ++r) x = mma(row[r], row[r], x);
+  return x;
+}
+// 1 / length of row c, from the diagonal.
+__device__ __forceinline__ float unit_of(f4 square, bool normalize, Lane l) {
+  float ss = square[0];
+#pragma unroll
+  for (int j = 1; j < 4; ++j) ss = (l.c & 3) == j ? square[j] : ss;
+  ss = from_lane(ss, (l.c & 12) * 4 + l.c);
   return normalize ? rsqrtf(ss + kUnitEps) : 1.0f;
 }
 
@@ -115,28 +359,21 @@ struct Decay {
 };
 // `gate`: step c's, in powers of two, zero outside of the span
 __device__ __forceinline__ Decay decay_of(double gate, Lane l) {
-  double sum = gate;
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
-    const double o = __shfl_up(sum, m, 16);
-    sum += l.c >= m ? o : 0.0;
-  }
-  const double end = __shfl(sum, 15, 16);
+  const double sum = sum_up_to(gate), end = row_lane<kOf + 15>(sum);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, sum);
   Decay d;
   d.all = exp2_fast((float)end);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double o = __shfl(sum, l.in(j), 16);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (20 * l.g + j), (int)(uint32_t)bits);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (20 * l.g + j), (int)(uint32_t)(bits >> 32));
+    const double o = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
     d.in[j] = exp2_fast((float)o);
     d.tail[j] = exp2_fast((float)(end - o));
-    d.pair[j] = exp2_fast((float)(l.in(j) < l.c ? sum - o : o - sum));
+    const float apart = (float)(sum - o);
+    d.pair[j] = exp2_fast(l.in(j) < l.c ? apart : -apart);
   }
   return d;
-}
-
-template <int LANE>
-__device__ __forceinline__ float quad_lane(float v) {  // of the four lanes around
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), LANE * 0x55, 0xF, 0xF, true));
 }
 
 // The inverse of 1 + L, L strictly lower triangular; `row`: row c, places
@@ -150,26 +387,26 @@ struct Both {
   f4 row, col;
 };
 __device__ __forceinline__ Both inverse(Both L, Lane l) {
-  const int b = l.c >> 2, n = l.c & 3;
+  const int b = l.c >> 2;
   f4 ar, ac, lr, lc;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    ar[j] = ac[j] = l.g == b && j == n ? 1.0f : 0.0f;
+    ar[j] = ac[j] = l.in(j) == l.c ? 1.0f : 0.0f;
     lr[j] = l.g == b ? L.row[j] : 0.0f;
     lc[j] = l.g == b ? L.col[j] : 0.0f;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[0], quad_lane<0>(ar[j]), ar[j]);
+  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[0], row_lane<0 * kQuad>(ar[j]), ar[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[1], quad_lane<1>(ar[j]), ar[j]);
+  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[1], row_lane<1 * kQuad>(ar[j]), ar[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[2], quad_lane<2>(ar[j]), ar[j]);
+  for (int j = 0; j < 4; ++j) ar[j] = fmaf(-lr[2], row_lane<2 * kQuad>(ar[j]), ar[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[3], quad_lane<3>(ac[j]), ac[j]);
+  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[3], row_lane<3 * kQuad>(ac[j]), ac[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[2], quad_lane<2>(ac[j]), ac[j]);
+  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[2], row_lane<2 * kQuad>(ac[j]), ac[j]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[1], quad_lane<1>(ac[j]), ac[j]);
+  for (int j = 0; j < 4; ++j) ac[j] = fmaf(-lc[1], row_lane<1 * kQuad>(ac[j]), ac[j]);
   f4 m8, m16;  // minus M: pairs of blocks, then of pairs
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -191,31 +428,34 @@ struct Unit {
 };
 
 // State tiles: tile (r, t), place in(j): channel NT * in(j) + r, column VT * c + t.
-template <int NT, int VT>
-__device__ __forceinline__ void load_state(const float* p, const DeltaArgs& a, const Unit<NT, VT>& u, f4 (&s)[NT][VT]) {
-#pragma unroll
-  for (int r = 0; r < NT; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = NT * u.l.in(j) + r;
-      float x[VT];
-      load_row<VT>(p + (int64_t)row * a.values + u.col(), row < a.keys ? a.values - u.col() : 0, x);
-#pragma unroll
-      for (int t = 0; t < VT; ++t) s[r][t][j] = x[t];
-    }
+// f(r, j, address, columns that there are): p is the same in all lanes.
+template <bool FULL, int NT, int VT, typename P, typename F>
+__device__ __forceinline__ void each_row(P* p, const DeltaArgs& a, const Unit<NT, VT>& u, F&& f) {
+  const int rows = opaque(a.keys - 4 * NT * u.l.g), wide = opaque(a.values - u.col());
+  const uint32_t at = (uint32_t)opaque((4 * NT * u.l.g * a.values + u.col()) * 4);  // in bytes
+  each<NT * 4>([&](auto n) {
+    constexpr int r = n / 4, j = n % 4, row = NT * j + r;
+    f(r, j, (P*)((uintptr_t)(p + row * a.values) + at), FULL ? VT : row < rows ? wide : 0);
+  });
 }
-template <int NT, int VT>
+template <bool FULL, int NT, int VT>
+__device__ __forceinline__ void load_state(const float* p, const DeltaArgs& a, const Unit<NT, VT>& u, f4 (&s)[NT][VT]) {
+  each_row<FULL>(p, a, u, [&](int r, int j, const float* at, int wide) {
+    Words<float, VT> x;
+    if constexpr (FULL) x = load_whole<VT>(at);
+    else x = load_words<VT>(at, wide);
+#pragma unroll
+    for (int t = 0; t < VT; ++t) s[r][t][j] = __uint_as_float(x.w[t]);
+  });
+}
+template <bool FULL, int NT, int VT>
 __device__ __forceinline__ void store_state(float* p, const DeltaArgs& a, const Unit<NT, VT>& u, const f4 (&s)[NT][VT]) {
+  each_row<FULL>(p, a, u, [&](int r, int j, float* at, int wide) {
+    float x[VT];
 #pragma unroll
-  for (int r = 0; r < NT; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = NT * u.l.in(j) + r;
-      float x[VT];
-#pragma unroll
-      for (int t = 0; t < VT; ++t) x[t] = s[r][t][j];
-      store_row<VT>(p + (int64_t)row * a.values + u.col(), row < a.keys ? a.values - u.col() : 0, x);
-    }
+    for (int t = 0; t < VT; ++t) x[t] = s[r][t][j];
+    store_row<VT>(at, wide, x);
+  });
 }
 template <int NT, int VT>
 __device__ __forceinline__ void clear_state(f4 (&s)[NT][VT]) {
@@ -252,27 +492,77 @@ __device__ __forceinline__ int next_cut(const Gates& r, int lo) {
 }
 __device__ __forceinline__ bool cut_at(const Gates& r, int t) { return r.cuts >> t & 1u; }
 
-// The triangular system of a span, with keys of unit length `kap` (row c) and `kin`.
-struct System {
-  Both T;    // inverse
-  f4 plain;  // L without its betas, row c
-};
-template <int NT>
-__device__ __forceinline__ System system_of(const f4 (&k)[NT], float kap, f4 kin, float beta, f4 bin, const Decay& d, Lane l) {
-  f4 kk = zero4();
-#pragma unroll
-  for (int r = 0; r < NT; ++r) kk = mma(k[r], k[r], kk);
-  System s;
+// The inverse of the triangular system, from the keys' inner products times what is
+// left between their steps (`p`, both ways round).  Forward it is solved for u /
+// beta, so that the gradient finds that without a division:
+//   (1 + P beta) (u / beta) = v - g S0^T k;  the gradient solves (1 + beta P)^T.
+template <bool GRAD>
+__device__ __forceinline__ Both solve(f4 p, float beta, f4 bin, Lane l) {
   Both L;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float p = kk[j] * (kap * kin[j]) * d.pair[j];
-    s.plain[j] = l.in(j) < l.c ? p : 0.0f;
-    L.row[j] = l.in(j) < l.c ? beta * p : 0.0f;
-    L.col[j] = l.in(j) > l.c ? bin[j] * p : 0.0f;
+    L.row[j] = l.in(j) < l.c ? p[j] * (GRAD ? beta : bin[j]) : 0.0f;
+    L.col[j] = l.in(j) <= l.c ? 0.0f : p[j] * (GRAD ? bin[j] : beta);
   }
-  s.T = inverse(L, l);
-  return s;
+  return inverse(L, l);
+}
+
+// What a chunk's products need that does not depend on the state, made by one
+// wavefront for all of a workgroup's: kGroup chunks at a time, side by side.
+constexpr int kGroup = 4;
+template <bool GRAD>
+struct Solved {
+  f4 t[64];                   // solve()'s rows; GRAD: columns
+  f4 m[64];                   // scale G_ij (q_i . k_j), row i; GRAD: row j
+  f4 pair[GRAD ? 64 : 1];     // what is left between two steps, zero across a cut
+  double sums[16];
+  float beta[16], kap[16], qap[16], in[16], tail[16];  // 1 / lengths; qap times the scale, but for GRAD
+  float all;
+  uint32_t cuts;
+  int steps, pad;
+};
+__device__ __forceinline__ f4 of_rows(const float* p, Lane l) { return *reinterpret_cast<const f4*>(p + 4 * l.g); }
+
+// Cuts are gates that let nothing through, which is the same as long as
+// everything in the chunk is finite; where it is not, so is T or the result.
+template <bool GRAD, typename T, int NT, bool FULL>
+__device__ __forceinline__ void solve_chunk(const DeltaArgs& a, int t0, int env, int head, const Steps<T, NT, FULL>& q, const Steps<T, NT, FULL>& k, Lane l, Solved<GRAD>& z) {
+  const Gates gates = load_gates(a, t0, env, head, l);
+  const Span s{0, gates.steps};
+  Raw<T> kr[NT], qr[NT];
+  k.rows(t0, s, l, kr);
+  q.rows(t0, s, l, qr);
+  const f4 kk = square_of(kr);
+  const float kap = unit_of(kk, a.normalize, l);
+  const float qap = (a.normalize ? unit_of(square_of(qr), true, l) : 1.0f) * (GRAD ? 1.0f : a.scale);
+  f4 kq = zero4();
+#pragma unroll
+  for (int r = 0; r < NT; ++r) kq = GRAD ? mma(qr[r], kr[r], kq) : mma(kr[r], qr[r], kq);
+  const double sum = sum_up_to(gates.gate), end = row_lane<kOf + 15>(sum);
+  const uint32_t upto = (2u << l.c) - 1u;  // bits of the steps up to c
+  if (l.g == 0) {
+    z.sums[l.c] = sum;
+    z.beta[l.c] = gates.beta, z.kap[l.c] = kap, z.qap[l.c] = qap;
+    z.in[l.c] = gates.cuts & upto ? 0.0f : exp2_fast((float)sum);
+    z.tail[l.c] = gates.cuts & ~upto ? 0.0f : exp2_fast((float)(end - sum));
+    if (l.c == 0) z.all = gates.cuts ? 0.0f : exp2_fast((float)end), z.cuts = gates.cuts, z.steps = gates.steps;
+  }
+  const int lane = 16 * l.g + l.c;
+  const f4 bin = of_rows(z.beta, l), kin = of_rows(z.kap, l), qin = of_rows(z.qap, l);
+  f4 p, m, pair;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float apart = (float)(sum - z.sums[l.in(j)]);
+    const bool same = ((upto ^ ((2u << l.in(j)) - 1u)) & gates.cuts) == 0u;
+    pair[j] = same ? exp2_fast(l.in(j) < l.c ? apart : -apart) : 0.0f;
+    p[j] = kk[j] * (kap * kin[j]) * pair[j];
+    if constexpr (GRAD) m[j] = l.in(j) < l.c ? 0.0f : kq[j] * (kap * qin[j] * a.scale) * pair[j];
+    else m[j] = l.in(j) <= l.c ? kq[j] * (qap * kin[j]) * pair[j] : 0.0f;
+  }
+  const Both t = solve<GRAD>(p, gates.beta, bin, l);
+  z.t[lane] = GRAD ? t.col : t.row;
+  z.m[lane] = m;
+  if constexpr (GRAD) z.pair[lane] = pair;
 }
 
 __device__ __forceinline__ bool finite4(f4 v) {
@@ -286,6 +576,11 @@ void by_keys(int keys, F&& f) {
   if (keys <= 32) f(std::integral_constant<int, 2>{});
   else if (keys <= 64) f(std::integral_constant<int, 4>{});
   else f(std::integral_constant<int, 8>{});
+}
+template <typename F>
+void by_truth(bool yes, F&& f) {
+  if (yes) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 }  // namespace

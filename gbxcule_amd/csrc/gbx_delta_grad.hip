@@ -26,319 +26,534 @@
 namespace gbx {
 namespace {
 
-// The state with the summed index on its columns: tile (t, r), place in(j):
-// column VT * in(j) + t, channel NT * c + r.
-template <int NT, int VT>
-__device__ __forceinline__ void load_turned(const float* p, const DeltaArgs& a, const Unit<NT, VT>& u, f4 (&s)[VT][NT]) {
-  const int col = u.first + 4 * VT * u.l.g;
+// The state with the summed index on its columns, channels NT * c + r: tile t,
+// place in(j): column VT * in(j) + t.
+template <bool FULL, int NT, int VT>
+__device__ __forceinline__ void load_turned(const float* p, const DeltaArgs& a, const Unit<NT, VT>& u, int r, f4 (&s)[VT]) {
+  const uint32_t at = (uint32_t)opaque((NT * u.l.c * a.values + u.first + 4 * VT * u.l.g) * 4);  // in bytes
+  const float* from = (const float*)((uintptr_t)(p + r * a.values) + at);
+  Words<float, 4 * VT> x;
+  if constexpr (FULL) x = load_whole<4 * VT>(from);
+  else x = load_words<4 * VT>(from, NT * u.l.c + r < a.keys ? a.values - u.first - 4 * VT * u.l.g : 0);
 #pragma unroll
-  for (int r = 0; r < NT; ++r) {
-    const int row = NT * u.l.c + r;
-    float x[4 * VT];
-    load_row<4 * VT>(p + (int64_t)row * a.values + col, row < a.keys ? a.values - col : 0, x);
+  for (int t = 0; t < VT; ++t)
 #pragma unroll
-    for (int t = 0; t < VT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[t][r][j] = x[VT * j + t];
-  }
+    for (int j = 0; j < 4; ++j) s[t][j] = __uint_as_float(x.w[VT * j + t]);
 }
 
-template <typename T, int NT, int VT>
+// The state before a span, both ways round: as the forward pass kept it,
+// or nothing, read where it is used; or moved on from there, in registers.
+template <int NT, int VT>
+struct Kept {
+  const float* p;  // NULL: zeros
+};
+template <int NT, int VT>
+struct Moved {
+  f4 S[NT][VT], St[NT][VT];
+};
+
+template <typename T, int NT, int VT, bool FULL>
 struct Grad {
-  static constexpr int kKeys = 16 * NT;
+  using F = Factor<T>;
   DeltaArgs a;
   Unit<NT, VT> u;
   Lane l;
-  const T *q, *k, *v, *dy;  // of the chunk's first step
-  T* dv;
+  Steps<T, NT, FULL> q, k;
+  Steps<T, VT, FULL> v, dy;
+  int t0;  // the chunk's first step
+  T* dv;   // of that step
+  int64_t dv_lane;
+  float* part;  // in LDS: dq and dk of the chunk's steps, this wavefront's columns' part
   Gates gates;
-  f4 D[NT][VT], Dt[VT][NT];  // gradient of the state, both ways round
-  f4 S[NT][VT], St[VT][NT];  // the state before the span
+  f4 D[NT][VT], Dt[NT][VT];  // gradient of the state, both ways round
 
-  __device__ __forceinline__ void start(const float* saved, bool cut) {
-    if (cut) {
-      clear_state(S);
-      clear_state(St);
+  __device__ __forceinline__ void state(const Kept<NT, VT>& from, f4 (&s)[NT][VT]) const {
+    if (from.p) load_state<FULL>(from.p, a, u, s);
+    else clear_state(s);
+  }
+  __device__ __forceinline__ void turned(const Kept<NT, VT>& from, int r, f4 (&s)[VT]) const {
+    if (from.p) {
+      load_turned<FULL>(from.p, a, u, r, s);
     } else {
-      load_state(saved, a, u, S);
-      load_turned(saved, a, u, St);
+#pragma unroll
+      for (int t = 0; t < VT; ++t) s[t] = zero4();
     }
   }
+  __device__ __forceinline__ void state(const Moved<NT, VT>& from, f4 (&s)[NT][VT]) const {
+#pragma unroll
+    for (int r = 0; r < NT; ++r)
+#pragma unroll
+      for (int t = 0; t < VT; ++t) s[r][t] = from.S[r][t];
+  }
+  __device__ __forceinline__ void turned(const Moved<NT, VT>& from, int r, f4 (&s)[VT]) const {
+#pragma unroll
+    for (int t = 0; t < VT; ++t) s[t] = from.St[r][t];
+  }
+
   // One step of the forward pass.
-  __device__ __forceinline__ void advance(int t0) {
-    const Span s{t0, t0 + 1};
-    f4 kr[NT], kc[NT], vc[VT];
-    load_rows(k, a.k_step, a.keys, s, l, kr);
-    load_cols(k, a.k_step, a.keys, s, l, kc);
-    load_cols(v, a.v_step, a.values - u.first, s, l, vc);
-    const f4 bin = across(s.has(l.c) ? gates.beta : 0.0f, l), kin = across(unit_of(kr, a.normalize), l);
+  __device__ __forceinline__ void advance(int t, Moved<NT, VT>& m) const {
+    const Span s{t, t + 1};
+    Raw<T> kr[NT], kc[NT], vc[VT];
+    k.rows(t0, s, l, kr);
+    k.cols(t0, s, l, kc);
+    v.cols(t0, s, l, vc);
+    const f4 bin = across(s.has(l.c) ? gates.beta : 0.0f, l), kin = across(unit_of(square_of(kr), a.normalize, l), l);
     const Decay d = decay_of(s.has(l.c) ? gates.gate : 0.0, l);
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
       f4 x = zero4();
+      const f4 vt = F::wide(vc[t]);
 #pragma unroll
-      for (int r = 0; r < NT; ++r) x = mma(kr[r], S[r][t], x);
+      for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(m.S[r][t]), x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = s.has(l.in(j)) ? kin[j] * bin[j] * fmaf(-d.in[j] * kin[j], x[j], vc[t][j]) : 0.0f;
+      for (int j = 0; j < 4; ++j) x[j] = s.has(l.in(j)) ? kin[j] * bin[j] * fmaf(-d.in[j] * kin[j], x[j], vt[j]) : 0.0f;
+      const Fine<T> xf = F::fine(x);
 #pragma unroll
       for (int r = 0; r < NT; ++r) {
-        S[r][t] = mma(kc[r], x, S[r][t] * d.all);
-        St[t][r] = mma(x, kc[r], St[t][r] * d.all);
+        m.S[r][t] = mma(kc[r], xf, m.S[r][t] * d.all);
+        m.St[r][t] = mma(xf, kc[r], m.St[r][t] * d.all);
       }
     }
   }
 
-  // Walks a span back.  False, and nothing done, if a value is not finite: in a
-  // product zero times infinity would reach steps that the formulas keep from it.
-  __device__ __forceinline__ bool back(Span s, f4 (&dq)[NT], f4 (&dk)[NT], float& dgate, f4& dbeta) {
-    f4 kr[NT], qr[NT], kc[NT], qc[NT], dyr[VT], dyc[VT], vc[VT];
-    load_rows(k, a.k_step, a.keys, s, l, kr);
-    load_rows(q, a.q_step, a.keys, s, l, qr);
+  // Walks a chunk back whose system is solved.  False, and nothing done, if a
+  // value is not finite: in a product zero times infinity would reach steps that the
+  // formulas keep from it.
+  __device__ __forceinline__ bool chunk(const Solved<true>& z, const float* kept, const Steps<float, VT, FULL>& over, float& dgate, f4& dbeta) {
+    const Span s{0, z.steps};
+    const int lane = 16 * l.g + l.c;
+    Raw<T> kr[NT], dyc[VT];
+    Whole ec[VT], er[VT];
+    k.template rows<true>(t0, s, l, kr);
+    dy.cols(t0, s, l, dyc);
+    over.template cols<true>(t0, s, l, ec);
+    over.template rows<true>(t0, s, l, er);
+    const f4 bin = of_rows(z.beta, l), kin = of_rows(z.kap, l), qin = of_rows(z.qap, l), in = of_rows(z.in, l), tail = of_rows(z.tail, l);
+    const float beta = z.beta[l.c], all = z.all;
+    f4 W[VT], bsum = zero4();
+    Fine<T> Utf[VT], Wtf[VT];  // rows c
+    float whole = 0.0f;        // <S, D> after the chunk: what it wrote, then what it kept
+    {
+      const f4 T_col = z.t[lane];
+      const Fine<T> aq = F::fine(z.m[lane]);
+      bool fine = true;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        f4 x = zero4();
+#pragma unroll
+        for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(D[r][t]), x);
+        x *= tail * kin;
+        const f4 part = x * bin * ec[t].v;
+        whole += (part[0] + part[1]) + (part[2] + part[3]);
+        x = mma(aq, dyc[t], x);
+        W[t] = mma(T_col, x, zero4());
+        Wtf[t] = F::fine(mma(x, T_col, zero4()));
+        Utf[t] = F::fine(er[t].v * beta);
+        bsum += W[t] * ec[t].v;
+        fine = fine && finite4(W[t]) && finite4(ec[t].v);
+      }
+      if (!__all(fine)) return false;
+    }
+    Raw<T> dyr[VT], kc[NT], qc[NT];
+    dy.rows(t0, s, l, dyr);
+    k.template cols<true>(t0, s, l, kc);
+    q.template cols<true>(t0, s, l, qc);
+    Fine<T> asks[VT], gives[VT];  // what D takes up
+    {
+      const f4 ask = a.scale * qin * in, give = -in * kin;
+      float out[4][VT];
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        const f4 v = bin * W[t];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j][t] = v[j];
+        asks[t] = F::fine(ask * F::wide(dyc[t]));
+        gives[t] = F::fine(give * v);
+      }
+      const int64_t v_step = (int64_t)a.envs * a.heads * a.values;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store_row<VT>((dv + j * v_step) + dv_lane, opaque(s.has(l.in(j)) ? FULL ? VT : a.values - u.col() : 0), out[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dbeta[j] = row_sum(bsum[j]);
+    Fine<T> pf, ptf, mf, mtf;
+    {
+      const f4 pair = z.pair[lane];
+      f4 p = zero4(), pt = zero4(), m = zero4(), mt = zero4();
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        p = mma(Utf[t], dyr[t], p);
+        pt = mma(dyr[t], Utf[t], pt);
+        m = mma(Utf[t], Wtf[t], m);
+        mt = mma(Wtf[t], Utf[t], mt);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[j] = l.in(j) <= l.c ? p[j] * (a.scale * kin[j]) * pair[j] : 0.0f;
+        pt[j] = l.in(j) < l.c ? 0.0f : pt[j] * (a.scale * qin[j]) * pair[j];
+        m[j] = l.in(j) < l.c ? -m[j] * (beta * kin[j]) * pair[j] : 0.0f;
+        mt[j] = l.in(j) <= l.c ? 0.0f : -mt[j] * (bin[j] * kin[j]) * pair[j];
+      }
+      pf = F::fine(p), ptf = F::fine(pt), mf = F::fine(m), mtf = F::fine(mt);
+    }
+    const f4 qs = a.scale * in, rs = -in * bin;
+    f4 e = zero4();  // q . dq + k . dk_reads - k . dk_writes
+    float held = 0.0f;
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+      f4 x = zero4(), reads = zero4(), writes = zero4(), St[VT];
+      load_turned<FULL>(kept, a, u, r, St);
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        const auto sf = F::big(St[t]);
+        x = mma(dyr[t], sf, x);
+        reads = mma(Wtf[t], sf, reads);
+        writes = mma(Utf[t], F::big(Dt[r][t]), writes);
+        const f4 part = St[t] * Dt[r][t];
+        held += (part[0] + part[1]) + (part[2] + part[3]);
+      }
+      x = mma(pf, kc[r], x * qs);
+      reads = mma(mf, kc[r], reads * rs);
+      writes = mma(ptf, qc[r], writes * tail);
+      writes = mma(mtf, kc[r], writes);
+      e += qin * F::wide(qc[r]) * x + kin * F::wide(kc[r]) * (reads - writes);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        part[(r * 4 + j) * 64] = x[j];
+        part[((NT + r) * 4 + j) * 64] = reads[j] + writes[j];
+      }
+#pragma unroll
+      for (int t = 0; t < VT; ++t) {
+        D[r][t] = mma(kc[r], gives[t], mma(qc[r], asks[t], D[r][t] * all));
+        Dt[r][t] = mma(gives[t], kc[r], mma(asks[t], qc[r], Dt[r][t] * all));
+      }
+    }
+    whole = row_sum(whole + all * held);
+    whole = from_lane(whole, l.c) + from_lane(whole, l.c + 16) + from_lane(whole, l.c + 32) + from_lane(whole, l.c + 48);
+    float own = 0.0f;  // e of step c, then the sum from there to before the next cut
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float other = from_lane(row_sum(e[j]), (l.c & 12) * 4);
+      own = (l.c & 3) == j ? other : own;
+    }
+    const uint32_t later = z.cuts >> l.c >> 1;
+    const int far = later ? __builtin_ctz(later) + 1 : 16;
+    float v = row_lane<kLeft + 1>(own);
+    own += far > 1 ? v : 0.0f;
+    v = row_lane<kLeft + 2>(own);
+    own += far > 2 ? v : 0.0f;
+    v = row_lane<kLeft + 4>(own);
+    own += far > 4 ? v : 0.0f;
+    v = row_lane<kLeft + 8>(own);
+    own += far > 8 ? v : 0.0f;
+    dgate = z.cuts >> l.c & 1u ? 0.0f : later ? own : own + whole;
+    return true;
+  }
+
+  // Walks a span back, likewise.
+  template <typename From>
+  __device__ __forceinline__ bool back(Span s, const From& from, float& dgate, f4& dbeta) {
+    Raw<T> kr[NT], qr[NT], kc[NT], qc[NT], dyr[VT], dyc[VT], vc[VT];
+    k.rows(t0, s, l, kr);
+    q.rows(t0, s, l, qr);
+    v.cols(t0, s, l, vc);
+    dy.cols(t0, s, l, dyc);
     const float beta = s.has(l.c) ? gates.beta : 0.0f;
-    const float kap = unit_of(kr, a.normalize), qap = unit_of(qr, a.normalize);
+    const f4 kk = square_of(kr);
+    const float kap = unit_of(kk, a.normalize, l), qap = a.normalize ? unit_of(square_of(qr), true, l) : 1.0f;
     const f4 bin = across(beta, l), kin = across(kap, l), qin = across(qap, l);
     const Decay d = decay_of(s.has(l.c) ? gates.gate : 0.0, l);
-    const System sys = system_of(kr, kap, kin, beta, bin, d, l);
-    load_cols(v, a.v_step, a.values - u.first, s, l, vc);
-    load_cols(dy, a.dy_step, a.values - u.first, s, l, dyc);
-    load_rows(dy, a.dy_step, a.values - u.first, s, l, dyr);
+    const f4 plain = kk * (kap * kin) * d.pair;
+    const Both sys = solve<true>(plain, beta, bin, l);
     f4 aq = zero4();  // A^T: row c, places in(j) >= c
 #pragma unroll
     for (int r = 0; r < NT; ++r) aq = mma(qr[r], kr[r], aq);
+    f4 less;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) aq[j] = l.in(j) >= l.c ? aq[j] * (kap * qin[j] * a.scale) * d.pair[j] : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      aq[j] = l.in(j) < l.c ? 0.0f : aq[j] * (kap * qin[j] * a.scale) * d.pair[j];
+      less[j] = l.in(j) < l.c ? -plain[j] : 0.0f;
+    }
+    const Fine<T> aqf = F::fine(aq);
 
-    f4 U[VT], Ut[VT], W[VT], Wt[VT], over[VT];  // over: u / beta
-    float whole = 0.0f;                         // the part of <S, D> that the span wrote
+    f4 W[VT], over[VT];          // over: u / beta
+    Fine<T> Utf[VT], Wtf[VT];    // rows c
+    float whole = 0.0f;          // <S, D> after the span: what it wrote, then what it kept
     bool fine = true;
+    {
+      f4 S[NT][VT];
+      state(from, S);
+      float held = 0.0f;
 #pragma unroll
-    for (int t = 0; t < VT; ++t) {
-      f4 x = zero4(), rhs, plain;
+      for (int t = 0; t < VT; ++t) {
+        f4 x = zero4(), rhs;
+        const f4 vt = F::wide(vc[t]);
 #pragma unroll
-      for (int r = 0; r < NT; ++r) x = mma(kr[r], S[r][t], x);
+        for (int r = 0; r < NT; ++r) {
+          x = mma(kr[r], F::big(S[r][t]), x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        over[t][j] = s.has(l.in(j)) ? fmaf(-d.in[j] * kin[j], x[j], vc[t][j]) : 0.0f;
-        rhs[j] = s.has(l.in(j)) ? bin[j] * over[t][j] : 0.0f;
-        plain[j] = -sys.plain[j];
+          for (int j = 0; j < 4; ++j) held = fmaf(S[r][t][j], D[r][t][j], held);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          over[t][j] = s.has(l.in(j)) ? fmaf(-d.in[j] * kin[j], x[j], vt[j]) : 0.0f;
+          rhs[j] = s.has(l.in(j)) ? bin[j] * over[t][j] : 0.0f;
+        }
+        const f4 U = mma(sys.row, rhs, zero4());
+        Utf[t] = F::fine(mma(rhs, sys.row, zero4()));
+        over[t] = mma(less, U, over[t]);
+        x = zero4();
+#pragma unroll
+        for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(D[r][t]), x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = s.has(l.in(j)) ? d.tail[j] * kin[j] * x[j] : 0.0f;
+          whole = fmaf(x[j], U[j], whole);
+        }
+        x = mma(aqf, dyc[t], x);
+        W[t] = mma(sys.col, x, zero4());
+        Wtf[t] = F::fine(mma(x, sys.col, zero4()));
+        fine = fine && finite4(U) && finite4(W[t]);
       }
-      U[t] = mma(sys.T.row, rhs, zero4());
-      Ut[t] = mma(rhs, sys.T.row, zero4());
-      over[t] = mma(plain, U[t], over[t]);
-      x = zero4();
-#pragma unroll
-      for (int r = 0; r < NT; ++r) x = mma(kr[r], D[r][t], x);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = s.has(l.in(j)) ? d.tail[j] * kin[j] * x[j] : 0.0f;
-        whole = fmaf(x[j], U[t][j], whole);
-      }
-      x = mma(aq, dyc[t], x);
-      W[t] = mma(sys.T.col, x, zero4());
-      Wt[t] = mma(x, sys.T.col, zero4());
-      fine = fine && finite4(U[t]) && finite4(W[t]);
+      whole = fmaf(d.all, held, whole);
     }
     if (s.hi - s.lo > 1 && !__all(fine)) return false;
 
+    dy.rows(t0, s, l, dyr);
     f4 p = zero4(), pt = zero4(), m = zero4(), mt = zero4();
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
-      p = mma(Ut[t], dyr[t], p);
-      pt = mma(dyr[t], Ut[t], pt);
-      m = mma(Ut[t], Wt[t], m);
-      mt = mma(Wt[t], Ut[t], mt);
+      p = mma(Utf[t], dyr[t], p);
+      pt = mma(dyr[t], Utf[t], pt);
+      m = mma(Utf[t], Wtf[t], m);
+      mt = mma(Wtf[t], Utf[t], mt);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       p[j] = l.in(j) <= l.c ? p[j] * (a.scale * kin[j]) * d.pair[j] : 0.0f;
-      pt[j] = l.in(j) >= l.c ? pt[j] * (a.scale * qin[j]) * d.pair[j] : 0.0f;
+      pt[j] = l.in(j) < l.c ? 0.0f : pt[j] * (a.scale * qin[j]) * d.pair[j];
       m[j] = l.in(j) < l.c ? -m[j] * (beta * kin[j]) * d.pair[j] : 0.0f;
-      mt[j] = l.in(j) > l.c ? -mt[j] * (bin[j] * kin[j]) * d.pair[j] : 0.0f;
+      mt[j] = l.in(j) <= l.c ? 0.0f : -mt[j] * (bin[j] * kin[j]) * d.pair[j];
     }
+    const Fine<T> pf = F::fine(p), ptf = F::fine(pt), mf = F::fine(m), mtf = F::fine(mt);
     // dv, dbeta, and what D takes up
-    f4 asks[VT], gives[VT], bsum = zero4();
+    Fine<T> asks[VT], gives[VT];
+    f4 bsum = zero4();
     float out[4][VT];
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
-      Wt[t] *= beta;  // dv's rows
+      f4 x = F::wide(dyc[t]), y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bsum[j] = fmaf(W[t][j], over[t][j], bsum[j]);
         out[j][t] = bin[j] * W[t][j];
-        asks[t][j] = a.scale * qin[j] * d.in[j] * dyc[t][j];
-        gives[t][j] = -d.in[j] * kin[j] * out[j][t];
+        x[j] *= a.scale * qin[j] * d.in[j];
+        y[j] = -d.in[j] * kin[j] * out[j][t];
       }
+      asks[t] = F::fine(x);
+      gives[t] = F::fine(y);
     }
     const int64_t v_step = (int64_t)a.envs * a.heads * a.values;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      store_row<VT>(dv + l.in(j) * v_step, s.has(l.in(j)) ? a.values - u.col() : 0, out[j]);
-#pragma unroll
-      for (int n = 1; n < 16; n <<= 1) bsum[j] += __shfl_xor(bsum[j], n, 16);
-      dbeta[j] = s.has(l.in(j)) ? bsum[j] : dbeta[j];
+      store_row<VT>((dv + j * v_step) + dv_lane, opaque(s.has(l.in(j)) ? FULL ? VT : a.values - u.col() : 0), out[j]);
+      dbeta[j] = s.has(l.in(j)) ? row_sum(bsum[j]) : dbeta[j];
     }
-    load_cols(k, a.k_step, a.keys, s, l, kc);
-    load_cols(q, a.q_step, a.keys, s, l, qc);
+    k.cols(t0, s, l, kc);
+    q.cols(t0, s, l, qc);
     f4 e = zero4();  // q . dq + k . dk_reads - k . dk_writes
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
-      f4 x = zero4(), reads = zero4(), writes = zero4();
+      f4 x = zero4(), reads = zero4(), writes = zero4(), St[VT];
+      turned(from, r, St);
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
-        x = mma(dyr[t], St[t][r], x);
-        reads = mma(Wt[t], St[t][r], reads);
-        writes = mma(Ut[t], Dt[t][r], writes);
+        const auto sf = F::big(St[t]);
+        x = mma(dyr[t], sf, x);
+        reads = mma(Wtf[t], sf, reads);
+        writes = mma(Utf[t], F::big(Dt[r][t]), writes);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] *= a.scale * d.in[j];
-        reads[j] *= -d.in[j];
+        reads[j] *= -d.in[j] * bin[j];
         writes[j] *= d.tail[j];
       }
-      x = mma(p, kc[r], x);
-      reads = mma(m, kc[r], reads);
-      writes = mma(pt, qc[r], writes);
-      writes = mma(mt, kc[r], writes);
+      x = mma(pf, kc[r], x);
+      reads = mma(mf, kc[r], reads);
+      writes = mma(ptf, qc[r], writes);
+      writes = mma(mtf, kc[r], writes);
+      const f4 qw = F::wide(qc[r]), kw = F::wide(kc[r]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        e[j] = fmaf(qin[j] * qc[r][j], x[j], e[j]);
-        e[j] = fmaf(kin[j] * kc[r][j], reads[j] - writes[j], e[j]);
-        dq[r][j] = s.has(l.in(j)) ? x[j] : dq[r][j];
-        dk[r][j] = s.has(l.in(j)) ? reads[j] + writes[j] : dk[r][j];
+        e[j] = fmaf(qin[j] * qw[j], x[j], e[j]);
+        e[j] = fmaf(kin[j] * kw[j], reads[j] - writes[j], e[j]);
+        if (s.has(l.in(j))) {
+          part[(r * 4 + j) * 64] = x[j];
+          part[((NT + r) * 4 + j) * 64] = reads[j] + writes[j];
+        }
       }
-    }
-    float held = 0.0f;
-#pragma unroll
-    for (int r = 0; r < NT; ++r)
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) held = fmaf(S[r][t][j], D[r][t][j], held);
         D[r][t] = mma(kc[r], gives[t], mma(qc[r], asks[t], D[r][t] * d.all));
-        Dt[t][r] = mma(gives[t], kc[r], mma(asks[t], qc[r], Dt[t][r] * d.all));
+        Dt[r][t] = mma(gives[t], kc[r], mma(asks[t], qc[r], Dt[r][t] * d.all));
       }
-    whole = fmaf(d.all, held, whole);
-#pragma unroll
-    for (int n = 1; n < 64; n <<= 1) whole += __shfl_xor(whole, n, 64);
+    }
+    whole = row_sum(whole);
+    whole = from_lane(whole, l.c) + from_lane(whole, l.c + 16) + from_lane(whole, l.c + 32) + from_lane(whole, l.c + 48);
     float own = 0.0f;  // e of step c, then the sum from there on
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int n = 1; n < 16; n <<= 1) e[j] += __shfl_xor(e[j], n, 16);
-      const float other = __shfl(e[j], l.c / 4 * 16, 64);
+      const float other = from_lane(row_sum(e[j]), (l.c & 12) * 4);
       own = (l.c & 3) == j && s.has(l.c) ? other : own;
     }
-#pragma unroll
-    for (int n = 1; n < 16; n <<= 1) {
-      const float later = __shfl_down(own, n, 16);
-      own += l.c + n < 16 ? later : 0.0f;
-    }
+    own = sum_from(own);
     if (s.has(l.c)) dgate = cut_at(gates, l.c) ? 0.0f : whole + own;
     return true;
   }
+
+  // The span one step at a time, each from the state moved on from `known`.
+  __device__ __forceinline__ void back_singly(Span s, const Kept<NT, VT>& known, float& dgate, f4& dbeta) {
+    for (int hi = s.hi; hi > s.lo; --hi) {
+      Moved<NT, VT> m;
+      state(known, m.S);
+#pragma unroll
+      for (int r = 0; r < NT; ++r) turned(known, r, m.St[r]);
+      for (int t = s.lo; t < hi - 1; ++t) advance(t, m);
+      back(Span{hi - 1, hi}, m, dgate, dbeta);
+    }
+  }
 };
 
-// A workgroup is a head of an env, a wavefront some columns of its state.  The
-// columns' parts of dq, dk, dgate and dbeta are added in LDS, in one order.
-template <typename T, int NT, int VT>
-__global__ __launch_bounds__(512 / VT) void delta_grad_kernel(DeltaArgs a) {
-  extern __shared__ float lds[];
-  constexpr int kKeys = 16 * NT, kPart = 2 * kDeltaChunk * kKeys;
-  const int lane = threadIdx.x & 63, slab = threadIdx.x >> 6, slabs = blockDim.x >> 6;
-  float* sums = lds + slabs * kPart;  // [slab][dgate, dbeta][step]
-  Grad<T, NT, VT> w;
-  w.a = a;
-  const int64_t unit = block_id();
-  if (unit >= (int64_t)a.envs * a.heads) return;
-  w.u = {{lane & 15, lane >> 4}, (int)(unit / a.heads), (int)(unit % a.heads), slab * 16 * VT};
-  w.l = w.u.l;
-  const Lane l = w.l;
-  const int env = w.u.env, head = w.u.head;
-  const T* q = (const T*)a.q + env * a.q_env + head / a.share * a.q_head;
-  const T* k = (const T*)a.k + env * a.k_env + head / a.share * a.k_head;
-  const T* v = (const T*)a.v + env * a.v_env + head * a.v_head + w.u.first;
-  const T* dy = (const T*)a.dy + env * a.dy_env + head * a.dy_head + w.u.first;
-  T* dv = (T*)a.dv + unit * a.values + w.u.col();
+// The columns' parts of dq, dk, dgate and dbeta of a chunk, added in one order.
+// lds: [slab][dq, dk][r][j][lane], then [slab][dgate, dbeta][step].
+template <typename T, int NT, int VT, bool FULL>
+__device__ __forceinline__ void join(const Grad<T, NT, VT, FULL>& w, int64_t unit, const float* lds, int slabs) {
+  constexpr int kPart = 2 * NT * 256;
+  const DeltaArgs& a = w.a;
+  const int t0 = w.t0, steps = a.steps - t0;  // (more than a chunk's do no harm)
   const int64_t heads = (int64_t)a.envs * a.heads;
+  for (int i = opaque(threadIdx.x); i < 256; i += blockDim.x) {
+    const int j = i >> 6, c = i & 15, t = 4 * (i >> 4 & 3) + j, rest = opaque(a.keys - NT * c);
+    const bool live = t < steps;
+    const int64_t row = (t0 + t) * heads + unit;
+    auto turn = [&](const T* p, int64_t step, int kind, void* to) {
+      float x[NT], dx[NT] = {}, ss = 0.0f, dot = 0.0f;
+      load_row<NT>(p + t * step + NT * c, live ? rest : 0, x);
+      for (int n = 0; n < slabs; ++n)
+#pragma unroll
+        for (int r = 0; r < NT; ++r) dx[r] += lds[n * kPart + ((kind * NT + r) * 4 + j) * 64 + (i & 63)];
+      if (a.normalize) {  // x / length: the gradient's part along x goes
+#pragma unroll
+        for (int r = 0; r < NT; ++r) {
+          ss = fmaf(x[r], x[r], ss);
+          dot = fmaf(x[r], dx[r], dot);
+        }
+        const float unit_x = rsqrtf(row_sum(ss) + kUnitEps);
+        dot = row_sum(dot) * (unit_x * unit_x);
+#pragma unroll
+        for (int r = 0; r < NT; ++r) dx[r] = unit_x * fmaf(-x[r], dot, dx[r]);
+      }
+      if (a.share == 1) store_row<NT>((T*)to + row * a.keys + NT * c, live ? rest : 0, dx);
+      else store_row<NT>((float*)to + row * a.keys + NT * c, live ? rest : 0, dx);
+    };
+    turn(w.q.p + t0 * a.q_step, a.q_step, 0, a.share == 1 ? a.dq : a.work);
+    turn(w.k.p + t0 * a.k_step, a.k_step, 1, a.share == 1 ? a.dk : a.work + a.steps * heads * a.keys);
+    if (i < 2 * kDeltaChunk && (i & 15) < steps) {
+      float x = 0.0f;
+      for (int n = 0; n < slabs; ++n) x += lds[slabs * kPart + n * 2 * kDeltaChunk + i];
+      (i < kDeltaChunk ? a.dgate : a.dbeta)[(t0 + (i & 15)) * heads + unit] = x;
+    }
+  }
+}
+
+// A workgroup is a head of an env, a wavefront some columns of its state.
+#ifndef GMINW
+#define GMINW 2
+#define GCOLS(nt) (nt == 8 ? 1 : 2)
+#endif
+template <typename T, int NT, int VT, bool FULL>
+__global__ __launch_bounds__(512 / VT, GMINW) void delta_grad_kernel(DeltaArgs a) {
+  extern __shared__ float lds[];
+  __shared__ Solved<true> solved[kGroup];
+  __shared__ int bad;
+  constexpr int kPart = 2 * NT * 256;
+  const int lane = threadIdx.x & 63, slab = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slabs = blockDim.x >> 6;
+  float* sums = lds + slabs * kPart + slab * 2 * kDeltaChunk;
+  const int64_t unit = block_id(), heads = (int64_t)a.envs * a.heads, v_step = heads * a.values;
+  if (unit >= heads) return;
+  const int env = (int)(unit / a.heads), head = (int)(unit % a.heads);
+  const Unit<NT, VT> u{{lane & 15, lane >> 4}, env, head, slab * 16 * VT};
+  Grad<T, NT, VT, FULL> w{a,
+                          u,
+                          u.l,
+                          {(const T*)a.q + env * a.q_env + head / a.share * a.q_head, a.q_step, a.keys, u.l},
+                          {(const T*)a.k + env * a.k_env + head / a.share * a.k_head, a.k_step, a.keys, u.l},
+                          {(const T*)a.v + env * a.v_env + head * a.v_head + u.first, a.v_step, a.values - u.first, u.l},
+                          {(const T*)a.dy + env * a.dy_env + head * a.dy_head + u.first, a.dy_step, a.values - u.first, u.l},
+                          0,
+                          nullptr,
+                          4 * u.l.g * v_step + u.col(),
+                          lds + slab * kPart + lane};
+  const int chunks = (a.steps + kDeltaChunk - 1) / kDeltaChunk;
+  const float* kept = a.saved + unit * a.keys * a.values;
+  const int64_t state = heads * a.keys * a.values;  // of all heads
+  const Steps<float, VT, FULL> over(a.saved + chunks * state + unit * a.values + u.first, v_step, a.values - u.first, u.l);
+  auto at = [&](int chunk) {
+    w.l = again(u.l), w.t0 = chunk * kDeltaChunk;
+    w.dv = (T*)a.dv + unit * a.values + w.t0 * v_step;
+  };
+  auto hand_in = [&](float dgate, const f4& dbeta) {
+    if (w.l.c == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sums[kDeltaChunk + w.l.in(j)] = dbeta[j];
+    }
+    if (w.l.g == 0) sums[w.l.c] = dgate;
+  };
+  if (threadIdx.x == 0) bad = 0;
   clear_state(w.D);
   clear_state(w.Dt);
-  for (int t0 = (a.steps - 1) / kDeltaChunk * kDeltaChunk; t0 >= 0; t0 -= kDeltaChunk) {
-    w.gates = load_gates(a, t0, env, head, l);
-    w.q = q + t0 * a.q_step, w.k = k + t0 * a.k_step, w.v = v + t0 * a.v_step, w.dy = dy + t0 * a.dy_step;
-    w.dv = dv + t0 * heads * a.values;
-    const float* saved = a.saved + ((int64_t)(t0 / kDeltaChunk) * heads + unit) * a.keys * a.values;
-    f4 dq[NT], dk[NT], dbeta = zero4();
+  bool fine = true;
+  for (int last = chunks; last > 0 && fine; last -= kGroup) {
+    const int first = last > kGroup ? last - kGroup : 0;
+    for (int n = slab; n < last - first; n += slabs) solve_chunk(a, (first + n) * kDeltaChunk, env, head, w.q, w.k, again(u.l), solved[n]);
+    __syncthreads();
+    for (int n = last - first - 1; n >= 0 && fine; --n) {
+      at(first + n);
+      f4 dbeta;
+      float dgate;
+      if (w.chunk(solved[n], kept + (first + n) * state, over, dgate, dbeta)) hand_in(dgate, dbeta);
+      else bad = 1;
+      __syncthreads();
+      fine = !bad;  // nobody sets it again before the next barrier
+      if (fine) join(w, unit, lds, slabs);
+      __syncthreads();
+    }
+  }
+  if (fine) return;
+  // the whole rollout span by span, and where a value is not finite step by step
+  clear_state(w.D);
+  clear_state(w.Dt);
+  for (int chunk = chunks - 1; chunk >= 0; --chunk) {
+    at(chunk);
+    w.gates = load_gates(a, w.t0, env, head, w.l);
+    f4 dbeta = zero4();
     float dgate = 0.0f;
-#pragma unroll
-    for (int r = 0; r < NT; ++r) dq[r] = dk[r] = zero4();
-    int singles = kDeltaChunk;  // steps from this one on go one by one
     for (int hi = w.gates.steps; hi > 0;) {
       const uint32_t before = w.gates.cuts & ((1u << hi) - 1u);
-      const int from = before ? 31 - __builtin_clz(before) : 0;  // where the state is known
-      const int lo = hi > singles ? hi - 1 : from;
-      w.start(saved, cut_at(w.gates, from));
-      for (int t = from; t < lo; ++t) w.advance(t);
-      if (!w.back({lo, hi}, dq, dk, dgate, dbeta)) {
-        singles = lo;
-        continue;
-      }
-      if (cut_at(w.gates, lo)) {
+      const Span s{before ? 31 - __builtin_clz(before) : 0, hi};
+      const bool cut = cut_at(w.gates, s.lo);
+      const Kept<NT, VT> known{cut ? nullptr : kept + chunk * state};
+      if (!w.back(s, known, dgate, dbeta)) w.back_singly(s, known, dgate, dbeta);
+      if (cut) {
         clear_state(w.D);
         clear_state(w.Dt);
       }
-      hi = lo;
+      hi = s.lo;
     }
-    float* part = lds + slab * kPart;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float x[NT];
-#pragma unroll
-      for (int r = 0; r < NT; ++r) x[r] = dq[r][j];
-      store_row<NT>(part + l.in(j) * kKeys + NT * l.c, NT, x);
-#pragma unroll
-      for (int r = 0; r < NT; ++r) x[r] = dk[r][j];
-      store_row<NT>(part + (kDeltaChunk + l.in(j)) * kKeys + NT * l.c, NT, x);
-      if (l.c == 0) sums[(slab * 2 + 1) * kDeltaChunk + l.in(j)] = dbeta[j];
-    }
-    if (l.g == 0) sums[slab * 2 * kDeltaChunk + l.c] = dgate;
+    hand_in(dgate, dbeta);
     __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) {
-      const int t = i >> 4, c = i & 15, rest = a.keys - NT * c;
-      const bool live = t < w.gates.steps;
-      const int64_t row = (t0 + t) * heads + unit;
-      auto turn = [&](const T* p, int64_t step, int kind, void* to) {
-        float x[NT], dx[NT] = {}, ss = 0.0f, dot = 0.0f;
-        load_row<NT>(p + t * step + NT * c, live ? rest : 0, x);
-        for (int n = 0; n < slabs; ++n)
-#pragma unroll
-          for (int r = 0; r < NT; ++r) dx[r] += lds[n * kPart + (kind * kDeltaChunk + t) * kKeys + NT * c + r];
-        if (a.normalize) {  // x / length: the gradient's part along x goes
-#pragma unroll
-          for (int r = 0; r < NT; ++r) {
-            ss = fmaf(x[r], x[r], ss);
-            dot = fmaf(x[r], dx[r], dot);
-          }
-#pragma unroll
-          for (int n = 1; n < 16; n <<= 1) {
-            ss += __shfl_xor(ss, n, 16);
-            dot += __shfl_xor(dot, n, 16);
-          }
-          const float unit_x = rsqrtf(ss + kUnitEps);
-          dot *= unit_x * unit_x;
-#pragma unroll
-          for (int r = 0; r < NT; ++r) dx[r] = unit_x * fmaf(-x[r], dot, dx[r]);
-        }
-        if (a.share == 1) store_row<NT>((T*)to + row * a.keys + NT * c, live ? rest : 0, dx);
-        else store_row<NT>((float*)to + row * a.keys + NT * c, live ? rest : 0, dx);
-      };
-      turn(w.q, a.q_step, 0, a.share == 1 ? a.dq : a.work);
-      turn(w.k, a.k_step, 1, a.share == 1 ? a.dk : a.work + a.steps * heads * a.keys);
-      if (i < 2 * kDeltaChunk && c < w.gates.steps) {
-        float x = 0.0f;
-        for (int n = 0; n < slabs; ++n) x += sums[n * 2 * kDeltaChunk + i];
-        (t == 0 ? a.dgate : a.dbeta)[(t0 + c) * heads + unit] = x;
-      }
-    }
+    join(w, unit, lds, slabs);
     __syncthreads();
   }
 }
@@ -360,22 +575,25 @@ __global__ __launch_bounds__(256) void delta_share_kernel(const float* in, int64
 int64_t delta_grad_work(const DeltaArgs& a) { return a.share == 1 ? 0 : 2 * (int64_t)a.steps * a.envs * a.heads * a.keys; }
 
 hipError_t launch_delta_grad(const DeltaArgs& a, hipStream_t st) {
+  hipError_t failed = hipSuccess;
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_keys(a.keys, [&](auto nt) {
-      constexpr int kCols = nt == 8 ? 1 : 2;
+      constexpr int kCols = GCOLS(nt);
       const int slabs = (a.values + 16 * kCols - 1) / (16 * kCols);
-      const size_t shared = (size_t)slabs * (2 * kDeltaChunk * 16 * nt + 2 * kDeltaChunk) * 4;
-      auto* kernel = delta_grad_kernel<T, nt, kCols>;
-      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-      hipLaunchKernelGGL(kernel, wide_grid((int64_t)a.envs * a.heads), dim3(64 * slabs), shared, st, a);
+      const size_t shared = (size_t)slabs * (2 * 256 * nt + 2 * kDeltaChunk) * 4;
+      by_truth(a.keys == 16 * nt && a.values % (16 * kCols) == 0, [&](auto full) {
+        auto* kernel = delta_grad_kernel<T, nt, kCols, full>;
+        if (shared > 64 * 1024) failed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (failed == hipSuccess) hipLaunchKernelGGL(kernel, wide_grid((int64_t)a.envs * a.heads), dim3(64 * slabs), shared, st, a);
+      });
     });
-    if (a.share > 1) {
+    if (a.share > 1 && failed == hipSuccess) {
       const int64_t count = (int64_t)a.steps * a.envs * (a.heads / a.share) * a.keys;
       hipLaunchKernelGGL((delta_share_kernel<T>), dim3((unsigned)std::min<int64_t>((2 * count + 255) / 256, 1 << 16)), dim3(256), 0, st, a.work, count, a.share, a.keys, (T*)a.dq, (T*)a.dk);
     }
   });
-  return hipGetLastError();
+  return failed == hipSuccess ? hipGetLastError() : failed;
 }
 
 }  // namespace gbx

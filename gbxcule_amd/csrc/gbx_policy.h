@@ -89,7 +89,7 @@ struct DeltaArgs {
   const float* state;     // [envs][heads][keys][values] or NULL
   const uint8_t* resets;  // [steps][envs] or NULL
   void* y;                // contiguous
-  float *last, *saved;    // saved: [chunks][envs][heads][keys][values] or NULL
+  float *last, *saved;    // saved: [chunks][envs][heads][keys][values], [steps][envs][heads][values]; or NULL
   float* work;
   const void* dy;  // the rest: gradient only
   int64_t dy_step, dy_env, dy_head;
@@ -149,6 +149,7 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t st);
 int64_t scan_grad_work(int steps, int envs, int dim, int groups, int states);
 hipError_t launch_scan_grad(const ScanArgs& a, hipStream_t st);
 hipError_t launch_scan_step(const ScanArgs& a, hipStream_t st);
+int64_t delta_saved(const DeltaArgs& a);
 int64_t delta_work(const DeltaArgs& a);
 hipError_t launch_delta(const DeltaArgs& a, hipStream_t st);
 int64_t delta_grad_work(const DeltaArgs& a);

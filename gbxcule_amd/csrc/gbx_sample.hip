@@ -111,29 +111,39 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
 
 // ---- longer rows: a workgroup each
 
-// The workgroup's wavefronts, and one place of LDS for each.
+// Sums over a workgroup, in one order.  Two halves of LDS in turn: what one
+// call writes is not what the call before may still read.
 template <int THREADS>
 struct Group {
   static constexpr int kWaves = THREADS / 64;
-  double* lds;  // kWaves
+  double* lds;  // 2 * kWaves
+  int turn;
+  template <typename V>
+  __device__ __forceinline__ const V* share(V v) {
+    V* at = reinterpret_cast<V*>(lds + (turn ^= kWaves));
+    if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return at;
+  }
   template <typename V, typename F>
-  __device__ __forceinline__ V all(V v, F&& f) const {
+  __device__ __forceinline__ V all(V v, F&& f) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) v = f(v, __shfl_xor(v, m, 64));
     if constexpr (kWaves > 1) {
-      V* at = reinterpret_cast<V*>(lds);
-      __syncthreads();  // the last use has been read
-      if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
-      __syncthreads();
+      const V* at = share(v);
       v = at[0];
 #pragma unroll
       for (int n = 1; n < kWaves; ++n) v = f(v, at[n]);
     }
     return v;
   }
+  template <typename V>
+  __device__ __forceinline__ V sum(V v) {
+    return all(v, [](V p, V q) { return p + q; });
+  }
   // sum of the threads before this one, and of all
   template <typename V>
-  __device__ __forceinline__ V before(V v, V& total) const {
+  __device__ __forceinline__ V before(V v, V& total) {
     const int lane = threadIdx.x & 63;
     V run = v;
 #pragma unroll
@@ -144,10 +154,7 @@ struct Group {
     V first = V(0);
     total = __shfl(run, 63, 64);
     if constexpr (kWaves > 1) {
-      V* at = reinterpret_cast<V*>(lds);
-      __syncthreads();
-      if (lane == 0) at[threadIdx.x >> 6] = total;
-      __syncthreads();
+      const V* at = share(total);
       total = V(0);
 #pragma unroll
       for (int n = 0; n < kWaves; ++n) {
@@ -157,6 +164,17 @@ struct Group {
     }
     run = __shfl_up(run, 1, 64);
     return first + (lane ? run : V(0));
+  }
+  // threads for which it holds
+  __device__ __forceinline__ int count(bool yes) {
+    int n = __builtin_popcountll(__ballot(yes));
+    if constexpr (kWaves > 1) {
+      const int* at = share(n);
+      n = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) n += at[w];
+    }
+    return n;
   }
 };
 
@@ -169,62 +187,24 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return (b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) >> (32 - kKeyBits<T>);
 }
 
-// HELD consecutive logits a thread stay in registers (0: rows of any length,
-// read again at each turn).  Cuts are found by halving the range of keys, one
-// count or sum over the row a bit.
-template <typename T, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
-  __shared__ double lds[THREADS / 64];
-  __shared__ int choice[2];
-  const Group<THREADS> group{lds};
-  const int64_t row = block_id();
-  if (row >= a.rows) return;
-  const T* logits = (const T*)a.logits + row * a.stride;
-  const int each = HELD ? HELD : (a.actions + THREADS - 1) / THREADS, first = threadIdx.x * each;
-  float held[HELD ? HELD : 1];
-  if constexpr (HELD > 0) {
-    load_row<HELD>(logits + first, a.actions - first, held);
-#pragma unroll
-    for (int e = 0; e < HELD; ++e) held[e] = first + e < a.actions ? logit(held[e]) : -INFINITY;
-  }
-  auto over = [&](auto&& f) {  // f(place, logit) of this thread's
-    if constexpr (HELD > 0) {
-#pragma unroll
-      for (int e = 0; e < HELD; ++e) f(e, held[e]);
-    } else {
-      for (int e = 0; e < each && first + e < a.actions; ++e) f(e, logit(logits[first + e]));
-    }
-  };
-  auto add = [](auto p, auto q) { return p + q; };
-  float most = -INFINITY;
-  over([&](int, float x) { most = fmaxf(most, x); });
-  most = group.all(most, [](float p, float q) { return fmaxf(p, q); });
-  if (most == -INFINITY) {
-    if (threadIdx.x == 0) write_none(a, row);
-    return;
-  }
-  const Cuts c = cuts_of(a, row);
-  double weights[HELD ? HELD : 1];
-  if constexpr (HELD > 0) {
-#pragma unroll
-    for (int e = 0; e < HELD; ++e) weights[e] = weight_of(held[e], most, c.heat);
-  }
-  auto weight = [&](int e, float x) {
-    if constexpr (HELD > 0) return weights[e];
-    else return weight_of(x, most, c.heat);
-  };
+// Draws from the row's logits, or from those of them that can stay, which
+// over(f) hands to f(logit, weight, index) thread by thread in the order of
+// their indexes.  `full`: the weight of all.  Cuts are found by halving the range
+// of keys, one count or sum over the row a bit.
+template <typename T, int THREADS, typename Over>
+__device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Cuts& c, double full, Group<THREADS>& group, int* choice, Over&& over) {
   // what stays: keys above `edge`, and the first `equals` of those at it
   uint32_t edge = 0;
   int equals = a.actions;
   auto count_from = [&](uint32_t t) {
     int n = 0;
-    over([&](int, float x) { n += key_of<T>(x) >= t; });
-    return group.all(n, add);
+    over([&](float x, double, int) { n += key_of<T>(x) >= t; });
+    return group.sum(n);
   };
   auto mass_from = [&](uint32_t t) {
     double n = 0.0;
-    over([&](int e, float x) { n += key_of<T>(x) >= t ? weight(e, x) : 0.0; });
-    return group.all(n, add);
+    over([&](float x, double w, int) { n += key_of<T>(x) >= t ? w : 0.0; });
+    return group.sum(n);
   };
   if (c.k) {
     for (int bit = kKeyBits<T> - 1; bit >= 0; --bit)
@@ -232,23 +212,22 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
     equals = c.k - count_from(edge + 1u);
   }
   if (c.p < 1.0) {
-    // the logit at an edge: weights of equals are equal
-    auto at_edge = [&](uint32_t t, double& w) {
-      w = 0.0;
+    auto at_edge = [&](uint32_t t, double& weight) {  // equals have equal weights
+      weight = 0.0;
       int n = 0;
-      over([&](int e, float x) {
+      over([&](float x, double w, int) {
         if (key_of<T>(x) == t) {
-          w = weight(e, x);
+          weight = w;
           ++n;
         }
       });
-      w = group.all(w, [](double p, double q) { return p > q ? p : q; });
-      return group.all(n, add);
+      weight = group.all(weight, [](double p, double q) { return p > q ? p : q; });
+      return group.sum(n);
     };
     double w;
     const int there = at_edge(edge, w);
     if (equals > there) equals = there;
-    const double above = mass_from(edge + 1u), need = c.p * (above + equals * w);
+    const double above = mass_from(edge + 1u), need = c.p * (c.k ? above + equals * w : full);
     if (above >= need) {  // the edge goes up
       uint32_t t = 0;
       for (int bit = kKeyBits<T> - 1; bit >= 0; --bit)
@@ -263,43 +242,147 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
     equals = fewest < 1 ? 1 : fewest;
   }
   int mine = 0, there;
-  over([&](int, float x) { mine += key_of<T>(x) == edge; });
-  int rank = group.before(mine, there);
-  auto kept = [&](int e, float x, int& rank) {
+  over([&](float x, double, int) { mine += key_of<T>(x) == edge; });
+  const int rank = group.before(mine, there);
+  auto kept = [&](float x, double w, int& r) {
     const uint32_t key = key_of<T>(x);
-    const double w = weight(e, x);
-    const bool stays = key > edge || (key == edge && rank < equals);
-    rank += key == edge;
+    const bool stays = key > edge || (key == edge && r < equals);
+    r += key == edge;
     return stays && w >= c.least ? w : 0.0;
   };
   double sum = 0.0, all;
-  {
-    int r = rank;
-    over([&](int e, float x) { sum += kept(e, x, r); });
-  }
-  const double start = group.before(sum, all);
+  int r = rank;
+  over([&](float x, double w, int) { sum += kept(x, w, r); });
   if (threadIdx.x < 2) choice[threadIdx.x] = threadIdx.x ? -1 : a.actions;
-  __syncthreads();
+  double run = group.before(sum, all);
+  if constexpr (THREADS == 64) __syncthreads();
   const double target = (double)a.uniform[row] * all;
-  {
-    double run = start;
-    int r = rank, past = a.actions, last = -1;
-    over([&](int e, float x) {
-      const double w = kept(e, x, r);
-      run += w;
-      if (w > 0.0) {
-        last = first + e;
-        if (past == a.actions && run > target) past = first + e;
-      }
-    });
-    if (past < a.actions) atomicMin(&choice[0], past);
-    if (last >= 0) atomicMax(&choice[1], last);
-  }
+  int past = a.actions, last = -1;
+  r = rank;
+  over([&](float x, double w, int index) {
+    w = kept(x, w, r);
+    run += w;
+    if (w > 0.0) {
+      last = index;
+      if (past == a.actions && run > target) past = index;
+    }
+  });
+  if (past < a.actions) atomicMin(&choice[0], past);
+  if (last >= 0) atomicMax(&choice[1], last);
   __syncthreads();
   const int action = choice[0] < a.actions ? choice[0] : choice[1];
-  over([&](int e, float x) {
-    if (first + e == action) write(a, row, action, weight(e, x) / all);
+  over([&](float, double w, int index) {
+    if (index == action) write(a, row, action, w / all);
   });
+}
+
+// HELD consecutive logits a thread stay in registers (0: rows of any length, read
+// again at each turn), and with KEEP their weights.
+//
+// Where few logits can stay they are put together first, one a thread, which
+// makes the turns of the search short: those from the k-th largest of the
+// threads' own largest on hold the k largest of the row; and those that weigh
+// less than (1 - p) / actions of the row are together less than what top_p leaves
+// out.
+template <typename T, int THREADS, int HELD, bool KEEP>
+__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
+  __shared__ double lds[2 * THREADS / 64];
+  __shared__ float some[THREADS];
+  __shared__ int places[THREADS], choice[2];
+  Group<THREADS> group{lds, 0};
+  const int64_t row = block_id();
+  if (row >= a.rows) return;
+  const T* logits = (const T*)a.logits + row * a.stride;
+  const int each = HELD ? HELD : (a.actions + THREADS - 1) / THREADS, first = threadIdx.x * each;
+  float held[HELD ? HELD : 1];
+  double weights[KEEP ? HELD : 1];
+  float most = -INFINITY;
+  if constexpr (HELD > 0) {
+#pragma unroll
+    for (int e = 0; e < HELD; e += 8) {
+      float x[8];
+      load_row<8>(logits + first + e, a.actions - first - e, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        held[e + i] = first + e + i < a.actions ? logit(x[i]) : -INFINITY;
+        most = fmaxf(most, held[e + i]);
+      }
+    }
+  } else {
+    for (int e = first; e < first + each && e < a.actions; ++e) most = fmaxf(most, logit(logits[e]));
+  }
+  const uint32_t own = key_of<T>(most);
+  most = group.all(most, [](float p, float q) { return fmaxf(p, q); });
+  if (most == -INFINITY) {
+    if (threadIdx.x == 0) write_none(a, row);
+    return;
+  }
+  const Cuts c = cuts_of(a, row);
+  auto logits_of = [&](auto&& f) {  // f(logit, index)
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int e = 0; e < HELD; ++e) f(held[e], first + e);
+    } else {
+      for (int e = first; e < first + each && e < a.actions; ++e) f(logit(logits[e]), e);
+    }
+  };
+  auto over = [&](auto&& f) {  // f(logit, weight, index)
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int e = 0; e < HELD; ++e) f(held[e], weights[e], first + e);
+    } else {
+      logits_of([&](float x, int index) { f(x, weight_of(x, most, c.heat), index); });
+    }
+  };
+  // Draws from the logits that each_of(f) hands to f, if there are no more of them than threads.
+  auto from_some = [&](double full, auto&& each_of) {
+    int mine = 0, count;
+    each_of([&](float, int) { ++mine; });
+    int at = group.before(mine, count);
+    if (count > THREADS) return false;
+    each_of([&](float x, int index) {
+      some[at] = x;
+      places[at++] = index;
+    });
+    __syncthreads();
+    const bool live = (int)threadIdx.x < count;
+    const float x = live ? some[threadIdx.x] : -INFINITY;
+    const int index = live ? places[threadIdx.x] : a.actions;
+    const double w = weight_of(x, most, c.heat);
+    draw<T>(a, row, c, full, group, choice, [&](auto&& f) { f(x, w, index); });
+    return true;
+  };
+  if (c.k && c.k <= THREADS) {
+    uint32_t from = 0;
+    for (int bit = kKeyBits<T> - 1; bit >= 0; --bit)
+      if (group.count(own >= (from | 1u << bit)) >= c.k) from |= 1u << bit;
+    if (from_some(0.0, [&](auto&& f) {
+          logits_of([&](float x, int index) {
+            if (key_of<T>(x) >= from && x > -INFINITY) f(x, index);
+          });
+        }))
+      return;
+  }
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int e = 0; e < HELD; ++e) weights[e] = weight_of(held[e], most, c.heat);
+  }
+  double full = 0.0;
+  if (!c.k && (c.p < 1.0 || c.least > 0.0)) {
+    double least = c.least;
+    if (c.p < 1.0) {
+      over([&](float, double w, int) { full += w; });
+      full = group.sum(full);
+      least = fmax(least, (1.0 - c.p) * full / a.actions * (1.0 - 1e-9));
+    }
+    if (from_some(full, [&](auto&& f) {
+          over([&](float x, double w, int index) {
+            if (w >= least && w > 0.0) f(x, index);
+          });
+        }))
+      return;
+  }
+  draw<T>(a, row, c, full, group, choice, over);
 }
 
 }  // namespace
@@ -308,7 +391,13 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     auto few = [&](auto lanes) { hipLaunchKernelGGL((sample_few_kernel<T, lanes>), wide_grid((a.rows + 256 / lanes - 1) / (256 / lanes)), dim3(256), 0, st, a); };
-    auto many = [&](auto threads, auto held) { hipLaunchKernelGGL((sample_kernel<T, threads, held>), wide_grid(a.rows), dim3(threads), 0, st, a); };
+    auto many = [&](auto threads, auto held) {
+      // one top_k for all, of which every row finds few logits to draw from: their
+      // weights alone are computed, and without 128 registers for all of them two
+      // long rows share a compute unit
+      if (held == 0 || (!a.top_ks && a.top_k > 0 && a.top_k <= threads)) hipLaunchKernelGGL((sample_kernel<T, threads, held, false>), wide_grid(a.rows), dim3(threads), 0, st, a);
+      else hipLaunchKernelGGL((sample_kernel<T, threads, held, (held > 0)>), wide_grid(a.rows), dim3(threads), 0, st, a);
+    };
     using std::integral_constant;
     if (a.actions <= 8) few(integral_constant<int, 8>{});
     else if (a.actions <= 16) few(integral_constant<int, 16>{});
@@ -316,7 +405,8 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
     else if (a.actions <= 64) few(integral_constant<int, 64>{});
     else if (a.actions <= 512) many(integral_constant<int, 64>{}, integral_constant<int, 8>{});
     else if (a.actions <= 2048) many(integral_constant<int, 256>{}, integral_constant<int, 8>{});
-    else if (a.actions <= 16384) many(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+    else if (a.actions <= 8192) many(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+    else if (a.actions <= 32768) many(integral_constant<int, 512>{}, integral_constant<int, 64>{});
     else many(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
   });
   return hipGetLastError();

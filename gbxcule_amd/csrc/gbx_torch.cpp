@@ -488,10 +488,11 @@ gbx_delta_in delta_in(const Delta& d, double scale, bool normalize, int elem) {
 }
 variable_list delta_forward(const Delta& d, const Tensor& state, double scale, bool normalize, int elem, bool save) {
   const c10::DeviceGuard guard(d.v.device());
-  const int64_t steps = d.v.size(0), envs = d.v.size(1), heads = d.v.size(2), values = d.v.size(3), keys = d.q.size(3);
-  const Tensor y = blank(d.v), last = floats(d.v, {envs, heads, keys, values}), saved = save ? floats(d.v, {(steps + 15) / 16, envs, heads, keys, values}) : Tensor();
-  if (d.v.numel() == 0) return {y, unmoved(state, last), saved};
+  const int64_t envs = d.v.size(1), heads = d.v.size(2), values = d.v.size(3), keys = d.q.size(3);
+  const Tensor y = blank(d.v), last = floats(d.v, {envs, heads, keys, values});
+  if (d.v.numel() == 0) return {y, unmoved(state, last), Tensor()};
   const gbx_delta_in g = delta_in(d, scale, normalize, elem);
+  const Tensor saved = save ? work(d.v, gbx_delta_rule_saved(&g)) : Tensor();
   const Tensor scratch = work(d.v, gbx_delta_rule_work(&g));
   check(gbx_delta_rule(&g, fin(state), out(y), fout(last), fout(saved), fout(scratch), stream(d.v)));
   return {y, last, saved};

@@ -322,7 +322,8 @@ typedef struct gbx_delta_in {
 } gbx_delta_in;
 /* state[envs][heads][keys][values] (NULL: zeros) before the first step, last
  * after the last one.  saved, if not NULL, receives what the gradient starts
- * from: [steps / 16 rounded up][envs][heads][keys][values]. */
+ * from, as many floats as gbx_delta_rule_saved returns. */
+int64_t gbx_delta_rule_saved(const gbx_delta_in* in);
 int64_t gbx_delta_rule_work(const gbx_delta_in* in);
 int gbx_delta_rule(const gbx_delta_in* in, const float* state, void* y, float* last, float* saved,
                    float* work, void* stream);

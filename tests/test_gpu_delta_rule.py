@@ -256,7 +256,9 @@ def test_nothing_from_before_an_episode():
         clean = [r.detach().requires_grad_() for r in rows]
         want = torch.autograd.grad(delta_rule(*clean, state=s["state"], resets=s["resets"])[0], clean, dy)
         for a, b, name in zip(got, want, NAMES):
-            assert torch.equal(a[at:], b[at:]), name
+            # a rollout with a value that is not finite is walked back span by span, with u computed anew where the
+            # other has the forward pass's: two orders of the same sums, each within _roundings of the formulas
+            assert float((a[at:] - b[at:]).abs().max()) <= 2 * 4 * _roundings(36, 24) * 2.0**-23 * float(b.abs().max()), name
         one = delta_rule_step(*(r.detach()[at] for r in dirty), state=state, resets=s["resets"][at])
         ref.check(one, ref.f64(y[at]), 64, "step")
         assert torch.isfinite(state).all()
