@@ -510,6 +510,7 @@ __device__ __forceinline__ Both solve(f4 p, float beta, f4 bin, Lane l) {
 // What a chunk's products need that does not depend on the state, made by one
 // wavefront for all of a workgroup's: kGroup chunks at a time, side by side.
 constexpr int kGroup = 4;
+constexpr int kManyWaves = 1024;  // one for each SIMD
 template <bool GRAD>
 struct Solved {
   f4 t[64];                   // solve()'s rows; GRAD: columns
@@ -576,6 +577,15 @@ void by_keys(int keys, F&& f) {
   if (keys <= 32) f(std::integral_constant<int, 2>{});
   else if (keys <= 64) f(std::integral_constant<int, 4>{});
   else f(std::integral_constant<int, 8>{});
+}
+// f(tiles of columns a wavefront takes): two share what does not depend on the
+// columns, but registers do for no more with 128 keys, and a few heads need all the
+// wavefronts that they can make.
+constexpr int slabs_of(int values, int cols) { return (values + 16 * cols - 1) / (16 * cols); }
+template <int MOST, typename F>
+void by_columns(const DeltaArgs& a, F&& f) {
+  if (MOST > 1 && (int64_t)a.envs * a.heads * slabs_of(a.values, 2) >= kManyWaves) f(std::integral_constant<int, MOST>{});
+  else f(std::integral_constant<int, 1>{});
 }
 template <typename F>
 void by_truth(bool yes, F&& f) {

@@ -63,9 +63,10 @@ struct Grad {
   int t0;  // the chunk's first step
   T* dv;   // of that step
   int64_t dv_lane;
-  float* part;  // in LDS: dq and dk of the chunk's steps, this wavefront's columns' part
+  float *tiles, *part;  // in LDS: dq and dk of the chunk's steps, this wavefront's columns' part; the lane's place
   Gates gates;
-  f4 D[NT][VT], Dt[NT][VT];  // gradient of the state, both ways round
+  f4 D[NT][VT];   // gradient of the state
+  f4 Dt[NT][VT];  // the other way round; a chunk whose system is solved turns D in LDS
 
   __device__ __forceinline__ void state(const Kept<NT, VT>& from, f4 (&s)[NT][VT]) const {
     if (from.p) load_state<FULL>(from.p, a, u, s);
@@ -123,13 +124,23 @@ struct Grad {
     const Span s{0, z.steps};
     const int lane = 16 * l.g + l.c;
     Raw<T> kr[NT], dyc[VT];
-    Whole ec[VT], er[VT];
+    Whole ec[VT], er[VT];  // u / beta
     k.template rows<true>(t0, s, l, kr);
-    dy.cols(t0, s, l, dyc);
     over.template cols<true>(t0, s, l, ec);
     over.template rows<true>(t0, s, l, er);
+    dy.cols(t0, s, l, dyc);
     const f4 bin = of_rows(z.beta, l), kin = of_rows(z.kap, l), qin = of_rows(z.qap, l), in = of_rows(z.in, l), tail = of_rows(z.tail, l);
     const float beta = z.beta[l.c], all = z.all;
+    // D goes through LDS to be read the other way round, tile (r, t) where dq's (t = 0) and dk's (t = 1) tile
+    // r comes to lie afterwards.  Every other four rows lie two by two the other way, so that
+    // 16 columns of four rows fall on all banks.
+#pragma unroll
+    for (int r = 0; r < NT; ++r)
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tiles[(t * NT + r) * 256 + (l.in(j) ^ (l.g & 1)) * 16 + l.c] = D[r][t][j];
+    const int turned = (l.c ^ (l.c >> 2 & 1)) * 16 + 4 * l.g;
     f4 W[VT], bsum = zero4();
     Fine<T> Utf[VT], Wtf[VT];  // rows c
     float whole = 0.0f;        // <S, D> after the chunk: what it wrote, then what it kept
@@ -155,11 +166,12 @@ struct Grad {
       if (!__all(fine)) return false;
     }
     Raw<T> dyr[VT], kc[NT], qc[NT];
+    f4 St[VT];
     dy.rows(t0, s, l, dyr);
     k.template cols<true>(t0, s, l, kc);
     q.template cols<true>(t0, s, l, qc);
-    Fine<T> asks[VT], gives[VT];  // what D takes up
-    {
+    {  // dv, and what D takes up
+      Fine<T> asks[VT], gives[VT];
       const f4 ask = a.scale * qin * in, give = -in * kin;
       float out[4][VT];
 #pragma unroll
@@ -173,7 +185,12 @@ struct Grad {
       const int64_t v_step = (int64_t)a.envs * a.heads * a.values;
 #pragma unroll
       for (int j = 0; j < 4; ++j) store_row<VT>((dv + j * v_step) + dv_lane, opaque(s.has(l.in(j)) ? FULL ? VT : a.values - u.col() : 0), out[j]);
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+#pragma unroll
+        for (int t = 0; t < VT; ++t) D[r][t] = mma(kc[r], gives[t], mma(qc[r], asks[t], D[r][t] * all));
     }
+    load_turned<FULL>(kept, a, u, 0, St);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dbeta[j] = row_sum(bsum[j]);
     Fine<T> pf, ptf, mf, mtf;
@@ -201,16 +218,18 @@ struct Grad {
     float held = 0.0f;
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
-      f4 x = zero4(), reads = zero4(), writes = zero4(), St[VT];
-      load_turned<FULL>(kept, a, u, r, St);
+      f4 x = zero4(), reads = zero4(), writes = zero4(), next[VT];
+      if (r + 1 < NT) load_turned<FULL>(kept, a, u, r + 1, next);
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
         const auto sf = F::big(St[t]);
+        const f4 Dr = *reinterpret_cast<const f4*>(tiles + (t * NT + r) * 256 + turned);
         x = mma(dyr[t], sf, x);
         reads = mma(Wtf[t], sf, reads);
-        writes = mma(Utf[t], F::big(Dt[r][t]), writes);
-        const f4 part = St[t] * Dt[r][t];
+        writes = mma(Utf[t], F::big(Dr), writes);
+        const f4 part = St[t] * Dr;
         held += (part[0] + part[1]) + (part[2] + part[3]);
+        if (r + 1 < NT) St[t] = next[t];
       }
       x = mma(pf, kc[r], x * qs);
       reads = mma(mf, kc[r], reads * rs);
@@ -221,11 +240,6 @@ struct Grad {
       for (int j = 0; j < 4; ++j) {
         part[(r * 4 + j) * 64] = x[j];
         part[((NT + r) * 4 + j) * 64] = reads[j] + writes[j];
-      }
-#pragma unroll
-      for (int t = 0; t < VT; ++t) {
-        D[r][t] = mma(kc[r], gives[t], mma(qc[r], asks[t], D[r][t] * all));
-        Dt[r][t] = mma(gives[t], kc[r], mma(asks[t], qc[r], Dt[r][t] * all));
       }
     }
     whole = row_sum(whole + all * held);
@@ -468,12 +482,8 @@ __device__ __forceinline__ void join(const Grad<T, NT, VT, FULL>& w, int64_t uni
 }
 
 // A workgroup is a head of an env, a wavefront some columns of its state.
-#ifndef GMINW
-#define GMINW 2
-#define GCOLS(nt) (nt == 8 ? 1 : 2)
-#endif
 template <typename T, int NT, int VT, bool FULL>
-__global__ __launch_bounds__(512 / VT, GMINW) void delta_grad_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(512 / VT, 2) void delta_grad_kernel(DeltaArgs a) {
   extern __shared__ float lds[];
   __shared__ Solved<true> solved[kGroup];
   __shared__ int bad;
@@ -494,6 +504,7 @@ __global__ __launch_bounds__(512 / VT, GMINW) void delta_grad_kernel(DeltaArgs a
                           0,
                           nullptr,
                           4 * u.l.g * v_step + u.col(),
+                          lds + slab * kPart,
                           lds + slab * kPart + lane};
   const int chunks = (a.steps + kDeltaChunk - 1) / kDeltaChunk;
   const float* kept = a.saved + unit * a.keys * a.values;
@@ -510,9 +521,9 @@ __global__ __launch_bounds__(512 / VT, GMINW) void delta_grad_kernel(DeltaArgs a
     }
     if (w.l.g == 0) sums[w.l.c] = dgate;
   };
+  static_assert(VT <= 2, "a tile of D for each of dq and dk");
   if (threadIdx.x == 0) bad = 0;
   clear_state(w.D);
-  clear_state(w.Dt);
   bool fine = true;
   for (int last = chunks; last > 0 && fine; last -= kGroup) {
     const int first = last > kGroup ? last - kGroup : 0;
@@ -579,13 +590,14 @@ hipError_t launch_delta_grad(const DeltaArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     by_keys(a.keys, [&](auto nt) {
-      constexpr int kCols = GCOLS(nt);
-      const int slabs = (a.values + 16 * kCols - 1) / (16 * kCols);
-      const size_t shared = (size_t)slabs * (2 * 256 * nt + 2 * kDeltaChunk) * 4;
-      by_truth(a.keys == 16 * nt && a.values % (16 * kCols) == 0, [&](auto full) {
-        auto* kernel = delta_grad_kernel<T, nt, kCols, full>;
-        if (shared > 64 * 1024) failed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-        if (failed == hipSuccess) hipLaunchKernelGGL(kernel, wide_grid((int64_t)a.envs * a.heads), dim3(64 * slabs), shared, st, a);
+      by_columns<nt == 8 ? 1 : 2>(a, [&](auto cols) {
+        const int slabs = slabs_of(a.values, cols);
+        const size_t shared = (size_t)slabs * (2 * 256 * nt + 2 * kDeltaChunk) * 4;
+        by_truth(a.keys == 16 * nt && a.values % (16 * cols) == 0, [&](auto full) {
+          auto* kernel = delta_grad_kernel<T, nt, cols, full>;
+          if (shared > 48 * 1024) failed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+          if (failed == hipSuccess) hipLaunchKernelGGL(kernel, wide_grid((int64_t)a.envs * a.heads), dim3(64 * slabs), shared, st, a);
+        });
       });
     });
     if (a.share > 1 && failed == hipSuccess) {

@@ -91,6 +91,11 @@ struct DeltaArgs {
   void* y;                // contiguous
   float *last, *saved;    // saved: [chunks][envs][heads][keys][values], [steps][envs][heads][values]; or NULL
   float* work;
+  // a rollout in pieces of so many steps (pieces 1: none); the states that pieces after the first start from;
+  // what a piece makes of the state before it; which of both are not finite
+  int pieces, piece_steps;
+  float *starts, *maps;
+  int32_t* flags;
   const void* dy;  // the rest: gradient only
   int64_t dy_step, dy_env, dy_head;
   void *dq, *dk, *dv;

@@ -145,6 +145,12 @@ CASES = [
     (21, 2, 2, 128, 2, 1, F32, 0.3, False, True),
     (100, 3, 2, 24, 48, 1, BF16, 0.05, True, True),
     (200, 2, 1, 64, 64, 1, F32, 0.01, True, True),
+    # few heads and many steps, which are cut into pieces
+    (256, 1, 1, 64, 64, 1, F32, 0.0, True, True),
+    (700, 1, 2, 40, 24, 2, F32, 0.005, True, True),
+    (555, 2, 1, 128, 100, 1, BF16, 0.01, True, False),
+    (430, 1, 3, 32, 48, 1, F16, 0.0, True, True),
+    (321, 1, 1, 100, 128, 1, F32, 0.02, False, True),
 ]
 
 
@@ -295,6 +301,38 @@ def test_a_value_that_is_not_finite_reaches_later_steps_alone():
     want = torch.autograd.grad(delta_rule(*clean, state=s["state"])[0], clean, dy)
     for a, b, name in zip(got, want, NAMES):
         assert float((a[:at] - b[:at]).abs().max()) <= 4 * _roundings(30, 24) * 2.0**-23 * float(b.abs().max()), name
+
+
+def test_pieces_and_what_is_not_finite():
+    """Few heads and many steps: what a value that is not finite reaches, and what an episode's start keeps from it."""
+    from gbxcule_amd.rl import delta_rule
+
+    steps, keys = 520, 32
+    s = _inputs(60, steps, 2, 1, keys, 24)
+    s["resets"] = torch.zeros(steps, 2, dtype=torch.bool, device="cuda")
+    s["resets"][300, 1] = True
+    rows = [s[k] for k in NAMES]
+    y, last = delta_rule(*rows, state=s["state"], resets=s["resets"])
+    near = _roundings(steps, keys) * 2.0**-23 * float(y.abs().max())
+    for which, at, bad in ((0, 200, math.nan), (1, 7, math.inf), (2, 290, math.nan), (3, 130, math.nan), (4, 299, math.inf), (2, 500, math.inf)):
+        dirty = [r.clone() for r in rows]
+        dirty[which][at, 1].view(-1)[0] = bad
+        y2, last2 = delta_rule(*dirty, state=s["state"], resets=s["resets"])
+        assert torch.equal(y2[:, 0], y[:, 0]) and torch.equal(last2[0], last[0])  # the other env
+        assert float((y2[:at, 1] - y[:at, 1]).abs().max()) <= near
+        assert not torch.isfinite(y2[at : at + 1, 1]).all()
+        if at < 300:  # the episode after it
+            assert float((y2[300:, 1] - y[300:, 1]).abs().max()) <= near
+            assert float((last2[1] - last[1]).abs().max()) <= _roundings(steps, keys) * 2.0**-23 * float(last.abs().max())
+    state = s["state"].clone()
+    state[1, 0, 3, 5] = math.nan  # one column, until the episode ends
+    y2, last2 = delta_rule(*rows, state=state, resets=s["resets"])
+    assert torch.isnan(y2[:300, 1, 0, 5]).all() and torch.isfinite(y2[:, 1, 0, 6:]).all() and torch.isfinite(last2).all()
+    assert float((y2[300:] - y[300:]).abs().max()) <= near
+    # nothing grows from a state of zero, however open the gates: without steps that write there is nothing
+    rows[3], rows[4] = torch.full_like(rows[3], 2.0), torch.zeros_like(rows[4])
+    y2, last2 = delta_rule(*rows)
+    assert not y2.any() and not last2.any()
 
 
 def test_gradient_against_differences():
