@@ -2,13 +2,14 @@
 with the actor and the learner around ``collect_rollout``.
 
 ``python -m gbxcule_amd.rl.memory`` plays the synthetic PPU cart and learns
-from a few rollouts.
+from a few rollouts (``... memory delta``: with the other kind of memory).
 
-The policy reads packed frames, carries a selective state space through the
-steps of an episode and returns action logits and a value.  The actor holds one
-state per env and makes one step of all envs at a time, with the projection at
-each block's entry in 8 bits on request; the learner reads the same rollout as
-``[T, N]`` with the episode starts, from the state the rollout began with.
+The policy reads packed frames, carries a selective state space, or a matrix for
+each head that it corrects by the gated delta rule, through the steps of an
+episode and returns action logits and a value.  The actor holds one state per env
+and makes one step of all envs at a time, with the projection at each scan
+block's entry in 8 bits on request; the learner reads the same rollout as ``[T,
+N]`` with the episode starts, from the state the rollout began with.
 """
 
 from __future__ import annotations
@@ -21,7 +22,18 @@ from torch import nn
 from torch.nn import functional as F
 
 from ..abi import DOWNSAMPLE_H, DOWNSAMPLE_W
-from .ops import causal_conv, causal_conv_step, rms_norm, rms_norm_fp8, selective_scan, selective_scan_step
+from .ops import (
+    causal_conv,
+    causal_conv_step,
+    delta_rule,
+    delta_rule_step,
+    layer_norm,
+    rms_norm,
+    rms_norm_fp8,
+    sample_actions,
+    selective_scan,
+    selective_scan_step,
+)
 from .packed import unpack_2bpp_u8
 
 E4M3_MAX = 448.0
@@ -29,7 +41,8 @@ E4M3_MAX = 448.0
 
 class BlockState(NamedTuple):
     """What a block carries: the convolution's last inputs ``[N, 3, inner]`` and
-    the scan's state ``[N, inner, states]``."""
+    the scan's state ``[N, inner, states]``, or the delta rule's ``[N, heads, keys,
+    values]``."""
 
     window: torch.Tensor
     scan: torch.Tensor
@@ -102,15 +115,80 @@ class MemoryBlock(nn.Module):
         return (w / scale[:, None]).to(torch.float8_e4m3fn), scale.unsqueeze(0)
 
 
-class MemoryPolicy(nn.Module):
-    """Packed frames ``[..., 1, 72, 20]`` -> action logits and values."""
+class DeltaBlock(nn.Module):
+    """layer norm -> projection -> causal convolution -> gated delta rule -> norm
+    of each head, gated -> projection.  ``share`` heads of values have a head of
+    queries and keys together."""
 
-    def __init__(self, num_actions: int, *, dim: int = 256, blocks: int = 2, states: int = 16, dtype=torch.bfloat16) -> None:
+    def __init__(self, dim: int, heads: int = 4, keys: int = 64, values: int = 64, share: int = 1, width: int = 4, dtype=torch.bfloat16) -> None:
         super().__init__()
+        if heads % share:
+            raise ValueError(f"heads ({heads}) must be a multiple of share ({share})")
+        self.heads, self.keys, self.values, self.shared, self.width = heads, keys, values, heads // share, width
+        self.inner = 2 * self.shared * keys + heads * values  # q, k and v
+        self.norm = nn.Parameter(torch.ones(dim))
+        self.norm_bias = nn.Parameter(torch.zeros(dim))
+        self.entry = nn.Parameter(torch.randn(self.inner + heads * values + 2 * heads, dim, dtype=dtype) * dim**-0.5)
+        self.conv = nn.Parameter(torch.randn(self.inner, width) * width**-0.5)
+        self.log_rate = nn.Parameter(torch.log(1.0 + 15.0 * torch.rand(heads)))
+        size = torch.exp(torch.rand(heads) * math.log(100.0) + math.log(1e-3))  # steps of 0.001 to 0.1
+        self.dt_bias = nn.Parameter(size + torch.log(-torch.expm1(-size)))
+        self.head_norm = nn.Parameter(torch.ones(values))
+        self.exit = nn.Parameter(torch.randn(dim, heads * values, dtype=dtype) * (heads * values) ** -0.5)
+
+    def initial_state(self, envs: int) -> BlockState:
+        return BlockState(self.entry.new_zeros(envs, self.width - 1, self.inner),
+                          self.norm.new_zeros(envs, self.heads, self.keys, self.values))  # fmt: skip
+
+    def _enter(self, hidden, stream):
+        """What the convolution reads, the gate, the decays and the step sizes of
+        the corrections (both in 32 bits), and the stream."""
+        out = layer_norm(hidden, self.norm, self.norm_bias, stream)
+        y, stream = (out, hidden) if stream is None else out
+        x, z, dt, beta = F.linear(y, self.entry).split([self.inner, self.heads * self.values, self.heads, self.heads], dim=-1)
+        g = -torch.exp(self.log_rate) * F.softplus(dt.float() + self.dt_bias)
+        return x, z, g, torch.sigmoid(beta.float()), stream
+
+    def _heads(self, x):
+        q, k, v = x.split([self.shared * self.keys, self.shared * self.keys, self.heads * self.values], dim=-1)
+        return q.unflatten(-1, (self.shared, self.keys)), k.unflatten(-1, (self.shared, self.keys)), v.unflatten(-1, (self.heads, self.values))
+
+    def _leave(self, y, z):
+        return F.linear((rms_norm(y, self.head_norm).flatten(-2) * F.silu(z)), self.exit)
+
+    def forward(self, hidden, stream, state: BlockState, resets):
+        """A rollout: ``[T, N, dim]`` and ``resets`` ``[T, N]``; the state stays
+        as it is.  Returns ``(hidden, stream)``."""
+        x, z, g, beta, stream = self._enter(hidden, stream)
+        x, _ = causal_conv(x, self.conv, state=state.window, resets=resets)
+        y, _ = delta_rule(*self._heads(x), g, beta, state=state.scan, resets=resets)
+        return self._leave(y, z), stream
+
+    def step(self, hidden, stream, state: BlockState, resets, entry_fp8=None):
+        """One step of all envs, ``[N, dim]``; the state moves on in place."""
+        if entry_fp8 is not None:
+            raise ValueError("a DeltaBlock has no projection in 8 bits")
+        x, z, g, beta, stream = self._enter(hidden, stream)
+        x = causal_conv_step(x, self.conv, None, state.window, resets=resets)
+        return self._leave(delta_rule_step(*self._heads(x), g, beta, state=state.scan, resets=resets), z), stream
+
+
+class MemoryPolicy(nn.Module):
+    """Packed frames ``[..., 1, 72, 20]`` -> action logits and values.
+    ``memory``: ``"scan"`` or ``"delta"``, the kind of its blocks."""
+
+    def __init__(self, num_actions: int, *, dim: int = 256, blocks: int = 2, states: int = 16, dtype=torch.bfloat16, memory: str = "scan") -> None:
+        super().__init__()
+        if memory not in ("scan", "delta"):
+            raise ValueError(f"memory must be 'scan' or 'delta', got {memory!r}")
         pixels = DOWNSAMPLE_H * DOWNSAMPLE_W
         self.dtype = dtype
         self.eye = nn.Parameter(torch.randn(dim, pixels, dtype=dtype) * pixels**-0.5)
-        self.blocks = nn.ModuleList(MemoryBlock(dim, states, dtype=dtype) for _ in range(blocks))
+        self.memory = memory
+        if memory == "scan":
+            self.blocks = nn.ModuleList(MemoryBlock(dim, states, dtype=dtype) for _ in range(blocks))
+        else:
+            self.blocks = nn.ModuleList(DeltaBlock(dim, heads=max(1, dim // 64), dtype=dtype) for _ in range(blocks))
         self.norm = nn.Parameter(torch.ones(dim))
         self.heads = nn.Parameter(torch.zeros(num_actions + 1, dim, dtype=dtype))
 
@@ -144,10 +222,16 @@ class MemoryPolicy(nn.Module):
 
 class MemoryActor:
     """The ``policy`` argument of ``collect_rollout``: keeps the envs' states and
-    takes the episode starts from the rollout's rows of the step before."""
+    takes the episode starts from the rollout's rows of the step before.
 
-    def __init__(self, policy: MemoryPolicy, num_envs: int, rollout, *, fp8: bool = False) -> None:
-        self.policy, self.rollout, self.fp8 = policy, rollout, fp8
+    ``sampling``: options of ``sample_actions`` (numbers, or tensors with one for
+    each env, such as a ladder of temperatures); the log-probabilities are then those
+    that the actions were drawn with.  None: from the policy's own distribution."""
+
+    def __init__(self, policy: MemoryPolicy, num_envs: int, rollout, *, fp8: bool = False, sampling: dict | None = None) -> None:
+        if fp8 and policy.memory != "scan":
+            raise ValueError("fp8 needs a policy with memory='scan'")
+        self.policy, self.rollout, self.fp8, self.sampling = policy, rollout, fp8, sampling
         self.state = policy.initial_state(num_envs)
         self.begin_rollout(torch.ones(num_envs, dtype=torch.bool, device=policy.eye.device))
 
@@ -163,6 +247,9 @@ class MemoryActor:
         t = self.rollout.step
         resets = self.starts if t == 0 else self.rollout.dones[t - 1]
         logits, values = self.policy.step(frames, self.state, resets, self.entries)
+        if self.sampling is not None:
+            actions, logp = sample_actions(logits, torch.rand_like(values), **self.sampling)
+            return actions, values, logp
         logp = torch.log_softmax(logits, -1)
         noise = -torch.log(-torch.log(torch.rand_like(logp).clamp_min(1e-20)).clamp_min(1e-20))
         actions = (logp + noise).argmax(-1)
@@ -213,7 +300,7 @@ def learn(actor: MemoryActor, optimizer, last_frames, *, passes: int = 2, clip: 
     return losses
 
 
-def main(num_envs: int = 1024, steps: int = 32, rollouts: int = 4) -> None:
+def main(num_envs: int = 1024, steps: int = 32, rollouts: int = 4, memory: str = "scan") -> None:
     import time
 
     from ..carts.synth import cart_c3
@@ -228,9 +315,9 @@ def main(num_envs: int = 1024, steps: int = 32, rollouts: int = 4) -> None:
     env = PackedPixelEnv(cart_c3(2), num_envs=num_envs, reward_fn=reward)
     env.reset(seed=0)
     rollout = RolloutBuffer(steps=steps, num_envs=num_envs, stack_k=1, obs_format="packed2", obs_steps=steps + 1)
-    policy = MemoryPolicy(env.num_actions).cuda()
+    policy = MemoryPolicy(env.num_actions, memory=memory).cuda()
     optimizer = AdamW(policy.parameters(), lr=1e-3, state_bits=8)
-    actor = MemoryActor(policy, num_envs, rollout, fp8=True)
+    actor = MemoryActor(policy, num_envs, rollout, fp8=True) if memory == "scan" else MemoryActor(policy, num_envs, rollout, sampling={})
     for k in range(rollouts):
         if k:
             actor.begin_rollout()
@@ -246,4 +333,6 @@ def main(num_envs: int = 1024, steps: int = 32, rollouts: int = 4) -> None:
 
 
 if __name__ == "__main__":
-    main()
+    import sys
+
+    main(memory=sys.argv[1] if len(sys.argv) > 1 else "scan")
