@@ -142,27 +142,44 @@ __device__ __forceinline__ void mask(Words<T, COUNT>& r, bool has) {
 #pragma unroll
   for (int i = 0; i < r.kWords; ++i) r.w[i] = has ? r.w[i] : 0u;
 }
-// COUNT elements, zero from `valid` on.  (Zeros and loads meet in whole words:
-// where they met in 16-bit elements, each took a register.)
+// COUNT elements, zero from `valid` on, in pieces of up to 8.  A piece that ends
+// inside is loaded element by element, its last one again and again: without
+// conditions of their own the loads go out together.  (Zeros and loads meet in whole
+// words: where they met in 16-bit elements, each took a register.)
 template <int COUNT, typename T>
 __device__ __forceinline__ Words<T, COUNT> load_words(const T* p, int valid) {
+  constexpr int kPiece = COUNT < 8 ? COUNT : 8, kWords = Words<T, kPiece>::kWords;
+  static_assert(COUNT % kPiece == 0, "whole pieces");
   Words<T, COUNT> r{};
   valid = opaque(valid);
-  if (valid >= COUNT) {
-    __builtin_memcpy(r.w, p, COUNT * sizeof(T));
-  } else {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        if (i < valid) __builtin_memcpy(&r.w[i], p + i, 4);
-      } else {
-        uint16_t h = 0;
-        if (i < valid) __builtin_memcpy(&h, p + i, 2);
-        r.w[i / 2] |= (uint32_t)h << (16 * (i & 1));
+  for (int n = 0; n < COUNT; n += kPiece) {
+    uint32_t* to = r.w + n / kPiece * kWords;
+    const int rest = valid - n;
+    if (rest >= kPiece) {
+      __builtin_memcpy(to, p + n, kPiece * sizeof(T));
+    } else if (rest > 0) {
+      T x[kPiece];
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) x[i] = p[n + (i < rest ? i : rest - 1)];
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        if constexpr (sizeof(T) == 4) to[i] = i < rest ? __builtin_bit_cast(uint32_t, x[i]) : 0u;
+        else to[i / 2] |= i < rest ? (uint32_t)__builtin_bit_cast(uint16_t, x[i]) << (16 * (i & 1)) : 0u;
       }
     }
   }
   return r;
+}
+// the same as floats
+template <int COUNT, typename T>
+__device__ __forceinline__ void load_floats(const T* p, int valid, float (&v)[COUNT]) {
+  const Words<T, COUNT> x = load_words<COUNT>(p, valid);
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(x.w[i]);
+    else v[i] = (float)__builtin_bit_cast(T, (uint16_t)(x.w[i / 2] >> (16 * (i & 1))));
+  }
 }
 // elements I and J of 16 bits as one word
 template <int I, int J>

@@ -311,12 +311,12 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs a, int slabs,
   const float gate = a.gate[env * a.gate_env + head], beta = a.beta[env * a.beta_env + head];
   const bool cut = (a.resets && a.resets[env]) || gate < kClosed;
   float k[R], q[R], v[4], S[R][4];
-  load_row<R>((const T*)a.k + env * a.k_env + head / a.share * a.k_head + row, a.keys - row, k);
-  load_row<R>((const T*)a.q + env * a.q_env + head / a.share * a.q_head + row, a.keys - row, q);
-  load_row<4>((const T*)a.v + env * a.v_env + head * a.v_head + col, wide, v);
+  load_floats<R>((const T*)a.k + env * a.k_env + head / a.share * a.k_head + row, a.keys - row, k);
+  load_floats<R>((const T*)a.q + env * a.q_env + head / a.share * a.q_head + row, a.keys - row, q);
+  load_floats<4>((const T*)a.v + env * a.v_env + head * a.v_head + col, wide, v);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    load_row<4>(state + (int64_t)i * a.values, row + i < a.keys && !cut ? wide : 0, S[i]);
+    load_floats<4>(state + (int64_t)i * a.values, row + i < a.keys && !cut ? wide : 0, S[i]);
   }
   float p[4] = {}, w[4] = {}, kk = 0.0f, qq = 0.0f, qk = 0.0f;
 #pragma unroll

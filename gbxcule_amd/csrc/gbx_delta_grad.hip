@@ -453,7 +453,7 @@ __device__ __forceinline__ void join(const Grad<T, NT, VT, FULL>& w, int64_t uni
     const int64_t row = (t0 + t) * heads + unit;
     auto turn = [&](const T* p, int64_t step, int kind, void* to) {
       float x[NT], dx[NT] = {}, ss = 0.0f, dot = 0.0f;
-      load_row<NT>(p + t * step + NT * c, live ? rest : 0, x);
+      load_floats<NT>(p + t * step + NT * c, live ? rest : 0, x);
       for (int n = 0; n < slabs; ++n)
 #pragma unroll
         for (int r = 0; r < NT; ++r) dx[r] += lds[n * kPart + ((kind * NT + r) * 4 + j) * 64 + (i & 63)];
