@@ -115,6 +115,36 @@ __device__ __forceinline__ f4 mma(const Parts<A>& a, const Parts<B>& b, f4 d) {
   }
 }
 
+// Two tiles that follow each other in the sum: an instruction takes a term of both,
+// with no place left empty.
+struct WholeTwo {
+  f4 v[2];
+};
+template <int N>
+struct PartsTwo {
+  w4 p[N];
+};
+__device__ __forceinline__ WholeTwo two(Whole a, Whole b) { return {{a.v, b.v}}; }
+template <int N>
+__device__ __forceinline__ PartsTwo<N> two(const Parts<N>& a, const Parts<N>& b) {
+  PartsTwo<N> r;
+#pragma unroll
+  for (int n = 0; n < N; ++n) r.p[n] = w4{a.p[n][0], a.p[n][1], b.p[n][0], b.p[n][1]};
+  return r;
+}
+__device__ __forceinline__ f4 mma(const WholeTwo& a, const WholeTwo& b, f4 d) { return mma(a.v[0], b.v[0], mma(a.v[1], b.v[1], d)); }
+template <int A, int B>
+__device__ __forceinline__ f4 mma(const PartsTwo<A>& a, const PartsTwo<B>& b, f4 d) {
+#pragma unroll
+  for (int n = (A > B ? A : B) - 1; n >= 0; --n)  // the small terms first
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j)
+        if (i + j == n) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a.p[i]), __builtin_bit_cast(b8, b.p[j]), d, 0, 0, 0);
+  return d;
+}
+
 // Inputs in words as they lie in memory.
 template <typename T, int COUNT>
 struct Words {
@@ -236,10 +266,18 @@ struct Factor<float> {
   static __device__ __forceinline__ Fine fine(f4 x) { return {x}; }
   static __device__ __forceinline__ Big big(f4 x) { return {x}; }
 };
+// The tiles of a sum over a wavefront's VT tiles of columns.
+template <int VT, typename R>
+__device__ __forceinline__ auto columns(const R (&x)[VT]) {
+  if constexpr (VT == 2) return two(x[0], x[1]);
+  else return x[0];
+}
 template <typename T>
 using Raw = typename Factor<T>::Raw;
 template <typename T>
 using Fine = typename Factor<T>::Fine;
+template <typename T>
+using Big = typename Factor<T>::Big;
 
 struct Lane {
   int c, g;  // place among 16 lanes (a row or column), group of 16 (four places of the other index)
@@ -351,11 +389,15 @@ struct Steps {
 
 // Inner products of the rows with each other: row c, places in(j), or the other way round.
 template <int NT, typename R>
-__device__ __forceinline__ f4 square_of(const R (&row)[NT]) {
+__device__ __forceinline__ f4 product_of(const R (&row)[NT], const R (&col)[NT]) {
   f4 x = zero4();
 #pragma unroll
-  for (int r = 0; r < NT; ++r) x = mma(row[r], row[r], x);
+  for (int r = 0; r < NT; r += 2) x = mma(two(row[r], row[r + 1]), two(col[r], col[r + 1]), x);
   return x;
+}
+template <int NT, typename R>
+__device__ __forceinline__ f4 square_of(const R (&row)[NT]) {
+  return product_of(row, row);
 }
 // 1 / length of row c, from the diagonal.
 __device__ __forceinline__ float unit_of(f4 square, bool normalize, Lane l) {
@@ -553,9 +595,7 @@ __device__ __forceinline__ void solve_chunk(const DeltaArgs& a, int t0, int env,
   const f4 kk = square_of(kr);
   const float kap = unit_of(kk, a.normalize, l);
   const float qap = (a.normalize ? unit_of(square_of(qr), true, l) : 1.0f) * (GRAD ? 1.0f : a.scale);
-  f4 kq = zero4();
-#pragma unroll
-  for (int r = 0; r < NT; ++r) kq = GRAD ? mma(qr[r], kr[r], kq) : mma(kr[r], qr[r], kq);
+  const f4 kq = GRAD ? product_of(qr, kr) : product_of(kr, qr);
   const double sum = sum_up_to(gates.gate), end = row_lane<kOf + 15>(sum);
   const uint32_t upto = (2u << l.c) - 1u;  // bits of the steps up to c
   if (l.g == 0) {

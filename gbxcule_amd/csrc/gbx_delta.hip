@@ -106,10 +106,10 @@ struct Forward {
       f4 x = zero4();
       Y[t] = zero4();
 #pragma unroll
-      for (int r = 0; r < NT; ++r) {
-        const auto b = F::big(S[r][t]);
-        x = mma(kr[r], b, x);
-        if (!MAP) Y[t] = mma(qr[r], b, Y[t]);
+      for (int r = 0; r < NT; r += 2) {
+        const auto b = two(F::big(S[r][t]), F::big(S[r + 1][t]));
+        x = mma(two(kr[r], kr[r + 1]), b, x);
+        if (!MAP) Y[t] = mma(two(qr[r], qr[r + 1]), b, Y[t]);
       }
       x = F::wide(vc[t]) - in * kin * x;
       E[t] = mma(T_row, x, zero4());
@@ -160,10 +160,10 @@ struct Forward {
           Y[t] = zero4();
           const f4 vt = F::wide(vc[t]);
 #pragma unroll
-          for (int r = 0; r < NT; ++r) {
-            const auto b = F::big(S[r][t]);
-            x = mma(kr[r], b, x);
-            Y[t] = mma(qr[r], b, Y[t]);
+          for (int r = 0; r < NT; r += 2) {
+            const auto b = two(F::big(S[r][t]), F::big(S[r + 1][t]));
+            x = mma(two(kr[r], kr[r + 1]), b, x);
+            Y[t] = mma(two(qr[r], qr[r + 1]), b, Y[t]);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = s.has(l.in(j)) ? vt[j] - d.in[j] * kin[j] * x[j] : 0.0f;
@@ -175,9 +175,7 @@ struct Forward {
           continue;
         }
         if (!MAP && over) store(over, t0, s, l, E);
-        f4 kq = zero4();  // row c, places in(j): q_c . k_j
-#pragma unroll
-        for (int r = 0; r < NT; ++r) kq = mma(kr[r], qr[r], kq);
+        f4 kq = product_of(kr, qr);  // row c, places in(j): q_c . k_j
 #pragma unroll
         for (int j = 0; j < 4; ++j) kq[j] = l.in(j) <= l.c ? kq[j] * (qap * kin[j]) * d.pair[j] : 0.0f;
         const Fine<T> kqf = F::fine(kq);

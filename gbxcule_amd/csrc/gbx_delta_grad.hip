@@ -129,6 +129,12 @@ struct Grad {
     over.template cols<true>(t0, s, l, ec);
     over.template rows<true>(t0, s, l, er);
     dy.cols(t0, s, l, dyc);
+    Raw<T> dyr[VT], kc[NT], qc[NT];
+    f4 St[VT];
+    dy.rows(t0, s, l, dyr);
+    k.template cols<true>(t0, s, l, kc);
+    q.template cols<true>(t0, s, l, qc);
+    load_turned<FULL>(kept, a, u, 0, St);
     const f4 bin = of_rows(z.beta, l), kin = of_rows(z.kap, l), qin = of_rows(z.qap, l), in = of_rows(z.in, l), tail = of_rows(z.tail, l);
     const float beta = z.beta[l.c], all = z.all;
     // D goes through LDS to be read the other way round, tile (r, t) where dq's (t = 0) and dk's (t = 1) tile
@@ -141,9 +147,8 @@ struct Grad {
 #pragma unroll
         for (int j = 0; j < 4; ++j) tiles[(t * NT + r) * 256 + (l.in(j) ^ (l.g & 1)) * 16 + l.c] = D[r][t][j];
     const int turned = (l.c ^ (l.c >> 2 & 1)) * 16 + 4 * l.g;
-    f4 W[VT], bsum = zero4();
-    Fine<T> Utf[VT], Wtf[VT];  // rows c
-    float whole = 0.0f;        // <S, D> after the chunk: what it wrote, then what it kept
+    f4 W[VT], Ut[VT], Wt[VT], bsum = zero4();  // Ut and Wt: rows c
+    float whole = 0.0f;                        // <S, D> after the chunk: what it wrote, then what it kept
     {
       const f4 T_col = z.t[lane];
       const Fine<T> aq = F::fine(z.m[lane]);
@@ -152,26 +157,20 @@ struct Grad {
       for (int t = 0; t < VT; ++t) {
         f4 x = zero4();
 #pragma unroll
-        for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(D[r][t]), x);
+        for (int r = 0; r < NT; r += 2) x = mma(two(kr[r], kr[r + 1]), two(F::big(D[r][t]), F::big(D[r + 1][t])), x);
         x *= tail * kin;
         const f4 part = x * bin * ec[t].v;
         whole += (part[0] + part[1]) + (part[2] + part[3]);
         x = mma(aq, dyc[t], x);
         W[t] = mma(T_col, x, zero4());
-        Wtf[t] = F::fine(mma(x, T_col, zero4()));
-        Utf[t] = F::fine(er[t].v * beta);
+        Wt[t] = mma(x, T_col, zero4());
+        Ut[t] = er[t].v * beta;
         bsum += W[t] * ec[t].v;
         fine = fine && finite4(W[t]) && finite4(ec[t].v);
       }
       if (!__all(fine)) return false;
     }
-    Raw<T> dyr[VT], kc[NT], qc[NT];
-    f4 St[VT];
-    dy.rows(t0, s, l, dyr);
-    k.template cols<true>(t0, s, l, kc);
-    q.template cols<true>(t0, s, l, qc);
     {  // dv, and what D takes up
-      Fine<T> asks[VT], gives[VT];
       const f4 ask = a.scale * qin * in, give = -in * kin;
       float out[4][VT];
 #pragma unroll
@@ -179,31 +178,24 @@ struct Grad {
         const f4 v = bin * W[t];
 #pragma unroll
         for (int j = 0; j < 4; ++j) out[j][t] = v[j];
-        asks[t] = F::fine(ask * F::wide(dyc[t]));
-        gives[t] = F::fine(give * v);
+        const auto takes = two(F::fine(ask * F::wide(dyc[t])), F::fine(give * v));
+#pragma unroll
+        for (int r = 0; r < NT; ++r) D[r][t] = mma(two(qc[r], kc[r]), takes, D[r][t] * all);
       }
       const int64_t v_step = (int64_t)a.envs * a.heads * a.values;
 #pragma unroll
       for (int j = 0; j < 4; ++j) store_row<VT>((dv + j * v_step) + dv_lane, opaque(s.has(l.in(j)) ? FULL ? VT : a.values - u.col() : 0), out[j]);
-#pragma unroll
-      for (int r = 0; r < NT; ++r)
-#pragma unroll
-        for (int t = 0; t < VT; ++t) D[r][t] = mma(kc[r], gives[t], mma(qc[r], asks[t], D[r][t] * all));
     }
-    load_turned<FULL>(kept, a, u, 0, St);
 #pragma unroll
     for (int j = 0; j < 4; ++j) dbeta[j] = row_sum(bsum[j]);
-    Fine<T> pf, ptf, mf, mtf;
+    Fine<T> Utf[VT], Wtf[VT], pf, mf, ptf, mtf;
+#pragma unroll
+    for (int t = 0; t < VT; ++t) Utf[t] = F::fine(Ut[t]), Wtf[t] = F::fine(Wt[t]);
+    const auto Us = columns<VT>(Utf), Ws = columns<VT>(Wtf);
+    const auto dys = columns<VT>(dyr);
     {
       const f4 pair = z.pair[lane];
-      f4 p = zero4(), pt = zero4(), m = zero4(), mt = zero4();
-#pragma unroll
-      for (int t = 0; t < VT; ++t) {
-        p = mma(Utf[t], dyr[t], p);
-        pt = mma(dyr[t], Utf[t], pt);
-        m = mma(Utf[t], Wtf[t], m);
-        mt = mma(Wtf[t], Utf[t], mt);
-      }
+      f4 p = mma(Us, dys, zero4()), pt = mma(dys, Us, zero4()), m = mma(Us, Ws, zero4()), mt = mma(Ws, Us, zero4());
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         p[j] = l.in(j) <= l.c ? p[j] * (a.scale * kin[j]) * pair[j] : 0.0f;
@@ -213,28 +205,27 @@ struct Grad {
       }
       pf = F::fine(p), ptf = F::fine(pt), mf = F::fine(m), mtf = F::fine(mt);
     }
+    const auto writers = two(ptf, mtf);
     const f4 qs = a.scale * in, rs = -in * bin;
     f4 e = zero4();  // q . dq + k . dk_reads - k . dk_writes
     float held = 0.0f;
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
-      f4 x = zero4(), reads = zero4(), writes = zero4(), next[VT];
+      f4 next[VT];
       if (r + 1 < NT) load_turned<FULL>(kept, a, u, r + 1, next);
+      Big<T> sf[VT], df[VT];
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
-        const auto sf = F::big(St[t]);
         const f4 Dr = *reinterpret_cast<const f4*>(tiles + (t * NT + r) * 256 + turned);
-        x = mma(dyr[t], sf, x);
-        reads = mma(Wtf[t], sf, reads);
-        writes = mma(Utf[t], F::big(Dr), writes);
         const f4 part = St[t] * Dr;
         held += (part[0] + part[1]) + (part[2] + part[3]);
+        sf[t] = F::big(St[t]), df[t] = F::big(Dr);
         if (r + 1 < NT) St[t] = next[t];
       }
-      x = mma(pf, kc[r], x * qs);
-      reads = mma(mf, kc[r], reads * rs);
-      writes = mma(ptf, qc[r], writes * tail);
-      writes = mma(mtf, kc[r], writes);
+      const auto Ss = columns<VT>(sf), Ds = columns<VT>(df);
+      const f4 x = mma(pf, kc[r], mma(dys, Ss, zero4()) * qs);
+      const f4 reads = mma(mf, kc[r], mma(Ws, Ss, zero4()) * rs);
+      const f4 writes = mma(writers, two(qc[r], kc[r]), mma(Us, Ds, zero4()) * tail);
       e += qin * F::wide(qc[r]) * x + kin * F::wide(kc[r]) * (reads - writes);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -440,46 +431,56 @@ struct Grad {
 };
 
 // The columns' parts of dq, dk, dgate and dbeta of a chunk, added in one order.
-// lds: [slab][dq, dk][r][j][lane], then [slab][dgate, dbeta][step].
+// lds: [slab][dq, dk][r][j][lane], then [slab][dgate, dbeta][step].  A thread's rows
+// are loaded before the others' parts are waited for.
 template <typename T, int NT, int VT, bool FULL>
-__device__ __forceinline__ void join(const Grad<T, NT, VT, FULL>& w, int64_t unit, const float* lds, int slabs) {
-  constexpr int kPart = 2 * NT * 256;
-  const DeltaArgs& a = w.a;
-  const int t0 = w.t0, steps = a.steps - t0;  // (more than a chunk's do no harm)
-  const int64_t heads = (int64_t)a.envs * a.heads;
-  for (int i = opaque(threadIdx.x); i < 256; i += blockDim.x) {
-    const int j = i >> 6, c = i & 15, t = 4 * (i >> 4 & 3) + j, rest = opaque(a.keys - NT * c);
-    const bool live = t < steps;
-    const int64_t row = (t0 + t) * heads + unit;
-    auto turn = [&](const T* p, int64_t step, int kind, void* to) {
-      float x[NT], dx[NT] = {}, ss = 0.0f, dot = 0.0f;
-      load_floats<NT>(p + t * step + NT * c, live ? rest : 0, x);
-      for (int n = 0; n < slabs; ++n)
+struct Join {
+  static constexpr int kPart = 2 * NT * 256;
+  float q[NT], k[NT];  // of the thread's first turn
+  __device__ __forceinline__ void load(const Grad<T, NT, VT, FULL>& w, int i, float (&q)[NT], float (&k)[NT]) const {
+    const int c = i & 15, t = w.t0 + 4 * (i >> 4 & 3) + (i >> 6), rest = t < w.a.steps ? w.a.keys - NT * c : 0;
+    load_floats<NT>(w.q.p + t * w.a.q_step + NT * c, rest, q);
+    load_floats<NT>(w.k.p + t * w.a.k_step + NT * c, rest, k);
+  }
+  __device__ __forceinline__ void begin(const Grad<T, NT, VT, FULL>& w) { load(w, opaque(threadIdx.x), q, k); }
+  __device__ __forceinline__ void end(const Grad<T, NT, VT, FULL>& w, int64_t unit, const float* lds, int slabs) {
+    const DeltaArgs& a = w.a;
+    const int t0 = w.t0, steps = a.steps - t0, first = opaque(threadIdx.x);  // (more steps than a chunk's do no harm)
+    const int64_t heads = (int64_t)a.envs * a.heads;
+    for (int i = first; i < 256; i += blockDim.x) {
+      const int j = i >> 6, c = i & 15, t = 4 * (i >> 4 & 3) + j, rest = opaque(a.keys - NT * c);
+      const bool live = t < steps;
+      const int64_t row = (t0 + t) * heads + unit;
+      if (i != first) load(w, i, q, k);
+      auto turn = [&](const float (&x)[NT], int kind, void* to) {
+        float dx[NT] = {}, ss = 0.0f, dot = 0.0f;
+        for (int n = 0; n < slabs; ++n)
 #pragma unroll
-        for (int r = 0; r < NT; ++r) dx[r] += lds[n * kPart + ((kind * NT + r) * 4 + j) * 64 + (i & 63)];
-      if (a.normalize) {  // x / length: the gradient's part along x goes
+          for (int r = 0; r < NT; ++r) dx[r] += lds[n * kPart + ((kind * NT + r) * 4 + j) * 64 + (i & 63)];
+        if (a.normalize) {  // x / length: the gradient's part along x goes
 #pragma unroll
-        for (int r = 0; r < NT; ++r) {
-          ss = fmaf(x[r], x[r], ss);
-          dot = fmaf(x[r], dx[r], dot);
+          for (int r = 0; r < NT; ++r) {
+            ss = fmaf(x[r], x[r], ss);
+            dot = fmaf(x[r], dx[r], dot);
+          }
+          const float unit_x = rsqrtf(row_sum(ss) + kUnitEps);
+          dot = row_sum(dot) * (unit_x * unit_x);
+#pragma unroll
+          for (int r = 0; r < NT; ++r) dx[r] = unit_x * fmaf(-x[r], dot, dx[r]);
         }
-        const float unit_x = rsqrtf(row_sum(ss) + kUnitEps);
-        dot = row_sum(dot) * (unit_x * unit_x);
-#pragma unroll
-        for (int r = 0; r < NT; ++r) dx[r] = unit_x * fmaf(-x[r], dot, dx[r]);
+        if (a.share == 1) store_row<NT>((T*)to + row * a.keys + NT * c, live ? rest : 0, dx);
+        else store_row<NT>((float*)to + row * a.keys + NT * c, live ? rest : 0, dx);
+      };
+      turn(q, 0, a.share == 1 ? a.dq : a.work);
+      turn(k, 1, a.share == 1 ? a.dk : a.work + a.steps * heads * a.keys);
+      if (i < 2 * kDeltaChunk && (i & 15) < steps) {
+        float x = 0.0f;
+        for (int n = 0; n < slabs; ++n) x += lds[slabs * kPart + n * 2 * kDeltaChunk + i];
+        (i < kDeltaChunk ? a.dgate : a.dbeta)[(t0 + (i & 15)) * heads + unit] = x;
       }
-      if (a.share == 1) store_row<NT>((T*)to + row * a.keys + NT * c, live ? rest : 0, dx);
-      else store_row<NT>((float*)to + row * a.keys + NT * c, live ? rest : 0, dx);
-    };
-    turn(w.q.p + t0 * a.q_step, a.q_step, 0, a.share == 1 ? a.dq : a.work);
-    turn(w.k.p + t0 * a.k_step, a.k_step, 1, a.share == 1 ? a.dk : a.work + a.steps * heads * a.keys);
-    if (i < 2 * kDeltaChunk && (i & 15) < steps) {
-      float x = 0.0f;
-      for (int n = 0; n < slabs; ++n) x += lds[slabs * kPart + n * 2 * kDeltaChunk + i];
-      (i < kDeltaChunk ? a.dgate : a.dbeta)[(t0 + (i & 15)) * heads + unit] = x;
     }
   }
-}
+};
 
 // A workgroup is a head of an env, a wavefront some columns of its state.
 template <typename T, int NT, int VT, bool FULL>
@@ -535,9 +536,11 @@ __global__ __launch_bounds__(512 / VT, 2) void delta_grad_kernel(DeltaArgs a) {
       float dgate;
       if (w.chunk(solved[n], kept + (first + n) * state, over, dgate, dbeta)) hand_in(dgate, dbeta);
       else bad = 1;
+      Join<T, NT, VT, FULL> join;
+      join.begin(w);
       __syncthreads();
       fine = !bad;  // nobody sets it again before the next barrier
-      if (fine) join(w, unit, lds, slabs);
+      if (fine) join.end(w, unit, lds, slabs);
       __syncthreads();
     }
   }
@@ -563,8 +566,10 @@ __global__ __launch_bounds__(512 / VT, 2) void delta_grad_kernel(DeltaArgs a) {
       hi = s.lo;
     }
     hand_in(dgate, dbeta);
+    Join<T, NT, VT, FULL> join;
+    join.begin(w);
     __syncthreads();
-    join(w, unit, lds, slabs);
+    join.end(w, unit, lds, slabs);
     __syncthreads();
   }
 }
