@@ -60,39 +60,48 @@ __device__ __forceinline__ void write_none(const SampleArgs& a, int64_t row) {
   a.logp[row] = __builtin_nanf("");
 }
 
-// Up to 64 actions: L lanes hold a row, one action each, and compare each with each.
-template <typename T, int L>
-__global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
+// What lane n of the next L lanes holds (n counts from lane i where rows share a
+// wavefront; with a row a wavefront it is the same lane for all, read as a scalar).
+template <int L>
+__device__ __forceinline__ int turn_of(int i, int n) { return L == 64 ? n : (i + n) % L; }
+template <int L>
+__device__ __forceinline__ int held_by(int v, int j) {
+  if constexpr (L == 64) return __builtin_amdgcn_readlane(v, j);
+  else return __shfl(v, j, L);
+}
+template <int L>
+__device__ __forceinline__ float held_by(float v, int j) { return __int_as_float(held_by<L>(__float_as_int(v), j)); }
+template <int L>
+__device__ __forceinline__ double held_by(double v, int j) {
+  return __hiloint2double(held_by<L>(__double2hiint(v), j), held_by<L>(__double2loint(v), j));
+}
+
+// Draws from up to 64 logits in the order of their indexes: L lanes hold one each
+// (-infinity where there are fewer) and compare each with each.  `full`: the weight
+// of the whole row; negative: that of these.
+template <int L>
+__device__ __forceinline__ void draw_few(const SampleArgs& a, int64_t row, const Cuts& c, float x, float most, int index, double full) {
   const int i = threadIdx.x % L, base = (threadIdx.x & 63) / L * L;
-  const int64_t row = block_id() * (256 / L) + threadIdx.x / L;
-  if (row >= a.rows) return;
-  const float x = i < a.actions ? logit(((const T*)a.logits)[row * a.stride + i]) : -INFINITY;
-  float most = x;
-#pragma unroll
-  for (int m = 1; m < L; m <<= 1) most = fmaxf(most, __shfl_xor(most, m, L));
-  if (most == -INFINITY) {
-    if (i == 0) write_none(a, row);
-    return;
-  }
-  const Cuts c = cuts_of(a, row);
   double w = weight_of(x, most, c.heat);
   if (c.k || c.p < 1.0) {
     int rank = 0;
-    for (int n = 1; n < L; ++n) {
-      const int j = (i + n) % L;
-      const float o = __shfl(x, j, L);
+#pragma unroll 8
+    for (int n = 0; n < L; ++n) {
+      const int j = turn_of<L>(i, n);
+      const float o = held_by<L>(x, j);
       rank += o > x || (o == x && j < i);
     }
     if (c.k && rank >= c.k) w = 0.0;
     if (c.p < 1.0) {
-      double before = 0.0, all = w;
-      for (int n = 1; n < L; ++n) {
-        const int j = (i + n) % L;
-        const double o = __shfl(w, j, L);
+      double before = 0.0, all = 0.0;
+#pragma unroll 8
+      for (int n = 0; n < L; ++n) {
+        const int j = turn_of<L>(i, n);
+        const double o = held_by<L>(w, j);
         all += o;
-        before += __shfl(rank, j, L) < rank ? o : 0.0;
+        before += held_by<L>(rank, j) < rank ? o : 0.0;
       }
-      if (rank > 0 && !(before < c.p * all)) w = 0.0;
+      if (rank > 0 && !(before < c.p * (c.k || full < 0.0 ? all : full))) w = 0.0;
     }
   }
   if (!(w >= c.least)) w = 0.0;
@@ -106,7 +115,26 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
   constexpr uint64_t kRow = L == 64 ? ~0ull : (1ull << L) - 1;
   const uint64_t kept = __ballot(w > 0.0) >> base & kRow;
   const uint64_t past = __ballot(w > 0.0 && run > (double)a.uniform[row] * all) >> base & kRow;
-  if (i == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(kept))) write(a, row, i, w / all);
+  if (i == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(kept))) write(a, row, index, w / all);
+}
+
+// Up to 64 actions: L lanes a row.  Bound by a launch at 64 x 8 (6.2 us); at
+// 131,072 x 8 with every option its own a row by the arithmetic in 64 bits (12.5 us,
+// of which reading 8 MB is 2).
+template <typename T, int L>
+__global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
+  const int i = threadIdx.x % L;
+  const int64_t row = block_id() * (256 / L) + threadIdx.x / L;
+  if (row >= a.rows) return;
+  const float x = i < a.actions ? logit(((const T*)a.logits)[row * a.stride + i]) : -INFINITY;
+  float most = x;
+#pragma unroll
+  for (int m = 1; m < L; m <<= 1) most = fmaxf(most, __shfl_xor(most, m, L));
+  if (most == -INFINITY) {
+    if (i == 0) write_none(a, row);
+    return;
+  }
+  draw_few<L>(a, row, cuts_of(a, row), x, most, i, -1.0);
 }
 
 // ---- longer rows: a workgroup each
@@ -279,38 +307,69 @@ __device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Cut
 // HELD consecutive logits a thread stay in registers (0: rows of any length, read
 // again at each turn), and with KEEP their weights.
 //
-// Where few logits can stay they are put together first, one a thread, which
-// makes the turns of the search short: those from the k-th largest of the
+// The search for a cut goes over the row once a bit, so where few logits can stay
+// they are put together first, one a thread: those from the k-th largest of the
 // threads' own largest on hold the k largest of the row; and those that weigh
 // less than (1 - p) / actions of the row are together less than what top_p leaves
-// out.
+// out.  512 x 32,768 in 16 bits, top_k 50, top_p 0.95: 20 us, where reading the
+// row once is 7; the rest are the 20 turns of a workgroup's counts, each a barrier
+// that two workgroups a compute unit cannot hide.
 template <typename T, int THREADS, int HELD, bool KEEP>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   __shared__ double lds[2 * THREADS / 64];
   __shared__ float some[THREADS];
-  __shared__ int places[THREADS], choice[2];
+  __shared__ int places[THREADS], order[THREADS], found, choice[2];
   Group<THREADS> group{lds, 0};
   const int64_t row = block_id();
   if (row >= a.rows) return;
   const T* logits = (const T*)a.logits + row * a.stride;
-  const int each = HELD ? HELD : (a.actions + THREADS - 1) / THREADS, first = threadIdx.x * each;
+  // (whole vectors of 8 a thread)
+  const int each = HELD ? HELD : ((a.actions + THREADS - 1) / THREADS + 7) & ~7, first = threadIdx.x * each;
+  auto eight = [&](int e, float (&x)[8]) {
+    load_row<8>(logits + e, a.actions - e, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = e + i < a.actions ? logit(x[i]) : -INFINITY;
+  };
   float held[HELD ? HELD : 1];
   double weights[KEEP ? HELD : 1];
+  // f(logit, index) in any order: what is not held is read in whole lines, four
+  // vectors a thread under way together
+  auto logits_of = [&](auto&& f) {
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int e = 0; e < HELD; ++e) f(held[e], first + e);
+    } else {
+      constexpr int kStep = THREADS * 8;
+      int e = threadIdx.x * 8;
+      for (; e + 3 * kStep + 8 <= a.actions; e += 4 * kStep) {
+        float x[4][8];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) load_row<8>(logits + e + n * kStep, 8, x[n]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f(logit(x[n][i]), e + n * kStep + i);
+      }
+      for (; e < a.actions; e += kStep) {
+        float x[8];
+        eight(e, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f(x[i], e + i);
+      }
+    }
+  };
   float most = -INFINITY;
   if constexpr (HELD > 0) {
 #pragma unroll
     for (int e = 0; e < HELD; e += 8) {
       float x[8];
-      load_row<8>(logits + first + e, a.actions - first - e, x);
+      eight(first + e, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        held[e + i] = first + e + i < a.actions ? logit(x[i]) : -INFINITY;
-        most = fmaxf(most, held[e + i]);
-      }
+      for (int i = 0; i < 8; ++i) held[e + i] = x[i];
     }
-  } else {
-    for (int e = first; e < first + each && e < a.actions; ++e) most = fmaxf(most, logit(logits[e]));
   }
+  logits_of([&](float x, int) { most = fmaxf(most, x); });
+  if (threadIdx.x == 0) found = 0;
   const uint32_t own = key_of<T>(most);
   most = group.all(most, [](float p, float q) { return fmaxf(p, q); });
   if (most == -INFINITY) {
@@ -318,36 +377,55 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
     return;
   }
   const Cuts c = cuts_of(a, row);
-  auto logits_of = [&](auto&& f) {  // f(logit, index)
-    if constexpr (HELD > 0) {
-#pragma unroll
-      for (int e = 0; e < HELD; ++e) f(held[e], first + e);
-    } else {
-      for (int e = first; e < first + each && e < a.actions; ++e) f(logit(logits[e]), e);
-    }
-  };
-  auto over = [&](auto&& f) {  // f(logit, weight, index)
+  auto over = [&](auto&& f) {  // f(logit, weight, index), in order
     if constexpr (KEEP) {
 #pragma unroll
       for (int e = 0; e < HELD; ++e) f(held[e], weights[e], first + e);
     } else {
-      logits_of([&](float x, int index) { f(x, weight_of(x, most, c.heat), index); });
+      for (int e = first; e < first + each && e < a.actions; e += 8) {
+        float x[8];
+        eight(e, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f(x[i], weight_of(x[i], most, c.heat), e + i);
+      }
     }
   };
-  // Draws from the logits that each_of(f) hands to f, if there are no more of them than threads.
+  auto any = [&](auto&& f) {  // the same in any order
+    if constexpr (KEEP) over(f);
+    else logits_of([&](float x, int index) { f(x, weight_of(x, most, c.heat), index); });
+  };
+  // Draws from the logits that each_of(f) hands to f, if there are no more of
+  // them than threads.  They come as they come, and are ordered by their indexes.
   auto from_some = [&](double full, auto&& each_of) {
-    int mine = 0, count;
-    each_of([&](float, int) { ++mine; });
-    int at = group.before(mine, count);
-    if (count > THREADS) return false;
     each_of([&](float x, int index) {
-      some[at] = x;
-      places[at++] = index;
+      const int at = atomicAdd(&found, 1);
+      if (at < THREADS) {
+        some[at] = x;
+        places[at] = index;
+      }
     });
     __syncthreads();
+    const int count = found;
+    if (count > THREADS) return false;
     const bool live = (int)threadIdx.x < count;
-    const float x = live ? some[threadIdx.x] : -INFINITY;
-    const int index = live ? places[threadIdx.x] : a.actions;
+    float x = live ? some[threadIdx.x] : -INFINITY;
+    int index = live ? places[threadIdx.x] : a.actions;
+    if (live) {
+      int rank = 0;
+#pragma unroll 8
+      for (int n = 0; n < count; ++n) rank += places[n] < index;
+      order[rank] = threadIdx.x;
+    }
+    __syncthreads();
+    if (live) {
+      const int from = order[threadIdx.x];
+      x = some[from];
+      index = places[from];
+    }
+    if (count <= 64) {
+      if (threadIdx.x < 64) draw_few<64>(a, row, c, x, most, index, full);
+      return true;
+    }
     const double w = weight_of(x, most, c.heat);
     draw<T>(a, row, c, full, group, choice, [&](auto&& f) { f(x, w, index); });
     return true;
@@ -371,12 +449,12 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   if (!c.k && (c.p < 1.0 || c.least > 0.0)) {
     double least = c.least;
     if (c.p < 1.0) {
-      over([&](float, double w, int) { full += w; });
+      any([&](float, double w, int) { full += w; });
       full = group.sum(full);
       least = fmax(least, (1.0 - c.p) * full / a.actions * (1.0 - 1e-9));
     }
     if (from_some(full, [&](auto&& f) {
-          over([&](float x, double w, int index) {
+          any([&](float x, double w, int index) {
             if (w >= least && w > 0.0) f(x, index);
           });
         }))
@@ -391,13 +469,13 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
   by_element(a.elem, [&](auto t) {
     using T = decltype(t);
     auto few = [&](auto lanes) { hipLaunchKernelGGL((sample_few_kernel<T, lanes>), wide_grid((a.rows + 256 / lanes - 1) / (256 / lanes)), dim3(256), 0, st, a); };
-    auto many = [&](auto threads, auto held) {
-      // one top_k for all, of which every row finds few logits to draw from: their
-      // weights alone are computed, and without 128 registers for all of them two
-      // long rows share a compute unit
-      if (held == 0 || (!a.top_ks && a.top_k > 0 && a.top_k <= threads)) hipLaunchKernelGGL((sample_kernel<T, threads, held, false>), wide_grid(a.rows), dim3(threads), 0, st, a);
-      else hipLaunchKernelGGL((sample_kernel<T, threads, held, (held > 0)>), wide_grid(a.rows), dim3(threads), 0, st, a);
-    };
+    auto many = [&](auto threads, auto held) { hipLaunchKernelGGL((sample_kernel<T, threads, held, (held > 0)>), wide_grid(a.rows), dim3(threads), 0, st, a); };
+    // With one top_k for all, every row finds few logits to draw from, and only
+    // their weights are needed: a long row is then read twice in whole lines and
+    // not held (512 x 32,768 in 16 bits, top_k 50: 20 us, held 70).  Other cuts
+    // may leave the whole row to search, with a weight for each turn, and hold it
+    // (the same with top_p alone: 248 us, read again at each turn 893).
+    const bool cut = !a.top_ks && a.top_k > 0 && a.top_k <= 512;
     using std::integral_constant;
     if (a.actions <= 8) few(integral_constant<int, 8>{});
     else if (a.actions <= 16) few(integral_constant<int, 16>{});
@@ -406,7 +484,8 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
     else if (a.actions <= 512) many(integral_constant<int, 64>{}, integral_constant<int, 8>{});
     else if (a.actions <= 2048) many(integral_constant<int, 256>{}, integral_constant<int, 8>{});
     else if (a.actions <= 8192) many(integral_constant<int, 512>{}, integral_constant<int, 16>{});
-    else if (a.actions <= 32768) many(integral_constant<int, 512>{}, integral_constant<int, 64>{});
+    else if (a.actions <= 32768 && !cut) many(integral_constant<int, 512>{}, integral_constant<int, 64>{});
+    else if (a.actions <= 32768) many(integral_constant<int, 512>{}, integral_constant<int, 0>{});
     else many(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
   });
   return hipGetLastError();
