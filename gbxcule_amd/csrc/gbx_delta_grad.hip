@@ -17,8 +17,12 @@
 // and a later step: with "reads" the terms of dq and of dk before the gap above
 // and "writes" those behind it,
 //   dgate_i = <S, D> after the chunk + sum over m >= i of (q . dq + k . dk_reads - k . dk_writes)_m.
-// The inner product is computed anew at the end of every span, so its error does not
+// The inner product is computed anew at the end of every chunk, so its error does not
 // grow with the length of the rollout.
+//
+// D is needed both ways round, and registers hold one: it is turned in LDS.  S0 is
+// needed with its columns summed alone, as <S, D> is taken apart into what the chunk
+// wrote and what it kept, and is read so from what the forward pass kept.
 #include "gbx_delta.h"
 
 #include <algorithm>
@@ -105,7 +109,7 @@ struct Grad {
       f4 x = zero4();
       const f4 vt = F::wide(vc[t]);
 #pragma unroll
-      for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(m.S[r][t]), x);
+      for (int r = 0; r < NT; ++r) x = mma(kr[r], F::fine(m.S[r][t]), x);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = s.has(l.in(j)) ? kin[j] * bin[j] * fmaf(-d.in[j] * kin[j], x[j], vt[j]) : 0.0f;
       const Fine<T> xf = F::fine(x);
@@ -157,7 +161,7 @@ struct Grad {
       for (int t = 0; t < VT; ++t) {
         f4 x = zero4();
 #pragma unroll
-        for (int r = 0; r < NT; r += 2) x = mma(two(kr[r], kr[r + 1]), two(F::big(D[r][t]), F::big(D[r + 1][t])), x);
+        for (int r = 0; r < NT; r += 2) x = mma(two(kr[r], kr[r + 1]), two(F::fine(D[r][t]), F::fine(D[r + 1][t])), x);
         x *= tail * kin;
         const f4 part = x * bin * ec[t].v;
         whole += (part[0] + part[1]) + (part[2] + part[3]);
@@ -213,13 +217,13 @@ struct Grad {
     for (int r = 0; r < NT; ++r) {
       f4 next[VT];
       if (r + 1 < NT) load_turned<FULL>(kept, a, u, r + 1, next);
-      Big<T> sf[VT], df[VT];
+      Fine<T> sf[VT], df[VT];
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
         const f4 Dr = *reinterpret_cast<const f4*>(tiles + (t * NT + r) * 256 + turned);
         const f4 part = St[t] * Dr;
         held += (part[0] + part[1]) + (part[2] + part[3]);
-        sf[t] = F::big(St[t]), df[t] = F::big(Dr);
+        sf[t] = F::fine(St[t]), df[t] = F::fine(Dr);
         if (r + 1 < NT) St[t] = next[t];
       }
       const auto Ss = columns<VT>(sf), Ds = columns<VT>(df);
@@ -295,7 +299,7 @@ struct Grad {
         const f4 vt = F::wide(vc[t]);
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-          x = mma(kr[r], F::big(S[r][t]), x);
+          x = mma(kr[r], F::fine(S[r][t]), x);
 #pragma unroll
           for (int j = 0; j < 4; ++j) held = fmaf(S[r][t][j], D[r][t][j], held);
         }
@@ -309,7 +313,7 @@ struct Grad {
         over[t] = mma(less, U, over[t]);
         x = zero4();
 #pragma unroll
-        for (int r = 0; r < NT; ++r) x = mma(kr[r], F::big(D[r][t]), x);
+        for (int r = 0; r < NT; ++r) x = mma(kr[r], F::fine(D[r][t]), x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[j] = s.has(l.in(j)) ? d.tail[j] * kin[j] * x[j] : 0.0f;
@@ -373,10 +377,10 @@ struct Grad {
       turned(from, r, St);
 #pragma unroll
       for (int t = 0; t < VT; ++t) {
-        const auto sf = F::big(St[t]);
+        const auto sf = F::fine(St[t]);
         x = mma(dyr[t], sf, x);
         reads = mma(Wtf[t], sf, reads);
-        writes = mma(Utf[t], F::big(Dt[r][t]), writes);
+        writes = mma(Utf[t], F::fine(Dt[r][t]), writes);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -574,7 +578,8 @@ __global__ __launch_bounds__(512 / VT, 2) void delta_grad_kernel(DeltaArgs a) {
   }
 }
 
-// dq or dk of heads that share their rows: added in 32 bits, rounded once.
+// dq or dk of heads that share their rows: added in 32 bits, rounded once.  Bound by
+// reading the heads' rows.
 template <typename T>
 __global__ __launch_bounds__(256) void delta_share_kernel(const float* in, int64_t count, int share, int keys, T* dq, T* dk) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * count; i += (int64_t)gridDim.x * 256) {

@@ -303,6 +303,35 @@ def test_a_value_that_is_not_finite_reaches_later_steps_alone():
         assert float((a[:at] - b[:at]).abs().max()) <= 4 * _roundings(30, 24) * 2.0**-23 * float(b.abs().max()), name
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("which", range(5))
+def test_a_value_that_is_not_finite_at_any_step_of_a_chunk(which, dtype):
+    """The last step of a chunk, whose system does not reach it, as well as the first."""
+    from gbxcule_amd.rl import delta_rule
+
+    s = _inputs(41, 19, 1, 2, 24, 40, dtype=dtype)
+    rows = [s[k] for k in NAMES]
+    clean = [t.detach().requires_grad_() for t in rows]
+    y, _ = delta_rule(*clean, state=s["state"])
+    near = (_roundings(19, 24) * 2.0**-23 + 2 * ref.UNIT[dtype]) * float(y.detach().abs().max())
+    for at in range(19):
+        for bad in (math.nan, math.inf):
+            dirty = [t.detach().clone() for t in rows]
+            dirty[which][at].view(-1)[0] = bad
+            leaves = [t.requires_grad_() for t in dirty]
+            y2, _ = delta_rule(*leaves, state=s["state"])
+            assert not torch.isfinite(y2[at]).all()
+            if at:
+                assert float((y2[:at] - y[:at]).detach().abs().max()) <= near, (at, bad)
+            if which == 0 and at < 18:  # no later step's gradient asks for an earlier query
+                assert float((y2[at + 1 :] - y[at + 1 :]).detach().abs().max()) <= near, (at, bad)
+                found = torch.autograd.grad(y2, leaves, s["dy"])
+                want = torch.autograd.grad(y, clean, s["dy"], retain_graph=True)
+                for a, b, name in zip(found, want, NAMES):
+                    off = (4 * _roundings(19, 24) * 2.0**-23 + 2 * ref.UNIT[b.dtype]) * float(b.abs().max())
+                    assert float((a[at + 1 :] - b[at + 1 :]).abs().max()) <= off, (at, bad, name)
+
+
 def test_pieces_and_what_is_not_finite():
     """Few heads and many steps: what a value that is not finite reaches, and what an episode's start keeps from it."""
     from gbxcule_amd.rl import delta_rule
