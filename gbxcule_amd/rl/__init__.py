@@ -3,8 +3,9 @@ the reference's RL engines (``src/gbxcule/rl/``) -- preallocated rollout
 buffers, double-buffer stream coordination, packed-pixel helpers and a
 game-agnostic packed-pixel env that chains step -> render into a rollout slot
 -> RAM senses -> masked reset on torch's current stream with no host sync --
-and the operators of a policy that remembers its episode: norm, causal
-convolution, selective scan, and the optimizer that trains it."""
+and the operators of a policy that remembers its episode: norms, causal
+convolution, selective scan, gated delta rule, the drawing of actions, and the
+optimizer that trains it."""
 
 from .async_buffers import AsyncPPOBufferManager, AsyncPPOBufferState
 from .env import PackedPixelEnv, collect_rollout

@@ -1,9 +1,10 @@
 """Operators of a policy that remembers an episode, as HIP kernels.
 
-A memory block normalises its input (``rms_norm``), mixes the last few steps
-of each env (``causal_conv``), carries a state along the steps
-(``selective_scan``) and adds the result to the residual stream.  All tensors
-are time-major, as ``RolloutBuffer`` stores them: ``[T, N, ...]`` for T steps
+A memory block normalises its input (``rms_norm``, ``layer_norm``), mixes the
+last few steps of each env (``causal_conv``), carries a state along the steps
+(``selective_scan``, or a matrix a head: ``delta_rule``) and adds the result to
+the residual stream; an actor draws from the logits that come out
+(``sample_actions``).  All tensors are time-major, as ``RolloutBuffer`` stores them: ``[T, N, ...]`` for T steps
 of N envs.  ``resets`` (bool or uint8 ``[T, N]``) is set where an env begins an
 episode at that step: nothing from before reaches it, whatever it holds, so
 episodes of any length lie one after the other in a row.
@@ -131,7 +132,8 @@ def delta_rule(q, k, v, g, beta, *, scale: float | None = None, normalize: bool 
     ``sqrt(sum of squares + 1e-6)``.  ``scale=None``: ``keys ** -0.5``.
     ``state`` ``[N, heads, keys, values]`` float32 before the first step (None:
     zeros).  Returns ``(y, state after the last step)``; differentiable in
-    everything but the state.  For the gradient every 16th state is kept."""
+    everything but the state.  For the gradient every 16th state is kept, and
+    a value's correction at every step."""
     return tuple(ext.delta_rule(q, k, v, g, beta, scale, normalize, state, resets))
 
 
