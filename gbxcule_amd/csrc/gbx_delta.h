@@ -36,8 +36,8 @@
 // What bounds it: a chunk follows the one before, and of the three parts of every
 // 32-bit factor 24 bits of work come for each 8 that a matrix instruction
 // takes.  At 128 steps x 1,024 envs x 4 heads of 64 x 64 the forward pass takes
-// 298 us (moving 0.93 GB with what it keeps for the gradient, 190 us) and the
-// gradient 763 (1.4 GB, 290 us): 2,400 vector and 175 matrix instructions a
+// 289 us (moving 0.94 GB with what it keeps for the gradient, 190 us) and the
+// gradient 753 (1.1 GB, 230 us): 2,400 vector and 175 matrix instructions a
 // wavefront and chunk, and two wavefronts a SIMD to hide their waits.
 #pragma once
 #include <type_traits>

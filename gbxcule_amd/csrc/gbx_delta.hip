@@ -299,8 +299,8 @@ __global__ __launch_bounds__(64) void delta_join_kernel(DeltaArgs a, int slabs) 
 // head.  With p = sum over rows of S k and w = that of S q, the state is read
 // once, moved on in registers and written:
 //   e = beta (v - a p),  S = a S + k e^T,  y = scale (a w + (q . k) e).
-// Bound by reading and writing the state: 8,192 envs x 4 heads of 64 x 64 in 201 us,
-// 5.4 TB/s (a copy to other memory reaches 4.9); 64 envs in 6.8 us, a launch.
+// Bound by reading and writing the state: 8,192 envs x 4 heads of 64 x 64 in 203 us,
+// 5.4 TB/s (a copy to other memory reaches 4.9); 64 envs in 6.9 us, a launch.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs a, int slabs, int64_t units) {
   const int lane = threadIdx.x & 63, g = lane >> 3, c = lane & 7;
@@ -363,8 +363,8 @@ namespace {
 // Few heads and many steps are cut into pieces that run side by side: what each
 // makes of the state before it (two passes of the recurrence, over the values'
 // and over the keys' columns), the states one after the other, and the pieces again
-// from those: 8,192 steps of 8 heads of 64 x 64 in 186 us, of which the maps are 72
-// and the last pass 53; one after the other 1,568.  More pieces make the passes shorter and the join longer, which
+// from those: 8,192 steps of 8 heads of 64 x 64 in 187 us, of which the maps are 74
+// and the last pass 54; one after the other 1,568.  More pieces make the passes shorter and the join longer, which
 // takes about two thirds of a chunk's time a piece.
 DeltaArgs in_pieces(DeltaArgs a) {
   const int64_t units = (int64_t)a.envs * a.heads, waves = units * slabs_of(a.values, 1), chunks = (a.steps + kDeltaChunk - 1) / kDeltaChunk;

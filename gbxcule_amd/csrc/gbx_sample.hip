@@ -118,8 +118,8 @@ __device__ __forceinline__ void draw_few(const SampleArgs& a, int64_t row, const
   if (i == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(kept))) write(a, row, index, w / all);
 }
 
-// Up to 64 actions: L lanes a row.  Bound by a launch at 64 x 8 (6.2 us); at
-// 131,072 x 8 with every option its own a row by the arithmetic in 64 bits (12.5 us,
+// Up to 64 actions: L lanes a row.  Bound by a launch at 64 x 8 (6.4 us); at
+// 131,072 x 8 with every option its own a row by the arithmetic in 64 bits (12.8 us,
 // of which reading 8 MB is 2).
 template <typename T, int L>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
