@@ -578,16 +578,23 @@ __global__ __launch_bounds__(512 / VT, 2) void delta_grad_kernel(DeltaArgs a) {
   }
 }
 
-// dq or dk of heads that share their rows: added in 32 bits, rounded once.  Bound by
-// reading the heads' rows.
+// dq or dk of heads that share their rows: added in 32 bits, rounded once.  A thread
+// takes four channels of a row.  Bound by reading the heads' rows.
 template <typename T>
-__global__ __launch_bounds__(256) void delta_share_kernel(const float* in, int64_t count, int share, int keys, T* dq, T* dk) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * count; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / keys;
-    const float* p = in + row * share * keys + i % keys;
-    float x = 0.0f;
-    for (int n = 0; n < share; ++n) x += p[(int64_t)n * keys];
-    (i < count ? dq[i] : dk[i - count]) = (T)x;
+__global__ __launch_bounds__(256) void delta_share_kernel(const float* in, int64_t rows, int share, int keys, T* dq, T* dk) {
+  const int pieces = (keys + 3) / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * rows * pieces; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / pieces;
+    const int c = (int)(i - row * pieces) * 4;
+    const float* p = in + row * share * keys + c;
+    float x[4] = {};
+    for (int n = 0; n < share; ++n) {
+      float o[4];
+      load_row<4>(p + n * keys, keys - c, o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += o[j];
+    }
+    store_row<4>((row < rows ? dq + row * keys : dk + (row - rows) * keys) + c, keys - c, x);
   }
 }
 
@@ -611,8 +618,8 @@ hipError_t launch_delta_grad(const DeltaArgs& a, hipStream_t st) {
       });
     });
     if (a.share > 1 && failed == hipSuccess) {
-      const int64_t count = (int64_t)a.steps * a.envs * (a.heads / a.share) * a.keys;
-      hipLaunchKernelGGL((delta_share_kernel<T>), dim3((unsigned)std::min<int64_t>((2 * count + 255) / 256, 1 << 16)), dim3(256), 0, st, a.work, count, a.share, a.keys, (T*)a.dq, (T*)a.dk);
+      const int64_t rows = (int64_t)a.steps * a.envs * (a.heads / a.share), pieces = 2 * rows * ((a.keys + 3) / 4);
+      hipLaunchKernelGGL((delta_share_kernel<T>), dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16)), dim3(256), 0, st, a.work, rows, a.share, a.keys, (T*)a.dq, (T*)a.dk);
     }
   });
   return failed == hipSuccess ? hipGetLastError() : failed;
