@@ -147,3 +147,44 @@ def test_threads():
     for t in threads:
         t.join()
     assert not wrong and len(done) == len(nets), wrong
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: what is at the end equals the same rows by themselves, bit for bit."""
+    from gbxcule_amd.rl import delta_rule, delta_rule_step, layer_norm, sample_actions
+
+    gen = _gen(9)
+    some = lambda *shape, dtype=BF16: torch.empty(shape, dtype=dtype, device="cuda").normal_(generator=gen)  # noqa: E731
+    # layer norm and drawing, a row each
+    x = some(1_100_000, 2000)
+    w, b = 1 + 0.1 * some(2000, dtype=F32), some(2000, dtype=F32)
+    assert torch.equal(layer_norm(x, w, b)[-700:], layer_norm(x[-700:].clone(), w, b))
+    u = torch.rand(1_100_000, device="cuda", generator=gen)
+    for got, want in zip(sample_actions(x, u, top_k=30), sample_actions(x[-700:].clone(), u[-700:], top_k=30)):
+        assert torch.equal(got[-700:], want)
+    leaf, part = x.requires_grad_(), x[-700:].detach().clone().requires_grad_()
+    dy = some(700, 2000)
+    wide = torch.zeros_like(x)
+    wide[-700:] = dy
+    (found,) = torch.autograd.grad(layer_norm(leaf, w, b), [leaf], wide)
+    assert torch.equal(found[-700:], torch.autograd.grad(layer_norm(part, w, b), [part], dy)[0])
+    del x, leaf, found, wide
+    # the delta rule: 33 x 8,192 x 64 heads of 8 x 128, of whose envs the last 64 alone make as many wavefronts a compute unit
+    q, k, v = some(33, 8192, 64, 8), some(33, 8192, 64, 8), some(33, 8192, 64, 128)
+    g, beta = -0.1 * torch.rand(33, 8192, 64, device="cuda", generator=gen), torch.rand(33, 8192, 64, device="cuda", generator=gen)
+    rows = [q, k, v, g, beta]
+    last = lambda t: t[:, -64:].clone()  # noqa: E731
+    whole, part = [t.requires_grad_() for t in rows], [last(t.detach()).requires_grad_() for t in rows]
+    y, s = delta_rule(*whole)
+    y2, s2 = delta_rule(*part)
+    assert torch.equal(y[:, -64:], y2) and torch.equal(s[-64:], s2)
+    dy = some(33, 8192, 64, 128)
+    for got, want in zip(torch.autograd.grad(y, whole, dy), torch.autograd.grad(y2, part, last(dy))):
+        assert torch.equal(got[:, -64:], want)
+    del whole, part, y, dy, rows, got, want
+    # a step, with more than 2^31 numbers of state
+    state = some(33_000, 16, 64, 64, dtype=F32)
+    kept = state[-64:].clone()
+    rows = [some(33_000, 16, 64) for _ in range(3)] + [g.detach().flatten()[: 33_000 * 16].view(33_000, 16), beta.detach().flatten()[: 33_000 * 16].view(33_000, 16)]
+    y = delta_rule_step(*rows, state=state)
+    assert torch.equal(y[-64:], delta_rule_step(*(t[-64:].clone() for t in rows), state=kept)) and torch.equal(state[-64:], kept)

@@ -99,3 +99,13 @@ def test_sample_outputs():
     _bad(lib.gbx_sample_actions(_sample_in(), None, P, None), b"NULL")
     _bad(lib.gbx_sample_actions(_sample_in(), P, None, None), b"NULL")
     assert lib.gbx_sample_actions(_sample_in(rows=0), None, None, None) == 0
+
+
+def test_delta_rule_work_of_pieces():
+    """Few heads and many steps go in pieces, whose states are in scratch memory; many heads need none."""
+    lib = _lib.load()
+    long = _delta_in(steps=8192, envs=1, heads=8, share=1)
+    floats = lib.gbx_delta_rule_work(long)
+    assert floats >= 3 * 8 * 16 * (24 + 16)
+    _bad(lib.gbx_delta_rule(long, None, P, P, None, None, None), b"work")
+    assert lib.gbx_delta_rule_work(_delta_in(steps=8192, envs=4096)) == 0
