@@ -136,6 +136,8 @@ struct Forward {
     for (int t0 = from; t0 < upto; t0 += kDeltaChunk) {
       const Lane l = again(u.l);
       const Gates gates = load_gates(a, t0, u.env, u.head, l);
+      // a state that nothing of the chunk sees is not kept either: the gradient multiplies what is kept, and only then decays it
+      if (cut_at(gates, 0)) clear_state(S);
       keep(t0);
       int singles = 0;  // steps before this one go one by one
       for (int lo = 0; lo < gates.steps;) {

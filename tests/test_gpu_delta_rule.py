@@ -497,3 +497,58 @@ def test_refusals():
     version = state._version
     delta_rule_step(*one, state=state)
     assert state._version == version + 1
+
+
+def _behind(s, at, leaves, got, normalize=True):
+    """Gradients of the steps from `at` on, where every env begins an episode, against those of these steps alone."""
+    rest = {k: s[k][at:] for k in (*NAMES, "dy")}
+    wide = [ref.f64(rest[k]).requires_grad_() for k in NAMES]
+    want, _ = _plain(*wide, None, None, normalize)
+    n = _roundings(len(rest["q"]), s["q"].shape[3])
+    for a, b, leaf, name in zip(got, torch.autograd.grad(want, wide, ref.f64(rest["dy"])), leaves, NAMES):
+        assert torch.isfinite(a[at:]).all(), name
+        terms = _terms(wide, {**rest, "state": None, "resets": None}, None)[name] if normalize and name in "qk" else 0.0
+        # what is redone span by span computes u anew, another order of the same sums
+        _check_terms(a[at:], b, 2 * 4 * n + s["v"].shape[3], terms, f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("keys, values", [(64, 64), (24, 40)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("closed", [False, True])
+def test_a_state_that_an_episode_at_the_first_step_leaves_behind(dtype, keys, values, bad, closed):
+    """Fresh memory as a state, with an episode that begins, or a gate that closes, at step 0: no gradient sees it."""
+    from gbxcule_amd.rl import delta_rule
+
+    s = _inputs(70, 19, 2, 2, keys, values, dtype=dtype)
+    state = s["state"].clone()
+    state[1, 0, 3, 5] = bad
+    state[0] = bad
+    resets = None
+    if closed:
+        s["g"][0] = -200.0
+    else:
+        resets = torch.zeros(19, 2, dtype=torch.bool, device="cuda")
+        resets[0] = True
+    leaves = _leaves(s)
+    y, last = delta_rule(*leaves, state=state, resets=resets)
+    assert torch.isfinite(y).all() and torch.isfinite(last).all()
+    _behind(s, 0, leaves, torch.autograd.grad(y, leaves, s["dy"]))
+
+
+def test_a_state_that_overflows_right_before_an_episode():
+    """The last correction of a chunk is finite and takes the state past the largest number; an episode begins with the next chunk."""
+    from gbxcule_amd.rl import delta_rule
+
+    s = _inputs(71, 36, 1, 1, 16, 16, normalize=False)
+    for k in ("q", "k", "v", "g", "beta", "dy"):
+        s[k][:16] = 0.0
+    s["k"][15, ..., :2], s["beta"][15], s["v"][15] = 0.5, 1.0, 1e38
+    state = torch.zeros(1, 1, 16, 16, device="cuda")
+    state[..., 0, :], state[..., 1, :] = 3.3e38, -3.3e38  # of which the key reads nothing, and adds 0.5e38 to the one
+    resets = torch.zeros(36, 1, dtype=torch.bool, device="cuda")
+    resets[16] = True
+    leaves = _leaves(s)
+    y, last = delta_rule(*leaves, state=state, resets=resets, normalize=False)
+    assert torch.isfinite(y[16:]).all() and torch.isfinite(last).all()
+    _behind(s, 16, leaves, torch.autograd.grad(y, leaves, s["dy"]), False)
