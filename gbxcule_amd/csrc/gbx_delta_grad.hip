@@ -123,7 +123,11 @@ struct Grad {
 
   // Walks a chunk back whose system is solved.  False, and nothing done, if a
   // value is not finite: in a product zero times infinity would reach steps that the
-  // formulas keep from it.
+  // formulas keep from it.  Looked at is what the other products take: w, which all
+  // that the system or D holds goes through, and u itself, whose first step no row
+  // of the system has (its beta may be infinite, or u overflow, with u / beta finite;
+  // a u / beta that is not finite makes u so for any beta).  The kept state is finite
+  // where u is: where it is read, u has read it, and where it is not, it is zero.
   __device__ __forceinline__ bool chunk(const Solved<true>& z, const float* kept, const Steps<float, VT, FULL>& over, float& dgate, f4& dbeta) {
     const Span s{0, z.steps};
     const int lane = 16 * l.g + l.c;
@@ -170,7 +174,7 @@ struct Grad {
         Wt[t] = mma(x, T_col, zero4());
         Ut[t] = er[t].v * beta;
         bsum += W[t] * ec[t].v;
-        fine = fine && finite4(W[t]) && finite4(ec[t].v);
+        fine = fine && finite4(W[t]) && finite4(Ut[t]);
       }
       if (!__all(fine)) return false;
     }

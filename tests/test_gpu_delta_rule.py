@@ -552,3 +552,23 @@ def test_a_state_that_overflows_right_before_an_episode():
     y, last = delta_rule(*leaves, state=state, resets=resets, normalize=False)
     assert torch.isfinite(y[16:]).all() and torch.isfinite(last).all()
     _behind(s, 16, leaves, torch.autograd.grad(y, leaves, s["dy"]), False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("keys, values", [(64, 64), (24, 40)])
+@pytest.mark.parametrize("at", [0, 16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e38])
+def test_a_correction_right_before_an_episode(dtype, keys, values, at, bad):
+    """The correction of a chunk's first step is in no other's: one that is not finite, or is only with what it
+    is made of, leaves the system as it is, and no gradient of the episode that begins behind it sees it."""
+    from gbxcule_amd.rl import delta_rule
+
+    s = _inputs(72, 36, 2, 2, keys, values, dtype=dtype)
+    s["beta"][at] = bad
+    s["v"][at, ..., ::2], s["v"][at, ..., 1::2] = 100.0, -100.0
+    resets = torch.zeros(36, 2, dtype=torch.bool, device="cuda")
+    resets[at + 1] = True
+    leaves = _leaves(s)
+    y, last = delta_rule(*leaves, state=s["state"], resets=resets)
+    assert torch.isfinite(y[at + 1 :]).all() and torch.isfinite(last).all()
+    _behind(s, at + 1, leaves, torch.autograd.grad(y, leaves, s["dy"]))
