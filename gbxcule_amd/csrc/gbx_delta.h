@@ -56,6 +56,15 @@ constexpr float kUnitEps = 1e-6f;  // added to a squared length before its root
 
 __device__ __forceinline__ f4 zero4() { return f4{0.0f, 0.0f, 0.0f, 0.0f}; }
 
+// What a decay leaves of a sum: of none nothing, though the sum be infinite (of finite
+// values from before an episode, say, as large as memory may hold that nothing has written).
+__device__ __forceinline__ float left_of(float x, float decay) { return decay == 0.0f ? 0.0f : x * decay; }
+__device__ __forceinline__ f4 left_of(f4 x, f4 decay) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = left_of(x[j], decay[j]);
+  return x;
+}
+
 // Factors of a product, four places of the summed index a lane.
 //
 // Whole: 32 bits, on the 32-bit matrix instructions, which sum 4 places in twice
@@ -611,9 +620,9 @@ __device__ __forceinline__ void solve_chunk(const DeltaArgs& a, int t0, int env,
     const float apart = (float)(sum - z.sums[l.in(j)]);
     const bool same = ((upto ^ ((2u << l.in(j)) - 1u)) & gates.cuts) == 0u;
     pair[j] = same ? exp2_fast(l.in(j) < l.c ? apart : -apart) : 0.0f;
-    p[j] = kk[j] * (kap * kin[j]) * pair[j];
-    if constexpr (GRAD) m[j] = l.in(j) < l.c ? 0.0f : kq[j] * (kap * qin[j] * a.scale) * pair[j];
-    else m[j] = l.in(j) <= l.c ? kq[j] * (qap * kin[j]) * pair[j] : 0.0f;
+    p[j] = left_of(kk[j] * (kap * kin[j]), pair[j]);
+    if constexpr (GRAD) m[j] = l.in(j) < l.c ? 0.0f : left_of(kq[j] * (kap * qin[j] * a.scale), pair[j]);
+    else m[j] = l.in(j) <= l.c ? left_of(kq[j] * (qap * kin[j]), pair[j]) : 0.0f;
   }
   const Both t = solve<GRAD>(p, gates.beta, bin, l);
   z.t[lane] = GRAD ? t.col : t.row;

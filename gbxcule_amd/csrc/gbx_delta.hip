@@ -121,7 +121,7 @@ struct Forward {
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
       const f4 U = bin * E[t];
-      if (!MAP) Y[t] = mma(kq, F::fine(U), Y[t] * qin);
+      if (!MAP) Y[t] = mma(kq, F::fine(U), left_of(Y[t], qin));
       const Fine<T> x = F::fine(U * tail);
 #pragma unroll
       for (int r = 0; r < NT; ++r) S[r][t] = mma(kc[r], x, S[r][t] * all);

@@ -206,10 +206,10 @@ struct Grad {
       f4 p = mma(Us, dys, zero4()), pt = mma(dys, Us, zero4()), m = mma(Us, Ws, zero4()), mt = mma(Ws, Us, zero4());
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        p[j] = l.in(j) <= l.c ? p[j] * (a.scale * kin[j]) * pair[j] : 0.0f;
-        pt[j] = l.in(j) < l.c ? 0.0f : pt[j] * (a.scale * qin[j]) * pair[j];
-        m[j] = l.in(j) < l.c ? -m[j] * (beta * kin[j]) * pair[j] : 0.0f;
-        mt[j] = l.in(j) <= l.c ? 0.0f : -mt[j] * (bin[j] * kin[j]) * pair[j];
+        p[j] = l.in(j) <= l.c ? left_of(p[j] * (a.scale * kin[j]), pair[j]) : 0.0f;
+        pt[j] = l.in(j) < l.c ? 0.0f : left_of(pt[j] * (a.scale * qin[j]), pair[j]);
+        m[j] = l.in(j) < l.c ? left_of(-m[j] * (beta * kin[j]), pair[j]) : 0.0f;
+        mt[j] = l.in(j) <= l.c ? 0.0f : left_of(-mt[j] * (bin[j] * kin[j]), pair[j]);
       }
       pf = F::fine(p), ptf = F::fine(pt), mf = F::fine(m), mtf = F::fine(mt);
     }
@@ -231,9 +231,9 @@ struct Grad {
         if (r + 1 < NT) St[t] = next[t];
       }
       const auto Ss = columns<VT>(sf), Ds = columns<VT>(df);
-      const f4 x = mma(pf, kc[r], mma(dys, Ss, zero4()) * qs);
-      const f4 reads = mma(mf, kc[r], mma(Ws, Ss, zero4()) * rs);
-      const f4 writes = mma(writers, two(qc[r], kc[r]), mma(Us, Ds, zero4()) * tail);
+      const f4 x = mma(pf, kc[r], left_of(mma(dys, Ss, zero4()), qs));
+      const f4 reads = mma(mf, kc[r], left_of(mma(Ws, Ss, zero4()), rs));
+      const f4 writes = mma(writers, two(qc[r], kc[r]), left_of(mma(Us, Ds, zero4()), tail));
       e += qin * F::wide(qc[r]) * x + kin * F::wide(kc[r]) * (reads - writes);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -241,7 +241,7 @@ struct Grad {
         part[((NT + r) * 4 + j) * 64] = reads[j] + writes[j];
       }
     }
-    whole = row_sum(whole + all * held);
+    whole = row_sum(whole + left_of(held, all));
     whole = from_lane(whole, l.c) + from_lane(whole, l.c + 16) + from_lane(whole, l.c + 32) + from_lane(whole, l.c + 48);
     float own = 0.0f;  // e of step c, then the sum from there to before the next cut
 #pragma unroll

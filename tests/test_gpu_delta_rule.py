@@ -572,3 +572,54 @@ def test_a_correction_right_before_an_episode(dtype, keys, values, at, bad):
     y, last = delta_rule(*leaves, state=s["state"], resets=resets)
     assert torch.isfinite(y[at + 1 :]).all() and torch.isfinite(last).all()
     _behind(s, at + 1, leaves, torch.autograd.grad(y, leaves, s["dy"]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("keys, values", [(64, 64), (24, 40)])
+@pytest.mark.parametrize("at", [1, 7, 16, 21])
+@pytest.mark.parametrize("big", [1e19, 1e30, 3e38])
+def test_large_values_before_an_episode(dtype, keys, values, at, big):
+    """Memory that nothing has written holds such numbers as often as ones that are not finite: products of
+    them overflow, and zero, which is what an episode's start leaves of them, times infinity is no zero."""
+    from gbxcule_amd.rl import delta_rule
+
+    big = min(big, torch.finfo(dtype).max)
+    for which in ("q", "k", "v", "beta", "g", "state", "q k", "k v", "q k v g beta state"):
+        for normalize in (True, False):
+            s = _inputs(73, 40, 2, 2, keys, values, dtype=dtype, normalize=normalize)
+            gen = _gen(74)
+            for name in which.split():
+                t = s[name] if name == "state" else s[name][:at]
+                t.copy_(torch.where(_rand(gen, *t.shape) < 0.3, big * torch.sign(_randn(gen, *t.shape)), t.float()))
+            resets = torch.zeros(40, 2, dtype=torch.bool, device="cuda")
+            resets[at] = True
+            leaves = _leaves(s)
+            y, last = delta_rule(*leaves, state=s["state"], resets=resets, normalize=normalize)
+            want, want_last = _plain(*(ref.f64(s[k][at:]) for k in NAMES), None, None, normalize)
+            ref.check(y[at:], want, _roundings(40, keys), f"y after {which}")
+            ref.check(last, want_last, _roundings(40, keys), f"state after {which}")
+            _behind(s, at, leaves, torch.autograd.grad(y, leaves, s["dy"]), normalize)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("steps, at, keys, values", [(40, 1, 64, 64), (40, 16, 24, 40), (40, 23, 64, 64), (33, 32, 128, 48), (520, 300, 32, 24)])
+def test_memory_that_nothing_has_written_before_an_episode(dtype, steps, at, keys, values):
+    """Any bits at all, in everything from before it."""
+    from gbxcule_amd.rl import delta_rule
+
+    for seed in range(6):
+        s = _inputs(75 + seed, steps, 1, 2, keys, values, dtype=dtype)
+        gen = _gen(90 + seed)
+        for name in (*NAMES, "state"):
+            t = s[name] if name == "state" else s[name][:at]
+            word = torch.int32 if t.dtype is F32 else torch.int16
+            bits = torch.randint(-(2**31), 2**31, t.shape, device="cuda", generator=gen)
+            t.copy_(bits.to(word).view(t.dtype))
+        resets = torch.zeros(steps, 1, dtype=torch.bool, device="cuda")
+        resets[at] = True
+        leaves = _leaves(s)
+        y, last = delta_rule(*leaves, state=s["state"], resets=resets)
+        want, want_last = _plain(*(ref.f64(s[k][at:]) for k in NAMES), None, None)
+        ref.check(y[at:], want, _roundings(steps, keys), "y")
+        ref.check(last, want_last, _roundings(steps, keys), "state")
+        _behind(s, at, leaves, torch.autograd.grad(y, leaves, s["dy"]))
