@@ -136,13 +136,12 @@ struct Forward {
     for (int t0 = from; t0 < upto; t0 += kDeltaChunk) {
       const Lane l = again(u.l);
       const Gates gates = load_gates(a, t0, u.env, u.head, l);
-      // a state that nothing of the chunk sees is not kept either: the gradient multiplies what is kept, and only then decays it
-      if (cut_at(gates, 0)) clear_state(S);
-      keep(t0);
       int singles = 0;  // steps before this one go one by one
       for (int lo = 0; lo < gates.steps;) {
         const Span s{lo, lo < singles ? lo + 1 : next_cut(gates, lo)};
         if (cut_at(gates, lo)) clear_state(S);
+        // (a state that nothing of the chunk sees is kept as zeros: the gradient multiplies what is kept, and only then decays it)
+        if (lo == 0) keep(t0);
         Raw<T> kr[NT], qr[NT], kc[NT], vc[VT];
         k.rows(t0, s, l, kr);
         q.rows(t0, s, l, qr);
