@@ -72,6 +72,9 @@ __device__ __forceinline__ f4 left_of(f4 x, f4 decay) {
 // values, each what the ones before leave; an input's bfloat16 is one part, a
 // float16 exactly two.  A product of two sums is their terms' products, added in
 // 32 bits, two of them in an instruction that sums 32 places.
+// Three parts hold a 32-bit value whole; two lose its last eight bits, which brought
+// the learner's recurrence from 1,400 to 1,020 us and its results from 3e-7 to 4e-6.
+constexpr int kParts = 3;
 struct Whole {
   f4 v;
 };
@@ -115,7 +118,7 @@ __device__ __forceinline__ f4 two_terms(w2 a, w2 b, w2 a2, w2 b2, f4 d) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, w4{a[0], a[1], a2[0], a2[1]}), __builtin_bit_cast(b8, w4{b[0], b[1], b2[0], b2[1]}), d, 0, 0, 0);
 }
 __device__ __forceinline__ f4 one_term(w2 a, w2 b, f4 d) { return two_terms(a, b, a, w2{0u, 0u}, d); }
-// Terms whose places add up to more than the longer sum's last are below its
+// Terms whose places add up to more than a whole value's last, kParts - 1, are below its
 // rounding and left out, but where an instruction has room for one.
 template <int A, int B>
 __device__ __forceinline__ f4 mma(const Parts<A>& a, const Parts<B>& b, f4 d) {
@@ -155,7 +158,7 @@ __device__ __forceinline__ f4 mma(const WholeTwo& a, const WholeTwo& b, f4 d) { 
 template <int A, int B>
 __device__ __forceinline__ f4 mma(const PartsTwo<A>& a, const PartsTwo<B>& b, f4 d) {
 #pragma unroll
-  for (int n = (A > B ? A : B) - 1; n >= 0; --n)  // the small terms first
+  for (int n = kParts - 1; n >= 0; --n)  // the small terms first
 #pragma unroll
     for (int i = 0; i < A; ++i)
 #pragma unroll
@@ -237,9 +240,6 @@ __device__ __forceinline__ uint32_t pick(const uint32_t* p, const uint32_t* q) {
 }
 
 // How the products take the inputs, of type T, and values computed from them.
-// Three parts hold a 32-bit value whole; two lose its last eight bits, which brought
-// the learner's recurrence from 1,400 to 1,020 us and its results from 3e-7 to 4e-6.
-constexpr int kParts = 3;
 template <typename T>
 struct Factor {
   using Raw = Parts<1>;

@@ -623,3 +623,30 @@ def test_memory_that_nothing_has_written_before_an_episode(dtype, steps, at, key
         ref.check(y[at:], want, _roundings(steps, keys), "y")
         ref.check(last, want_last, _roundings(steps, keys), "state")
         _behind(s, at, leaves, torch.autograd.grad(y, leaves, s["dy"]))
+
+
+@pytest.mark.parametrize("keys", [16, 33, 64, 128])
+def test_products_of_keys_in_float16(keys):
+    """1 + 2^-8 and its products have no more digits than 32-bit sums hold in any order, so that all
+    that is off in a state is its few roundings, of 2^-24 each: two of a length's root and sum, one of u, two of what
+    scales it, one of its parts and up to six of the terms added. A bfloat16 holds the 1, and the square of what it
+    leaves is 2^-16 of the product: half of that, of a length's root, would be 128 of these roundings."""
+    from gbxcule_amd.rl import delta_rule, delta_rule_step
+
+    gen = _gen(80)
+    sign = torch.where(_rand(gen, 1, 3, 2, keys) < 0.5, -1.0, 1.0)
+    q = k = (sign * (1.0 + 2.0**-8)).to(F16)
+    v, g, beta = _randn(gen, 1, 3, 2, 40, dtype=F16), torch.zeros(1, 3, 2, device="cuda"), torch.full((1, 3, 2), 0.75, device="cuda")
+    _, last = delta_rule(q, k, v, g, beta)
+    _, want = _plain(*(ref.f64(t) for t in (q, k, v, g, beta)), None, None)
+    ref.check(last, want, 8, "state of unit keys")
+    state = torch.zeros_like(last)
+    delta_rule_step(*(t[0] for t in (q, k, v, g, beta)), state=state)
+    ref.check(state, want, 8, "state of a single step")
+    # keys of their own length, the same one at two steps, the second of which corrects the first: the product is in
+    # what is recalled, and both steps' roundings in the state, which is half of what they are of
+    k2 = torch.cat([k, k]) * 2.0**-3 if keys == 64 else torch.cat([k, k]) * 2.0**-4
+    rows = [k2, k2, torch.cat([v, torch.zeros_like(v)]), torch.cat([g, g]), torch.cat([beta, beta])]
+    _, last = delta_rule(*rows, normalize=False)
+    _, want = _plain(*(ref.f64(t) for t in rows), None, None, False)
+    ref.check(last, want, 32, "state of plain keys")
