@@ -33,9 +33,9 @@ __device__ __forceinline__ Cuts cuts_of(const SampleArgs& a, int64_t row) {
   c.k = a.top_ks ? a.top_ks[row] : a.top_k;
   if (!(c.heat > 0.0)) c.heat = 0.0;
   if (c.heat == 0.0 || !(c.p > 0.0) || !(c.least <= 1.0)) c.k = 1;
+  if (c.k == 1) c.p = 1.0, c.least = 0.0;  // before k becomes `all`, as it does where there is one action
   if (c.k < 0 || c.k >= a.actions) c.k = 0;
-  if (c.k == 1 || c.p >= 1.0) c.p = 1.0;
-  if (c.k == 1) c.least = 0.0;
+  if (c.p >= 1.0) c.p = 1.0;
   return c;
 }
 // NaN stands for an action that is not allowed, as -infinity does.

@@ -5,6 +5,7 @@ random numbers, streams, graphs, and refusals."""
 
 from __future__ import annotations
 
+import itertools
 import math
 
 import pytest
@@ -247,3 +248,31 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError, match="no gradient"):
         sample_actions(x.clone().requires_grad_(), u)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_one_action_with_any_options(dtype):
+    """It is always drawn, whatever the cuts are: every output is written."""
+    from gbxcule_amd import _lib
+
+    lib = _lib.load()
+    values = {
+        "temperatures": [0.0, -1.0, math.nan, 1e-30, 1.0, math.inf],
+        "top_ps": [0.0, -1.0, math.nan, 1e-30, 0.5, 1.0],
+        "min_ps": [-1.0, 0.0, 1.0, 1.5, math.inf, math.nan],
+    }
+    grid = torch.tensor(list(itertools.product(*values.values())), device="cuda")
+    rows = len(grid)
+    ks = torch.tensor([-1, 0, 1, 2], dtype=torch.int32, device="cuda").repeat(rows)[:rows]
+    logits = torch.tensor([0.5, -3.0, math.inf, -math.inf, math.nan], device="cuda").repeat(rows)[:rows].to(dtype)
+    uniform = torch.rand(rows, device="cuda", generator=_gen(8))
+    action, logp = torch.full((rows,), 77, dtype=torch.int32, device="cuda"), torch.full((rows,), 77.0, device="cuda")
+    each = [grid[:, i].contiguous() for i in range(3)]
+    given = _lib.SampleIn(rows=rows, actions=1, elem={F32: 0, BF16: 1, F16: 2}[dtype], logits=logits.data_ptr(), stride=1, uniform=uniform.data_ptr(),
+                          top_ks=ks.data_ptr(), **{k: t.data_ptr() for k, t in zip(values, each)})  # fmt: skip
+    assert lib.gbx_sample_actions(given, action.data_ptr(), logp.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    allowed = logits > -math.inf  # not NaN either
+    assert torch.equal(action, torch.where(allowed, 0, -1).int())
+    assert not logp[allowed].any() and torch.isnan(logp[~allowed]).all()
+    for name, option in zip(("temperature", "top_p", "min_p"), each):  # one of them alone, by the public name
+        _check(logits.unsqueeze(1), uniform, **{name: option})
