@@ -574,7 +574,9 @@ Tensor delta_rule_step(const Tensor& q, const Tensor& k, const Tensor& v, const 
 std::vector<Tensor> sample_actions(const Tensor& logits, const Tensor& uniform, const std::variant<double, Tensor>& temperature, const std::variant<int64_t, Tensor>& top_k,
                                    const std::variant<double, Tensor>& top_p, const std::variant<double, Tensor>& min_p) {
   const int elem = input("logits", logits);
-  no_grad("sample_actions", {&logits});
+  const auto tensor = [](const auto& o) { return std::get_if<Tensor>(&o); };
+  no_grad("sample_actions", {&logits, &uniform, tensor(temperature), tensor(top_p), tensor(min_p)});
+  no_tangent("sample_actions", {&logits, &uniform, tensor(temperature), tensor(top_p), tensor(min_p)});
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits: expected [..., actions], got ", logits.sizes());
   const IntArrayRef lead(logits.sizes().data(), logits.dim() - 1);
   const auto row = [&](const char* name, const Tensor& t, at::ScalarType kind) {

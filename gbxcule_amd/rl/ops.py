@@ -160,5 +160,6 @@ def sample_actions(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
     number or a tensor ``[...]`` with one for each row (float32, ``top_k`` int32).
 
     NaN and -infinity are never drawn; a row of nothing else has action -1 and
-    logp NaN.  Weights and sums are in 64 bits.  No gradient."""
+    logp NaN.  Weights and sums are in 64 bits.  No gradient, of the logits or
+    the options."""
     return tuple(ext.sample_actions(logits, uniform, temperature, top_k, top_p, min_p))

@@ -276,3 +276,23 @@ def test_one_action_with_any_options(dtype):
     assert not logp[allowed].any() and torch.isnan(logp[~allowed]).all()
     for name, option in zip(("temperature", "top_p", "min_p"), each):  # one of them alone, by the public name
         _check(logits.unsqueeze(1), uniform, **{name: option})
+
+
+def test_no_derivative_is_dropped():
+    """Tangents and gradients are refused, of the logits and of the options."""
+    import torch.autograd.forward_ad as fwad
+
+    from gbxcule_amd.rl import sample_actions
+
+    x, u, one = torch.randn(4, 8, device="cuda"), torch.rand(4, device="cuda"), torch.full((4,), 0.5, device="cuda")
+    tensors = {"logits": x, "uniform": u, "temperature": one, "top_p": one, "min_p": one}
+    for name in tensors:
+        leaf = tensors[name].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            sample_actions(**{**tensors, name: leaf})
+        with torch.no_grad():
+            action, logp = sample_actions(**{**tensors, name: leaf})
+        want = sample_actions(**tensors)
+        assert torch.equal(action, want[0]) and torch.equal(logp, want[1])
+        with fwad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            sample_actions(**{**tensors, name: fwad.make_dual(tensors[name], torch.ones_like(tensors[name]))})
