@@ -249,7 +249,8 @@ class MemoryActor:
         logits, values = self.policy.step(frames, self.state, resets, self.entries)
         if self.sampling is not None:
             actions, logp = sample_actions(logits, torch.rand_like(values), **self.sampling)
-            return actions, values, logp
+            # -1 is no action: where all logits are NaN the env plays 0, and logp stays NaN
+            return actions.clamp_min(0), values, logp
         logp = torch.log_softmax(logits, -1)
         noise = -torch.log(-torch.log(torch.rand_like(logp).clamp_min(1e-20)).clamp_min(1e-20))
         actions = (logp + noise).argmax(-1)

@@ -138,3 +138,29 @@ def test_refusals():
     policy = _policy(torch.bfloat16)
     with pytest.raises(ValueError, match="fp8"):
         MemoryActor(policy, 4, None, fp8=True)
+
+
+def test_an_env_whose_state_is_not_finite_plays_an_action(carts):
+    """Its logits are NaN, so nothing can be drawn from them: it plays on, and rollout and loss say so."""
+    from gbxcule_amd.rl import AdamW, PackedPixelEnv, RolloutBuffer, collect_rollout
+    from gbxcule_amd.rl.memory import MemoryActor, learn
+
+    n, steps = 8, 5
+    env = PackedPixelEnv(carts["c3"], num_envs=n, frames_per_step=2)
+    try:
+        env.reset(seed=0)
+        rollout = RolloutBuffer(steps=steps, num_envs=n, stack_k=1, obs_format="packed2", obs_steps=steps + 1)
+        policy = _policy(torch.bfloat16)
+        actor = MemoryActor(policy, n, rollout, sampling={"temperature": 0.9})
+        actor.begin_rollout(torch.zeros(n, dtype=torch.bool, device="cuda"))
+        for s in actor.state:
+            s.scan[2] = float("nan")
+        actor.begin_rollout(actor.starts)
+        last = collect_rollout(env, actor, rollout)
+        assert int(rollout.actions.min()) >= 0 and int(rollout.actions.max()) < 8
+        bad = torch.isnan(rollout.logprobs)
+        assert bad[:, 2].all() and int(bad.sum()) == steps
+        (loss,) = learn(actor, AdamW(policy.parameters(), lr=1e-3), last, passes=1)
+        assert torch.isnan(loss)
+    finally:
+        env.close()

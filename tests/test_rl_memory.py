@@ -1,0 +1,89 @@
+"""The actor and the learner of ``gbxcule_amd.rl.memory`` around a policy whose
+logits are given, on the CPU: what the actor stores of a draw, and what the
+learner makes of it."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from gbxcule_amd.rl import RolloutBuffer, memory
+
+STEPS, ENVS, ACTIONS = 5, 6, 4
+
+
+class GivenPolicy(nn.Module):
+    """Logits and values of each step and env as parameters."""
+
+    memory = "delta"
+
+    def __init__(self) -> None:
+        super().__init__()
+        gen = torch.Generator().manual_seed(1)
+        self.logits = nn.Parameter(torch.randn(STEPS, ENVS, ACTIONS, generator=gen))
+        self.values = nn.Parameter(torch.randn(STEPS, ENVS, generator=gen))
+        self.eye = torch.zeros(1)
+        self.blocks = nn.ModuleList()
+        self.at = 0
+
+    def initial_state(self, envs):
+        return []
+
+    def forward(self, frames, state, resets):
+        return self.logits, self.values
+
+    @torch.no_grad()
+    def step(self, frames, state, resets, entries=None):
+        k = min(self.at, STEPS - 1)
+        self.at += 1
+        return self.logits[k].detach(), self.values[k].detach()
+
+
+class Kept:
+    """An optimizer that moves nothing and keeps the gradients of each step."""
+
+    def __init__(self, policy) -> None:
+        self.policy, self.seen = policy, []
+
+    def zero_grad(self) -> None:
+        self.policy.zero_grad()
+
+    def step(self, grad_scale) -> None:
+        self.seen.append([p.grad.clone() for p in self.policy.parameters()])
+
+
+def _draw(logits, uniform, *, temperature=1.0, **_):
+    """``sample_actions`` on the CPU, with temperatures alone."""
+    heat = torch.as_tensor(temperature, dtype=torch.float64).expand(len(logits)).unsqueeze(-1)
+    sharp = torch.log_softmax(logits.double() / heat.clamp_min(1e-6), -1)
+    action = (sharp.exp().cumsum(-1) <= uniform.double().unsqueeze(-1)).sum(-1).clamp_max(logits.shape[-1] - 1)
+    logp = sharp.gather(-1, action.unsqueeze(-1)).squeeze(-1)
+    nothing = torch.isnan(logits).all(-1)
+    return torch.where(nothing, -1, action).int(), torch.where(nothing, math.nan, logp).float()
+
+
+def _played(monkeypatch, policy, sampling):
+    monkeypatch.setattr(memory, "sample_actions", _draw)
+    torch.manual_seed(2)
+    rollout = RolloutBuffer(steps=STEPS, num_envs=ENVS, stack_k=1, obs_format="packed2", device="cpu", obs_steps=STEPS + 1)
+    actor = memory.MemoryActor(policy, ENVS, rollout, sampling=sampling)
+    rollout.reset()
+    for t in range(STEPS):
+        actions, values, logp = actor(rollout.obs_slot(t))
+        rollout.set_step_fields(t, actions, torch.randn(ENVS), torch.zeros(ENVS, dtype=torch.bool), values, logp)
+    return actor, rollout
+
+
+def test_an_env_with_nothing_to_draw_from_plays_an_action(monkeypatch):
+    """A policy that has diverged: the sampler's -1 is no action, and the learner reads logits by the actions."""
+    policy = GivenPolicy()
+    with torch.no_grad():
+        policy.logits[:, 2] = math.nan
+    actor, rollout = _played(monkeypatch, policy, {})
+    assert int(rollout.actions.min()) >= 0 and int(rollout.actions.max()) < ACTIONS
+    assert torch.isnan(rollout.logprobs[:, 2]).all() and torch.isfinite(rollout.logprobs[:, :2]).all()
+    (loss,) = memory.learn(actor, Kept(policy), rollout.obs_slot(STEPS), passes=1)
+    assert torch.isnan(loss)  # as with the default actor: it shows
