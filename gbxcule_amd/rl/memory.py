@@ -226,7 +226,8 @@ class MemoryActor:
 
     ``sampling``: options of ``sample_actions`` (numbers, or tensors with one for
     each env, such as a ladder of temperatures); the log-probabilities are then those
-    that the actions were drawn with.  None: from the policy's own distribution."""
+    that the actions were drawn with, and ``learn`` takes them for what they are.
+    None: from the policy's own distribution."""
 
     def __init__(self, policy: MemoryPolicy, num_envs: int, rollout, *, fp8: bool = False, sampling: dict | None = None) -> None:
         if fp8 and policy.memory != "scan":
@@ -275,7 +276,11 @@ def advantages(rewards, dones, values, last_value, *, discount: float = 0.99, tr
 
 def learn(actor: MemoryActor, optimizer, last_frames, *, passes: int = 2, clip: float = 0.2, max_norm: float = 1.0) -> list:
     """Clipped policy-gradient passes over the collected rollout; returns the
-    losses as device scalars (nothing here synchronises)."""
+    losses as device scalars (nothing here synchronises).
+
+    The clip is around the policy's own probability of an action before the first
+    pass.  Where the actor drew with ``sampling``, that is another one than it was
+    drawn with, and their ratio, at most 1, weighs the action's gain."""
     policy, r = actor.policy, actor.rollout
     # the value after the last step, from a copy of the states the rollout ended with
     state = [BlockState(*(t.clone() for t in s)) for s in actor.state]
@@ -285,10 +290,15 @@ def learn(actor: MemoryActor, optimizer, last_frames, *, passes: int = 2, clip: 
     gain = (gain - gain.mean()) / (gain.std() + 1e-6)
     frames, resets, actions = r.obs[: r.steps], actor.resets(), r.actions.long().unsqueeze(-1)
     losses = []
+    before = r.logprobs if actor.sampling is None else None
     for _ in range(passes):
         logits, values = policy(frames, actor.first_state, resets)
         logp = torch.log_softmax(logits, -1)
-        ratio = torch.exp(logp.gather(-1, actions).squeeze(-1) - r.logprobs)
+        taken = logp.gather(-1, actions).squeeze(-1)
+        if before is None:
+            before = taken.detach()
+            gain = gain * torch.exp(before - r.logprobs).clamp_max(1.0)
+        ratio = torch.exp(taken - before)
         gained = torch.minimum(ratio * gain, ratio.clamp(1 - clip, 1 + clip) * gain)
         entropy = -(logp.exp() * logp).sum(-1)
         loss = -gained.mean() + 0.5 * (values - target).square().mean() - 0.01 * entropy.mean()

@@ -87,3 +87,43 @@ def test_an_env_with_nothing_to_draw_from_plays_an_action(monkeypatch):
     assert torch.isnan(rollout.logprobs[:, 2]).all() and torch.isfinite(rollout.logprobs[:, :2]).all()
     (loss,) = memory.learn(actor, Kept(policy), rollout.obs_slot(STEPS), passes=1)
     assert torch.isnan(loss)  # as with the default actor: it shows
+
+
+def _advantage(rollout):
+    gain = memory.advantages(rollout.rewards, rollout.dones, rollout.values, rollout.values[-1])
+    return (gain - gain.mean()) / (gain.std() + 1e-6)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0, 2.0])
+def test_the_clip_is_around_the_policy_that_drew(monkeypatch, temperature):
+    """The first pass's gradient is that of the weighted gains, with every ratio 1 and so no action
+    clipped away: an env that always takes its likeliest action learns from the bad ones, too."""
+    policy = GivenPolicy()
+    actor, rollout = _played(monkeypatch, policy, {"temperature": temperature})
+    kept = Kept(policy)
+    memory.learn(actor, kept, rollout.obs_slot(STEPS), passes=1)
+    logits = policy.logits.detach().double().requires_grad_()
+    logp = torch.log_softmax(logits, -1)
+    taken = logp.gather(-1, rollout.actions.long().unsqueeze(-1)).squeeze(-1)
+    weight = torch.exp(taken.detach() - rollout.logprobs.double()).clamp_max(1.0)
+    gain = _advantage(rollout).double()
+    (-(weight * gain * taken).mean() + 0.01 * (logp.exp() * logp).sum(-1).mean()).backward()
+    torch.testing.assert_close(kept.seen[0][0].double(), logits.grad, rtol=1e-4, atol=1e-6)
+    if temperature == 0.0:
+        assert bool(((taken.detach().exp() < 1 - 0.2) & (gain < 0)).any())  # which a clip around the draw's own 1 would drop
+
+
+def test_an_actor_without_options_is_learned_from_as_before(monkeypatch):
+    """The clip is around what the actor stored."""
+    policy = GivenPolicy()
+    actor, rollout = _played(monkeypatch, policy, None)
+    rollout.logprobs.sub_(0.05)  # as 16-bit rounding may move them
+    kept = Kept(policy)
+    memory.learn(actor, kept, rollout.obs_slot(STEPS), passes=1, clip=0.01)
+    logits = policy.logits.detach().double().requires_grad_()
+    logp = torch.log_softmax(logits, -1)
+    ratio = torch.exp(logp.gather(-1, rollout.actions.long().unsqueeze(-1)).squeeze(-1) - rollout.logprobs.double())
+    gain = _advantage(rollout).double()
+    gained = torch.minimum(ratio * gain, ratio.clamp(0.99, 1.01) * gain)
+    (-gained.mean() + 0.01 * (logp.exp() * logp).sum(-1).mean()).backward()
+    torch.testing.assert_close(kept.seen[0][0].double(), logits.grad, rtol=1e-4, atol=1e-6)
