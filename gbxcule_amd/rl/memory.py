@@ -177,6 +177,8 @@ class MemoryPolicy(nn.Module):
     """Packed frames ``[..., 1, 72, 20]`` -> action logits and values.
     ``memory``: ``"scan"`` or ``"delta"``, the kind of its blocks."""
 
+    memory = "scan"  # of policies saved whole before there was a choice
+
     def __init__(self, num_actions: int, *, dim: int = 256, blocks: int = 2, states: int = 16, dtype=torch.bfloat16, memory: str = "scan") -> None:
         super().__init__()
         if memory not in ("scan", "delta"):
@@ -229,8 +231,10 @@ class MemoryActor:
     that the actions were drawn with, and ``learn`` takes them for what they are.
     None: from the policy's own distribution."""
 
+    sampling = None  # of actors saved whole before there was a choice
+
     def __init__(self, policy: MemoryPolicy, num_envs: int, rollout, *, fp8: bool = False, sampling: dict | None = None) -> None:
-        if fp8 and policy.memory != "scan":
+        if fp8 and getattr(policy, "memory", "scan") != "scan":
             raise ValueError("fp8 needs a policy with memory='scan'")
         self.policy, self.rollout, self.fp8, self.sampling = policy, rollout, fp8, sampling
         self.state = policy.initial_state(num_envs)
@@ -290,7 +294,7 @@ def learn(actor: MemoryActor, optimizer, last_frames, *, passes: int = 2, clip: 
     gain = (gain - gain.mean()) / (gain.std() + 1e-6)
     frames, resets, actions = r.obs[: r.steps], actor.resets(), r.actions.long().unsqueeze(-1)
     losses = []
-    before = r.logprobs if actor.sampling is None else None
+    before = r.logprobs if getattr(actor, "sampling", None) is None else None
     for _ in range(passes):
         logits, values = policy(frames, actor.first_state, resets)
         logp = torch.log_softmax(logits, -1)

@@ -5,6 +5,7 @@ learner makes of it."""
 from __future__ import annotations
 
 import math
+import types
 
 import pytest
 import torch
@@ -127,3 +128,33 @@ def test_an_actor_without_options_is_learned_from_as_before(monkeypatch):
     gained = torch.minimum(ratio * gain, ratio.clamp(0.99, 1.01) * gain)
     (-gained.mean() + 0.01 * (logp.exp() * logp).sum(-1).mean()).backward()
     torch.testing.assert_close(kept.seen[0][0].double(), logits.grad, rtol=1e-4, atol=1e-6)
+
+
+def test_policies_and_actors_from_before_the_options():
+    """One that was saved whole, or a policy of a user's own, has no kind of memory and no options of a draw."""
+    policy = memory.MemoryPolicy(ACTIONS, dim=16, blocks=1)
+    policy.__dict__.pop("memory", None)
+    rollout = RolloutBuffer(steps=STEPS, num_envs=ENVS, stack_k=1, obs_format="packed2", device="cpu", obs_steps=STEPS + 1)
+    actor = memory.MemoryActor(policy, ENVS, rollout, fp8=True)
+    assert policy.memory == "scan" and len(actor.entries) == 1
+    actor.__dict__.pop("sampling", None)
+    assert actor.sampling is None
+
+    class Own(GivenPolicy):
+        @property
+        def memory(self):
+            raise AttributeError("memory")
+
+    assert memory.MemoryActor(Own(), ENVS, rollout, fp8=True).entries == []
+
+
+def test_an_actor_of_a_users_own(monkeypatch):
+    """What ``learn`` reads of it is what it read before there were options."""
+    policy = GivenPolicy()
+    actor, rollout = _played(monkeypatch, policy, None)
+    names = ("policy", "rollout", "state", "first_state", "entries", "resets")
+    own = types.SimpleNamespace(**{name: getattr(actor, name) for name in names})
+    both = Kept(policy)
+    for a in (actor, own):
+        memory.learn(a, both, rollout.obs_slot(STEPS), passes=1)
+    assert all(torch.equal(p, q) for p, q in zip(*both.seen))
