@@ -301,7 +301,10 @@ __global__ __launch_bounds__(64) void delta_join_kernel(DeltaArgs a, int slabs) 
 // once, moved on in registers and written:
 //   e = beta (v - a p),  S = a S + k e^T,  y = scale (a w + (q . k) e).
 // Bound by reading and writing the state: 8,192 envs x 4 heads of 64 x 64 in 203 us,
-// 5.4 TB/s (a copy to other memory reaches 4.9); 64 envs in 6.9 us, a launch.
+// 5.4 TB/s (a copy to other memory reaches 4.9).  64 envs take 6.9 us, the kernel 6.1
+// where one that is no more than a launch takes 3.2: a wavefront's own chain, the state's
+// loads behind the gate's and the episode start's and sums over rows behind those,
+// in 128 workgroups, which leave half of the compute units without one.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs a, int slabs, int64_t units) {
   const int lane = threadIdx.x & 63, g = lane >> 3, c = lane & 7;

@@ -14,8 +14,9 @@ namespace {
 // those of what is left when the mean is gone: the mean of the squares minus
 // the mean's square would lose as many digits as the mean is larger than the
 // spread.  Bound by HBM where there are many rows and by a launch where there are
-// few: 131,072 x 512 in 16 bits with a residual, forward and gradient, in 205 us
-// (941 MB, 4.6 TB/s), 64 x 256 in 6.9 us.
+// few: 131,072 x 512 in 16 bits with a residual in 91 us (537 MB, 5.9 TB/s), with the
+// gradient in 205 (1,074 MB, 5.2 TB/s); to 8,192 channels at 5.3 TB/s, over
+// that, where each pass reads the row again, 3.8; 64 x 256 in 6.9 us.
 template <typename T, int LANES, int NV, int ENDS>
 __global__ __launch_bounds__(threads_of(LANES)) void layer_norm_kernel(LayerNormArgs a) {
   constexpr int kRows = threads_of(LANES) / LANES, kHeld = NV ? NV : 1;
@@ -103,11 +104,16 @@ __device__ __forceinline__ float less(float g, float mean) {
 //   dweight = sum over rows of dy * c * r,  dbias = sum over rows of dy.
 // The row stays in registers as in the forward kernel and its mean is summed
 // again, so nothing but s itself has to be kept from the forward; the other
-// three sums go together.  A workgroup sums dweight and dbias over its rows in
+// three sums are made in one pass over the row, each with an exchange of its own.  A workgroup sums dweight and dbias over its rows in
 // registers, then over its row slots in LDS, and writes one row of partial
 // sums, dbias's columns after dweight's: no atomics, one order.  Bound by HBM; rows
 // that no 16-byte load divides cost what their split lines do (20,011 x 1,023 in 32
-// bits, forward and gradient: 95 us, 410 MB, 4.3 TB/s).
+// bits, forward and gradient: 95 us, 410 MB with x once for each, 4.3 TB/s).  Two pieces
+// a lane leave registers for three wavefronts a SIMD (65,536 x 1,024 in 16 bits with a
+// residual: 162 us, 3.3 TB/s); rows over 1,024 channels are a workgroup's, whose eight
+// barriers a row nothing else fills (32,768 x 2,048 135 us, 4.0 TB/s; 8,192 x 8,192 182 us,
+// 2.9); over 8,192 every pass reads the row again, and a workgroup's partial sums are in
+// memory (4,096 x 16,384: 784 us).
 template <typename T, int LANES, int NV, int ENDS>
 __global__ __launch_bounds__(threads_of(LANES)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
   constexpr int kThreads = threads_of(LANES), kRows = kThreads / LANES, kHeld = NV ? NV : 1;

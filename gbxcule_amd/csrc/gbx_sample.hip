@@ -118,9 +118,10 @@ __device__ __forceinline__ void draw_few(const SampleArgs& a, int64_t row, const
   if (i == (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(kept))) write(a, row, index, w / all);
 }
 
-// Up to 64 actions: L lanes a row.  Bound by a launch at 64 x 8 (6.4 us); at
-// 131,072 x 8 with every option its own a row by the arithmetic in 64 bits (12.8 us,
-// of which reading 8 MB is 2).
+// Up to 64 actions: L lanes a row.  Bound by a launch at 64 x 8 (6.4 us).  131,072 x
+// 8 with every option its own a row takes 12.8 us, of which reading 8 MB is 2: every lane
+// goes over its row's others by exchanges, so the sums for ranks and shares, in 64 bits,
+// are made eight times, and the logarithm and the division for one lane in eight.
 template <typename T, int L>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs a) {
   const int i = threadIdx.x % L;
@@ -474,7 +475,8 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
     // their weights are needed: a long row is then read twice in whole lines and
     // not held (512 x 32,768 in 16 bits, top_k 50: 20 us, held 70).  Other cuts
     // may leave the whole row to search, with a weight for each turn, and hold it
-    // (the same with top_p alone: 248 us, read again at each turn 893).
+    // (the same with top_p alone: 248 us, read again at each turn 893).  A top_k of
+    // each row's own takes the held form, 35 us: a row's may be 0.
     const bool cut = !a.top_ks && a.top_k > 0 && a.top_k <= 512;
     using std::integral_constant;
     if (a.actions <= 8) few(integral_constant<int, 8>{});
